@@ -20,6 +20,13 @@ __all__ = [
     "MixedRound",
     "SparseAttention",
     "sparse_attention",
+    "TreeAttention",
+    "tree_attention",
+    "DraftVerifier",
+    "Rotary",
+    "rotary_frequencies",
+    "KvRowStore",
+    "PageTables",
     "VllmIndexSelector",
     "PagedIndexer",
     "RequestPlan",
@@ -49,6 +56,13 @@ _EXPORTS = {
     "MixedRound": ("operators.mixed", "MixedRound"),
     "SparseAttention": ("operators.sfa", "SparseAttention"),
     "sparse_attention": ("operators.sfa", "sparse_attention"),
+    "TreeAttention": ("operators.tree", "TreeAttention"),
+    "tree_attention": ("operators.tree", "tree_attention"),
+    "DraftVerifier": ("operators.verify", "DraftVerifier"),
+    "Rotary": ("operators.rotary", "Rotary"),
+    "rotary_frequencies": ("operators.rotary", "rotary_frequencies"),
+    "KvRowStore": ("operators.rotary", "KvRowStore"),
+    "PageTables": ("cache.page_tables", "PageTables"),
     "VllmIndexSelector": ("adapters.vllm.selector", "VllmIndexSelector"),
     "PagedIndexer": ("adapters.vllm.selector", "PagedIndexer"),
     "RequestPlan": ("adapters.vllm.selector", "RequestPlan"),

@@ -1,0 +1,333 @@
+// Verification of drafted tokens against the target's probabilities (kvip_hip_draft.h).
+//
+// The walk needs one probability per drafted token, p(its parent's row, the token), so it is decided
+// before any row is read whole; then one row per request is (two after a refused child of a drawn
+// chain): its weights' sum, and the place where the running sum passes the drawn share.
+// What bounds it: reading those rows. They are split over workgroups of 4096 weights. Each repeats the
+// walk (one wave, a lane per token: one gather, then register work) instead of a launch before it,
+// sums its weights in 64 bits and counts itself on the request's ticket; the last one adds up the
+// sums in order, finds the part that holds the place and goes through it again (from the cache).
+// The sums cross workgroups as atomics of agent scope between a release and an acquire of the ticket; as
+// a workgroup writes eight bytes, the release has next to nothing to write back.
+#include "kvip_device.h"
+#include "kvip_hip_draft.h"
+
+namespace kvip {
+namespace {
+
+constexpr int kVerifyThreads = 256;
+constexpr int kPerLane = 16;                              // weights per thread
+constexpr int kPart = kVerifyThreads * kPerLane;          // weights per workgroup
+constexpr int kMaxParts = (1 << 20) / kPart;
+
+template <typename T> struct Weights;  // 16 bytes of them, at any element address
+template <> struct Weights<float> { typedef float vec __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Weights<__bf16> { typedef __bf16 vec __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Weights<_Float16> { typedef _Float16 vec __attribute__((ext_vector_type(8), aligned(2))); };
+
+KVIP_DEVICE double shuffle_double(double v, int lane) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(__shfl(static_cast<int>(bits), lane));
+    const uint32_t hi = static_cast<uint32_t>(__shfl(static_cast<int>(bits >> 32), lane));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+KVIP_DEVICE double wave_sum(double v) {
+    for (int d = 32; d > 0; d >>= 1) v += shuffle_double(v, lane_id() ^ d);
+    return v;
+}
+
+// Inclusive running sum over the lanes.
+KVIP_DEVICE double wave_running(double v) {
+    for (int d = 1; d < 64; d <<= 1) {
+        const double before = shuffle_double(v, max(lane_id() - d, 0));
+        if (lane_id() >= d) v += before;
+    }
+    return v;
+}
+
+struct Walk {
+    int end;                              // row (within the request) where the walk ends
+    int kept;                             // its rows
+    int residual;                         // weights are max(probs - draft_probs, 0)
+    int excluded;                         // tokens whose weight is 0
+    int tokens[KVIP_DRAFT_MAX_NODES];
+};
+
+// The walk of request b, by one wave. `write`: also its path, and the tokens taken.
+template <typename T>
+KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, bool write, Walk* w) {
+    const int lane = lane_id();
+    const T* probs = static_cast<const T*>(p.probs);
+    const T* draft = static_cast<const T*>(p.draft_probs);
+    const bool live = lane < n;
+    const int64_t token = live ? p.tokens[begin + lane] : -1;
+    const bool named = token >= 0 && token < p.vocab;
+    int up = !live || lane == 0 ? -1 : p.parents != nullptr ? p.parents[begin + lane] : lane - 1;
+    uint32_t err = live && lane > 0 && !named ? KVIP_STATUS_BAD_TOKEN : 0u;
+    if (up < -1 || up >= lane) {
+        if (live && lane > 0) err |= KVIP_STATUS_BAD_TREE;
+        up = -1;
+    }
+    const bool child = up >= 0 && named;
+    double mine = 0.0, drawn = 0.0;
+    if (child) {
+        mine = static_cast<double>(static_cast<float>(probs[(begin + up) * p.probs_stride + token]));
+        if (draft != nullptr) drawn = static_cast<double>(static_cast<float>(draft[(begin + up) * p.draft_stride + token]));
+    }
+    if (!(mine > 0.0)) mine = 0.0;
+    const double uniform = live ? static_cast<double>(p.uniforms[begin + lane]) : 0.0;
+    int at = 0, kept = 1, residual = 0;
+    int place = lane == 0 ? 0 : -1;  // lane i: row of the walk's i-th token
+    unsigned long long tried;
+    for (;;) {  // at most n rounds: a child comes after its parent
+        tried = __ballot(child && up == at);
+        const double u = shuffle_double(uniform, at);
+        int next = -1;
+        if (draft != nullptr) {
+            const int c = at + 1;
+            if (tried != 0) {
+                const double q = shuffle_double(drawn, c), t = shuffle_double(mine, c);
+                if (u * q < t) next = c;
+            }
+            // A token outside the vocabulary is refused too.
+            if (next < 0) residual = c < n;
+        } else {
+            double low = 0.0;
+            unsigned long long left = tried;
+            while (left != 0) {
+                const int c = __ffsll(left) - 1;
+                const int64_t name = static_cast<int64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(token), c)));
+                left &= ~__ballot(child && up == at && token == name);  // named again: nothing left
+                const double high = low + shuffle_double(mine, c);
+                if (low <= u && u < high) {
+                    next = c;
+                    break;
+                }
+                low = high;
+            }
+        }
+        if (next < 0) break;
+        at = next;
+        if (lane == kept) place = at;
+        ++kept;
+    }
+    if (lane == 0) {
+        w->end = at;
+        w->kept = kept;
+        w->residual = residual;
+        w->excluded = draft != nullptr ? 0 : __popcll(tried);
+    }
+    if (draft == nullptr && (tried >> lane & 1)) {
+        w->tokens[__popcll(tried & ((1ull << lane) - 1))] = static_cast<int>(token);
+    }
+    if (!write) return;
+    report(p.status, err);
+    const int64_t following = __shfl(static_cast<int>(token), max(__shfl(place, min(lane + 1, 63)), 0));
+    if (lane < p.max_nodes) {
+        p.path[static_cast<int64_t>(b) * p.max_nodes + lane] = place;
+        if (lane + 1 != kept) {  // the drawn token comes from the request's last workgroup
+            p.out_tokens[static_cast<int64_t>(b) * p.max_nodes + lane] = lane + 1 < kept ? following : -1;
+        }
+    }
+    if (lane == 0) p.kept[b] = kept;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerifyArgs p) {
+    typedef typename Weights<T>::vec V;
+    constexpr int kLoad = 16 / sizeof(T);
+    __shared__ Walk s_walk;
+    __shared__ double s_wave[kVerifyThreads / 64], s_before, s_left;
+    __shared__ int s_last, s_part, s_found, s_near, s_count, s_gone[KVIP_DRAFT_MAX_NODES];
+    const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int begin = min(max(p.cu_seqlens[b], 0), p.max_tokens);
+    const int all = min(max(p.cu_seqlens[b + 1], begin), p.max_tokens) - begin;
+    const int n = min(all, p.max_nodes);
+    if (part == 0 && tid == 0 && all > n) report(p.status, KVIP_STATUS_BAD_LENGTH);
+    if (n == 0) {  // uniform over the request's workgroups: its ticket is not used
+        if (part == 0 && tid < p.max_nodes) {
+            p.path[static_cast<int64_t>(b) * p.max_nodes + tid] = -1;
+            p.out_tokens[static_cast<int64_t>(b) * p.max_nodes + tid] = -1;
+            if (tid == 0) p.kept[b] = 0;
+        }
+        return;
+    }
+    if (wave == 0) walk_request<T>(p, b, begin, n, part == 0, &s_walk);
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    const int64_t row = begin + s_walk.end;
+    const T* probs = static_cast<const T*>(p.probs) + row * p.probs_stride;
+    const T* draft = s_walk.residual ? static_cast<const T*>(p.draft_probs) + row * p.draft_stride : nullptr;
+
+    // The weights [at, at + kLoad) of the row, in 64 bits: exact.
+    auto weights = [&](int at, double* out) {
+        V a{}, d{};
+        if (at + kLoad <= p.vocab) {
+            a = *reinterpret_cast<const V*>(probs + at);
+            if (draft != nullptr) d = *reinterpret_cast<const V*>(draft + at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kLoad; ++e) {
+                if (at + e < p.vocab) {
+                    a[e] = probs[at + e];
+                    if (draft != nullptr) d[e] = draft[at + e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kLoad; ++e) {
+            const double x = static_cast<double>(static_cast<float>(a[e])) - static_cast<double>(static_cast<float>(d[e]));
+            out[e] = x > 0.0 ? x : 0.0;  // also a NaN
+        }
+    };
+    auto exclude = [&](int at, double* x, int count, const int* gone) {
+        for (int k = 0; k < count; ++k) {
+#pragma unroll
+            for (int e = 0; e < kLoad; ++e) {
+                if (gone[k] == at + e) x[e] = 0.0;
+            }
+        }
+    };
+    // Of the excluded tokens, those of part `which` (few or none).
+    auto gather_gone = [&](int which) {
+        if (tid < s_walk.excluded) {
+            const int t = s_walk.tokens[tid];
+            if (t / kPart == which) s_gone[atomicAdd(&s_count, 1)] = t;
+        }
+        __syncthreads();
+    };
+    gather_gone(part);
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kPerLane / kLoad; ++j) {
+        const int at = part * kPart + (j * kVerifyThreads + tid) * kLoad;
+        double x[kLoad];
+        weights(at, x);
+        exclude(at, x, s_count, s_gone);
+#pragma unroll
+        for (int e = 0; e < kLoad; ++e) sum += x[e];
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) s_wave[wave] = sum;
+    __syncthreads();
+    double* sums = static_cast<double*>(p.workspace) + static_cast<int64_t>(b) * gridDim.x;
+    uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<double*>(p.workspace) + static_cast<int64_t>(p.batch) * gridDim.x) + b;
+    if (tid == 0) {
+        const double whole = (s_wave[0] + s_wave[1]) + (s_wave[2] + s_wave[3]);
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(sums + part), __builtin_bit_cast(uint64_t, whole), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+        s_last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        if (s_last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+
+    // The part in which the running sum passes the share, and the sum before it: one part per thread
+    // (at most 256), in order.
+    static_assert(kMaxParts <= kVerifyThreads, "a part per thread");
+    const double mine = tid < static_cast<int>(gridDim.x)
+                            ? __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<uint64_t*>(sums + tid),
+                                                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) : 0.0;
+    // Runs a block-wide inclusive sum of v; returns it, and the whole to *total.
+    auto running = [&](double v, double* total) {
+        const double in_wave = wave_running(v);
+        __syncthreads();
+        if (lane == 63) s_wave[wave] = in_wave;
+        __syncthreads();
+        double before = 0.0, whole = 0.0;
+#pragma unroll
+        for (int k = 0; k < kVerifyThreads / 64; ++k) {
+            before += k < wave ? s_wave[k] : 0.0;
+            whole += s_wave[k];
+        }
+        *total = whole;
+        return before + in_wave;
+    };
+    double whole;
+    const double upto = running(mine, &whole);
+    const double target = static_cast<double>(p.final_uniforms[b]) * whole;
+    if (tid == 0) {
+        s_part = kMaxParts;
+        s_near = -1;
+        s_found = 1 << 30;
+        s_count = 0;
+    }
+    __syncthreads();
+    const bool drawable = whole > 0.0 && whole <= 1.7976931348623157e308;
+    if (mine > 0.0) {
+        if (upto > target) atomicMin(&s_part, tid);
+        atomicMax(&s_near, tid);  // a share of 1 or one lost to rounding: the last part with a weight
+    }
+    __syncthreads();
+    const int chosen = s_part < kMaxParts ? s_part : s_near;
+    if (drawable && tid == chosen) {
+        s_before = upto - mine;
+        s_left = target;
+    }
+    __syncthreads();
+    int64_t drawn = -1;
+    if (drawable) {
+        gather_gone(chosen);
+        if (tid == 0) s_near = -1;
+        // In order: 16 weights in a row per thread.
+        const int at = chosen * kPart + tid * kPerLane;
+        double x[kPerLane], own = 0.0;
+#pragma unroll
+        for (int j = 0; j < kPerLane / kLoad; ++j) {
+            weights(at + j * kLoad, x + j * kLoad);
+            exclude(at + j * kLoad, x + j * kLoad, s_count, s_gone);
+        }
+#pragma unroll
+        for (int e = 0; e < kPerLane; ++e) own += x[e];
+        double unused;
+        double sum_to = running(own, &unused) - own + s_before;
+        int found = 1 << 30, last = -1;
+#pragma unroll
+        for (int e = 0; e < kPerLane; ++e) {
+            sum_to += x[e];
+            if (x[e] > 0.0) {
+                if (sum_to > s_left && found == 1 << 30) found = at + e;
+                last = at + e;
+            }
+        }
+        if (found < 1 << 30) atomicMin(&s_found, found);
+        if (last >= 0) atomicMax(&s_near, last);
+        __syncthreads();
+        drawn = s_found < 1 << 30 ? s_found : s_near;
+    }
+    if (tid == 0) {
+        if (!drawable) report(p.status, KVIP_STATUS_BAD_PROBS);
+        p.out_tokens[static_cast<int64_t>(b) * p.max_nodes + s_walk.kept - 1] = drawn;
+    }
+}
+
+int verify_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
+
+}  // namespace
+}  // namespace kvip
+
+extern "C" uint64_t kvip_hip_verify_drafts_workspace_bytes(int32_t batch, int32_t vocab) {
+    if (batch < 1 || vocab < 1) return 0;
+    return static_cast<uint64_t>(batch) * kvip::verify_parts(vocab) * sizeof(double) + (batch + 1) / 2 * 8;
+}
+
+extern "C" uint32_t kvip_hip_verify_drafts(const KvipVerifyArgs* a, void* stream) {
+    if (a == nullptr) return KVIP_ERR_INVALID;
+    const bool ok = a->probs && a->tokens && a->cu_seqlens && a->uniforms && a->final_uniforms && a->out_tokens && a->kept &&
+                    a->path && a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 7u) == 0 &&
+                    (a->draft_probs == nullptr || a->parents == nullptr) && a->batch >= 1 &&
+                    a->batch <= KVIP_DRAFT_MAX_BATCH && a->max_nodes >= 1 && a->max_nodes <= KVIP_DRAFT_MAX_NODES &&
+                    a->max_tokens >= 1 && a->max_tokens <= KVIP_DRAFT_MAX_TOKENS && a->vocab >= 1 && a->vocab <= (1 << 20) &&
+                    a->probs_stride >= a->vocab && (a->draft_probs == nullptr || a->draft_stride >= a->vocab) &&
+                    (a->dtype == KVIP_DTYPE_FP32 || a->dtype == KVIP_DTYPE_BF16 || a->dtype == KVIP_DTYPE_FP16);
+    if (!ok) return KVIP_ERR_INVALID;
+    const dim3 grid(kvip::verify_parts(a->vocab), a->batch), block(kvip::kVerifyThreads);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (a->dtype) {
+        case KVIP_DTYPE_FP32: hipLaunchKernelGGL(kvip::verify_kernel<float>, grid, block, 0, s, *a); break;
+        case KVIP_DTYPE_BF16: hipLaunchKernelGGL(kvip::verify_kernel<__bf16>, grid, block, 0, s, *a); break;
+        default: hipLaunchKernelGGL(kvip::verify_kernel<_Float16>, grid, block, 0, s, *a); break;
+    }
+    return static_cast<uint32_t>(hipGetLastError());
+}

@@ -10,6 +10,7 @@ from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parents[1] / "_lib" / "libkvip_hip.so"
 ABI_VERSION = 15
+DRAFT_ABI_VERSION = 1
 
 KVIP_OK = 0
 KVIP_ERR_INVALID = 100000
@@ -17,10 +18,15 @@ KVIP_ERR_INVALID = 100000
 DTYPE_FP8_E4M3 = 0
 DTYPE_BF16 = 1
 DTYPE_FP32 = 2
+DTYPE_FP16 = 3
 
 STATUS_BAD_BLOCK = 1
 STATUS_HISTOGRAM = 2
 STATUS_BAD_TOKEN = 4
+STATUS_NO_PAGE = 8       # this and the following: include/kvip_hip_draft.h
+STATUS_BAD_LENGTH = 16
+STATUS_BAD_TREE = 32
+STATUS_BAD_PROBS = 64
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -185,6 +191,67 @@ class SparseAttnArgs(ctypes.Structure):
     ]
 
 
+DRAFT_MAX_NODES = 64
+DRAFT_MAX_BATCH = 1024
+DRAFT_MAX_TOKENS = 1 << 20
+
+
+class PageTableArgs(ctypes.Structure):
+    _fields_ = [
+        ("block_table", _p), ("lengths", _p), ("free_pages", _p), ("free_count", _p), ("bases", _p), ("steps", _p),
+        ("ticket", _p), ("counts", _p), ("parents", _p), ("targets", _p), ("path", _p), ("rows", _p),
+        ("cu_seqlens", _p), ("positions", _p), ("slots", _p), ("visible", _p), ("status", _p),
+        ("batch", _i32), ("max_blocks", _i32), ("num_blocks", _i32), ("max_tokens", _i32), ("path_stride", _i32),
+        ("row_sets", _i32), ("kept", _i32), ("reserved", _i32),
+    ]
+
+
+class PagedRows(ctypes.Structure):
+    _fields_ = [("base", _i64), ("block_stride", _i64), ("row_stride", _i64), ("row_bytes", _i64)]
+
+
+class RotaryTensor(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("out", _p), ("x_token", _i64), ("x_head", _i64), ("out_token", _i64), ("out_head", _i64),
+        ("heads", _i32), ("dim", _i32),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("tensors", RotaryTensor * 2), ("positions", _p), ("frequencies", _p), ("tokens", _i64),
+        ("rotary_dim", _i32), ("half", _i32), ("inverse", _i32), ("dtype", _i32), ("magnitude", ctypes.c_float),
+        ("reserved", _i32),
+    ]
+
+
+class RowStoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("latent", _p), ("rope", _p), ("slots", _p), ("positions", _p), ("frequencies", _p), ("kv_cache", _p),
+        ("status", _p), ("latent_stride", _i64), ("rope_stride", _i64), ("kv_block_stride", _i64), ("tokens", _i64),
+        ("row_stride", _i32), ("num_blocks", _i32), ("half", _i32), ("dtype", _i32), ("magnitude", ctypes.c_float),
+        ("reserved", _i32),
+    ]
+
+
+class TreeAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", _p), ("kv_cache", _p), ("block_table", _p), ("seq_lens", _p), ("cu_seqlens", _p), ("visible", _p),
+        ("output", _p), ("lse", _p), ("workspace", _p), ("status", _p), ("kv_block_stride", _i64),
+        ("row_stride", _i32), ("batch", _i32), ("heads", _i32), ("max_nodes", _i32), ("max_tokens", _i32),
+        ("max_blocks", _i32), ("num_blocks", _i32), ("output_dtype", _i32), ("scale", ctypes.c_float), ("reserved", _i32),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("probs", _p), ("draft_probs", _p), ("tokens", _p), ("cu_seqlens", _p), ("parents", _p), ("uniforms", _p),
+        ("final_uniforms", _p), ("out_tokens", _p), ("kept", _p), ("path", _p), ("workspace", _p), ("status", _p),
+        ("probs_stride", _i64), ("draft_stride", _i64), ("batch", _i32), ("max_nodes", _i32), ("max_tokens", _i32),
+        ("vocab", _i32), ("dtype", _i32), ("reserved", _i32),
+    ]
+
+
 # name -> (argtypes, restype); must list every function declared in include/kvip_hip.h.
 PROTOTYPES = {
     "kvip_hip_abi_version": ([], ctypes.c_uint32),
@@ -237,6 +304,20 @@ PROTOTYPES = {
                                    _p], ctypes.c_uint32),
 }
 
+# The same for include/kvip_hip_draft.h.
+DRAFT_PROTOTYPES = {
+    "kvip_hip_draft_abi_version": ([], ctypes.c_uint32),
+    "kvip_hip_page_tables_extend": ([ctypes.POINTER(PageTableArgs), _p], ctypes.c_uint32),
+    "kvip_hip_page_tables_move": ([ctypes.POINTER(PageTableArgs), _p], ctypes.c_uint32),
+    "kvip_hip_page_tables_truncate": ([ctypes.POINTER(PageTableArgs), _p], ctypes.c_uint32),
+    "kvip_hip_rotary": ([ctypes.POINTER(RotaryArgs), _p], ctypes.c_uint32),
+    "kvip_hip_store_rows": ([ctypes.POINTER(RowStoreArgs), _p], ctypes.c_uint32),
+    "kvip_hip_tree_attention": ([ctypes.POINTER(TreeAttnArgs), _p], ctypes.c_uint32),
+    "kvip_hip_tree_attention_workspace_bytes": ([_i32, _i32, _i32, _i32], ctypes.c_uint64),
+    "kvip_hip_verify_drafts": ([ctypes.POINTER(VerifyArgs), _p], ctypes.c_uint32),
+    "kvip_hip_verify_drafts_workspace_bytes": ([_i32, _i32], ctypes.c_uint64),
+}
+
 _LIB = None
 
 
@@ -257,12 +338,15 @@ def load_library(path: Path | None = None):
             "(kvip_amd has no CPU fallback)"
         )
     lib = ctypes.CDLL(str(path))
-    for name, (argtypes, restype) in PROTOTYPES.items():
+    for name, (argtypes, restype) in (*PROTOTYPES.items(), *DRAFT_PROTOTYPES.items()):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = argtypes, restype
     version = lib.kvip_hip_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"libkvip_hip.so ABI {version} != expected {ABI_VERSION}; rebuild")
+    version = lib.kvip_hip_draft_abi_version()
+    if version != DRAFT_ABI_VERSION:
+        raise RuntimeError(f"libkvip_hip.so draft ABI {version} != expected {DRAFT_ABI_VERSION}; rebuild")
     if path == LIBRARY:
         _LIB = lib
     return lib
@@ -290,3 +374,18 @@ def device_of(torch, device):
 
 def stream_handle(torch, device) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch(torch, device, entry, args, what: str) -> None:
+    """Calls a C entry with the current stream of `device`, which is made the current device around the
+    call where it is not (a stream handle of 0 names the current device's default stream)."""
+    if torch.cuda.current_device() == device.index:
+        check(entry(ctypes.byref(args), stream_handle(torch, device)), what)
+        return
+    with torch.cuda.device(device):
+        check(entry(ctypes.byref(args), stream_handle(torch, device)), what)
+
+
+def require(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
