@@ -3,12 +3,11 @@
 // and 64 bf16 rotary features: key = [nope * scale, rope], value = nope * scale.
 //
 // The rows of the problem are a request's (step token, head) pairs, which all read the same cache rows.
-// A workgroup of 4 waves takes R groups of 32 rows (R = 1, 2, 4) by 4 / R streams of 32-token tiles, a wave
-// per group and stream. A wave keeps its 32 queries (36 fragments, 144 registers) and its 32 x 512
-// accumulator (256 accumulation registers, one wave per SIMD has 512) and exchanges nothing until the
-// streams are merged at the end:
-//   - A tile stays as it is in the cache: direct-to-LDS loads put its fp8 bytes into a two-slot ring, the
-//     next tile landing while this one is computed.
+// A workgroup of 4 waves takes R groups of 32 rows (R = 2, 4) by 4 / R streams of 32-token tiles, a wave per
+// group and stream. A wave keeps its 32 queries (128 registers) and its 32 x 512 accumulator (the 256
+// accumulation registers; one wave per SIMD has 512 in all) and exchanges nothing until the streams are
+// merged at the end:
+//   - A tile stays as it is in the cache: direct-to-LDS loads put its fp8 bytes into a ring of three slots.
 //   - Logits are computed transposed (tokens x rows): bf16 MFMA of the key bytes, converted as they are read
 //     (exact), with the query; a scale group's dot products are summed on their own and added as
 //     fma(group, scale, s) in fp32.
@@ -17,6 +16,9 @@
 //     without leaving their registers, as the order of tokens along K is free. The value operand (8
 //     tokens of one feature per lane) comes from the token-major tile by transposing LDS reads.
 //   - The running maximum is raised lazily, when a tile exceeds it by kTaMargin.
+//   - One wave per SIMD hides nothing by itself, so the tile loop is one stretch of 68 MFMAs with everything
+//     else in between: the logits of tile t + 1, then the values of tile t with the softmax of tile t + 1
+//     beside them; operands are read from LDS several products ahead and converted one ahead.
 //
 // The (request, row tile, token steps) are laid out in one line and cut into equal shares, one per
 // workgroup, so that ragged batches keep every CU busy; what a share has of an item that others
@@ -42,6 +44,7 @@ constexpr int kTaThreads = 256;
 constexpr int kTaWaves = 4;
 constexpr int kTaRows = 32;                 // rows per wave (MFMA N)
 constexpr int kTaTile = 32;                 // tokens per tile
+constexpr int kTaSlots = 3;                 // tiles of a stream's ring
 constexpr int kKeyDim = 576;                // 512 nope + 64 rope
 constexpr int kValueDim = 512;
 constexpr int kScaleGroups = 4;
@@ -57,31 +60,28 @@ constexpr int kNopeSlot = kTaTile * kValueDim;
 constexpr int kRopeSlot = kTaTile * 128;
 constexpr int kScaleSlot = kScaleGroups * kTaTile * 4;
 
-// LDS of a workgroup with R row groups: per stream two slots of nope bytes, one (R = 1: LDS has no room
-// for two) or two of rope, two of scales [group][token]; then the work line's prefix sums. The merge of the
-// streams takes the front (8 blocks of 4 KB per wave).
+// LDS of a workgroup with R row groups: per stream the ring's nope bytes, rope and scales [group][token]; the
+// query's rope fragments; per wave and row visibility bits, later the softmax's state. The work line stands
+// in the ring's place at first, the merge of two streams at the end.
 template <int R>
 struct TaLds {
     static constexpr int kStreams = kTaWaves / R;
-    static constexpr int kRopeSlots = R == 1 ? 1 : 2;
-    static constexpr int kRope = kStreams * 2 * kNopeSlot;
-    static constexpr int kScale = kRope + kStreams * kRopeSlots * kRopeSlot;
-    static constexpr int kFront = kScale + kStreams * 2 * kScaleSlot;
-    static constexpr int kMerge = kStreams == 1 ? 0 : kTaWaves * 8 * 4096;
-    static constexpr int kState = kFront > kMerge ? kFront : kMerge;  // [wave][row] maximum and sum
-    static constexpr int kLine = kState + kTaWaves * kTaRows * 8;
-    static constexpr int kBytes = kLine + (KVIP_DRAFT_MAX_BATCH + 1) * 8 + 64;
+    static constexpr int kRope = kStreams * kTaSlots * kNopeSlot;
+    static constexpr int kScale = kRope + kStreams * kTaSlots * kRopeSlot;
+    static constexpr int kQuery = kScale + kStreams * kTaSlots * kScaleSlot;
+    static constexpr int kState = kQuery + R * 4096;
+    static constexpr int kBytes = kState + kTaWaves * kTaRows * 8;
+    static constexpr int kMerge = kTaWaves * 4 * 4096;  // 4 blocks of 4 KB per wave
     static_assert(kBytes <= 160 * 1024, "LDS of a CU");
+    static_assert(kStreams == 1 || kMerge <= kRope, "merge buffer in the ring");
+    static_assert((KVIP_DRAFT_MAX_BATCH + 1 + kTaWaves) * 8 <= kRope, "work line in the ring");
 };
 
-__host__ __device__ inline int ta_groups(int heads, int nodes) {  // R
-    const int rows = heads * nodes;
-    return rows <= kTaRows ? 1 : rows <= 2 * kTaRows ? 2 : 4;
-}
+__host__ __device__ inline int ta_groups(int heads, int nodes) { return heads * nodes <= 2 * kTaRows ? 2 : 4; }  // R
 
 __host__ __device__ inline int ta_tiles(int rows, int r) { return (rows + kTaRows * r - 1) / (kTaRows * r); }
 
-// Shares of a launch: no more than the longest contexts could fill.
+// Shares of a launch: one workgroup per CU, no more than the longest contexts could fill.
 __host__ __device__ inline int ta_shares(int batch, int heads, int nodes, int max_blocks) {
     const int r = ta_groups(heads, nodes), streams = kTaWaves / r;
     const int64_t steps = (static_cast<int64_t>(max_blocks) * kBlockTokens + kTaTile * streams - 1) / (kTaTile * streams);
@@ -125,28 +125,6 @@ KVIP_DEVICE float half_sum(float x) {
 // every bank once.
 KVIP_DEVICE constexpr int ta_swz(int t) { return ((t >> 2) & 1) | ((t & 1) << 1) | ((t & 2) << 1) | (t & 8); }
 
-// acc += a0 b0 + a1 b1 with the accumulator in accumulation registers. The compiler, left to choose, moves
-// parts of the 256 accumulators between the two halves of the register file in every tile. It does not
-// see what this block holds, so the block waits itself: two states between a vector write of an operand
-// and its reading. Nothing reads an accumulator within a tile of its last product (accumulators_done).
-KVIP_DEVICE void mma_pair(v16f& acc, bf16x8 a0, bf16x8 b0, bf16x8 a1, bf16x8 b1) {
-    asm volatile(
-        "s_nop 1\n\t"
-        "v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0\n\t"
-        "v_mfma_f32_32x32x16_bf16 %0, %3, %4, %0"
-        : "+a"(acc) : "v"(a0), "v"(b0), "v"(a1), "v"(b1));
-}
-
-// The products of mma_pair are in the accumulators (18 states after the last are enough).
-KVIP_DEVICE void accumulators_done(v16f (&o)[kBlocks]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        asm volatile("s_nop 15\n\ts_nop 7"
-                     : "+a"(o[8 * h]), "+a"(o[8 * h + 1]), "+a"(o[8 * h + 2]), "+a"(o[8 * h + 3]), "+a"(o[8 * h + 4]),
-                       "+a"(o[8 * h + 5]), "+a"(o[8 * h + 6]), "+a"(o[8 * h + 7]));
-    }
-}
-
 // Where the workspace holds what: per share two parts (its first item's, where others began it, and its
 // last one's, where others go on) of 32 R rows x 512 sums, their (maximum, sum) pairs, then per item the
 // first share and the number of shares.
@@ -162,6 +140,18 @@ struct TaWork {
         items = reinterpret_cast<int2*>(state + static_cast<size_t>(shares) * 2 * kRowsOf);
     }
 };
+
+// log sum_j exp(s_j) of a row: maximum in log2 units, sum (0 where the row sees nothing).
+KVIP_DEVICE float ta_lse(float m, float l) {
+    return l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+// Barrier for LDS data: unlike __syncthreads it leaves the direct-to-LDS loads in flight.
+KVIP_DEVICE void lds_sync() {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
 
 // A request as the kernel takes it.
 struct TaRequest {
@@ -191,31 +181,56 @@ KVIP_DEVICE int ta_steps(int length) {
 }
 
 template <int R>
+KVIP_DEVICE int64_t ta_cost(const KvipTreeAttnArgs& p, const TaRequest& q) {
+    return static_cast<int64_t>(ta_tiles(q.nodes * p.heads, R)) * ta_steps<R>(q.length);
+}
+
+// Direct-to-LDS loads from a wave-uniform address and a lane's offset below 2^32 (see lds_async.h).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+KVIP_DEVICE void dma16_at(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+KVIP_DEVICE void dma4_at(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Keeps an accumulator in accumulation registers from here to the next hold: left to itself the compiler
+// moves parts of the 256 between the two halves of the register file in every tile.
+KVIP_DEVICE void hold(v16f& acc) { asm volatile("" : "+a"(acc)); }
+
+template <int R>
 __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const KvipTreeAttnArgs p) {
     typedef TaLds<R> L;
     constexpr int kStreams = L::kStreams;
     __shared__ __align__(1024) uint8_t s_mem[L::kBytes];
-    int64_t* s_line = reinterpret_cast<int64_t*>(s_mem + L::kLine);  // steps before each request
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rg = w % R, st = w / R;
+    const int rg = w % R, st = w / R;  // row group, stream
     const int n = lane & 31, kg = lane >> 5;
+    const int shares = gridDim.x;
+    // Neighbouring shares, which read the same cache rows where an item or a request spans them, on one
+    // XCD (workgroups are dealt round the 8).
+    const int per_xcd = shares / 8;
+    const int g = static_cast<int>(blockIdx.x) < per_xcd * 8 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8
+                                                             : blockIdx.x;
 
-    // The line of work: 4 requests per thread, running sums in 64 bits.
+    // The line of work, in the ring's place: steps before each request, 4 requests per thread, running sums in
+    // 64 bits. Then this share's part of it: [pos, end), from request b, which starts at b_pos.
+    int b;
+    int64_t pos, end, b_pos, quota;
     {
         constexpr int kPer = KVIP_DRAFT_MAX_BATCH / kTaThreads;
+        int64_t* s_line = reinterpret_cast<int64_t*>(s_mem);
         int64_t* s_sum = s_line + KVIP_DRAFT_MAX_BATCH + 1;
-        int64_t steps[kPer], sum = 0;
+        int64_t cost[kPer], sum = 0;
         uint32_t err = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int b = tid * kPer + i;
-            steps[i] = 0;
-            if (b < p.batch) {
-                const TaRequest q = ta_request(p, b, &err);
-                steps[i] = static_cast<int64_t>(ta_tiles(q.nodes * p.heads, R)) * ta_steps<R>(q.length);
-            }
-            sum += steps[i];
+            const int at = tid * kPer + i;
+            cost[i] = at < p.batch ? ta_cost<R>(p, ta_request(p, at, &err)) : 0;
+            sum += cost[i];
         }
         if (blockIdx.x == 0) report(p.status, err);
         int64_t run = sum;
@@ -230,49 +245,50 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         for (int v = 0; v < w; ++v) before += s_sum[v];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int b = tid * kPer + i;
-            if (b <= p.batch) s_line[b] = before;
-            before += steps[i];
-            if (b == p.batch - 1) s_line[p.batch] = before;
+            const int at = tid * kPer + i;
+            if (at < p.batch) s_line[at] = before;
+            before += cost[i];
+            if (at == p.batch - 1) s_line[p.batch] = before;
         }
         __syncthreads();
+        const int64_t total = s_line[p.batch], even = (total + shares - 1) / shares;
+        quota = even < kMinSteps ? kMinSteps : even;
+        pos = min(g * quota, total);
+        end = min(pos + quota, total);
+        int lo = 0, hi = p.batch - 1;  // the last request that starts at or before pos
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_line[mid] <= pos) lo = mid;
+            else hi = mid - 1;
+        }
+        b = __builtin_amdgcn_readfirstlane(lo);
+        b_pos = s_line[b];
     }
-    const int64_t total = s_line[p.batch];
-    const int shares = gridDim.x;
-    const int64_t even = (total + shares - 1) / shares, quota = even < kMinSteps ? kMinSteps : even;
-    // Neighbouring shares, which read the same cache rows where an item or a request spans them, on one
-    // XCD (workgroups are dealt round the 8).
-    const int per_xcd = shares / 8;
-    const int g = static_cast<int>(blockIdx.x) < per_xcd * 8 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8
-                                                             : blockIdx.x;
-    int64_t pos = min(g * quota, total);
-    const int64_t end = min(pos + quota, total);
     const TaWork<R> work(p.workspace, shares);
-
-    uint8_t* ring = s_mem + st * 2 * kNopeSlot;
-    const uint32_t ring_lds = lds_addr(ring);
-    const uint32_t rope_lds = lds_addr(s_mem + L::kRope + st * L::kRopeSlots * kRopeSlot);
-    const uint32_t scales_lds = lds_addr(s_mem + L::kScale + st * 2 * kScaleSlot);
-    const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(p.scale * kLog2e)));
-    const int64_t row_stride = p.row_stride;
+    const uint32_t ring_lds = lds_addr(s_mem + st * kTaSlots * kNopeSlot);
+    const uint32_t rope_lds = lds_addr(s_mem + L::kRope + st * kTaSlots * kRopeSlot);
+    const uint32_t scales_lds = lds_addr(s_mem + L::kScale + st * kTaSlots * kScaleSlot);
+    // Logits are kept as they come and scaled on their way into the exponential. A negative scale turns the
+    // query's signs; one of 0 becomes 2^-100, which no logit shows.
+    const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(
+        __float_as_int(fmaxf(fabsf(p.scale * kLog2e), 0x1p-100f))));
+    const float margin = kTaMargin / scale2;
+    const int flip = p.scale < 0.f ? static_cast<int>(0x80008000u) : 0;
+    const int row_stride = p.row_stride;
 
     while (pos < end) {
         // The item at `pos`: request b, row tile rt, steps t0 .. t1 of its `steps`.
-        int b = 0;
-        {
-            int lo = 0, hi = p.batch - 1;  // the last request that starts at or before pos
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (s_line[mid] <= pos) lo = mid;
-                else hi = mid - 1;
-            }
-            b = __builtin_amdgcn_readfirstlane(lo);
-        }
         uint32_t err = 0;
-        const TaRequest req = ta_request(p, b, &err);
+        TaRequest req = ta_request(p, b, &err);
+        int64_t cost = ta_cost<R>(p, req);
+        while (pos >= b_pos + cost) {  // ends at the request that holds pos, as pos < end <= the line's length
+            b_pos += cost;
+            req = ta_request(p, ++b, &err);
+            cost = ta_cost<R>(p, req);
+        }
         err = 0;
         const int steps = ta_steps<R>(req.length);
-        const int64_t within = pos - s_line[b];
+        const int64_t within = pos - b_pos;
         const int rt = __builtin_amdgcn_readfirstlane(static_cast<int>(within / steps));
         const int t0 = __builtin_amdgcn_readfirstlane(static_cast<int>(within % steps));
         const int t1 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(steps), t0 + (end - pos))));
@@ -284,295 +300,104 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         const bool busy = rt * kTaRows * R + rg * kTaRows < rows;  // uniform: the wave's group has rows
         const int32_t* table = p.block_table + static_cast<int64_t>(b) * p.max_blocks;
 
-        // Page of the wave's tile of step k (-1: none of its tokens is there).
-        auto page_of = [&](int k) {
-            const int t = k * kStreams + st;
-            int page = -1;
-            if (k < t1 && t * kTaTile < req.length) {
-                page = table[t / (kBlockTokens / kTaTile)];
-                if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-                    err |= KVIP_STATUS_BAD_BLOCK;
-                    page = -1;
-                }
+        // Page of the wave's tile of step t (-1: none of its tokens is there), from the table entries of 64 pages
+        // that the lanes hold.
+        int held = 0, held_first = -64;
+        auto page_of = [&](int t) {
+            const int tile = t * kStreams + st, at = tile / (kBlockTokens / kTaTile);
+            if (t >= t1 || tile * kTaTile >= req.length) return -1;
+            if (at >= held_first + 64) {
+                held_first = at;
+                held = table[min(at + lane, p.max_blocks - 1)];
             }
-            return page;
+            const int page = __builtin_amdgcn_readlane(held, at - held_first);
+            if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks)) return page;
+            err |= KVIP_STATUS_BAD_BLOCK;
+            return -1;
         };
-        // First byte of the tile's first row.
-        auto tile_base = [&](int k, int page) {
-            const int t = k * kStreams + st;
-            return p.kv_cache + page * p.kv_block_stride + (t % (kBlockTokens / kTaTile)) * kTaTile * row_stride;
-        };
-        // This wave's share (1 / R) of the loads of a tile's nope bytes and scales into slot `slot`. LDS row t
-        // holds piece s ^ swz(t) at place s. Tokens past the length get zeros: their probabilities are
-        // zero, and zero times a stray NaN would not be.
-        auto load_nope = [&](int k, int page, int slot) {
-            const int ln = fresh(lane), up = ln >> 5;
-            const int live = min(req.length - (k * kStreams + st) * kTaTile, kTaTile);
-            constexpr int kLoads = 16 / R;  // of tokens 2 v and 2 v + 1 each
-            const uint8_t* base = tile_base(k, page) + up * row_stride;
-            const int from = ((ln & 31) ^ ta_swz(up)) * 16;
-            const uint32_t dst = ring_lds + slot * kNopeSlot;
+        // This wave's share (1 / R) of the loads of step t's tile into slot `slot`. LDS row i of the nope bytes holds
+        // piece s ^ ta_swz(i) at place s, of the rope features (128 bytes) piece s ^ (i / 2 % 8); scales stand as
+        // [group][token]. Tokens that are not there get zeros: their probabilities are zero, and zero times a
+        // stray NaN would not be (their rope keeps stale bytes: their logits are replaced).
+        auto load = [&](int t, int page, int slot) {
+            const int ln = fresh(lane), up = ln >> 5, tile = t * kStreams + st;
+            const int live = page < 0 ? 0 : min(req.length - tile * kTaTile, kTaTile);
+            const uint8_t* base = p.kv_cache + page * p.kv_block_stride +
+                                  static_cast<int64_t>(tile % (kBlockTokens / kTaTile)) * kTaTile * row_stride;
+            constexpr int kNopeLoads = 16 / R, kRopeLoads = 4 / R;
+            const uint32_t dst = ring_lds + slot * kNopeSlot, rope_dst = rope_lds + slot * kRopeSlot;
+            const uint32_t scale_dst = scales_lds + slot * kScaleSlot;
+            // Lane offsets: tokens 2 v and 2 v + 1 of nope bytes per load, 8 v .. 8 v + 7 of rope features, and scale
+            // groups 2 v and 2 v + 1.
+            auto nope_from = [&](int v) { return static_cast<uint32_t>(up * row_stride + ((ln & 31) ^ ta_swz(up) ^ ta_swz(2 * v)) * 16); };
+            auto rope_from = [&](int v) {
+                return static_cast<uint32_t>((ln >> 3) * row_stride + kValueDim + ((ln & 7) ^ (ln >> 4) ^ ((v & 1) * 4)) * 16);
+            };
+            const uint32_t scale_from = (ln & 31) * row_stride + 640 + 4 * up;
+            if (live == kTaTile) {
 #pragma unroll
-            for (int x = 0; x < kLoads; ++x) {
-                const int v = rg * kLoads + x;
-                const uint8_t* src = base + 2 * v * row_stride + (from ^ (ta_swz(2 * v) * 16));
-                if (live == kTaTile || 2 * v + up < live) {
-                    dma16(src, dst + v * 1024);
+                for (int x = 0; x < kNopeLoads; ++x) {
+                    const int v = rg * kNopeLoads + x;
+                    dma16_at(base + 2 * v * row_stride, nope_from(v), dst + v * 1024);
+                }
+#pragma unroll
+                for (int x = 0; x < kRopeLoads; ++x) {
+                    const int v = rg * kRopeLoads + x;
+                    dma16_at(base + 8 * v * row_stride, rope_from(v), rope_dst + v * 1024);
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    if (v == rg) dma4_at(base + 8 * v, scale_from, scale_dst + v * 256);
+                }
+                return;
+            }
+#pragma unroll 1
+            for (int x = 0; x < kNopeLoads; ++x) {
+                const int v = rg * kNopeLoads + x;
+                if (2 * v + up < live) {
+                    dma16_at(base + 2 * v * row_stride, nope_from(v), dst + v * 1024);
                 } else {
                     *(__attribute__((address_space(3))) v4i*)(dst + v * 1024 + ln * 16) = v4i{0, 0, 0, 0};
                 }
             }
-            // Scales, as [group][token]: groups 2 v and 2 v + 1 per load, v = 0 and 1.
-            const uint8_t* src = tile_base(k, page) + (ln & 31) * row_stride + 640 + 4 * up;
-            const uint32_t sc = scales_lds + slot * kScaleSlot;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                if (R > 1 && v != rg) continue;
-                if (live == kTaTile || (ln & 31) < live) dma4(src + 8 * v, sc + v * 256);
-                else *(__attribute__((address_space(3))) float*)(sc + v * 256 + ln * 4) = 0.f;
+#pragma unroll 1
+            for (int x = 0; x < kRopeLoads; ++x) {
+                const int v = rg * kRopeLoads + x;
+                if (8 * v + (ln >> 3) < live) dma16_at(base + 8 * v * row_stride, rope_from(v), rope_dst + v * 1024);
+            }
+            if (rg < 2) {
+                if ((ln & 31) < live) dma4_at(base + 8 * rg, scale_from, scale_dst + rg * 256);
+                else *(__attribute__((address_space(3))) float*)(scale_dst + rg * 256 + ln * 4) = 0.f;
             }
         };
-        // And of its rope features: LDS row t (128 bytes) holds piece s ^ (t / 2 % 8) at place s. Tokens past the
-        // length keep stale bytes: their logits are replaced.
-        auto load_rope = [&](int k, int page, int slot) {
-            const int ln = fresh(lane);
-            const int live = min(req.length - (k * kStreams + st) * kTaTile, kTaTile);
-            constexpr int kLoads = 4 / R;  // of tokens 8 v .. 8 v + 7 each
-#pragma unroll
-            for (int x = 0; x < kLoads; ++x) {
-                const int v = rg * kLoads + x, token = 8 * v + (ln >> 3);
-                const int piece = (ln & 7) ^ ((token >> 1) & 7);
-                if (token < live) {
-                    dma16(tile_base(k, page) + token * row_stride + kValueDim + piece * 16,
-                          rope_lds + (L::kRopeSlots == 1 ? 0 : slot * kRopeSlot) + v * 1024);
-                }
-            }
-        };
-        // Every load and LDS access of this wave is done, and (waves sharing a stream) of all waves.
+        // Every load and LDS access of this wave is done, and of all waves.
         auto settle = [&] {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-            if constexpr (R > 1) __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_s_barrier();
             asm volatile("" : : : "memory");
         };
 
-        __syncthreads();  // the LDS of the item before is free
+        __syncthreads();  // the LDS of the item before (at first: the line of work) is free
         int page = page_of(t0);
-        if (page >= 0) {
-            load_nope(t0, page, 0);
-            load_rope(t0, page, 0);
-        }
+        load(t0, page, 0);
         int page_next = page_of(t0 + 1);
-
-        // Queries of the wave's rows (rows past the last read it again; their outputs are not written). Fragment
-        // (group g, j, x): features 16 (8 g + 2 j + kg) + 8 x .. + 7, the half x of the key piece that the lane
-        // reads; the last four: rope features 16 i + 8 kg .. + 7.
-        bf16x8 qf[36];
-        uint64_t seen;
-        {
-            const int at = min(row, rows - 1), node = at / p.heads;
-            const uint16_t* q = p.query + (static_cast<int64_t>(req.begin) * p.heads + at) * kKeyDim;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                qf[i] = *reinterpret_cast<const bf16x8*>(q + (i >> 1) * 32 + kg * 16 + (i & 1) * 8);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qf[32 + i] = *reinterpret_cast<const bf16x8*>(q + kValueDim + i * 16 + kg * 8);
-            seen = p.visible != nullptr ? static_cast<uint64_t>(p.visible[req.begin + node]) : ~0ull >> (63 - node);
-        }
-        v16f o[kBlocks];
-#pragma unroll
-        for (int f = 0; f < kBlocks; ++f) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
-        }
-        float m_run = -INFINITY;  // reference maximum of the row, log2 units
-        float l_sum = 0.f;        // this lane's share of its probability sum
-        // Waited for here: the tile loop would wait for them each time round, and so for its own loads.
-#pragma unroll
-        for (int i = 0; i < 36; ++i) asm volatile("" : "+v"(qf[i]));
-
-        int slot = 0;
-#pragma unroll 1
-        for (int k = t0; k < t1; ++k, slot ^= 1) {
-            settle();  // the tile has landed; the other slot is free
-            const int ahead = page_next;
-            page_next = page_of(k + 2);
-            if (ahead >= 0) {
-                load_nope(k + 1, ahead, slot ^ 1);
-                if (L::kRopeSlots == 2) load_rope(k + 1, ahead, slot ^ 1);
-            }
-            const int ln = fresh(lane), tn = ln & 31, tk = ln >> 5;
-            const uint32_t ro = rope_lds + (L::kRopeSlots == 1 ? 0 : slot * kRopeSlot) + tn * 128;
-            const uint32_t ko = ring_lds + slot * kNopeSlot + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
-            const uint32_t sl = scales_lds + slot * kScaleSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
-            const int y = (ln & 15) >> 1, vt = 8 * (y >> 2) + 4 * tk + (y & 3);
-            const uint32_t vo = ring_lds + slot * kNopeSlot + vt * kValueDim + ((((ln >> 4) & 1) ^ ta_swz(vt)) << 4) + 8 * (ln & 1);
-
-            v16f s;
-            if (busy && page >= 0) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const v4i x = *(LdsV4i)(ro + (((2 * i + tk) ^ ((tn >> 1) & 7)) << 4));
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[32 + i], s, 0, 0, 0);
-                }
-            }
-            if (L::kRopeSlots == 1 && ahead >= 0) {  // the single rope slot has been read
-                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-                load_rope(k + 1, ahead, 0);
-            }
-            const int first = (k * kStreams + st) * kTaTile;  // position of the tile's first token
-            // A step with step tokens or the end of the context in it (the same for the workgroup's waves). What
-            // a row does not see must not reach it, and zero times a NaN would: tokens with a NaN feature or a
-            // scale that is not finite are found and zeroed in LDS, and rows that do see one become NaN as a whole
-            // (their logit is none).
-            uint32_t sees = 0xFFFFu;  // bit i: the row sees the token of register i
-            if ((k + 1) * kStreams * kTaTile > req.past) {
-                uint32_t nan = 0;
-                const uint32_t at = ring_lds + slot * kNopeSlot + tn * kValueDim;
-                const uint32_t sc = scales_lds + slot * kScaleSlot + tk * 2 * kTaTile * 4 + tn * 4;
-                if (page >= 0) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const v4i x = *(LdsV4i)(at + (((16 * tk + i) ^ ta_swz(tn)) << 4));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) nan |= (x[e] & 0x7F7F7F7Fu) + 0x01010101u;
-                    }
-                    nan &= 0x80808080u;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t x = __float_as_uint(*(LdsF32)(sc + i * kTaTile * 4));
-                        nan |= (x & 0x7F800000u) == 0x7F800000u ? 1u : 0u;
-                    }
-                }
-                const uint64_t found = __ballot(nan != 0);
-                const uint32_t bad = static_cast<uint32_t>(found | found >> 32);
-                if constexpr (R > 1) {  // the waves of the stream have all looked
-                    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-                    __builtin_amdgcn_s_barrier();
-                    asm volatile("" : : : "memory");
-                }
-                if (bad >> tn & 1) {
-#pragma unroll 1
-                    for (int i = 0; i < 16; ++i) {
-                        *(__attribute__((address_space(3))) v4i*)(at + (16 * tk + i) * 16) = v4i{0, 0, 0, 0};
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) *(__attribute__((address_space(3))) float*)(sc + i * kTaTile * 4) = 0.f;
-                }
-                sees = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int token = 8 * (i >> 2) + 4 * tk + (i & 3), rel = first + token - req.past;
-                    const bool in = rel < 0 || (rel < KVIP_DRAFT_MAX_NODES && rel < req.length - req.past &&
-                                                (seen >> (rel & 63) & 1) != 0);
-                    sees |= in ? 1u << i : 0u;
-                    if (in && (bad >> token & 1)) l_sum = NAN;
-                }
-            }
-            if (busy && page >= 0) {
-#pragma unroll
-                for (int gr = 0; gr < kScaleGroups; ++gr) {
-                    v16f dot;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) dot[i] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const v4i x = *(LdsV4i)(ko ^ ((8 * gr + 2 * j) * 16));
-                        dot = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(x[0], x[1]), qf[8 * gr + 2 * j], dot, 0, 0, 0);
-                        dot = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(x[2], x[3]), qf[8 * gr + 2 * j + 1], dot, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const f32x4 s4 = *(LdsF32x4)(sl + (gr * kTaTile + 8 * a) * 4);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) s[4 * a + c] = fmaf(dot[4 * a + c], s4[c], s[4 * a + c]);
-                    }
-                }
-                // Softmax: pr = 2^(logit - m), the logits of tokens that the row does not see at -inf.
-                float pr[16], mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) pr[i] = s[i] * scale2;
-                if (first + kTaTile > req.past) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (!(sees >> i & 1)) pr[i] = -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, pr[i]);
-                mx = half_max(mx);
-                const bool raise = mx > m_run + kTaMargin;  // also the first finite maximum
-                if (__ballot(raise) != 0ull) {
-                    const float m_new = raise ? mx : m_run;
-                    const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
-                    const float a = raise ? alpha : 1.f;
-                    l_sum *= a;
-#pragma unroll
-                    for (int f = 0; f < kBlocks; ++f) {
-                        asm volatile("" : "+a"(o[f]));  // read here, not in every tile
-                        o[f] *= a;
-                        asm volatile("" : "+a"(o[f]));
-                    }
-                    m_run = m_new;
-                }
-                const float bias = m_run == -INFINITY ? 0.f : -m_run;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    pr[i] = __builtin_amdgcn_exp2f(pr[i] + bias);
-                    l_sum += pr[i];
-                }
-                // Value product [features, rows].
-#pragma unroll
-                for (int gr = 0; gr < kScaleGroups; ++gr) {
-                    v4i packed[2];
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const f32x4 s4 = *(LdsF32x4)(sl + (gr * kTaTile + 8 * a) * 4);
-                        packed[a >> 1][2 * (a & 1)] = static_cast<int>(pack_bf16(pr[4 * a] * s4[0], pr[4 * a + 1] * s4[1]));
-                        packed[a >> 1][2 * (a & 1) + 1] = static_cast<int>(pack_bf16(pr[4 * a + 2] * s4[2], pr[4 * a + 3] * s4[3]));
-                    }
-                    const bf16x8 p0 = __builtin_bit_cast(bf16x8, packed[0]), p1 = __builtin_bit_cast(bf16x8, packed[1]);
-#pragma unroll
-                    for (int f = 4 * gr; f < 4 * gr + 4; ++f) {
-                        const i32x2 v0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsI32x2)(vo ^ (f * 32)));
-                        const i32x2 v1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsI32x2)((vo ^ (f * 32)) + 16 * kValueDim));
-                        mma_pair(o[f], fp8x8_to_bf16(v0[0], v0[1]), p0, fp8x8_to_bf16(v1[0], v1[1]), p1);
-                    }
-                }
-            }
-            page = ahead;
-        }
-        accumulators_done(o);
-        if (lane == 0) report(p.status, err);
-
-        // Merge of the streams: with the maximum M over them, sums = sum_w 2^(m_w - M) o_w and l likewise. A wave
-        // sums 16 / streams of the blocks, from halves of 8 blocks that the others put into LDS.
-        const float l_all = half_sum(l_sum);
-        float m = m_run, l = l_all, mine = 1.f;
-        float2* s_state = reinterpret_cast<float2*>(s_mem + L::kState);
-        if constexpr (kStreams > 1) {
-            if (kg == 0) s_state[w * kTaRows + n] = make_float2(m_run, l_all);
-            __syncthreads();  // and every wave is done with its ring
-            m = -INFINITY;
-#pragma unroll
-            for (int v = 0; v < kStreams; ++v) m = fmaxf(m, s_state[(v * R + rg) * kTaRows + n].x);
-            l = 0.f;
-#pragma unroll
-            for (int v = 0; v < kStreams; ++v) {
-                const float2 sv = s_state[(v * R + rg) * kTaRows + n];
-                const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sv.x - m);
-                l += f * sv.y;
-                if (v == st) mine = f;
-            }
-        }
+        if (t0 + 1 < t1) load(t0 + 1, page_next, 1);
+        // Step t: its tile has landed, the slot of step t - 1's is free and takes that of step t + 1 (but for the
+        // first two, which are under way).
+        auto arrive = [&](int t, int slot_free) {
+            settle();
+            if (t == t0) return;
+            const int ahead = page_of(t + 1);
+            if (t + 1 < t1) load(t + 1, ahead, slot_free);
+            page = page_next;
+            page_next = ahead;
+        };
+        auto last_tokens = [&](int t) { return (t + 1) * kStreams * kTaTile > req.past; };  // of the context, or step tokens
         const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
+        const size_t slot_row = (static_cast<size_t>(g) * 2 + (t0 == 0 ? 1 : 0)) * kTaRows * R + rg * kTaRows + n;
         // A whole item's rows are final; else the sums and their state go to the share's part 0 (others began
         // the item) or 1.
-        const float factor = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
-        const size_t slot_row = (static_cast<size_t>(g) * 2 + (t0 == 0 ? 1 : 0)) * kTaRows * R + rg * kTaRows + n;
-        auto put = [&](int f, const v16f& x) {
+        auto put = [&](int f, const v16f& x, float factor) {
             if (row >= rows) return;
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
@@ -588,53 +413,337 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 }
             }
         };
-        if constexpr (kStreams == 1) {
-            if (busy) {
-#pragma unroll
-                for (int f = 0; f < kBlocks; ++f) put(f, o[f]);
+        auto put_state = [&](float m, float l) {
+            if (st != 0 || kg != 0 || row >= rows) return;
+            if (!whole) work.state[slot_row] = make_float2(m, l);
+            else if (p.lse != nullptr) p.lse[out_row] = ta_lse(m, l);
+        };
+        if (!busy) {  // a row group without rows loads its share of the tiles
+            for (int t = t0; t < t1; ++t) {
+                arrive(t, (t + 1 - t0) % kTaSlots);
+                if (last_tokens(t)) lds_sync();
+            }
+            if constexpr (kStreams > 1) {  // the barriers of the merge
+                for (int i = 0; i < 5; ++i) __syncthreads();
             }
         } else {
-            constexpr int kOwn = 8 / kStreams;  // blocks of a half that a wave sums
-            const uint32_t buffer = lds_addr(s_mem);
+            // Queries of the wave's rows (rows past the last read it again; their outputs are not written). Fragment
+            // 2 i + x: features 16 (2 i + kg) + 8 x .. + 7, the half x of the key piece that the lane reads; rope
+            // fragment i: features 16 i + 8 kg .. + 7.
+            v4i qf[32];
+            uint64_t* s_seen = reinterpret_cast<uint64_t*>(s_mem + L::kState) + w * kTaRows + n;
+            const uint32_t q_rope = lds_addr(s_mem + L::kQuery) + rg * 4096 + lane * 16;
+            {
+                const int at = min(row, rows - 1), node = at / p.heads;
+                const uint16_t* q = p.query + (static_cast<int64_t>(req.begin) * p.heads + at) * kKeyDim;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                if (half > 0) __syncthreads();
+                for (int i = 0; i < 32; ++i) {
+                    qf[i] = *reinterpret_cast<const v4i*>(q + (i >> 1) * 32 + kg * 16 + (i & 1) * 8) ^ flip;
+                }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (j / kOwn == st || !busy) continue;
+                for (int i = 0; i < 4; ++i) {  // the streams of a row group write the same
+                    *(__attribute__((address_space(3))) v4i*)(q_rope + i * 1024) =
+                        *reinterpret_cast<const v4i*>(q + kValueDim + i * 16 + kg * 8) ^ flip;
+                }
+                *s_seen = p.visible != nullptr ? static_cast<uint64_t>(p.visible[req.begin + node]) : ~0ull >> (63 - node);
+            }
+            // Waited for here: the tile loop would wait for them each time round, and so for its own loads.
 #pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const v16f& x = o[8 * half + j];
-                        *(LdsF32x4Out)(buffer + ((w * 8 + j) * 4 + a) * 1024 + lane * 16) =
-                            f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * mine;
+            for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(qf[i]));
+            v16f o[kBlocks];
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
+                hold(o[f]);
+            }
+            float m_run = -INFINITY;  // reference maximum of the row
+            float l_sum = 0.f;        // this lane's share of its probability sum
+            float pr[16];             // probabilities of the tile whose values come next, relative to m_run
+            v16f s;                   // logits
+
+            constexpr int kAhead = 3;  // LDS reads stand so many products before their use, conversions one
+            // Logits of step t's tile, in slot `slot`.
+            auto logits = [&](int t, int slot) {
+                const int ln = fresh(lane), tn = ln & 31, tk = ln >> 5;
+                const int first = (t * kStreams + st) * kTaTile;  // position of the tile's first token
+                uint32_t sees = page < 0 ? 0u : 0xFFFFu;          // bit i: the row sees the token of register i
+                bool masked = page < 0;
+                // A step with step tokens or the end of the context in it (the same for the workgroup's waves). What
+                // a row does not see must not reach it, and zero times a NaN would: tokens with a NaN feature or a
+                // scale that is not finite are found and zeroed in LDS, and rows that do see one become NaN as a
+                // whole (their logit is none).
+                if (last_tokens(t)) {
+                    masked = true;
+                    uint32_t nan = 0;
+                    const uint32_t at = ring_lds + slot * kNopeSlot + tn * kValueDim;
+                    const uint32_t sc = scales_lds + slot * kScaleSlot + tk * 2 * kTaTile * 4 + tn * 4;
+#pragma unroll 4
+                    for (int i = 0; i < 16; ++i) {
+                        const v4i x = *(LdsV4i)(at + (((16 * tk + i) ^ ta_swz(tn)) << 4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) nan |= (x[e] & 0x7F7F7F7Fu) + 0x01010101u;
+                    }
+                    nan &= 0x80808080u;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t x = __float_as_uint(*(LdsF32)(sc + i * kTaTile * 4));
+                        nan |= (x & 0x7F800000u) == 0x7F800000u ? 1u : 0u;
+                    }
+                    const uint64_t found = __ballot(nan != 0);
+                    const uint32_t bad = static_cast<uint32_t>(found | found >> 32);
+                    lds_sync();  // the waves of the stream have all looked
+                    if (bad >> tn & 1) {
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i) {
+                            *(__attribute__((address_space(3))) v4i*)(at + (16 * tk + i) * 16) = v4i{0, 0, 0, 0};
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) *(__attribute__((address_space(3))) float*)(sc + i * kTaTile * 4) = 0.f;
+                    }
+                    sees = 0;
+                    const uint64_t seen = *s_seen;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int token = 8 * (i >> 2) + 4 * tk + (i & 3), rel = first + token - req.past;
+                        const bool in = page >= 0 && (rel < 0 || (rel < KVIP_DRAFT_MAX_NODES && rel < req.length - req.past &&
+                                                                  (seen >> (rel & 63) & 1) != 0));
+                        sees |= in ? 1u << i : 0u;
+                        if (in && (bad >> token & 1)) l_sum = NAN;
                     }
                 }
+                const uint32_t ro = rope_lds + slot * kRopeSlot + tn * 128;
+                const uint32_t ko = ring_lds + slot * kNopeSlot + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
+                const uint32_t sl = scales_lds + slot * kScaleSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
+                // Bit 8 of a key's address is its own: pieces 16 and up by an offset.
+                auto key = [&](int i) { return *(LdsV4i)((ko ^ ((i & 7) * 32)) + (i >> 3) * 256); };
+                v4i kr[4], kb[kAhead + 1];
+                v16f dot[2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kr[i] = *(LdsV4i)(ro + (((2 * i + tk) ^ ((tn >> 1) & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) kb[i] = key(i);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v4i y = *(LdsV4i)(q_rope + i * 1024);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), __builtin_bit_cast(bf16x8, y), s, 0, 0, 0);
+                }
+                bf16x8 ka[2] = {fp8x8_to_bf16(kb[0][0], kb[0][1]), fp8x8_to_bf16(kb[0][2], kb[0][3])};
+                // A quarter of a group's dot products (tokens 8 a + 4 kg .. + 3) joins the logits four products later, its
+                // scales two before that.
+                f32x4 s4[3];
+                auto scales = [&](int q) { s4[q % 3] = *(LdsF32x4)(sl + ((q >> 2) * kTaTile + 8 * (q & 3)) * 4); };
+                auto join = [&](int q) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int e = 4 * (q & 3) + c;
+                        s[e] = fmaf(dot[q >> 2 & 1][e], s4[q % 3][c], s[e]);
+                    }
+                };
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int gr = i >> 2;
+                    v16f& d = dot[gr & 1];
+                    if ((i & 3) == 0) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) d[e] = 0.f;
+                    }
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], __builtin_bit_cast(bf16x8, qf[2 * i]), d, 0, 0, 0);
+                    if (i + kAhead < 16) kb[(i + kAhead) % (kAhead + 1)] = key(i + kAhead);
+                    const v4i x = kb[(i + 1) % (kAhead + 1)];
+                    if (i < 15) ka[0] = fp8x8_to_bf16(x[0], x[1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[1], __builtin_bit_cast(bf16x8, qf[2 * i + 1]), d, 0, 0, 0);
+                    if (i < 15) ka[1] = fp8x8_to_bf16(x[2], x[3]);
+                    if (i >= 4) join(i - 4);
+                    if (i >= 2) scales(i - 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                join(12);
+                scales(14);
+                join(13);
+                scales(15);
+                join(14);
+                join(15);
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (!(sees >> i & 1)) s[i] = -INFINITY;
+                    }
+                }
+            };
+            // Softmax of the logits, p = 2^(scale2 (logit - m)), in 18 pieces. Its factor for what came before (alpha)
+            // counts once the values of the tile before are in.
+            float mx, bias, alpha, fresh_sum;
+            bool raise;
+            auto softmax = [&](int piece) {
+                if (piece == 0) {
+                    mx = s[0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+                    mx = half_max(mx);
+                    fresh_sum = 0.f;
+                } else if (piece == 1) {
+                    raise = mx > m_run + margin;  // also the first finite maximum
+                    const float m_new = raise ? mx : m_run;
+                    alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * scale2) : raise ? 0.f : 1.f;
+                    m_run = m_new;
+                    bias = m_new == -INFINITY ? 0.f : -m_new * scale2;
+                } else {
+                    s[piece - 2] = __builtin_amdgcn_exp2f(fmaf(s[piece - 2], scale2, bias));
+                    fresh_sum += s[piece - 2];
+                }
+            };
+            auto take = [&] {  // the softmax's results become those of the tile whose values come next
+                l_sum = l_sum * alpha + fresh_sum;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pr[i] = s[i];
+            };
+            // Values of the tile in slot `slot` [features, rows], the softmax of the next one beside them.
+            auto values = [&](int slot, auto with_softmax) {
+                constexpr bool kSoftmax = decltype(with_softmax)::value;
+                const int ln = fresh(lane), tk = ln >> 5;
+                const int y = (ln & 15) >> 1, vt = 8 * (y >> 2) + 4 * tk + (y & 3);
+                const uint32_t vo = ring_lds + slot * kNopeSlot + vt * kValueDim + ((((ln >> 4) & 1) ^ ta_swz(vt)) << 4) + 8 * (ln & 1);
+                const uint32_t sl = scales_lds + slot * kScaleSlot + 16 * tk;
+                auto value = [&](int f, int h) {
+                    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsI32x2)((vo ^ ((f & 7) * 32)) + (f >> 3) * 256 + h * 16 * kValueDim));
+                };
+                // A quarter of a group's operand: the probabilities of tokens 8 a + 4 kg .. + 3 times their scales, which
+                // are read two products earlier.
+                v4i pb[2][2];
+                f32x4 s4[4];
+                auto scales = [&](int q) { s4[q & 3] = *(LdsF32x4)(sl + ((q >> 2) * kTaTile + 8 * (q & 3)) * 4); };
+                auto weigh = [&](int q) {
+                    const int a = q & 3;
+                    v4i& d = pb[q >> 2 & 1][a >> 1];
+                    d[2 * (a & 1)] = static_cast<int>(pack_bf16(pr[4 * a] * s4[a][0], pr[4 * a + 1] * s4[a][1]));
+                    d[2 * (a & 1) + 1] = static_cast<int>(pack_bf16(pr[4 * a + 2] * s4[a][2], pr[4 * a + 3] * s4[a][3]));
+                };
+                i32x2 vb[kAhead + 1][2];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) scales(q);
+#pragma unroll
+                for (int f = 0; f < kAhead; ++f) {
+                    vb[f][0] = value(f, 0);
+                    vb[f][1] = value(f, 1);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) weigh(q);
+                scales(4);
+                scales(5);
+                bf16x8 va[2] = {fp8x8_to_bf16(vb[0][0][0], vb[0][0][1]), fp8x8_to_bf16(vb[0][1][0], vb[0][1][1])};
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int f = 0; f < kBlocks; ++f) {
+                    const int gr = f >> 2, next = (f + 1) % (kAhead + 1), far = (f + kAhead) % (kAhead + 1);
+                    hold(o[f]);
+                    o[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[0], __builtin_bit_cast(bf16x8, pb[gr & 1][0]), o[f], 0, 0, 0);
+                    if (f + kAhead < kBlocks) {
+                        vb[far][0] = value(f + kAhead, 0);
+                        vb[far][1] = value(f + kAhead, 1);
+                    }
+                    if (f + 1 < kBlocks) va[0] = fp8x8_to_bf16(vb[next][0][0], vb[next][0][1]);
+                    if (kSoftmax) softmax(f);
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[1], __builtin_bit_cast(bf16x8, pb[gr & 1][1]), o[f], 0, 0, 0);
+                    hold(o[f]);
+                    if (f + 1 < kBlocks) va[1] = fp8x8_to_bf16(vb[next][1][0], vb[next][1][1]);
+                    if (f + 4 < 16) weigh(f + 4);
+                    if (f + 6 < 16) scales(f + 6);
+                    if (kSoftmax && f == kBlocks - 1) {
+                        softmax(16);
+                        softmax(17);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+
+            arrive(t0, 0);
+            logits(t0, 0);
+#pragma unroll
+            for (int i = 0; i < 18; ++i) softmax(i);
+            take();
+            int slot = 0;
+#pragma unroll 1
+            for (int t = t0; t + 1 < t1; ++t) {
+                const int slot_next = slot == kTaSlots - 1 ? 0 : slot + 1;
+                arrive(t + 1, slot_next == kTaSlots - 1 ? 0 : slot_next + 1);
+                logits(t + 1, slot_next);
+                values(slot, std::true_type{});
+                if (__ballot(raise) != 0ull) {
+#pragma unroll
+                    for (int f = 0; f < kBlocks; ++f) {
+                        hold(o[f]);  // read here, not in every tile
+                        o[f] *= alpha;
+                        hold(o[f]);
+                    }
+                }
+                take();
+                slot = slot_next;
+            }
+            values(slot, std::false_type{});
+
+            const float l_all = half_sum(l_sum);
+            const float m_all = m_run * scale2;  // log2 units from here on
+            if constexpr (kStreams == 1) {
+                const float factor = whole ? (l_all > 0.f || l_all != l_all ? 1.f / l_all : 0.f) : 1.f;
+#pragma unroll
+                for (int f = 0; f < kBlocks; ++f) {
+                    hold(o[f]);
+                    put(f, o[f], factor);
+                }
+                put_state(m_all, l_all);
+            } else {
+                // Merge of the two streams: with the maximum M over them, sums = sum_w 2^(m_w - M) o_w and l likewise. A
+                // wave sums half of the blocks, whose other half it puts into LDS, 8 blocks at a time.
+                float2* s_state = reinterpret_cast<float2*>(s_mem + L::kState);
+                __syncthreads();  // every wave is done with its ring and its rows' bits
+                if (kg == 0) s_state[w * kTaRows + n] = make_float2(m_all, l_all);
                 __syncthreads();
+                const float2 other = s_state[(w ^ R) * kTaRows + n];
+                const float top = fmaxf(m_all, other.x);
+                const float mine = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_all - top);
+                const float theirs = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other.x - top);
+                const float l = mine * l_all + theirs * other.y;
+                const float factor = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
+                const uint32_t out_lds = lds_addr(s_mem) + w * 4 * 4096 + lane * 16;
+                const uint32_t in_lds = lds_addr(s_mem) + (w ^ R) * 4 * 4096 + lane * 16;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (j / kOwn != st || !busy) continue;
-                    v16f x = o[8 * half + j] * mine;
+                for (int half = 0; half < 2; ++half) {
+                    if (half > 0) __syncthreads();
 #pragma unroll
-                    for (int d = 1; d < kStreams; ++d) {
-                        const int v = (st + d) % kStreams * R + rg;
+                    for (int j = 0; j < 8; ++j) {
+                        if (j / 4 == st) continue;
+                        hold(o[8 * half + j]);
 #pragma unroll
                         for (int a = 0; a < 4; ++a) {
-                            const f32x4 add = *(LdsF32x4)(buffer + ((v * 8 + j) * 4 + a) * 1024 + lane * 16);
+                            const v16f& x = o[8 * half + j];
+                            *(LdsF32x4Out)(out_lds + ((j & 3) * 4 + a) * 1024) = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * mine;
+                        }
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (j / 4 != st) continue;
+                        hold(o[8 * half + j]);
+                        v16f x = o[8 * half + j] * mine;
+#pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            const f32x4 add = *(LdsF32x4)(in_lds + ((j & 3) * 4 + a) * 1024);
 #pragma unroll
                             for (int c = 0; c < 4; ++c) x[4 * a + c] += add[c];
                         }
+                        put(8 * half + j, x, factor);
                     }
-                    put(8 * half + j, x);
                 }
+                put_state(top, l);
             }
         }
-        if (st == 0 && kg == 0 && row < rows) {
-            if (!whole) {
-                work.state[slot_row] = make_float2(m, l);
-            } else if (p.lse != nullptr) {
-                p.lse[out_row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-            }
-        }
+        if (lane == 0) report(p.status, err);
         if (t0 == 0 && tid == 0) {  // which shares hold the item
             const int last = static_cast<int>((item_pos + steps - 1) / quota);
             work.items[static_cast<int64_t>(b) * ta_tiles(p.max_nodes * p.heads, R) + rt] = make_int2(g, last - g + 1);
@@ -686,7 +795,7 @@ __global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAtt
                 __builtin_convertvector(v, bf16x4);
         }
         if (f == 0 && p.lse != nullptr) {
-            p.lse[out_row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+            p.lse[out_row] = ta_lse(m, l);
         }
     }
 }
@@ -722,13 +831,12 @@ extern "C" uint32_t kvip_hip_tree_attention(const KvipTreeAttnArgs* a, void* str
                     a->max_nodes >= 1 && a->max_nodes <= KVIP_DRAFT_MAX_NODES && a->max_tokens >= 1 &&
                     a->max_tokens <= KVIP_DRAFT_MAX_TOKENS && a->max_blocks >= 1 && a->max_blocks <= (1 << 17) &&
                     a->num_blocks >= 1 && a->num_blocks < (1 << 24) && a->row_stride >= KVIP_KV_ROW_BYTES &&
-                    a->row_stride % 16 == 0 && a->kv_block_stride % 16 == 0 &&
+                    a->row_stride <= (1 << 24) && a->row_stride % 16 == 0 && a->kv_block_stride % 16 == 0 &&
                     a->kv_block_stride >= static_cast<int64_t>(kvip::kBlockTokens) * a->row_stride &&
                     (a->output_dtype == KVIP_DTYPE_BF16 || a->output_dtype == KVIP_DTYPE_FP32);
     if (!ok) return KVIP_ERR_INVALID;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     switch (kvip::ta_groups(a->heads, a->max_nodes)) {
-        case 1: kvip::launch_tree<1>(*a, s); break;
         case 2: kvip::launch_tree<2>(*a, s); break;
         default: kvip::launch_tree<4>(*a, s); break;
     }
