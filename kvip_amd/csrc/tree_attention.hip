@@ -51,7 +51,7 @@ constexpr int kScaleGroups = 4;
 constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
 constexpr int kMinSteps = 4;                // steps of a share, at least
-constexpr int kJoinRows = 8;                // rows per workgroup of the joining launch
+constexpr int kJoinRows = 2;                // rows per workgroup of the joining launch
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kTaMargin = 8.0f * kLog2e;
@@ -61,8 +61,9 @@ constexpr int kRopeSlot = kTaTile * 128;
 constexpr int kScaleSlot = kScaleGroups * kTaTile * 4;
 
 // LDS of a workgroup with R row groups: per stream the ring's nope bytes, rope and scales [group][token]; the
-// query's rope fragments; per wave and row visibility bits, later the softmax's state. The work line stands
-// in the ring's place at first, the merge of two streams at the end.
+// query's rope fragments; per wave and row visibility bits, later the softmax's state; per wave what its
+// registers have no room for while it works on the next tile's logits. The merge of two
+// streams takes the ring's place at the end.
 template <int R>
 struct TaLds {
     static constexpr int kStreams = kTaWaves / R;
@@ -70,22 +71,26 @@ struct TaLds {
     static constexpr int kScale = kRope + kStreams * kTaSlots * kRopeSlot;
     static constexpr int kQuery = kScale + kStreams * kTaSlots * kScaleSlot;
     static constexpr int kState = kQuery + R * 4096;
-    static constexpr int kBytes = kState + kTaWaves * kTaRows * 8;
+    static constexpr int kKept = kState + kTaWaves * kTaRows * 8;  // per wave a tile's probabilities
+    static constexpr int kBytes = kKept + kTaWaves * 4096;
     static constexpr int kMerge = kTaWaves * 4 * 4096;  // 4 blocks of 4 KB per wave
     static_assert(kBytes <= 160 * 1024, "LDS of a CU");
     static_assert(kStreams == 1 || kMerge <= kRope, "merge buffer in the ring");
-    static_assert((KVIP_DRAFT_MAX_BATCH + 1 + kTaWaves) * 8 <= kRope, "work line in the ring");
 };
 
 __host__ __device__ inline int ta_groups(int heads, int nodes) { return heads * nodes <= 2 * kTaRows ? 2 : 4; }  // R
 
 __host__ __device__ inline int ta_tiles(int rows, int r) { return (rows + kTaRows * r - 1) / (kTaRows * r); }
 
-// Shares of a launch: one workgroup per CU, no more than the longest contexts could fill.
-__host__ __device__ inline int ta_shares(int batch, int heads, int nodes, int max_blocks) {
+// Steps of a launch at most (the kernel counts them in 32 bits), and its shares: one workgroup per CU, no more
+// than these steps could fill.
+inline int64_t ta_most_steps(int batch, int heads, int nodes, int max_blocks) {
     const int r = ta_groups(heads, nodes), streams = kTaWaves / r;
     const int64_t steps = (static_cast<int64_t>(max_blocks) * kBlockTokens + kTaTile * streams - 1) / (kTaTile * streams);
-    const int64_t most = (steps * batch * ta_tiles(heads * nodes, r) + kMinSteps - 1) / kMinSteps;
+    return steps * batch * ta_tiles(heads * nodes, r);
+}
+inline int ta_shares(int batch, int heads, int nodes, int max_blocks) {
+    const int64_t most = (ta_most_steps(batch, heads, nodes, max_blocks) + kMinSteps - 1) / kMinSteps;
     return static_cast<int>(most < kTaGroups ? most : kTaGroups);
 }
 
@@ -181,8 +186,8 @@ KVIP_DEVICE int ta_steps(int length) {
 }
 
 template <int R>
-KVIP_DEVICE int64_t ta_cost(const KvipTreeAttnArgs& p, const TaRequest& q) {
-    return static_cast<int64_t>(ta_tiles(q.nodes * p.heads, R)) * ta_steps<R>(q.length);
+KVIP_DEVICE uint32_t ta_cost(const KvipTreeAttnArgs& p, const TaRequest& q) {
+    return static_cast<uint32_t>(ta_tiles(q.nodes * p.heads, R)) * ta_steps<R>(q.length);
 }
 
 // Direct-to-LDS loads from a wave-uniform address and a lane's offset below 2^32 (see lds_async.h).
@@ -208,7 +213,6 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w % R, st = w / R;  // row group, stream
-    const int n = lane & 31, kg = lane >> 5;
     const int shares = gridDim.x;
     // Neighbouring shares, which read the same cache rows where an item or a request spans them, on one
     // XCD (workgroups are dealt round the 8).
@@ -216,53 +220,47 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     const int g = static_cast<int>(blockIdx.x) < per_xcd * 8 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8
                                                              : blockIdx.x;
 
-    // The line of work, in the ring's place: steps before each request, 4 requests per thread, running sums in
-    // 64 bits. Then this share's part of it: [pos, end), from request b, which starts at b_pos.
+    // The line of work: steps before each request, 4 requests per thread. Then this share's part of it:
+    // [pos, end), from request b, which starts at b_pos.
     int b;
-    int64_t pos, end, b_pos, quota;
+    uint32_t pos, end, b_pos, quota;
     {
         constexpr int kPer = KVIP_DRAFT_MAX_BATCH / kTaThreads;
-        int64_t* s_line = reinterpret_cast<int64_t*>(s_mem);
-        int64_t* s_sum = s_line + KVIP_DRAFT_MAX_BATCH + 1;
-        int64_t cost[kPer], sum = 0;
-        uint32_t err = 0;
+        uint32_t* s_sum = reinterpret_cast<uint32_t*>(s_mem);
+        uint32_t* s_found = s_sum + kTaWaves;  // request, where it starts
+        uint32_t cost[kPer], sum = 0, err = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int at = tid * kPer + i;
-            cost[i] = at < p.batch ? ta_cost<R>(p, ta_request(p, at, &err)) : 0;
+            cost[i] = at < p.batch ? ta_cost<R>(p, ta_request(p, at, &err)) : 0u;
             sum += cost[i];
         }
         if (blockIdx.x == 0) report(p.status, err);
-        int64_t run = sum;
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t lo = static_cast<uint32_t>(__shfl_up(static_cast<int>(run), d));
-            const uint32_t hi = static_cast<uint32_t>(__shfl_up(static_cast<int>(run >> 32), d));
-            if (lane >= d) run += static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-        }
+        const uint32_t run = wave_inclusive_scan(sum);
         if (lane == 63) s_sum[w] = run;
         __syncthreads();
-        int64_t before = run - sum;
-        for (int v = 0; v < w; ++v) before += s_sum[v];
+        uint32_t before = run - sum, total = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int at = tid * kPer + i;
-            if (at < p.batch) s_line[at] = before;
-            before += cost[i];
-            if (at == p.batch - 1) s_line[p.batch] = before;
+        for (int v = 0; v < kTaWaves; ++v) {
+            before += v < w ? s_sum[v] : 0u;
+            total += s_sum[v];
         }
-        __syncthreads();
-        const int64_t total = s_line[p.batch], even = (total + shares - 1) / shares;
+        const uint32_t even = (total + shares - 1) / shares;
         quota = even < kMinSteps ? kMinSteps : even;
         pos = min(g * quota, total);
         end = min(pos + quota, total);
-        int lo = 0, hi = p.batch - 1;  // the last request that starts at or before pos
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_line[mid] <= pos) lo = mid;
-            else hi = mid - 1;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (before <= pos && pos < before + cost[i]) {
+                s_found[0] = tid * kPer + i;
+                s_found[1] = before;
+            }
+            before += cost[i];
         }
-        b = __builtin_amdgcn_readfirstlane(lo);
-        b_pos = s_line[b];
+        __syncthreads();
+        if (pos >= end) return;  // the whole workgroup: more shares than steps
+        b = __builtin_amdgcn_readfirstlane(s_found[0]);
+        b_pos = __builtin_amdgcn_readfirstlane(s_found[1]);
     }
     const TaWork<R> work(p.workspace, shares);
     const uint32_t ring_lds = lds_addr(s_mem + st * kTaSlots * kNopeSlot);
@@ -280,7 +278,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         // The item at `pos`: request b, row tile rt, steps t0 .. t1 of its `steps`.
         uint32_t err = 0;
         TaRequest req = ta_request(p, b, &err);
-        int64_t cost = ta_cost<R>(p, req);
+        uint32_t cost = ta_cost<R>(p, req);
         while (pos >= b_pos + cost) {  // ends at the request that holds pos, as pos < end <= the line's length
             b_pos += cost;
             req = ta_request(p, ++b, &err);
@@ -288,86 +286,65 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         }
         err = 0;
         const int steps = ta_steps<R>(req.length);
-        const int64_t within = pos - b_pos;
-        const int rt = __builtin_amdgcn_readfirstlane(static_cast<int>(within / steps));
-        const int t0 = __builtin_amdgcn_readfirstlane(static_cast<int>(within % steps));
-        const int t1 = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(steps), t0 + (end - pos))));
-        const int64_t item_pos = pos - t0;
+        const uint32_t within = pos - b_pos;
+        const int rt = __builtin_amdgcn_readfirstlane(within / steps);
+        const int t0 = __builtin_amdgcn_readfirstlane(within - rt * steps);
+        const int t1 = __builtin_amdgcn_readfirstlane(min(steps, static_cast<int>(t0 + (end - pos))));
+        const uint32_t item_pos = pos - t0;
         pos += t1 - t0;
         const bool whole = t0 == 0 && t1 == steps;
         const int rows = req.nodes * p.heads;
-        const int row = rt * kTaRows * R + rg * kTaRows + n;
-        const bool busy = rt * kTaRows * R + rg * kTaRows < rows;  // uniform: the wave's group has rows
+        const int first_row = rt * kTaRows * R + rg * kTaRows;
+        const bool busy = first_row < rows;  // uniform: the wave's group has rows
         const int32_t* table = p.block_table + static_cast<int64_t>(b) * p.max_blocks;
 
         // Page of the wave's tile of step t (-1: none of its tokens is there), from the table entries of 64 pages
         // that the lanes hold.
-        int held = 0, held_first = -64;
+        int held_first = t0 * kStreams / (kBlockTokens / kTaTile);
+        int held = table[min(held_first + lane, p.max_blocks - 1)];
         auto page_of = [&](int t) {
             const int tile = t * kStreams + st, at = tile / (kBlockTokens / kTaTile);
             if (t >= t1 || tile * kTaTile >= req.length) return -1;
             if (at >= held_first + 64) {
                 held_first = at;
                 held = table[min(at + lane, p.max_blocks - 1)];
+                asm volatile("" : "+v"(held));  // waited for here, not at every use
             }
             const int page = __builtin_amdgcn_readlane(held, at - held_first);
             if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks)) return page;
             err |= KVIP_STATUS_BAD_BLOCK;
             return -1;
         };
-        // This wave's share (1 / R) of the loads of step t's tile into slot `slot`. LDS row i of the nope bytes holds
-        // piece s ^ ta_swz(i) at place s, of the rope features (128 bytes) piece s ^ (i / 2 % 8); scales stand as
-        // [group][token]. Tokens that are not there get zeros: their probabilities are zero, and zero times a
-        // stray NaN would not be (their rope keeps stale bytes: their logits are replaced).
-        auto load = [&](int t, int page, int slot) {
-            const int ln = fresh(lane), up = ln >> 5, tile = t * kStreams + st;
-            const int live = page < 0 ? 0 : min(req.length - tile * kTaTile, kTaTile);
-            const uint8_t* base = p.kv_cache + page * p.kv_block_stride +
-                                  static_cast<int64_t>(tile % (kBlockTokens / kTaTile)) * kTaTile * row_stride;
-            constexpr int kNopeLoads = 16 / R, kRopeLoads = 4 / R;
-            const uint32_t dst = ring_lds + slot * kNopeSlot, rope_dst = rope_lds + slot * kRopeSlot;
-            const uint32_t scale_dst = scales_lds + slot * kScaleSlot;
-            // Lane offsets: tokens 2 v and 2 v + 1 of nope bytes per load, 8 v .. 8 v + 7 of rope features, and scale
-            // groups 2 v and 2 v + 1.
-            auto nope_from = [&](int v) { return static_cast<uint32_t>(up * row_stride + ((ln & 31) ^ ta_swz(up) ^ ta_swz(2 * v)) * 16); };
-            auto rope_from = [&](int v) {
-                return static_cast<uint32_t>((ln >> 3) * row_stride + kValueDim + ((ln & 7) ^ (ln >> 4) ^ ((v & 1) * 4)) * 16);
-            };
-            const uint32_t scale_from = (ln & 31) * row_stride + 640 + 4 * up;
-            if (live == kTaTile) {
-#pragma unroll
-                for (int x = 0; x < kNopeLoads; ++x) {
-                    const int v = rg * kNopeLoads + x;
-                    dma16_at(base + 2 * v * row_stride, nope_from(v), dst + v * 1024);
-                }
-#pragma unroll
-                for (int x = 0; x < kRopeLoads; ++x) {
-                    const int v = rg * kRopeLoads + x;
-                    dma16_at(base + 8 * v * row_stride, rope_from(v), rope_dst + v * 1024);
-                }
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    if (v == rg) dma4_at(base + 8 * v, scale_from, scale_dst + v * 256);
-                }
-                return;
-            }
-#pragma unroll 1
-            for (int x = 0; x < kNopeLoads; ++x) {
-                const int v = rg * kNopeLoads + x;
-                if (2 * v + up < live) {
-                    dma16_at(base + 2 * v * row_stride, nope_from(v), dst + v * 1024);
-                } else {
-                    *(__attribute__((address_space(3))) v4i*)(dst + v * 1024 + ln * 16) = v4i{0, 0, 0, 0};
-                }
-            }
-#pragma unroll 1
-            for (int x = 0; x < kRopeLoads; ++x) {
-                const int v = rg * kRopeLoads + x;
-                if (8 * v + (ln >> 3) < live) dma16_at(base + 8 * v * row_stride, rope_from(v), rope_dst + v * 1024);
-            }
-            if (rg < 2) {
-                if ((ln & 31) < live) dma4_at(base + 8 * rg, scale_from, scale_dst + rg * 256);
-                else *(__attribute__((address_space(3))) float*)(scale_dst + rg * 256 + ln * 4) = 0.f;
+        // The tile under way: the first row of this wave's share (1 / R) of its tokens, and its LDS slot. A tile is
+        // part of one page, so its 32 rows are in the cache, whatever the length; where there is no page the
+        // cache's first rows stand in. `logits` zeroes in LDS what is not there.
+        constexpr int kShare = kTaTile / R;
+        const uint8_t* from = nullptr;
+        int from_slot = 0;
+        auto aim = [&](int t, int page, int slot) {
+            const int first = page < 0 ? 0 : (t * kStreams + st) % (kBlockTokens / kTaTile) * kTaTile;
+            from = p.kv_cache + max(page, 0) * p.kv_block_stride + static_cast<int64_t>(first + rg * kShare) * row_stride;
+            from_slot = slot;
+        };
+        // The share's loads, in kFetches pieces that are called in order. LDS row i of the nope bytes holds piece
+        // s ^ ta_swz(i) at place s, of the rope features (128 bytes) piece s ^ (i / 2 % 8); scales stand as
+        // [group][token].
+        constexpr int kNopeLoads = kShare / 2, kRopeLoads = kShare / 8, kFetches = kNopeLoads + kRopeLoads + 1;
+        constexpr int kEvery = 16 / kFetches;  // products of the logits from one piece to the next
+        auto fetch = [&](int x, int ln) {
+            if (x < kNopeLoads) {  // the share's tokens 2 x and 2 x + 1 (ta_swz is linear over XOR)
+                const int up = ln >> 5;
+                dma16_at(from, up * row_stride + ((ln & 31) ^ ta_swz(up) ^ ta_swz(rg * kShare) ^ ta_swz(2 * x)) * 16,
+                         ring_lds + from_slot * kNopeSlot + rg * (kShare * kValueDim) + x * 1024);
+                from += x + 1 < kNopeLoads ? 2 * row_stride : -(2 * kNopeLoads - 2) * row_stride;
+            } else if (x < kNopeLoads + kRopeLoads) {  // tokens 8 y .. 8 y + 7
+                const int y = x - kNopeLoads, v = rg * kRopeLoads + y;
+                dma16_at(from, (ln >> 3) * row_stride + kValueDim + ((ln & 7) ^ (ln >> 4) ^ ((v & 1) * 4)) * 16,
+                         rope_lds + from_slot * kRopeSlot + rg * (kShare * 128) + y * 1024);
+                from += y + 1 < kRopeLoads ? 8 * row_stride : -(8 * kRopeLoads - 8 + rg * kShare) * row_stride;
+            } else {  // scale groups 2 v and 2 v + 1 of all tokens (with 4 row groups, two of them load the same)
+                const int v = rg & 1;
+                dma4_at(from + 8 * v, (ln & 31) * row_stride + 640 + 4 * (ln >> 5), scales_lds + from_slot * kScaleSlot + v * 256);
             }
         };
         // Every load and LDS access of this wave is done, and of all waves.
@@ -377,79 +354,48 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             asm volatile("" : : : "memory");
         };
 
+        // Queries of the wave's rows (rows past the last read it again; their outputs are not written). Fragment
+        // 2 i + x: features 16 (2 i + kg) + 8 x .. + 7, the half x of the key piece that the lane reads; rope
+        // fragment i: features 16 i + 8 kg .. + 7.
+        v4i qf[32], q_rope[4];
+        uint64_t seen_by = 0;
+        if (busy) {
+            const int n = lane & 31, kg = lane >> 5;
+            const int at = min(first_row + n, rows - 1), node = at / p.heads;
+            const uint16_t* q = p.query + (static_cast<int64_t>(req.begin) * p.heads + at) * kKeyDim;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) qf[i] = *reinterpret_cast<const v4i*>(q + (i >> 1) * 32 + kg * 16 + (i & 1) * 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q_rope[i] = *reinterpret_cast<const v4i*>(q + kValueDim + i * 16 + kg * 8);
+            seen_by = p.visible != nullptr ? static_cast<uint64_t>(p.visible[req.begin + node]) : ~0ull >> (63 - node);
+        }
         __syncthreads();  // the LDS of the item before (at first: the line of work) is free
-        int page = page_of(t0);
-        load(t0, page, 0);
-        int page_next = page_of(t0 + 1);
-        if (t0 + 1 < t1) load(t0 + 1, page_next, 1);
-        // Step t: its tile has landed, the slot of step t - 1's is free and takes that of step t + 1 (but for the
-        // first two, which are under way).
+        int page = page_of(t0), page_next = page;
+        aim(t0, page, 0);
+#pragma unroll
+        for (int x = 0; x < kFetches; ++x) fetch(x, lane);
+        // Step t: its tile has landed, and the slot of step t - 2's is free for that of step t + 1, which is aimed at.
         auto arrive = [&](int t, int slot_free) {
             settle();
-            if (t == t0) return;
-            const int ahead = page_of(t + 1);
-            if (t + 1 < t1) load(t + 1, ahead, slot_free);
             page = page_next;
-            page_next = ahead;
+            page_next = page_of(t + 1);
+            aim(t + 1, page_next, slot_free);
         };
         auto last_tokens = [&](int t) { return (t + 1) * kStreams * kTaTile > req.past; };  // of the context, or step tokens
-        const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
-        const size_t slot_row = (static_cast<size_t>(g) * 2 + (t0 == 0 ? 1 : 0)) * kTaRows * R + rg * kTaRows + n;
-        // A whole item's rows are final; else the sums and their state go to the share's part 0 (others began
-        // the item) or 1.
-        auto put = [&](int f, const v16f& x, float factor) {
-            if (row >= rows) return;
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const int feature = 32 * f + 8 * a + 4 * kg;
-                const f32x4 v = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * factor;
-                if (!whole) {
-                    *reinterpret_cast<f32x4*>(work.sums + slot_row * kValueDim + feature) = v;
-                } else if (p.output_dtype == KVIP_DTYPE_FP32) {
-                    *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + out_row * kValueDim + feature) = v;
-                } else {
-                    *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + feature) =
-                        __builtin_convertvector(v, bf16x4);
-                }
-            }
-        };
-        auto put_state = [&](float m, float l) {
-            if (st != 0 || kg != 0 || row >= rows) return;
-            if (!whole) work.state[slot_row] = make_float2(m, l);
-            else if (p.lse != nullptr) p.lse[out_row] = ta_lse(m, l);
-        };
         if (!busy) {  // a row group without rows loads its share of the tiles
             for (int t = t0; t < t1; ++t) {
                 arrive(t, (t + 1 - t0) % kTaSlots);
                 if (last_tokens(t)) lds_sync();
+#pragma unroll
+                for (int x = 0; x < kFetches; ++x) fetch(x, lane);
             }
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
             if constexpr (kStreams > 1) {  // the barriers of the merge
                 for (int i = 0; i < 5; ++i) __syncthreads();
             }
         } else {
-            // Queries of the wave's rows (rows past the last read it again; their outputs are not written). Fragment
-            // 2 i + x: features 16 (2 i + kg) + 8 x .. + 7, the half x of the key piece that the lane reads; rope
-            // fragment i: features 16 i + 8 kg .. + 7.
-            v4i qf[32];
-            uint64_t* s_seen = reinterpret_cast<uint64_t*>(s_mem + L::kState) + w * kTaRows + n;
-            const uint32_t q_rope = lds_addr(s_mem + L::kQuery) + rg * 4096 + lane * 16;
-            {
-                const int at = min(row, rows - 1), node = at / p.heads;
-                const uint16_t* q = p.query + (static_cast<int64_t>(req.begin) * p.heads + at) * kKeyDim;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    qf[i] = *reinterpret_cast<const v4i*>(q + (i >> 1) * 32 + kg * 16 + (i & 1) * 8) ^ flip;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {  // the streams of a row group write the same
-                    *(__attribute__((address_space(3))) v4i*)(q_rope + i * 1024) =
-                        *reinterpret_cast<const v4i*>(q + kValueDim + i * 16 + kg * 8) ^ flip;
-                }
-                *s_seen = p.visible != nullptr ? static_cast<uint64_t>(p.visible[req.begin + node]) : ~0ull >> (63 - node);
-            }
-            // Waited for here: the tile loop would wait for them each time round, and so for its own loads.
-#pragma unroll
-            for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(qf[i]));
+            const uint32_t rope_q_lds = lds_addr(s_mem + L::kQuery) + rg * 4096;                 // + lane * 16
+            uint64_t* s_seen = reinterpret_cast<uint64_t*>(s_mem + L::kState) + w * kTaRows;  // + row of the wave
             v16f o[kBlocks];
 #pragma unroll
             for (int f = 0; f < kBlocks; ++f) {
@@ -457,23 +403,35 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
                 hold(o[f]);
             }
+            // Waited for here: the tile loop would wait for them each time round, and so for its own loads.
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                qf[i] ^= flip;
+                asm volatile("" : "+v"(qf[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // the streams of a row group write the same
+                *(__attribute__((address_space(3))) v4i*)(rope_q_lds + lane * 16 + i * 1024) = q_rope[i] ^ flip;
+            }
+            s_seen[lane & 31] = seen_by;
             float m_run = -INFINITY;  // reference maximum of the row
             float l_sum = 0.f;        // this lane's share of its probability sum
-            float pr[16];             // probabilities of the tile whose values come next, relative to m_run
+            // Probabilities of the tile whose values come next, relative to m_run: in LDS while the logits need the registers.
+            const uint32_t kept_lds = lds_addr(s_mem + L::kKept) + w * 4096;
             v16f s;                   // logits
 
             constexpr int kAhead = 3;  // LDS reads stand so many products before their use, conversions one
-            // Logits of step t's tile, in slot `slot`.
+            // Logits of step t's tile, in slot `slot`; the loads of the tile that is aimed at stand between the products.
             auto logits = [&](int t, int slot) {
                 const int ln = fresh(lane), tn = ln & 31, tk = ln >> 5;
                 const int first = (t * kStreams + st) * kTaTile;  // position of the tile's first token
                 uint32_t sees = page < 0 ? 0u : 0xFFFFu;          // bit i: the row sees the token of register i
                 bool masked = page < 0;
-                // A step with step tokens or the end of the context in it (the same for the workgroup's waves). What
-                // a row does not see must not reach it, and zero times a NaN would: tokens with a NaN feature or a
-                // scale that is not finite are found and zeroed in LDS, and rows that do see one become NaN as a
-                // whole (their logit is none).
-                if (last_tokens(t)) {
+                // A step with step tokens or the end of the context in it (the same for the workgroup's waves), or a
+                // tile that is not there. What a row does not see must not reach it, and zero times a NaN would:
+                // tokens that are not there, and those with a NaN feature or a scale that is not finite, are
+                // zeroed in LDS, and rows that do see one of the latter become NaN as a whole (their logit is none).
+                if (masked || last_tokens(t)) {
                     masked = true;
                     uint32_t nan = 0;
                     const uint32_t at = ring_lds + slot * kNopeSlot + tn * kValueDim;
@@ -492,8 +450,8 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     }
                     const uint64_t found = __ballot(nan != 0);
                     const uint32_t bad = static_cast<uint32_t>(found | found >> 32);
-                    lds_sync();  // the waves of the stream have all looked
-                    if (bad >> tn & 1) {
+                    if (last_tokens(t)) lds_sync();  // the waves of the stream have all looked (or none needs to)
+                    if ((bad >> tn & 1) || page < 0 || first + tn >= req.length) {
 #pragma unroll 1
                         for (int i = 0; i < 16; ++i) {
                             *(__attribute__((address_space(3))) v4i*)(at + (16 * tk + i) * 16) = v4i{0, 0, 0, 0};
@@ -502,7 +460,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                         for (int i = 0; i < 2; ++i) *(__attribute__((address_space(3))) float*)(sc + i * kTaTile * 4) = 0.f;
                     }
                     sees = 0;
-                    const uint64_t seen = *s_seen;
+                    const uint64_t seen = s_seen[tn];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int token = 8 * (i >> 2) + 4 * tk + (i & 3), rel = first + token - req.past;
@@ -517,22 +475,10 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 const uint32_t sl = scales_lds + slot * kScaleSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
                 // Bit 8 of a key's address is its own: pieces 16 and up by an offset.
                 auto key = [&](int i) { return *(LdsV4i)((ko ^ ((i & 7) * 32)) + (i >> 3) * 256); };
-                v4i kr[4], kb[kAhead + 1];
+                v4i kr[4];
                 v16f dot[2];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) kr[i] = *(LdsV4i)(ro + (((2 * i + tk) ^ ((tn >> 1) & 7)) << 4));
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) kb[i] = key(i);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const v4i y = *(LdsV4i)(q_rope + i * 1024);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), __builtin_bit_cast(bf16x8, y), s, 0, 0, 0);
-                }
-                bf16x8 ka[2] = {fp8x8_to_bf16(kb[0][0], kb[0][1]), fp8x8_to_bf16(kb[0][2], kb[0][3])};
-                // A quarter of a group's dot products (tokens 8 a + 4 kg .. + 3) joins the logits four products later, its
-                // scales two before that.
+                // A quarter of a group's dot products (tokens 8 a + 4 kg .. + 3) joins the logits a group later, its
+                // scales are read a little before that.
                 f32x4 s4[3];
                 auto scales = [&](int q) { s4[q % 3] = *(LdsF32x4)(sl + ((q >> 2) * kTaTile + 8 * (q & 3)) * 4); };
                 auto join = [&](int q) {
@@ -542,25 +488,41 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                         s[e] = fmaf(dot[q >> 2 & 1][e], s4[q % 3][c], s[e]);
                     }
                 };
-                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int gr = i >> 2;
-                    v16f& d = dot[gr & 1];
-                    if ((i & 3) == 0) {
+                for (int i = 0; i < 4; ++i) kr[i] = *(LdsV4i)(ro + (((2 * i + tk) ^ ((tn >> 1) & 7)) << 4));
+                {
+                    v4i kb[kAhead + 1];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) d[e] = 0.f;
+                    for (int i = 0; i < kAhead; ++i) kb[i] = key(i);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const v4i y = *(LdsV4i)(rope_q_lds + ln * 16 + i * 1024);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), __builtin_bit_cast(bf16x8, y), s, 0, 0, 0);
                     }
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], __builtin_bit_cast(bf16x8, qf[2 * i]), d, 0, 0, 0);
-                    if (i + kAhead < 16) kb[(i + kAhead) % (kAhead + 1)] = key(i + kAhead);
-                    const v4i x = kb[(i + 1) % (kAhead + 1)];
-                    if (i < 15) ka[0] = fp8x8_to_bf16(x[0], x[1]);
+                    bf16x8 ka[2] = {fp8x8_to_bf16(kb[0][0], kb[0][1]), fp8x8_to_bf16(kb[0][2], kb[0][3])};
                     __builtin_amdgcn_sched_barrier(0);
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[1], __builtin_bit_cast(bf16x8, qf[2 * i + 1]), d, 0, 0, 0);
-                    if (i < 15) ka[1] = fp8x8_to_bf16(x[2], x[3]);
-                    if (i >= 4) join(i - 4);
-                    if (i >= 2) scales(i - 2);
-                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int gr = i >> 2;
+                        v16f& d = dot[gr & 1];
+                        if ((i & 3) == 0) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) d[e] = 0.f;
+                        }
+                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], __builtin_bit_cast(bf16x8, qf[2 * i]), d, 0, 0, 0);
+                        if (i + kAhead < 16) kb[(i + kAhead) % (kAhead + 1)] = key(i + kAhead);
+                        const v4i x = kb[(i + 1) % (kAhead + 1)];
+                        if (i < 15) ka[0] = fp8x8_to_bf16(x[0], x[1]);
+                        if (i % kEvery == 0 && i / kEvery < kFetches) fetch(i / kEvery, ln);
+                        __builtin_amdgcn_sched_barrier(0);
+                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[1], __builtin_bit_cast(bf16x8, qf[2 * i + 1]), d, 0, 0, 0);
+                        if (i < 15) ka[1] = fp8x8_to_bf16(x[2], x[3]);
+                        if (i >= 4) join(i - 4);
+                        if (i >= 2) scales(i - 2);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
                 join(12);
                 scales(14);
@@ -600,7 +562,9 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             auto take = [&] {  // the softmax's results become those of the tile whose values come next
                 l_sum = l_sum * alpha + fresh_sum;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) pr[i] = s[i];
+                for (int a = 0; a < 4; ++a) {
+                    *(LdsF32x4Out)(kept_lds + fresh(lane) * 16 + a * 1024) = f32x4{s[4 * a], s[4 * a + 1], s[4 * a + 2], s[4 * a + 3]};
+                }
             };
             // Values of the tile in slot `slot` [features, rows], the softmax of the next one beside them.
             auto values = [&](int slot, auto with_softmax) {
@@ -615,15 +579,17 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 // A quarter of a group's operand: the probabilities of tokens 8 a + 4 kg .. + 3 times their scales, which
                 // are read two products earlier.
                 v4i pb[2][2];
-                f32x4 s4[4];
+                f32x4 s4[4], pr[4];
                 auto scales = [&](int q) { s4[q & 3] = *(LdsF32x4)(sl + ((q >> 2) * kTaTile + 8 * (q & 3)) * 4); };
                 auto weigh = [&](int q) {
                     const int a = q & 3;
                     v4i& d = pb[q >> 2 & 1][a >> 1];
-                    d[2 * (a & 1)] = static_cast<int>(pack_bf16(pr[4 * a] * s4[a][0], pr[4 * a + 1] * s4[a][1]));
-                    d[2 * (a & 1) + 1] = static_cast<int>(pack_bf16(pr[4 * a + 2] * s4[a][2], pr[4 * a + 3] * s4[a][3]));
+                    d[2 * (a & 1)] = static_cast<int>(pack_bf16(pr[a][0] * s4[a][0], pr[a][1] * s4[a][1]));
+                    d[2 * (a & 1) + 1] = static_cast<int>(pack_bf16(pr[a][2] * s4[a][2], pr[a][3] * s4[a][3]));
                 };
                 i32x2 vb[kAhead + 1][2];
+#pragma unroll
+                for (int a = 0; a < 4; ++a) pr[a] = *(LdsF32x4)(kept_lds + ln * 16 + a * 1024);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) scales(q);
 #pragma unroll
@@ -662,7 +628,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 }
             };
 
-            arrive(t0, 0);
+            arrive(t0, 1);
             logits(t0, 0);
 #pragma unroll
             for (int i = 0; i < 18; ++i) softmax(i);
@@ -686,7 +652,35 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 slot = slot_next;
             }
             values(slot, std::false_type{});
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
 
+            const int le = fresh(lane), hn = le & 31, hk = le >> 5;  // not held over the tiles
+            const int row = first_row + hn;
+            const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
+            const size_t slot_row = (static_cast<size_t>(g) * 2 + (t0 == 0 ? 1 : 0)) * kTaRows * R + rg * kTaRows + hn;
+            // A whole item's rows are final; else the sums and their state go to the share's part 0 (others began
+            // the item) or 1.
+            auto put = [&](int f, const v16f& x, float factor) {
+                if (row >= rows) return;
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int feature = 32 * f + 8 * a + 4 * hk;
+                    const f32x4 v = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * factor;
+                    if (!whole) {
+                        *reinterpret_cast<f32x4*>(work.sums + slot_row * kValueDim + feature) = v;
+                    } else if (p.output_dtype == KVIP_DTYPE_FP32) {
+                        *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + out_row * kValueDim + feature) = v;
+                    } else {
+                        *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + feature) =
+                            __builtin_convertvector(v, bf16x4);
+                    }
+                }
+            };
+            auto put_state = [&](float m, float l) {
+                if (st != 0 || hk != 0 || row >= rows) return;
+                if (!whole) work.state[slot_row] = make_float2(m, l);
+                else if (p.lse != nullptr) p.lse[out_row] = ta_lse(m, l);
+            };
             const float l_all = half_sum(l_sum);
             const float m_all = m_run * scale2;  // log2 units from here on
             if constexpr (kStreams == 1) {
@@ -702,16 +696,16 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 // wave sums half of the blocks, whose other half it puts into LDS, 8 blocks at a time.
                 float2* s_state = reinterpret_cast<float2*>(s_mem + L::kState);
                 __syncthreads();  // every wave is done with its ring and its rows' bits
-                if (kg == 0) s_state[w * kTaRows + n] = make_float2(m_all, l_all);
+                if (hk == 0) s_state[w * kTaRows + hn] = make_float2(m_all, l_all);
                 __syncthreads();
-                const float2 other = s_state[(w ^ R) * kTaRows + n];
+                const float2 other = s_state[(w ^ R) * kTaRows + hn];
                 const float top = fmaxf(m_all, other.x);
                 const float mine = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_all - top);
                 const float theirs = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other.x - top);
                 const float l = mine * l_all + theirs * other.y;
                 const float factor = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
-                const uint32_t out_lds = lds_addr(s_mem) + w * 4 * 4096 + lane * 16;
-                const uint32_t in_lds = lds_addr(s_mem) + (w ^ R) * 4 * 4096 + lane * 16;
+                const uint32_t out_lds = lds_addr(s_mem) + w * 4 * 4096 + le * 16;
+                const uint32_t in_lds = lds_addr(s_mem) + (w ^ R) * 4 * 4096 + le * 16;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     if (half > 0) __syncthreads();
@@ -745,14 +739,13 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         }
         if (lane == 0) report(p.status, err);
         if (t0 == 0 && tid == 0) {  // which shares hold the item
-            const int last = static_cast<int>((item_pos + steps - 1) / quota);
+            const int last = (item_pos + steps - 1) / quota;
             work.items[static_cast<int64_t>(b) * ta_tiles(p.max_nodes * p.heads, R) + rt] = make_int2(g, last - g + 1);
         }
     }
 }
 
-// Joins the parts of items that several shares hold: 8 rows per workgroup, 128 threads of 4 features per
-// row and pass.
+// Joins the parts of items that several shares hold: 128 threads of 4 features per row.
 template <int R>
 __global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAttnArgs p, int shares) {
     constexpr int kPer = kTaRows * R / kJoinRows;
@@ -766,38 +759,38 @@ __global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAtt
     const TaWork<R> work(p.workspace, shares);
     const int2 of = work.items[item];
     if (of.y <= 1) return;
-    const int f = (threadIdx.x & 127) * 4;
-#pragma unroll 1
-    for (int i = threadIdx.x >> 7; i < kJoinRows; i += 2) {
-        const int row = rt * kTaRows * R + local + i;
-        if (row >= rows) return;
-        auto at = [&](int k) {  // the row of share of.x + k's part
-            return (static_cast<size_t>(of.x + k) * 2 + (k == 0 ? 1 : 0)) * kTaRows * R + local + i;
-        };
-        float m = -INFINITY;
-        for (int k = 0; k < of.y; ++k) m = fmaxf(m, work.state[at(k)].x);
-        float l = 0.f;
-        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int k = 0; k < of.y; ++k) {
-            const float2 sk = work.state[at(k)];
-            const f32x4 x = *reinterpret_cast<const f32x4*>(work.sums + at(k) * kValueDim + f);
-            const float wgt = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk.x - m);
-            l += wgt * sk.y;
-            v += wgt * x;
-        }
-        v *= l > 0.f || l != l ? 1.f / l : 0.f;
-        const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
-        if (p.output_dtype == KVIP_DTYPE_FP32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + out_row * kValueDim + f) = v;
-        } else {
-            *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + f) =
-                __builtin_convertvector(v, bf16x4);
-        }
-        if (f == 0 && p.lse != nullptr) {
-            p.lse[out_row] = ta_lse(m, l);
+    const int f = (threadIdx.x & 127) * 4, row = rt * kTaRows * R + local + (threadIdx.x >> 7);
+    if (row >= rows) return;
+    auto at = [&](int k) {  // the row of share of.x + k's part
+        return (static_cast<size_t>(of.x + k) * 2 + (k == 0 ? 1 : 0)) * kTaRows * R + row % (kTaRows * R);
+    };
+    // The parts' states by the lanes of a wave, 64 at a time, then their sums, several loads under way.
+    const int lane = threadIdx.x & 63;
+    float m = -INFINITY, l = 0.f;
+    for (int k = lane; k < of.y; k += 64) m = fmaxf(m, work.state[at(k)].x);
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first < of.y; first += 64) {
+        float2 state = make_float2(-INFINITY, 0.f);
+        if (first + lane < of.y) state = work.state[at(first + lane)];
+        const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
+        l += weight * state.y;
+        const int count = min(of.y - first, 64);
+#pragma unroll 8
+        for (int k = 0; k < count; ++k) {
+            const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
+            v += wk * *reinterpret_cast<const f32x4*>(work.sums + at(first + k) * kValueDim + f);
         }
     }
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d);
+    v *= l > 0.f || l != l ? 1.f / l : 0.f;
+    const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
+    if (p.output_dtype == KVIP_DTYPE_FP32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + out_row * kValueDim + f) = v;
+    } else {
+        *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + f) = __builtin_convertvector(v, bf16x4);
+    }
+    if (f == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(m, l);
 }
 
 template <int R>
@@ -814,7 +807,8 @@ void launch_tree(const KvipTreeAttnArgs& a, hipStream_t s) {
 extern "C" uint64_t kvip_hip_tree_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t max_nodes,
                                                             int32_t max_blocks) {
     if (batch < 1 || batch > KVIP_DRAFT_MAX_BATCH || heads < 1 || heads > 128 || max_nodes < 1 ||
-        max_nodes > KVIP_DRAFT_MAX_NODES || max_blocks < 1 || max_blocks > (1 << 17)) {
+        max_nodes > KVIP_DRAFT_MAX_NODES || max_blocks < 1 || max_blocks > (1 << 17) ||
+        kvip::ta_most_steps(batch, heads, max_nodes, max_blocks) > 0x7FFFFFFF) {
         return 0;
     }
     const int r = kvip::ta_groups(heads, max_nodes), shares = kvip::ta_shares(batch, heads, max_nodes, max_blocks);
@@ -833,7 +827,8 @@ extern "C" uint32_t kvip_hip_tree_attention(const KvipTreeAttnArgs* a, void* str
                     a->num_blocks >= 1 && a->num_blocks < (1 << 24) && a->row_stride >= KVIP_KV_ROW_BYTES &&
                     a->row_stride <= (1 << 24) && a->row_stride % 16 == 0 && a->kv_block_stride % 16 == 0 &&
                     a->kv_block_stride >= static_cast<int64_t>(kvip::kBlockTokens) * a->row_stride &&
-                    (a->output_dtype == KVIP_DTYPE_BF16 || a->output_dtype == KVIP_DTYPE_FP32);
+                    (a->output_dtype == KVIP_DTYPE_BF16 || a->output_dtype == KVIP_DTYPE_FP32) &&
+                    kvip::ta_most_steps(a->batch, a->heads, a->max_nodes, a->max_blocks) <= 0x7FFFFFFF;
     if (!ok) return KVIP_ERR_INVALID;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     switch (kvip::ta_groups(a->heads, a->max_nodes)) {
