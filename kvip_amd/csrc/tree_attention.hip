@@ -51,7 +51,6 @@ constexpr int kScaleGroups = 4;
 constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
 constexpr int kMinSteps = 4;                // steps of a share, at least
-constexpr int kJoinRows = 2;                // rows per workgroup of the joining launch
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kTaMargin = 8.0f * kLog2e;
@@ -131,24 +130,36 @@ KVIP_DEVICE float half_sum(float x) {
 KVIP_DEVICE constexpr int ta_swz(int t) { return ((t >> 2) & 1) | ((t & 1) << 1) | ((t & 2) << 1) | (t & 8); }
 
 // Where the workspace holds what: per share two parts (its first item's, where others began it, and its
-// last one's, where others go on) of 32 R rows x 512 sums, their (maximum, sum) pairs, then per item the
-// first share and the number of shares.
+// last one's, where others go on) of 32 R rows x 512 sums as a wave's lanes hold them ([row group][block][quarter]
+// [lane] 16 bytes: stored and read whole lines at a time), their (maximum, sum) pairs, then per item the first
+// share and the number of shares.
 template <int R>
 struct TaWork {
-    float* sums;
+    f32x4* sums;
     float2* state;
     int2* items;
     KVIP_DEVICE TaWork(void* base, int shares) {
-        constexpr int kRowsOf = kTaRows * R;
-        sums = static_cast<float*>(base);
-        state = reinterpret_cast<float2*>(sums + static_cast<size_t>(shares) * 2 * kRowsOf * kValueDim);
-        items = reinterpret_cast<int2*>(state + static_cast<size_t>(shares) * 2 * kRowsOf);
+        sums = static_cast<f32x4*>(base);
+        state = reinterpret_cast<float2*>(sums + static_cast<size_t>(shares) * 2 * R * (kBlocks * 4 * 64));
+        items = reinterpret_cast<int2*>(state + static_cast<size_t>(shares) * 2 * R * kTaRows);
     }
+    // Group `rg` of a part's rows: its sums (of lane 0) and states.
+    KVIP_DEVICE f32x4* group(int part, int rg) const { return sums + (static_cast<size_t>(part) * R + rg) * (kBlocks * 4 * 64); }
+    KVIP_DEVICE float2* rows(int part, int rg) const { return state + (static_cast<size_t>(part) * R + rg) * kTaRows; }
 };
 
 // log sum_j exp(s_j) of a row: maximum in log2 units, sum (0 where the row sees nothing).
 KVIP_DEVICE float ta_lse(float m, float l) {
     return l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+// Four features of the output.
+KVIP_DEVICE void ta_store(const KvipTreeAttnArgs& p, int64_t at, f32x4 v) {
+    if (p.output_dtype == KVIP_DTYPE_FP32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + at) = v;
+    } else {
+        *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + at) = __builtin_convertvector(v, bf16x4);
+    }
 }
 
 // Barrier for LDS data: unlike __syncthreads it leaves the direct-to-LDS loads in flight.
@@ -657,29 +668,27 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             const int le = fresh(lane), hn = le & 31, hk = le >> 5;  // not held over the tiles
             const int row = first_row + hn;
             const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
-            const size_t slot_row = (static_cast<size_t>(g) * 2 + (t0 == 0 ? 1 : 0)) * kTaRows * R + rg * kTaRows + hn;
+            const int part = g * 2 + (t0 == 0 ? 1 : 0);
             // A whole item's rows are final; else the sums and their state go to the share's part 0 (others began
             // the item) or 1.
             auto put = [&](int f, const v16f& x, float factor) {
+                if (!whole) {
+                    f32x4* out = work.group(part, rg) + le;
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) out[(f * 4 + a) * 64] = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]};
+                    return;
+                }
                 if (row >= rows) return;
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
-                    const int feature = 32 * f + 8 * a + 4 * hk;
                     const f32x4 v = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * factor;
-                    if (!whole) {
-                        *reinterpret_cast<f32x4*>(work.sums + slot_row * kValueDim + feature) = v;
-                    } else if (p.output_dtype == KVIP_DTYPE_FP32) {
-                        *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + out_row * kValueDim + feature) = v;
-                    } else {
-                        *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + feature) =
-                            __builtin_convertvector(v, bf16x4);
-                    }
+                    ta_store(p, out_row * kValueDim + 32 * f + 8 * a + 4 * hk, v);
                 }
             };
             auto put_state = [&](float m, float l) {
-                if (st != 0 || hk != 0 || row >= rows) return;
-                if (!whole) work.state[slot_row] = make_float2(m, l);
-                else if (p.lse != nullptr) p.lse[out_row] = ta_lse(m, l);
+                if (st != 0 || hk != 0) return;
+                if (!whole) work.rows(part, rg)[hn] = make_float2(m, l);
+                else if (p.lse != nullptr && row < rows) p.lse[out_row] = ta_lse(m, l);
             };
             const float l_all = half_sum(l_sum);
             const float m_all = m_run * scale2;  // log2 units from here on
@@ -745,52 +754,62 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     }
 }
 
-// Joins the parts of items that several shares hold: 128 threads of 4 features per row.
+// Joins the parts of items that several shares hold: a workgroup per 32 rows and 32 features, whose waves take
+// every fourth part. A lane holds four features of four quarters for one row, as the parts do; the waves' sums
+// meet in LDS, from where a row's features are stored side by side. Few items of many parts (two requests of
+// 131000 tokens, 9 tokens of 32 heads) and many items of few both have enough waves: with all of an item's
+// parts on one wave the join of the former took 44 us, this way 13.
 template <int R>
 __global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAttnArgs p, int shares) {
-    constexpr int kPer = kTaRows * R / kJoinRows;
+    constexpr int kPitch = 36;
+    __shared__ float s_sums[kTaWaves][kTaRows * kPitch];
+    __shared__ float2 s_state[kTaWaves][kTaRows];  // maximum and sum
     const int tiles = ta_tiles(p.max_nodes * p.heads, R);
-    const int item = blockIdx.x / kPer, b = item / tiles, rt = item % tiles;
+    const int f = blockIdx.x % kBlocks, rg = blockIdx.x / kBlocks % R, item = blockIdx.x / (kBlocks * R);
+    const int b = item / tiles, rt = item % tiles;
     uint32_t err = 0;
     const TaRequest req = ta_request(p, b, &err);
-    const int rows = req.nodes * p.heads;
-    const int local = static_cast<int>(blockIdx.x % kPer) * kJoinRows;
-    if (rt * kTaRows * R + local >= rows) return;
+    const int rows = req.nodes * p.heads, first_row = (rt * R + rg) * kTaRows;
+    if (first_row >= rows) return;
     const TaWork<R> work(p.workspace, shares);
     const int2 of = work.items[item];
     if (of.y <= 1) return;
-    const int f = (threadIdx.x & 127) * 4, row = rt * kTaRows * R + local + (threadIdx.x >> 7);
-    if (row >= rows) return;
-    auto at = [&](int k) {  // the row of share of.x + k's part
-        return (static_cast<size_t>(of.x + k) * 2 + (k == 0 ? 1 : 0)) * kTaRows * R + row % (kTaRows * R);
-    };
-    // The parts' states by the lanes of a wave, 64 at a time, then their sums, several loads under way.
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = lane & 31, kg = lane >> 5;
+    auto part = [&](int k) { return (of.x + k) * 2 + (k == 0 ? 1 : 0); };  // of share of.x + k
     float m = -INFINITY, l = 0.f;
-    for (int k = lane; k < of.y; k += 64) m = fmaxf(m, work.state[at(k)].x);
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first < of.y; first += 64) {
-        float2 state = make_float2(-INFINITY, 0.f);
-        if (first + lane < of.y) state = work.state[at(first + lane)];
+#pragma unroll 4
+    for (int k = w; k < of.y; k += kTaWaves) m = fmaxf(m, work.rows(part(k), rg)[n].x);
+    f32x4 v[4] = {};
+#pragma unroll 4
+    for (int k = w; k < of.y; k += kTaWaves) {
+        const float2 state = work.rows(part(k), rg)[n];
+        const f32x4* sums = work.group(part(k), rg) + f * 4 * 64 + lane;
         const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
         l += weight * state.y;
-        const int count = min(of.y - first, 64);
-#pragma unroll 8
-        for (int k = 0; k < count; ++k) {
-            const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
-            v += wk * *reinterpret_cast<const f32x4*>(work.sums + at(first + k) * kValueDim + f);
-        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a) v[a] += weight * sums[a * 64];
     }
-    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d);
-    v *= l > 0.f || l != l ? 1.f / l : 0.f;
-    const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + row;
-    if (p.output_dtype == KVIP_DTYPE_FP32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + out_row * kValueDim + f) = v;
-    } else {
-        *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + f) = __builtin_convertvector(v, bf16x4);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) *reinterpret_cast<f32x4*>(s_sums[w] + n * kPitch + 8 * a + 4 * kg) = v[a];
+    if (kg == 0) s_state[w][n] = make_float2(m, l);
+    __syncthreads();
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+    if (first_row + r >= rows) return;
+    float most = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTaWaves; ++i) most = fmaxf(most, s_state[i][r].x);
+    f32x4 out = {};
+#pragma unroll
+    for (int i = 0; i < kTaWaves; ++i) {
+        const float2 state = s_state[i][r];
+        const float weight = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - most);
+        sum += weight * state.y;
+        out += weight * *reinterpret_cast<const f32x4*>(s_sums[i] + r * kPitch + c);
     }
-    if (f == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(m, l);
+    const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + first_row + r;
+    ta_store(p, out_row * kValueDim + f * 32 + c, out * (sum > 0.f || sum != sum ? 1.f / sum : 0.f));
+    if (f == 0 && c == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(most, sum);
 }
 
 template <int R>
@@ -798,7 +817,7 @@ void launch_tree(const KvipTreeAttnArgs& a, hipStream_t s) {
     const int shares = ta_shares(a.batch, a.heads, a.max_nodes, a.max_blocks);
     hipLaunchKernelGGL(tree_attention_kernel<R>, dim3(shares), dim3(kTaThreads), 0, s, a);
     const int items = a.batch * ta_tiles(a.max_nodes * a.heads, R);
-    hipLaunchKernelGGL(tree_join_kernel<R>, dim3(items * (kTaRows * R / kJoinRows)), dim3(kTaThreads), 0, s, a, shares);
+    hipLaunchKernelGGL(tree_join_kernel<R>, dim3(items * R * kBlocks), dim3(kTaThreads), 0, s, a, shares);
 }
 
 }  // namespace
