@@ -7,8 +7,9 @@
 // walk (one wave, a lane per token: one gather, then register work) instead of a launch before it,
 // sums its weights in 64 bits and counts itself on the request's ticket; the last one adds up the
 // sums in order, finds the part that holds the place and goes through it again (from the cache).
-// The sums cross workgroups as atomics of agent scope between a release and an acquire of the ticket; as
-// a workgroup writes eight bytes, the release has next to nothing to write back.
+// The sums cross workgroups as atomics of agent scope, which are carried out where all XCDs see them: an
+// exchange whose answer is waited for before the ticket is drawn, and loads after the last ticket. (A
+// release and an acquire around the ticket write back and invalidate the XCD's L2 in every workgroup.)
 #include "kvip_device.h"
 #include "kvip_hip_draft.h"
 
@@ -19,31 +20,35 @@ constexpr int kVerifyThreads = 256;
 constexpr int kPerLane = 16;                              // weights per thread
 constexpr int kPart = kVerifyThreads * kPerLane;          // weights per workgroup
 constexpr int kMaxParts = (1 << 20) / kPart;
+constexpr int kTicketWords = 32;                          // a line per ticket: atomics on one line queue up, 12 ns each
 
 template <typename T> struct Weights;  // 16 bytes of them, at any element address
 template <> struct Weights<float> { typedef float vec __attribute__((ext_vector_type(4), aligned(4))); };
 template <> struct Weights<__bf16> { typedef __bf16 vec __attribute__((ext_vector_type(8), aligned(2))); };
 template <> struct Weights<_Float16> { typedef _Float16 vec __attribute__((ext_vector_type(8), aligned(2))); };
 
-KVIP_DEVICE double shuffle_double(double v, int lane) {
+// The value of lane `lane` (uniform), without an LDS round trip.
+KVIP_DEVICE double lane_double(double v, int lane) {
+    return __builtin_bit_cast(double, readlane64(__builtin_bit_cast(int64_t, v), lane));
+}
+
+// v of the lane that a DPP row shift names, 0 past the row of 16 lanes.
+template <int CTRL>
+KVIP_DEVICE double dpp_double(double v) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = static_cast<uint32_t>(__shfl(static_cast<int>(bits), lane));
-    const uint32_t hi = static_cast<uint32_t>(__shfl(static_cast<int>(bits >> 32), lane));
+    const uint32_t lo = dpp_row<CTRL>(static_cast<uint32_t>(bits)), hi = dpp_row<CTRL>(static_cast<uint32_t>(bits >> 32));
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-KVIP_DEVICE double wave_sum(double v) {
-    for (int d = 32; d > 0; d >>= 1) v += shuffle_double(v, lane_id() ^ d);
-    return v;
-}
-
-// Inclusive running sum over the lanes.
+// Inclusive running sum over the lanes; lane 63 has the whole.
 KVIP_DEVICE double wave_running(double v) {
-    for (int d = 1; d < 64; d <<= 1) {
-        const double before = shuffle_double(v, max(lane_id() - d, 0));
-        if (lane_id() >= d) v += before;
-    }
-    return v;
+    v += dpp_double<0x111>(v);  // row_shr:1
+    v += dpp_double<0x112>(v);
+    v += dpp_double<0x114>(v);
+    v += dpp_double<0x118>(v);
+    const double r0 = lane_double(v, 15), r1 = r0 + lane_double(v, 31), r2 = r1 + lane_double(v, 47);
+    const int row = lane_id() >> 4;
+    return v + (row == 0 ? 0.0 : row == 1 ? r0 : row == 2 ? r1 : r2);
 }
 
 struct Walk {
@@ -82,12 +87,12 @@ KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, 
     unsigned long long tried;
     for (;;) {  // at most n rounds: a child comes after its parent
         tried = __ballot(child && up == at);
-        const double u = shuffle_double(uniform, at);
+        const double u = lane_double(uniform, at);
         int next = -1;
         if (draft != nullptr) {
             const int c = at + 1;
             if (tried != 0) {
-                const double q = shuffle_double(drawn, c), t = shuffle_double(mine, c);
+                const double q = lane_double(drawn, c), t = lane_double(mine, c);
                 if (u * q < t) next = c;
             }
             // A token outside the vocabulary is refused too.
@@ -97,9 +102,9 @@ KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, 
             unsigned long long left = tried;
             while (left != 0) {
                 const int c = __ffsll(left) - 1;
-                const int64_t name = static_cast<int64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(token), c)));
+                const int64_t name = __builtin_amdgcn_readlane(static_cast<int>(token), c);  // named: below 2^20
                 left &= ~__ballot(child && up == at && token == name);  // named again: nothing left
-                const double high = low + shuffle_double(mine, c);
+                const double high = low + lane_double(mine, c);
                 if (low <= u && u < high) {
                     next = c;
                     break;
@@ -208,16 +213,18 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
 #pragma unroll
         for (int e = 0; e < kLoad; ++e) sum += x[e];
     }
-    sum = wave_sum(sum);
-    if (lane == 0) s_wave[wave] = sum;
+    sum = wave_running(sum);
+    if (lane == 63) s_wave[wave] = sum;
     __syncthreads();
     double* sums = static_cast<double*>(p.workspace) + static_cast<int64_t>(b) * gridDim.x;
-    uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<double*>(p.workspace) + static_cast<int64_t>(p.batch) * gridDim.x) + b;
+    uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<double*>(p.workspace) + static_cast<int64_t>(p.batch) * gridDim.x) +
+                       b * kTicketWords;
     if (tid == 0) {
         const double whole = (s_wave[0] + s_wave[1]) + (s_wave[2] + s_wave[3]);
-        __hip_atomic_store(reinterpret_cast<uint64_t*>(sums + part), __builtin_bit_cast(uint64_t, whole), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-        s_last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        uint64_t before = __hip_atomic_exchange(reinterpret_cast<uint64_t*>(sums + part), __builtin_bit_cast(uint64_t, whole),
+                                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" : "+v"(before));  // the exchange has been done
+        s_last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
         if (s_last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
@@ -309,7 +316,8 @@ int verify_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
 
 extern "C" uint64_t kvip_hip_verify_drafts_workspace_bytes(int32_t batch, int32_t vocab) {
     if (batch < 1 || vocab < 1) return 0;
-    return static_cast<uint64_t>(batch) * kvip::verify_parts(vocab) * sizeof(double) + (batch + 1) / 2 * 8;
+    return static_cast<uint64_t>(batch) * kvip::verify_parts(vocab) * sizeof(double) +
+           static_cast<uint64_t>(batch) * kvip::kTicketWords * sizeof(uint32_t);
 }
 
 extern "C" uint32_t kvip_hip_verify_drafts(const KvipVerifyArgs* a, void* stream) {
