@@ -88,11 +88,10 @@ class PageTables:
         [max_tokens] names every row's parent within its request (-1: none) where the tokens are trees of
         at most 64: positions then follow the depth, and `visible` gets each token's ancestors and itself.
         Returns (cu_seqlens, slots, positions)."""
-        a = abi.PageTableArgs.from_buffer_copy(self._args)
+        a = self._args  # copied by the launch
         a.counts = self._ints(counts, (self.batch,), "counts")
-        if parents is not None:
-            a.parents = self._ints(parents, (self.max_tokens,), "parents")
-            a.visible = self.visible.data_ptr()
+        a.parents = 0 if parents is None else self._ints(parents, (self.max_tokens,), "parents")
+        a.visible = 0 if parents is None else self.visible.data_ptr()
         abi.launch(self.torch, self.device, self.library.kvip_hip_page_tables_extend, a, "page tables")
         return self.cu_seqlens, self.slots, self.positions
 
@@ -101,7 +100,7 @@ class PageTables:
         the pages of the rest. path int32 [batch, places], as kvip_amd.DraftVerifier returns it, names the
         kept tokens of trees: their rows in `caches` are copied together first (without it the first
         kept[b] are kept). Returns lengths."""
-        a = abi.PageTableArgs.from_buffer_copy(self._args)
+        a = self._args  # copied by the launch
         a.targets, a.kept = self._ints(kept, (self.batch,), "kept"), 1
         if path is not None:
             abi.require(path.dim() == 2 and path.shape[1] >= 1, f"path must be int32 [{self.batch}, places]")
@@ -114,7 +113,7 @@ class PageTables:
         """Cuts request b to lengths[b] tokens (int32 [batch] on the device; one that is not shorter
         sets a status bit where it is longer) and gives back the pages that nothing needs; 0 ends a
         request. Pages come back in the order that undoes an `extend` from these lengths. Returns lengths."""
-        a = abi.PageTableArgs.from_buffer_copy(self._args)
-        a.targets = self._ints(lengths, (self.batch,), "lengths")
+        a = self._args  # copied by the launch
+        a.targets, a.kept = self._ints(lengths, (self.batch,), "lengths"), 0
         abi.launch(self.torch, self.device, self.library.kvip_hip_page_tables_truncate, a, "page tables")
         return self.lengths

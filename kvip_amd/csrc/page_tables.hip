@@ -7,9 +7,9 @@
 // over the batch (tokens, pages) are known, every table entry and slot is independent of the others.
 // What bounds it: latency (a few loads, two scans, one launch), then the 16 to 24 bytes written per token.
 // Every workgroup does both scans itself (4 requests per thread, at most 1024) instead of a launch before
-// it, writes the entries of the requests and rows that it takes in turn, and counts itself on a ticket;
-// the last one moves the lengths and the stack's top on, when every other has read them. Nothing
-// that one workgroup wrote is read by another in the same launch, so the ticket needs no fence.
+// it, counts itself on a ticket when it has read the state, and writes the entries of the requests and rows that
+// it takes in turn; the last one on the ticket moves the lengths and the stack's top on. Nothing that one
+// workgroup wrote is read by another in the same launch, so the ticket needs no fence.
 //
 // The ancestors of a tree's tokens (at most 64, one wave per request, one lane per token) come by
 // pointer doubling: after round r a lane's mask holds its nearest 2^r ancestors.
@@ -38,7 +38,8 @@ KVIP_DEVICE int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
 // Counts this workgroup; true in the last one, whose turn it is to write what the others have read.
 KVIP_DEVICE bool last_group(int32_t* ticket) {
     __shared__ int s_last;
-    __syncthreads();  // every read of this workgroup is done
+    __syncthreads();  // every read of the state by this workgroup is done
+    if (gridDim.x == 1) return true;
     if (threadIdx.x == 0) {
         // atomicInc wraps to 0 at the last one: ready for the next call.
         s_last = atomicInc(reinterpret_cast<uint32_t*>(ticket), gridDim.x - 1) == gridDim.x - 1;
@@ -122,7 +123,17 @@ __global__ __launch_bounds__(kTableThreads) void extend_tables_kernel(const Kvip
     if (tid == 0) s.start[p.batch] = static_cast<int>(min(total, static_cast<uint32_t>(p.max_tokens)));
     if (blockIdx.x == 0) report(p.status, err);
     block_exclusive_scan(given, s.wave_sums, &taken);
-    __syncthreads();
+
+    if (last_group(p.ticket)) {
+        for (int b = tid; b <= p.batch; b += kTableThreads) {
+            p.cu_seqlens[b] = s.start[b];
+            if (b == p.batch) break;
+            p.lengths[b] = s.length[b] + s.step[b];
+            p.bases[b] = s.length[b];
+            p.steps[b] = s.step[b];
+        }
+        if (tid == 0) p.free_count[0] = top - static_cast<int>(taken);
+    }
 
     // Table entries of the new pages; with a tree, also everything of its tokens: one wave per request.
     for (int b = blockIdx.x * kTableWaves + wave; b < p.batch; b += gridDim.x * kTableWaves) {
@@ -183,15 +194,6 @@ __global__ __launch_bounds__(kTableThreads) void extend_tables_kernel(const Kvip
         p.positions[t] = position;
         if (p.visible != nullptr) p.visible[t] = 0;
     }
-    if (!last_group(p.ticket)) return;
-    for (int b = tid; b <= p.batch; b += kTableThreads) {
-        p.cu_seqlens[b] = s.start[b];
-        if (b == p.batch) break;
-        p.lengths[b] = s.length[b] + s.step[b];
-        p.bases[b] = s.length[b];
-        p.steps[b] = s.step[b];
-    }
-    if (tid == 0) p.free_count[0] = top - static_cast<int>(taken);
 }
 
 __global__ __launch_bounds__(kTableThreads) void truncate_tables_kernel(const KvipPageTableArgs p) {
@@ -241,7 +243,13 @@ __global__ __launch_bounds__(kTableThreads) void truncate_tables_kernel(const Kv
     const int64_t height = static_cast<int64_t>(top) + freed;
     if (height > p.num_blocks) err |= KVIP_STATUS_BAD_BLOCK;  // pages that are in the stack already
     if (blockIdx.x == 0) report(p.status, err);
-    __syncthreads();
+    if (last_group(p.ticket)) {
+        for (int b = tid; b < p.batch; b += kTableThreads) {
+            p.lengths[b] = p.bases[b] = s.step[b];
+            p.steps[b] = 0;
+        }
+        if (tid == 0) p.free_count[0] = static_cast<int>(min(height, static_cast<int64_t>(p.num_blocks)));
+    }
     for (int b = blockIdx.x * kTableWaves + wave; b < p.batch; b += gridDim.x * kTableWaves) {
         const int first = blocks_of(s.step[b]);
         int32_t* table = p.block_table + static_cast<int64_t>(b) * p.max_blocks;
@@ -251,12 +259,6 @@ __global__ __launch_bounds__(kTableThreads) void truncate_tables_kernel(const Kv
             table[j] = -1;
         }
     }
-    if (!last_group(p.ticket)) return;
-    for (int b = tid; b < p.batch; b += kTableThreads) {
-        p.lengths[b] = p.bases[b] = s.step[b];
-        p.steps[b] = 0;
-    }
-    if (tid == 0) p.free_count[0] = static_cast<int>(min(height, static_cast<int64_t>(p.num_blocks)));
 }
 
 // One workgroup per (request, cache). A thread takes the same 4 bytes of every row, so the rows that it
