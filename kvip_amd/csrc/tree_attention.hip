@@ -58,23 +58,21 @@ constexpr float kTaMargin = 8.0f * kLog2e;
 constexpr int kNopeSlot = kTaTile * kValueDim;
 constexpr int kRopeSlot = kTaTile * 128;
 constexpr int kScaleSlot = kScaleGroups * kTaTile * 4;
+constexpr int kTaSlot = kNopeSlot + kRopeSlot + kScaleSlot;  // nope bytes, rope, scales [group][token] of a tile
 
-// LDS of a workgroup with R row groups: per stream the ring's nope bytes, rope and scales [group][token]; the
-// query's rope fragments; per wave and row visibility bits, later the softmax's state; per wave what its
-// registers have no room for while it works on the next tile's logits. The merge of two
-// streams takes the ring's place at the end.
+// LDS of a workgroup with R row groups: the ring's slots [slot][stream]; the query's rope fragments; per wave and
+// row visibility bits, later the softmax's state; per wave what its registers have no room for while it
+// works on the next tile's logits. The merge of two streams takes the ring's place at the end.
 template <int R>
 struct TaLds {
     static constexpr int kStreams = kTaWaves / R;
-    static constexpr int kRope = kStreams * kTaSlots * kNopeSlot;
-    static constexpr int kScale = kRope + kStreams * kTaSlots * kRopeSlot;
-    static constexpr int kQuery = kScale + kStreams * kTaSlots * kScaleSlot;
+    static constexpr int kQuery = kStreams * kTaSlots * kTaSlot;
     static constexpr int kState = kQuery + R * 4096;
     static constexpr int kKept = kState + kTaWaves * kTaRows * 8;  // per wave a tile's probabilities
     static constexpr int kBytes = kKept + kTaWaves * 4096;
     static constexpr int kMerge = kTaWaves * 4 * 4096;  // 4 blocks of 4 KB per wave
     static_assert(kBytes <= 160 * 1024, "LDS of a CU");
-    static_assert(kStreams == 1 || kMerge <= kRope, "merge buffer in the ring");
+    static_assert(kStreams == 1 || kMerge <= kQuery, "merge buffer in the ring");
 };
 
 __host__ __device__ inline int ta_groups(int heads, int nodes) { return heads * nodes <= 2 * kTaRows ? 2 : 4; }  // R
@@ -274,14 +272,12 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         b_pos = __builtin_amdgcn_readfirstlane(s_found[1]);
     }
     const TaWork<R> work(p.workspace, shares);
-    const uint32_t ring_lds = lds_addr(s_mem + st * kTaSlots * kNopeSlot);
-    const uint32_t rope_lds = lds_addr(s_mem + L::kRope + st * kTaSlots * kRopeSlot);
-    const uint32_t scales_lds = lds_addr(s_mem + L::kScale + st * kTaSlots * kScaleSlot);
+    const uint32_t ring_lds = lds_addr(s_mem) + st * kTaSlot;
+    auto slot_lds = [&](int slot) { return ring_lds + slot * (kStreams * kTaSlot); };
     // Logits are kept as they come and scaled on their way into the exponential. A negative scale turns the
     // query's signs; one of 0 becomes 2^-100, which no logit shows.
     const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(
         __float_as_int(fmaxf(fabsf(p.scale * kLog2e), 0x1p-100f))));
-    const float margin = kTaMargin / scale2;
     const int flip = p.scale < 0.f ? static_cast<int>(0x80008000u) : 0;
     const int row_stride = p.row_stride;
 
@@ -331,11 +327,11 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         // cache's first rows stand in. `logits` zeroes in LDS what is not there.
         constexpr int kShare = kTaTile / R;
         const uint8_t* from = nullptr;
-        int from_slot = 0;
+        uint32_t to = 0;
         auto aim = [&](int t, int page, int slot) {
             const int first = page < 0 ? 0 : (t * kStreams + st) % (kBlockTokens / kTaTile) * kTaTile;
             from = p.kv_cache + max(page, 0) * p.kv_block_stride + static_cast<int64_t>(first + rg * kShare) * row_stride;
-            from_slot = slot;
+            to = slot_lds(slot);
         };
         // The share's loads, in kFetches pieces that are called in order. LDS row i of the nope bytes holds piece
         // s ^ ta_swz(i) at place s, of the rope features (128 bytes) piece s ^ (i / 2 % 8); scales stand as
@@ -346,16 +342,16 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             if (x < kNopeLoads) {  // the share's tokens 2 x and 2 x + 1 (ta_swz is linear over XOR)
                 const int up = ln >> 5;
                 dma16_at(from, up * row_stride + ((ln & 31) ^ ta_swz(up) ^ ta_swz(rg * kShare) ^ ta_swz(2 * x)) * 16,
-                         ring_lds + from_slot * kNopeSlot + rg * (kShare * kValueDim) + x * 1024);
+                         to + rg * (kShare * kValueDim) + x * 1024);
                 from += x + 1 < kNopeLoads ? 2 * row_stride : -(2 * kNopeLoads - 2) * row_stride;
             } else if (x < kNopeLoads + kRopeLoads) {  // tokens 8 y .. 8 y + 7
                 const int y = x - kNopeLoads, v = rg * kRopeLoads + y;
                 dma16_at(from, (ln >> 3) * row_stride + kValueDim + ((ln & 7) ^ (ln >> 4) ^ ((v & 1) * 4)) * 16,
-                         rope_lds + from_slot * kRopeSlot + rg * (kShare * 128) + y * 1024);
+                         to + kNopeSlot + rg * (kShare * 128) + y * 1024);
                 from += y + 1 < kRopeLoads ? 8 * row_stride : -(8 * kRopeLoads - 8 + rg * kShare) * row_stride;
             } else {  // scale groups 2 v and 2 v + 1 of all tokens (with 4 row groups, two of them load the same)
                 const int v = rg & 1;
-                dma4_at(from + 8 * v, (ln & 31) * row_stride + 640 + 4 * (ln >> 5), scales_lds + from_slot * kScaleSlot + v * 256);
+                dma4_at(from + 8 * v, (ln & 31) * row_stride + 640 + 4 * (ln >> 5), to + kNopeSlot + kRopeSlot + v * 256);
             }
         };
         // Every load and LDS access of this wave is done, and of all waves.
@@ -365,21 +361,6 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             asm volatile("" : : : "memory");
         };
 
-        // Queries of the wave's rows (rows past the last read it again; their outputs are not written). Fragment
-        // 2 i + x: features 16 (2 i + kg) + 8 x .. + 7, the half x of the key piece that the lane reads; rope
-        // fragment i: features 16 i + 8 kg .. + 7.
-        v4i qf[32], q_rope[4];
-        uint64_t seen_by = 0;
-        if (busy) {
-            const int n = lane & 31, kg = lane >> 5;
-            const int at = min(first_row + n, rows - 1), node = at / p.heads;
-            const uint16_t* q = p.query + (static_cast<int64_t>(req.begin) * p.heads + at) * kKeyDim;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) qf[i] = *reinterpret_cast<const v4i*>(q + (i >> 1) * 32 + kg * 16 + (i & 1) * 8);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q_rope[i] = *reinterpret_cast<const v4i*>(q + kValueDim + i * 16 + kg * 8);
-            seen_by = p.visible != nullptr ? static_cast<uint64_t>(p.visible[req.begin + node]) : ~0ull >> (63 - node);
-        }
         __syncthreads();  // the LDS of the item before (at first: the line of work) is free
         int page = page_of(t0), page_next = page;
         aim(t0, page, 0);
@@ -407,6 +388,18 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         } else {
             const uint32_t rope_q_lds = lds_addr(s_mem + L::kQuery) + rg * 4096;                 // + lane * 16
             uint64_t* s_seen = reinterpret_cast<uint64_t*>(s_mem + L::kState) + w * kTaRows;  // + row of the wave
+            // Queries of the wave's rows (rows past the last read it again; their outputs are not written). Fragment
+            // 2 i + x: features 16 (2 i + kg) + 8 x .. + 7, the half x of the key piece that the lane reads; rope
+            // fragment i: features 16 i + 8 kg .. + 7.
+            const int at = min(first_row + (lane & 31), rows - 1), node = at / p.heads;
+            const uint16_t* q = p.query + (static_cast<int64_t>(req.begin) * p.heads + at) * kKeyDim + (lane >> 5) * 8;
+            v4i qf[32], q_rope[4];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) qf[i] = *reinterpret_cast<const v4i*>(q + (i >> 1) * 32 + (lane >> 5) * 8 + (i & 1) * 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q_rope[i] = *reinterpret_cast<const v4i*>(q + kValueDim + i * 16);
+            const uint64_t seen_by =
+                p.visible != nullptr ? static_cast<uint64_t>(p.visible[req.begin + node]) : ~0ull >> (63 - node);
             v16f o[kBlocks];
 #pragma unroll
             for (int f = 0; f < kBlocks; ++f) {
@@ -420,11 +413,6 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 qf[i] ^= flip;
                 asm volatile("" : "+v"(qf[i]));
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // the streams of a row group write the same
-                *(__attribute__((address_space(3))) v4i*)(rope_q_lds + lane * 16 + i * 1024) = q_rope[i] ^ flip;
-            }
-            s_seen[lane & 31] = seen_by;
             float m_run = -INFINITY;  // reference maximum of the row
             float l_sum = 0.f;        // this lane's share of its probability sum
             // Probabilities of the tile whose values come next, relative to m_run: in LDS while the logits need the registers.
@@ -445,8 +433,8 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 if (masked || last_tokens(t)) {
                     masked = true;
                     uint32_t nan = 0;
-                    const uint32_t at = ring_lds + slot * kNopeSlot + tn * kValueDim;
-                    const uint32_t sc = scales_lds + slot * kScaleSlot + tk * 2 * kTaTile * 4 + tn * 4;
+                    const uint32_t at = slot_lds(slot) + tn * kValueDim;
+                    const uint32_t sc = slot_lds(slot) + kNopeSlot + kRopeSlot + tk * 2 * kTaTile * 4 + tn * 4;
 #pragma unroll 4
                     for (int i = 0; i < 16; ++i) {
                         const v4i x = *(LdsV4i)(at + (((16 * tk + i) ^ ta_swz(tn)) << 4));
@@ -481,9 +469,9 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                         if (in && (bad >> token & 1)) l_sum = NAN;
                     }
                 }
-                const uint32_t ro = rope_lds + slot * kRopeSlot + tn * 128;
-                const uint32_t ko = ring_lds + slot * kNopeSlot + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
-                const uint32_t sl = scales_lds + slot * kScaleSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
+                const uint32_t ro = slot_lds(slot) + kNopeSlot + tn * 128;
+                const uint32_t ko = slot_lds(slot) + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
+                const uint32_t sl = slot_lds(slot) + kNopeSlot + kRopeSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
                 // Bit 8 of a key's address is its own: pieces 16 and up by an offset.
                 auto key = [&](int i) { return *(LdsV4i)((ko ^ ((i & 7) * 32)) + (i >> 3) * 256); };
                 v4i kr[4];
@@ -560,7 +548,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     mx = half_max(mx);
                     fresh_sum = 0.f;
                 } else if (piece == 1) {
-                    raise = mx > m_run + margin;  // also the first finite maximum
+                    raise = (mx - m_run) * scale2 > kTaMargin;  // also the first finite maximum
                     const float m_new = raise ? mx : m_run;
                     alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * scale2) : raise ? 0.f : 1.f;
                     m_run = m_new;
@@ -582,8 +570,8 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 constexpr bool kSoftmax = decltype(with_softmax)::value;
                 const int ln = fresh(lane), tk = ln >> 5;
                 const int y = (ln & 15) >> 1, vt = 8 * (y >> 2) + 4 * tk + (y & 3);
-                const uint32_t vo = ring_lds + slot * kNopeSlot + vt * kValueDim + ((((ln >> 4) & 1) ^ ta_swz(vt)) << 4) + 8 * (ln & 1);
-                const uint32_t sl = scales_lds + slot * kScaleSlot + 16 * tk;
+                const uint32_t vo = slot_lds(slot) + vt * kValueDim + ((((ln >> 4) & 1) ^ ta_swz(vt)) << 4) + 8 * (ln & 1);
+                const uint32_t sl = slot_lds(slot) + kNopeSlot + kRopeSlot + 16 * tk;
                 auto value = [&](int f, int h) {
                     return __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsI32x2)((vo ^ ((f & 7) * 32)) + (f >> 3) * 256 + h * 16 * kValueDim));
                 };
@@ -640,6 +628,11 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             };
 
             arrive(t0, 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // the streams of a row group write the same
+                *(__attribute__((address_space(3))) v4i*)(rope_q_lds + fresh(lane) * 16 + i * 1024) = q_rope[i] ^ flip;
+            }
+            s_seen[lane & 31] = seen_by;
             logits(t0, 0);
 #pragma unroll
             for (int i = 0; i < 18; ++i) softmax(i);
