@@ -50,7 +50,7 @@ constexpr int kValueDim = 512;
 constexpr int kScaleGroups = 4;
 constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
-constexpr int kMinSteps = 4;                // steps of a share, at least
+constexpr int kMinSteps = 2;                // steps of a share, at least: 900 cache rows take 20.8 us (1: 22.6, 3: 22.4, 4: 23.3)
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kTaMargin = 8.0f * kLog2e;
@@ -75,9 +75,16 @@ struct TaLds {
     static_assert(kStreams == 1 || kMerge <= kQuery, "merge buffer in the ring");
 };
 
-__host__ __device__ inline int ta_groups(int heads, int nodes) { return heads * nodes <= 2 * kTaRows ? 2 : 4; }  // R
-
 __host__ __device__ inline int ta_tiles(int rows, int r) { return (rows + kTaRows * r - 1) / (kTaRows * r); }
+
+// Row groups R. Four halve the cache rows that a workgroup reads per product, two waste less where the rows do not
+// fill a last tile of 128: a row's step costs 1.08 times as much with two (128 heads x 12 tokens on 2000-8192
+// cache rows: 227 us, 210 with four), so they pay where they save one of at most 12 half tiles (32 heads x 9
+// tokens on 131000 cache rows: 231 to 255 us, as the cache lies in memory, 254 with four).
+inline int ta_groups(int heads, int nodes) {
+    const int halves = ta_tiles(heads * nodes, 2), full = 2 * ta_tiles(heads * nodes, 4);
+    return halves * 13 < full * 12 ? 2 : 4;
+}
 
 // Steps of a launch at most (the kernel counts them in 32 bits), and its shares: one workgroup per CU, no more
 // than these steps could fill.
