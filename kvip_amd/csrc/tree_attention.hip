@@ -51,6 +51,7 @@ constexpr int kScaleGroups = 4;
 constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
 constexpr int kMinSteps = 2;                // steps of a share, at least: 900 cache rows take 20.8 us (1: 22.6, 3: 22.4, 4: 23.3)
+constexpr int kJoinGroups = 2048;            // workgroups of the join, at most, where items allow (8 per CU)
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kTaMargin = 8.0f * kLog2e;
@@ -240,15 +241,21 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     // [pos, end), from request b, which starts at b_pos.
     int b;
     uint32_t pos, end, b_pos, quota;
+    TaRequest req;
     {
         constexpr int kPer = KVIP_DRAFT_MAX_BATCH / kTaThreads;
         uint32_t* s_sum = reinterpret_cast<uint32_t*>(s_mem);
-        uint32_t* s_found = s_sum + kTaWaves;  // request, where it starts
+        int* s_found = reinterpret_cast<int*>(s_sum + kTaWaves);  // request, where it starts, what it is
+        TaRequest of[kPer];
         uint32_t cost[kPer], sum = 0, err = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int at = tid * kPer + i;
-            cost[i] = at < p.batch ? ta_cost<R>(p, ta_request(p, at, &err)) : 0u;
+            cost[i] = 0;
+            if (at < p.batch) {
+                of[i] = ta_request(p, at, &err);
+                cost[i] = ta_cost<R>(p, of[i]);
+            }
             sum += cost[i];
         }
         if (blockIdx.x == 0) report(p.status, err);
@@ -270,6 +277,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             if (before <= pos && pos < before + cost[i]) {
                 s_found[0] = tid * kPer + i;
                 s_found[1] = before;
+                *reinterpret_cast<TaRequest*>(s_found + 2) = of[i];
             }
             before += cost[i];
         }
@@ -277,6 +285,11 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         if (pos >= end) return;  // the whole workgroup: more shares than steps
         b = __builtin_amdgcn_readfirstlane(s_found[0]);
         b_pos = __builtin_amdgcn_readfirstlane(s_found[1]);
+        const TaRequest* found = reinterpret_cast<const TaRequest*>(s_found + 2);
+        req.begin = __builtin_amdgcn_readfirstlane(found->begin);
+        req.nodes = __builtin_amdgcn_readfirstlane(found->nodes);
+        req.past = __builtin_amdgcn_readfirstlane(found->past);
+        req.length = __builtin_amdgcn_readfirstlane(found->length);
     }
     const TaWork<R> work(p.workspace, shares);
     const uint32_t ring_lds = lds_addr(s_mem) + st * kTaSlot;
@@ -291,7 +304,6 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     while (pos < end) {
         // The item at `pos`: request b, row tile rt, steps t0 .. t1 of its `steps`.
         uint32_t err = 0;
-        TaRequest req = ta_request(p, b, &err);
         uint32_t cost = ta_cost<R>(p, req);
         while (pos >= b_pos + cost) {  // ends at the request that holds pos, as pos < end <= the line's length
             b_pos += cost;
@@ -426,7 +438,8 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             const uint32_t kept_lds = lds_addr(s_mem + L::kKept) + w * 4096;
             v16f s;                   // logits
 
-            constexpr int kAhead = 3;  // LDS reads stand so many products before their use, conversions one
+            auto landed = [] { __builtin_amdgcn_s_waitcnt(0xC07F); };  // lgkmcnt(0): one wait for the reads before
+            constexpr int kAhead = 3;  // LDS reads stand two or three products before their use, in pairs, conversions one
             // Logits of step t's tile, in slot `slot`; the loads of the tile that is aimed at stand between the products.
             auto logits = [&](int t, int slot) {
                 const int ln = fresh(lane), tn = ln & 31, tk = ln >> 5;
@@ -476,36 +489,42 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                         if (in && (bad >> token & 1)) l_sum = NAN;
                     }
                 }
-                const uint32_t ro = slot_lds(slot) + kNopeSlot + tn * 128;
-                const uint32_t ko = slot_lds(slot) + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
+                const uint32_t ro = slot_lds(slot) + kNopeSlot + tn * 128 + ((tk ^ ((tn >> 1) & 7)) << 4);
+                uint32_t ko = slot_lds(slot) + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
                 const uint32_t sl = slot_lds(slot) + kNopeSlot + kRopeSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
                 // Bit 8 of a key's address is its own: pieces 16 and up by an offset.
                 auto key = [&](int i) { return *(LdsV4i)((ko ^ ((i & 7) * 32)) + (i >> 3) * 256); };
-                v4i kr[4];
                 v16f dot[2];
                 // A quarter of a group's dot products (tokens 8 a + 4 kg .. + 3) joins the logits a group later, its
                 // scales are read a little before that.
-                f32x4 s4[3];
-                auto scales = [&](int q) { s4[q % 3] = *(LdsF32x4)(sl + ((q >> 2) * kTaTile + 8 * (q & 3)) * 4); };
+                f32x4 s4[16];
+                auto scales = [&](int q) { s4[q] = *(LdsF32x4)(sl + ((q >> 2) * kTaTile + 8 * (q & 3)) * 4); };
                 auto join = [&](int q) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int e = 4 * (q & 3) + c;
-                        s[e] = fmaf(dot[q >> 2 & 1][e], s4[q % 3][c], s[e]);
+                        s[e] = fmaf(dot[q >> 2 & 1][e], s4[q][c], s[e]);
                     }
                 };
-#pragma unroll
-                for (int i = 0; i < 4; ++i) kr[i] = *(LdsV4i)(ro + (((2 * i + tk) ^ ((tn >> 1) & 7)) << 4));
                 {
                     v4i kb[kAhead + 1];
+                    {
+                        const uint32_t yo = fresh(rope_q_lds + ln * 16);
+                        v4i kr[4], yr[4];
 #pragma unroll
-                    for (int i = 0; i < kAhead; ++i) kb[i] = key(i);
+                        for (int i = 0; i < 4; ++i) {
+                            kr[i] = *(LdsV4i)(ro ^ (i * 32));
+                            yr[i] = *(LdsV4i)(yo + i * 1024);
+                        }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+                        for (int i = 0; i < kAhead; ++i) kb[i] = key(i);
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const v4i y = *(LdsV4i)(rope_q_lds + ln * 16 + i * 1024);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), __builtin_bit_cast(bf16x8, y), s, 0, 0, 0);
+                        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), __builtin_bit_cast(bf16x8, yr[i]), s, 0, 0, 0);
+                        }
                     }
                     bf16x8 ka[2] = {fp8x8_to_bf16(kb[0][0], kb[0][1]), fp8x8_to_bf16(kb[0][2], kb[0][3])};
                     __builtin_amdgcn_sched_barrier(0);
@@ -518,24 +537,37 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                             for (int e = 0; e < 16; ++e) d[e] = 0.f;
                         }
                         d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], __builtin_bit_cast(bf16x8, qf[2 * i]), d, 0, 0, 0);
-                        if (i + kAhead < 16) kb[(i + kAhead) % (kAhead + 1)] = key(i + kAhead);
+                        if ((i & 1) == 0) {
+                            landed();
+                            if (i >= 4) {
+                                scales(i - 4);
+                                scales(i - 3);
+                            }
+#pragma unroll
+                            for (int k = i + kAhead; k < i + kAhead + 2 && k < 16; ++k) {
+                                if (k == 8) ko = fresh(ko);  // rather than hold eight addresses
+                                kb[k % (kAhead + 1)] = key(k);
+                            }
+                        }
                         const v4i x = kb[(i + 1) % (kAhead + 1)];
                         if (i < 15) ka[0] = fp8x8_to_bf16(x[0], x[1]);
                         if (i % kEvery == 0 && i / kEvery < kFetches) fetch(i / kEvery, ln);
                         __builtin_amdgcn_sched_barrier(0);
                         d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[1], __builtin_bit_cast(bf16x8, qf[2 * i + 1]), d, 0, 0, 0);
                         if (i < 15) ka[1] = fp8x8_to_bf16(x[2], x[3]);
-                        if (i >= 4) join(i - 4);
-                        if (i >= 2) scales(i - 2);
+                        if (i >= 4 && (i & 1) == 1) {
+                            join(i - 5);
+                            join(i - 4);
+                        }
+                        if (i == 15) {
+#pragma unroll
+                            for (int q = 12; q < 16; ++q) scales(q);
+                        }
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                join(12);
-                scales(14);
-                join(13);
-                scales(15);
-                join(14);
-                join(15);
+#pragma unroll
+                for (int q = 12; q < 16; ++q) join(q);
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -563,6 +595,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 } else {
                     s[piece - 2] = __builtin_amdgcn_exp2f(fmaf(s[piece - 2], scale2, bias));
                     fresh_sum += s[piece - 2];
+                    if ((piece & 1) == 1) asm volatile("" : "+v"(fresh_sum));  // here, not behind the products
                 }
             };
             auto take = [&] {  // the softmax's results become those of the tile whose values come next
@@ -605,18 +638,22 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) weigh(q);
-                scales(4);
-                scales(5);
                 bf16x8 va[2] = {fp8x8_to_bf16(vb[0][0][0], vb[0][0][1]), fp8x8_to_bf16(vb[0][1][0], vb[0][1][1])};
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int f = 0; f < kBlocks; ++f) {
-                    const int gr = f >> 2, next = (f + 1) % (kAhead + 1), far = (f + kAhead) % (kAhead + 1);
+                    const int gr = f >> 2, next = (f + 1) % (kAhead + 1);
                     hold(o[f]);
                     o[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[0], __builtin_bit_cast(bf16x8, pb[gr & 1][0]), o[f], 0, 0, 0);
-                    if (f + kAhead < kBlocks) {
-                        vb[far][0] = value(f + kAhead, 0);
-                        vb[far][1] = value(f + kAhead, 1);
+                    if ((f & 1) == 0) {
+                        landed();
+#pragma unroll
+                        for (int q = f + 4; q < f + 6 && q < 16; ++q) scales(q);
+#pragma unroll
+                        for (int k = f + kAhead; k < f + kAhead + 2 && k < kBlocks; ++k) {
+                            vb[k % (kAhead + 1)][0] = value(k, 0);
+                            vb[k % (kAhead + 1)][1] = value(k, 1);
+                        }
                     }
                     if (f + 1 < kBlocks) va[0] = fp8x8_to_bf16(vb[next][0][0], vb[next][0][1]);
                     if (kSoftmax) softmax(f);
@@ -624,8 +661,10 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     o[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[1], __builtin_bit_cast(bf16x8, pb[gr & 1][1]), o[f], 0, 0, 0);
                     hold(o[f]);
                     if (f + 1 < kBlocks) va[1] = fp8x8_to_bf16(vb[next][1][0], vb[next][1][1]);
-                    if (f + 4 < 16) weigh(f + 4);
-                    if (f + 6 < 16) scales(f + 6);
+                    if ((f & 1) == 1) {
+#pragma unroll
+                        for (int q = f + 3; q < f + 5 && q < 16; ++q) weigh(q);
+                    }
                     if (kSoftmax && f == kBlocks - 1) {
                         softmax(16);
                         softmax(17);
@@ -756,60 +795,65 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
 
 // Joins the parts of items that several shares hold: a workgroup per 32 rows and 32 features, whose waves take
 // every fourth part. A lane holds four features of four quarters for one row, as the parts do; the waves' sums
-// meet in LDS, from where a row's features are stored side by side. Few items of many parts (two requests of
+// meet in LDS, from where a row's features are stored side by side. It goes on to the features `slices` blocks
+// further, so that many items do not make for many workgroups that find nothing. Few items of many parts (two requests of
 // 131000 tokens, 9 tokens of 32 heads) and many items of few both have enough waves: with all of an item's
 // parts on one wave the join of the former took 44 us, this way 13.
 template <int R>
-__global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAttnArgs p, int shares) {
+__global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAttnArgs p, int shares, int slices) {
     constexpr int kPitch = 36;
     __shared__ float s_sums[kTaWaves][kTaRows * kPitch];
     __shared__ float2 s_state[kTaWaves][kTaRows];  // maximum and sum
     const int tiles = ta_tiles(p.max_nodes * p.heads, R);
-    const int f = blockIdx.x % kBlocks, rg = blockIdx.x / kBlocks % R, item = blockIdx.x / (kBlocks * R);
+    const int slice = blockIdx.x % slices, rg = blockIdx.x / slices % R, item = blockIdx.x / slices / R;
     const int b = item / tiles, rt = item % tiles;
+    const TaWork<R> work(p.workspace, shares);
+    const int2 of = work.items[item];  // where the item has rows
     uint32_t err = 0;
     const TaRequest req = ta_request(p, b, &err);
     const int rows = req.nodes * p.heads, first_row = (rt * R + rg) * kTaRows;
     if (first_row >= rows) return;
-    const TaWork<R> work(p.workspace, shares);
-    const int2 of = work.items[item];
     if (of.y <= 1) return;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int n = lane & 31, kg = lane >> 5;
     auto part = [&](int k) { return (of.x + k) * 2 + (k == 0 ? 1 : 0); };  // of share of.x + k
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;
 #pragma unroll 4
     for (int k = w; k < of.y; k += kTaWaves) m = fmaxf(m, work.rows(part(k), rg)[n].x);
-    f32x4 v[4] = {};
-#pragma unroll 4
-    for (int k = w; k < of.y; k += kTaWaves) {
-        const float2 state = work.rows(part(k), rg)[n];
-        const f32x4* sums = work.group(part(k), rg) + f * 4 * 64 + lane;
-        const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
-        l += weight * state.y;
-#pragma unroll
-        for (int a = 0; a < 4; ++a) v[a] += weight * sums[a * 64];
-    }
-#pragma unroll
-    for (int a = 0; a < 4; ++a) *reinterpret_cast<f32x4*>(s_sums[w] + n * kPitch + 8 * a + 4 * kg) = v[a];
-    if (kg == 0) s_state[w][n] = make_float2(m, l);
-    __syncthreads();
     const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
-    if (first_row + r >= rows) return;
-    float most = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTaWaves; ++i) most = fmaxf(most, s_state[i][r].x);
-    f32x4 out = {};
-#pragma unroll
-    for (int i = 0; i < kTaWaves; ++i) {
-        const float2 state = s_state[i][r];
-        const float weight = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - most);
-        sum += weight * state.y;
-        out += weight * *reinterpret_cast<const f32x4*>(s_sums[i] + r * kPitch + c);
-    }
     const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + first_row + r;
-    ta_store(p, out_row * kValueDim + f * 32 + c, out * (sum > 0.f || sum != sum ? 1.f / sum : 0.f));
-    if (f == 0 && c == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(most, sum);
+    for (int f = slice; f < kBlocks; f += slices) {
+        float l = 0.f;
+        f32x4 v[4] = {};
+#pragma unroll 4
+        for (int k = w; k < of.y; k += kTaWaves) {
+            const float2 state = work.rows(part(k), rg)[n];
+            const f32x4* sums = work.group(part(k), rg) + f * 4 * 64 + lane;
+            const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
+            l += weight * state.y;
+#pragma unroll
+            for (int a = 0; a < 4; ++a) v[a] += weight * sums[a * 64];
+        }
+        if (f != slice) __syncthreads();  // the sums before are read
+#pragma unroll
+        for (int a = 0; a < 4; ++a) *reinterpret_cast<f32x4*>(s_sums[w] + n * kPitch + 8 * a + 4 * kg) = v[a];
+        if (kg == 0) s_state[w][n] = make_float2(m, l);
+        __syncthreads();
+        float most = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kTaWaves; ++i) most = fmaxf(most, s_state[i][r].x);
+        f32x4 out = {};
+#pragma unroll
+        for (int i = 0; i < kTaWaves; ++i) {
+            const float2 state = s_state[i][r];
+            const float weight = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - most);
+            sum += weight * state.y;
+            out += weight * *reinterpret_cast<const f32x4*>(s_sums[i] + r * kPitch + c);
+        }
+        if (first_row + r >= rows) continue;
+        ta_store(p, out_row * kValueDim + f * 32 + c, out * (sum > 0.f || sum != sum ? 1.f / sum : 0.f));
+        if (f == 0 && c == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(most, sum);
+    }
 }
 
 template <int R>
@@ -817,7 +861,9 @@ void launch_tree(const KvipTreeAttnArgs& a, hipStream_t s) {
     const int shares = ta_shares(a.batch, a.heads, a.max_nodes, a.max_blocks);
     hipLaunchKernelGGL(tree_attention_kernel<R>, dim3(shares), dim3(kTaThreads), 0, s, a);
     const int items = a.batch * ta_tiles(a.max_nodes * a.heads, R);
-    hipLaunchKernelGGL(tree_join_kernel<R>, dim3(items * R * kBlocks), dim3(kTaThreads), 0, s, a, shares);
+    int slices = kBlocks;
+    while (slices > 1 && items * R * slices > kJoinGroups) slices /= 2;
+    hipLaunchKernelGGL(tree_join_kernel<R>, dim3(items * R * slices), dim3(kTaThreads), 0, s, a, shares, slices);
 }
 
 }  // namespace
