@@ -293,7 +293,6 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     }
     const TaWork<R> work(p.workspace, shares);
     const uint32_t ring_lds = lds_addr(s_mem) + st * kTaSlot;
-    auto slot_lds = [&](int slot) { return ring_lds + slot * (kStreams * kTaSlot); };
     // Logits are kept as they come and scaled on their way into the exponential. A negative scale turns the
     // query's signs; one of 0 becomes 2^-100, which no logit shows.
     const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         int held = table[min(held_first + lane, p.max_blocks - 1)];
         auto page_of = [&](int t) {
             const int tile = t * kStreams + st, at = tile / (kBlockTokens / kTaTile);
-            if (t >= t1 || tile * kTaTile >= req.length) return -1;
+            if (tile * kTaTile >= req.length) return -1;
             if (at >= held_first + 64) {
                 held_first = at;
                 held = table[min(at + lane, p.max_blocks - 1)];
@@ -341,16 +340,21 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             err |= KVIP_STATUS_BAD_BLOCK;
             return -1;
         };
-        // The tile under way: the first row of this wave's share (1 / R) of its tokens, and its LDS slot. A tile is
+        // The tile to load: the first row of this wave's share (1 / R) of its tokens, and its LDS slot. A tile is
         // part of one page, so its 32 rows are in the cache, whatever the length; where there is no page the
-        // cache's first rows stand in. `logits` zeroes in LDS what is not there.
-        constexpr int kShare = kTaTile / R;
-        const uint8_t* from = nullptr;
-        uint32_t to = 0;
-        auto aim = [&](int t, int page, int slot) {
-            const int first = page < 0 ? 0 : (t * kStreams + st) % (kBlockTokens / kTaTile) * kTaTile;
-            from = p.kv_cache + max(page, 0) * p.kv_block_stride + static_cast<int64_t>(first + rg * kShare) * row_stride;
-            to = slot_lds(slot);
+        // cache's first ones stand in. `logits` zeroes in LDS what is not there.
+        constexpr int kShare = kTaTile / R, kPageSteps = kBlockTokens / (kTaTile * kStreams);
+        const uint8_t *tile_from, *from;
+        uint32_t to, to_rope;
+        auto into = [&](uint32_t slot) {
+            from = tile_from;
+            to = slot + rg * (kShare * kValueDim);
+            to_rope = slot + kNopeSlot + rg * (kShare * 128);
+            asm volatile("" : "+s"(to), "+s"(to_rope));
+        };
+        auto aim = [&](int t, int page) {
+            const int first = (t * kStreams + st) % (kBlockTokens / kTaTile) * kTaTile;
+            tile_from = p.kv_cache + max(page, 0) * p.kv_block_stride + static_cast<int64_t>(first + rg * kShare) * row_stride;
         };
         // The share's loads, in kFetches pieces that are called in order. LDS row i of the nope bytes holds piece
         // s ^ ta_swz(i) at place s, of the rope features (128 bytes) piece s ^ (i / 2 % 8); scales stand as
@@ -361,16 +365,16 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             if (x < kNopeLoads) {  // the share's tokens 2 x and 2 x + 1 (ta_swz is linear over XOR)
                 const int up = ln >> 5;
                 dma16_at(from, up * row_stride + ((ln & 31) ^ ta_swz(up) ^ ta_swz(rg * kShare) ^ ta_swz(2 * x)) * 16,
-                         to + rg * (kShare * kValueDim) + x * 1024);
+                         to + x * 1024);
                 from += x + 1 < kNopeLoads ? 2 * row_stride : -(2 * kNopeLoads - 2) * row_stride;
             } else if (x < kNopeLoads + kRopeLoads) {  // tokens 8 y .. 8 y + 7
                 const int y = x - kNopeLoads, v = rg * kRopeLoads + y;
                 dma16_at(from, (ln >> 3) * row_stride + kValueDim + ((ln & 7) ^ (ln >> 4) ^ ((v & 1) * 4)) * 16,
-                         to + kNopeSlot + rg * (kShare * 128) + y * 1024);
+                         to_rope + y * 1024);
                 from += y + 1 < kRopeLoads ? 8 * row_stride : -(8 * kRopeLoads - 8 + rg * kShare) * row_stride;
             } else {  // scale groups 2 v and 2 v + 1 of all tokens (with 4 row groups, two of them load the same)
                 const int v = rg & 1;
-                dma4_at(from + 8 * v, (ln & 31) * row_stride + 640 + 4 * (ln >> 5), to + kNopeSlot + kRopeSlot + v * 256);
+                dma4_at(from + 8 * v, (ln & 31) * row_stride + 640 + 4 * (ln >> 5), to_rope + (kRopeSlot - rg * (kShare * 128) + v * 256));
             }
         };
         // Every load and LDS access of this wave is done, and of all waves.
@@ -382,21 +386,32 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
 
         __syncthreads();  // the LDS of the item before (at first: the line of work) is free
         int page = page_of(t0), page_next = page;
-        aim(t0, page, 0);
+        aim(t0, page);
+        into(ring_lds);
 #pragma unroll
         for (int x = 0; x < kFetches; ++x) fetch(x, lane);
-        // Step t: its tile has landed, and the slot of step t - 2's is free for that of step t + 1, which is aimed at.
-        auto arrive = [&](int t, int slot_free) {
+        // Step t: its tile has landed, and the slot of step t - 2's is free for that of step t + 1 (the last step loads
+        // its own again).
+        auto arrive = [&](int t, uint32_t slot_free) {
             settle();
             page = page_next;
-            page_next = page_of(t + 1);
-            aim(t + 1, page_next, slot_free);
+            if (t + 1 < t1) {
+                if ((t + 1) % kPageSteps == 0) {
+                    page_next = page_of(t + 1);
+                    aim(t + 1, page_next);
+                } else {
+                    tile_from += kTaTile * kStreams * row_stride;
+                }
+            }
+            into(slot_free);
         };
-        auto last_tokens = [&](int t) { return (t + 1) * kStreams * kTaTile > req.past; };  // of the context, or step tokens
+        // Steps with step tokens or the end of the context in them (the same for the workgroup's waves).
+        const int t_last = max(req.past, 0) / (kStreams * kTaTile);
+        constexpr int kSlotStep = kStreams * kTaSlot;
         if (!busy) {  // a row group without rows loads its share of the tiles
             for (int t = t0; t < t1; ++t) {
-                arrive(t, (t + 1 - t0) % kTaSlots);
-                if (last_tokens(t)) lds_sync();
+                arrive(t, ring_lds + (t + 1 - t0) % kTaSlots * kSlotStep);
+                if (t >= t_last) lds_sync();
 #pragma unroll
                 for (int x = 0; x < kFetches; ++x) fetch(x, lane);
             }
@@ -441,20 +456,19 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             auto landed = [] { __builtin_amdgcn_s_waitcnt(0xC07F); };  // lgkmcnt(0): one wait for the reads before
             constexpr int kAhead = 3;  // LDS reads stand two or three products before their use, in pairs, conversions one
             // Logits of step t's tile, in slot `slot`; the loads of the tile that is aimed at stand between the products.
-            auto logits = [&](int t, int slot) {
+            auto logits = [&](int t, uint32_t slot) {
                 const int ln = fresh(lane), tn = ln & 31, tk = ln >> 5;
                 const int first = (t * kStreams + st) * kTaTile;  // position of the tile's first token
                 uint32_t sees = page < 0 ? 0u : 0xFFFFu;          // bit i: the row sees the token of register i
                 bool masked = page < 0;
-                // A step with step tokens or the end of the context in it (the same for the workgroup's waves), or a
-                // tile that is not there. What a row does not see must not reach it, and zero times a NaN would:
+                // A step of the last, or a tile that is not there. What a row does not see must not reach it, and zero times a NaN would:
                 // tokens that are not there, and those with a NaN feature or a scale that is not finite, are
                 // zeroed in LDS, and rows that do see one of the latter become NaN as a whole (their logit is none).
-                if (masked || last_tokens(t)) {
+                if (masked || t >= t_last) {
                     masked = true;
                     uint32_t nan = 0;
-                    const uint32_t at = slot_lds(slot) + tn * kValueDim;
-                    const uint32_t sc = slot_lds(slot) + kNopeSlot + kRopeSlot + tk * 2 * kTaTile * 4 + tn * 4;
+                    const uint32_t at = slot + tn * kValueDim;
+                    const uint32_t sc = slot + kNopeSlot + kRopeSlot + tk * 2 * kTaTile * 4 + tn * 4;
 #pragma unroll 4
                     for (int i = 0; i < 16; ++i) {
                         const v4i x = *(LdsV4i)(at + (((16 * tk + i) ^ ta_swz(tn)) << 4));
@@ -469,7 +483,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     }
                     const uint64_t found = __ballot(nan != 0);
                     const uint32_t bad = static_cast<uint32_t>(found | found >> 32);
-                    if (last_tokens(t)) lds_sync();  // the waves of the stream have all looked (or none needs to)
+                    if (t >= t_last) lds_sync();  // the waves of the stream have all looked (or none needs to)
                     if ((bad >> tn & 1) || page < 0 || first + tn >= req.length) {
 #pragma unroll 1
                         for (int i = 0; i < 16; ++i) {
@@ -489,9 +503,9 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                         if (in && (bad >> token & 1)) l_sum = NAN;
                     }
                 }
-                const uint32_t ro = slot_lds(slot) + kNopeSlot + tn * 128 + ((tk ^ ((tn >> 1) & 7)) << 4);
-                uint32_t ko = slot_lds(slot) + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
-                const uint32_t sl = slot_lds(slot) + kNopeSlot + kRopeSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
+                const uint32_t ro = slot + kNopeSlot + tn * 128 + ((tk ^ ((tn >> 1) & 7)) << 4);
+                uint32_t ko = slot + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
+                const uint32_t sl = slot + kNopeSlot + kRopeSlot + 16 * tk;  // scales of tokens 8 a + 4 kg .. + 3
                 // Bit 8 of a key's address is its own: pieces 16 and up by an offset.
                 auto key = [&](int i) { return *(LdsV4i)((ko ^ ((i & 7) * 32)) + (i >> 3) * 256); };
                 v16f dot[2];
@@ -606,12 +620,12 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 }
             };
             // Values of the tile in slot `slot` [features, rows], the softmax of the next one beside them.
-            auto values = [&](int slot, auto with_softmax) {
+            auto values = [&](uint32_t slot, auto with_softmax) {
                 constexpr bool kSoftmax = decltype(with_softmax)::value;
                 const int ln = fresh(lane), tk = ln >> 5;
                 const int y = (ln & 15) >> 1, vt = 8 * (y >> 2) + 4 * tk + (y & 3);
-                const uint32_t vo = slot_lds(slot) + vt * kValueDim + ((((ln >> 4) & 1) ^ ta_swz(vt)) << 4) + 8 * (ln & 1);
-                const uint32_t sl = slot_lds(slot) + kNopeSlot + kRopeSlot + 16 * tk;
+                const uint32_t vo = slot + vt * kValueDim + ((((ln >> 4) & 1) ^ ta_swz(vt)) << 4) + 8 * (ln & 1);
+                const uint32_t sl = slot + kNopeSlot + kRopeSlot + 16 * tk;
                 auto value = [&](int f, int h) {
                     return __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsI32x2)((vo ^ ((f & 7) * 32)) + (f >> 3) * 256 + h * 16 * kValueDim));
                 };
@@ -673,21 +687,20 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 }
             };
 
-            arrive(t0, 1);
+            uint32_t slot = ring_lds, slot_next = ring_lds + kSlotStep, slot_free = ring_lds + 2 * kSlotStep;
+            arrive(t0, slot_next);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // the streams of a row group write the same
                 *(__attribute__((address_space(3))) v4i*)(rope_q_lds + fresh(lane) * 16 + i * 1024) = q_rope[i] ^ flip;
             }
             s_seen[lane & 31] = seen_by;
-            logits(t0, 0);
+            logits(t0, slot);
 #pragma unroll
             for (int i = 0; i < 18; ++i) softmax(i);
             take();
-            int slot = 0;
 #pragma unroll 1
             for (int t = t0; t + 1 < t1; ++t) {
-                const int slot_next = slot == kTaSlots - 1 ? 0 : slot + 1;
-                arrive(t + 1, slot_next == kTaSlots - 1 ? 0 : slot_next + 1);
+                arrive(t + 1, slot_free);
                 logits(t + 1, slot_next);
                 values(slot, std::true_type{});
                 if (__ballot(raise) != 0ull) {
@@ -699,7 +712,10 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     }
                 }
                 take();
+                const uint32_t used = slot;
                 slot = slot_next;
+                slot_next = slot_free;
+                slot_free = used;
             }
             values(slot, std::false_type{});
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
