@@ -51,6 +51,7 @@ constexpr int kScaleGroups = 4;
 constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
 constexpr int kMinSteps = 2;                // steps of a share, at least: 900 cache rows take 20.8 us (1: 22.6, 3: 22.4, 4: 23.3)
+constexpr int kHeadSteps = 6;               // what an item's start costs, in steps (the queries' loads, the first tile's)
 constexpr int kJoinGroups = 2048;            // workgroups of the join, at most, where items allow (8 per CU)
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
@@ -91,7 +92,7 @@ inline int ta_groups(int heads, int nodes) {
 // than these steps could fill.
 inline int64_t ta_most_steps(int batch, int heads, int nodes, int max_blocks) {
     const int r = ta_groups(heads, nodes), streams = kTaWaves / r;
-    const int64_t steps = (static_cast<int64_t>(max_blocks) * kBlockTokens + kTaTile * streams - 1) / (kTaTile * streams);
+    const int64_t steps = (static_cast<int64_t>(max_blocks) * kBlockTokens + kTaTile * streams - 1) / (kTaTile * streams) + kHeadSteps;
     return steps * batch * ta_tiles(heads * nodes, r);
 }
 inline int ta_shares(int batch, int heads, int nodes, int max_blocks) {
@@ -202,11 +203,6 @@ KVIP_DEVICE int ta_steps(int length) {
     return max((length + kTokens - 1) / kTokens, 1);
 }
 
-template <int R>
-KVIP_DEVICE uint32_t ta_cost(const KvipTreeAttnArgs& p, const TaRequest& q) {
-    return static_cast<uint32_t>(ta_tiles(q.nodes * p.heads, R)) * ta_steps<R>(q.length);
-}
-
 // Direct-to-LDS loads from a wave-uniform address and a lane's offset below 2^32 (see lds_async.h).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -237,49 +233,62 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     const int g = static_cast<int>(blockIdx.x) < per_xcd * 8 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8
                                                              : blockIdx.x;
 
-    // The line of work: steps before each request, 4 requests per thread. Then this share's part of it:
+    // The line of work: steps before each request, 4 requests per thread; an item has its start's cost (`head`, at
+    // most a tenth of a share) before its steps, as shares that start many would end last. This share's part:
     // [pos, end), from request b, which starts at b_pos.
     int b;
-    uint32_t pos, end, b_pos, quota;
+    uint32_t pos, end, b_pos, quota, head;
     TaRequest req;
     {
         constexpr int kPer = KVIP_DRAFT_MAX_BATCH / kTaThreads;
         uint32_t* s_sum = reinterpret_cast<uint32_t*>(s_mem);
-        int* s_found = reinterpret_cast<int*>(s_sum + kTaWaves);  // request, where it starts, what it is
+        uint32_t* s_items = s_sum + kTaWaves;
+        int* s_found = reinterpret_cast<int*>(s_items + kTaWaves);  // request, where it starts, what it is
         TaRequest of[kPer];
-        uint32_t cost[kPer], sum = 0, err = 0;
+        uint32_t tiles[kPer], steps[kPer], sum = 0, items = 0, err = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int at = tid * kPer + i;
-            cost[i] = 0;
+            tiles[i] = steps[i] = 0;
             if (at < p.batch) {
                 of[i] = ta_request(p, at, &err);
-                cost[i] = ta_cost<R>(p, of[i]);
+                tiles[i] = ta_tiles(of[i].nodes * p.heads, R);
+                steps[i] = ta_steps<R>(of[i].length);
             }
-            sum += cost[i];
+            items += tiles[i];
+            sum += tiles[i] * steps[i];
         }
         if (blockIdx.x == 0) report(p.status, err);
-        const uint32_t run = wave_inclusive_scan(sum);
-        if (lane == 63) s_sum[w] = run;
+        const uint32_t run = wave_inclusive_scan(sum), run_items = wave_inclusive_scan(items);
+        if (lane == 63) {
+            s_sum[w] = run;
+            s_items[w] = run_items;
+        }
         __syncthreads();
-        uint32_t before = run - sum, total = 0;
+        uint32_t before = run - sum, before_items = run_items - items, total = 0, all_items = 0;
 #pragma unroll
         for (int v = 0; v < kTaWaves; ++v) {
             before += v < w ? s_sum[v] : 0u;
+            before_items += v < w ? s_items[v] : 0u;
             total += s_sum[v];
+            all_items += s_items[v];
         }
+        head = min(total / shares / 10, static_cast<uint32_t>(kHeadSteps));
+        before += head * before_items;
+        total += head * all_items;
         const uint32_t even = (total + shares - 1) / shares;
         quota = even < kMinSteps ? kMinSteps : even;
         pos = min(g * quota, total);
         end = min(pos + quota, total);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            if (before <= pos && pos < before + cost[i]) {
+            const uint32_t cost = tiles[i] * (steps[i] + head);
+            if (before <= pos && pos < before + cost) {
                 s_found[0] = tid * kPer + i;
                 s_found[1] = before;
                 *reinterpret_cast<TaRequest*>(s_found + 2) = of[i];
             }
-            before += cost[i];
+            before += cost;
         }
         __syncthreads();
         if (pos >= end) return;  // the whole workgroup: more shares than steps
@@ -301,22 +310,27 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     const int row_stride = p.row_stride;
 
     while (pos < end) {
-        // The item at `pos`: request b, row tile rt, steps t0 .. t1 of its `steps`.
+        // The item at `pos`: request b, row tile rt, steps t0 .. t1 of its `steps`, which stand behind its head.
         uint32_t err = 0;
-        uint32_t cost = ta_cost<R>(p, req);
+        auto cost_of = [&](const TaRequest& q) {
+            return static_cast<uint32_t>(ta_tiles(q.nodes * p.heads, R)) * (ta_steps<R>(q.length) + head);
+        };
+        uint32_t cost = cost_of(req);
         while (pos >= b_pos + cost) {  // ends at the request that holds pos, as pos < end <= the line's length
             b_pos += cost;
             req = ta_request(p, ++b, &err);
-            cost = ta_cost<R>(p, req);
+            cost = cost_of(req);
         }
         err = 0;
-        const int steps = ta_steps<R>(req.length);
+        const int steps = ta_steps<R>(req.length), length = steps + head;
         const uint32_t within = pos - b_pos;
-        const int rt = __builtin_amdgcn_readfirstlane(within / steps);
-        const int t0 = __builtin_amdgcn_readfirstlane(within - rt * steps);
-        const int t1 = __builtin_amdgcn_readfirstlane(min(steps, static_cast<int>(t0 + (end - pos))));
-        const uint32_t item_pos = pos - t0;
-        pos += t1 - t0;
+        const int rt = __builtin_amdgcn_readfirstlane(within / length);
+        const int from_at = __builtin_amdgcn_readfirstlane(within - rt * length);
+        const int to_at = __builtin_amdgcn_readfirstlane(min(length, static_cast<int>(from_at + (end - pos))));
+        const uint32_t item_pos = pos - from_at;
+        pos += to_at - from_at;
+        const int t0 = max(from_at - static_cast<int>(head), 0), t1 = to_at - static_cast<int>(head);
+        if (t1 <= 0) break;  // the share ends in the item's head
         const bool whole = t0 == 0 && t1 == steps;
         const int rows = req.nodes * p.heads;
         const int first_row = rt * kTaRows * R + rg * kTaRows;
@@ -803,7 +817,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
         }
         if (lane == 0) report(p.status, err);
         if (t0 == 0 && tid == 0) {  // which shares hold the item
-            const int last = (item_pos + steps - 1) / quota;
+            const int last = (item_pos + length - 1) / quota;
             work.items[static_cast<int64_t>(b) * ta_tiles(p.max_nodes * p.heads, R) + rt] = make_int2(g, last - g + 1);
         }
     }
@@ -848,7 +862,7 @@ __global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAtt
             const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
             l += weight * state.y;
 #pragma unroll
-            for (int a = 0; a < 4; ++a) v[a] += weight * sums[a * 64];
+            for (int a = 0; a < 4; ++a) v[a] += weight * __builtin_nontemporal_load(sums + a * 64);
         }
         if (f != slice) __syncthreads();  // the sums before are read
 #pragma unroll
