@@ -187,6 +187,9 @@ void launch_rotary(const KvipRotaryArgs& a, int run, int64_t groups, hipStream_t
     }
 }
 
+// A launch has fewer than 2^32 threads: longer calls are made in runs of tokens.
+constexpr int64_t kLaunchTokens = 1 << 22;
+
 bool valid_tensor(const KvipRotaryTensor& t, int rotary_dim) {
     if (t.x == nullptr) return t.out == nullptr;
     return t.out && t.heads >= 1 && t.heads <= 65536 && t.dim >= rotary_dim && t.dim <= 65536;
@@ -213,12 +216,23 @@ extern "C" uint32_t kvip_hip_rotary(const KvipRotaryArgs* a, void* stream) {
     const int64_t room = kvip::kRunPairs / (a->rotary_dim / 2);
     const int64_t want = fill < share ? fill : share;
     const int run = static_cast<int>(want < 1 ? 1 : want > room ? room : want);
-    const int64_t groups = (a->tokens + run - 1) / run;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    switch (a->dtype) {
-        case KVIP_DTYPE_BF16: kvip::launch_rotary<__bf16>(*a, run, groups, s); break;
-        case KVIP_DTYPE_FP16: kvip::launch_rotary<_Float16>(*a, run, groups, s); break;
-        default: kvip::launch_rotary<float>(*a, run, groups, s); break;
+    const int64_t size = a->dtype == KVIP_DTYPE_FP32 ? 4 : 2;
+    for (int64_t first = 0; first < a->tokens; first += kvip::kLaunchTokens) {
+        KvipRotaryArgs part = *a;
+        part.positions += first;
+        part.tokens = a->tokens - first < kvip::kLaunchTokens ? a->tokens - first : kvip::kLaunchTokens;
+        for (KvipRotaryTensor& t : part.tensors) {
+            if (t.x == nullptr) continue;
+            t.x = static_cast<const char*>(t.x) + first * t.x_token * size;
+            t.out = static_cast<char*>(t.out) + first * t.out_token * size;
+        }
+        const int64_t groups = (part.tokens + run - 1) / run;
+        switch (a->dtype) {
+            case KVIP_DTYPE_BF16: kvip::launch_rotary<__bf16>(part, run, groups, s); break;
+            case KVIP_DTYPE_FP16: kvip::launch_rotary<_Float16>(part, run, groups, s); break;
+            default: kvip::launch_rotary<float>(part, run, groups, s); break;
+        }
     }
     return static_cast<uint32_t>(hipGetLastError());
 }
@@ -233,13 +247,22 @@ extern "C" uint32_t kvip_hip_store_rows(const KvipRowStoreArgs* a, void* stream)
                     (a->dtype == KVIP_DTYPE_BF16 || a->dtype == KVIP_DTYPE_FP16 || a->dtype == KVIP_DTYPE_FP32);
     if (!ok) return KVIP_ERR_INVALID;
     if (a->tokens == 0) return KVIP_OK;
-    const dim3 grid(static_cast<unsigned>((a->tokens + kvip::kStoreWaves - 1) / kvip::kStoreWaves));
     const dim3 block(kvip::kStoreWaves * 64);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    switch (a->dtype) {
-        case KVIP_DTYPE_BF16: hipLaunchKernelGGL(kvip::store_rows_kernel<__bf16>, grid, block, 0, s, *a); break;
-        case KVIP_DTYPE_FP16: hipLaunchKernelGGL(kvip::store_rows_kernel<_Float16>, grid, block, 0, s, *a); break;
-        default: hipLaunchKernelGGL(kvip::store_rows_kernel<float>, grid, block, 0, s, *a); break;
+    const int64_t size = a->dtype == KVIP_DTYPE_FP32 ? 4 : 2;
+    for (int64_t first = 0; first < a->tokens; first += kvip::kLaunchTokens) {
+        KvipRowStoreArgs part = *a;
+        part.latent = static_cast<const char*>(a->latent) + first * a->latent_stride * size;
+        part.rope = static_cast<const char*>(a->rope) + first * a->rope_stride * size;
+        part.slots += first;
+        if (part.positions != nullptr) part.positions += first;
+        part.tokens = a->tokens - first < kvip::kLaunchTokens ? a->tokens - first : kvip::kLaunchTokens;
+        const dim3 grid(static_cast<unsigned>((part.tokens + kvip::kStoreWaves - 1) / kvip::kStoreWaves));
+        switch (a->dtype) {
+            case KVIP_DTYPE_BF16: hipLaunchKernelGGL(kvip::store_rows_kernel<__bf16>, grid, block, 0, s, part); break;
+            case KVIP_DTYPE_FP16: hipLaunchKernelGGL(kvip::store_rows_kernel<_Float16>, grid, block, 0, s, part); break;
+            default: hipLaunchKernelGGL(kvip::store_rows_kernel<float>, grid, block, 0, s, part); break;
+        }
     }
     return static_cast<uint32_t>(hipGetLastError());
 }
