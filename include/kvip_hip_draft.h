@@ -163,11 +163,14 @@ typedef struct KvipRowStoreArgs {
  *   output = sum_j p_j value_j / sum_j p_j, p_j = exp(s_j - max s), s_j = scale <query, key_j>
  * over the rows it sees (0 where it sees none), lse = log sum_j exp(s_j) (-infinity).
  * Probabilities times a group's scale are rounded once to bf16; the rest is exact or in 32 bits.
- * Rows that a token does not see do not reach its output, whatever they hold. Blocks outside the cache set
+ * Rows that a token does not see do not reach its output, whatever they hold; a token that sees a row with a
+ * NaN or a scale that is not finite becomes NaN as a whole. Blocks outside the cache set
  * KVIP_STATUS_BAD_BLOCK and count as not there; lengths outside 0 .. max_blocks * 128, fewer
  * rows than step tokens or more than max_nodes of these set KVIP_STATUS_BAD_LENGTH (the length is
  * cut to the range, tokens past max_nodes are not computed). Rows of output and lse behind
- * cu_seqlens[batch] are left as they were. */
+ * cu_seqlens[batch] are left as they were. The launch counts steps of 32 rows x 128 (token, head) pairs in 32
+ * bits: where batch * heads * max_nodes * max_blocks could pass that, workspace_bytes is 0 and the
+ * call is refused. A workspace serves one call at a time. */
 typedef struct KvipTreeAttnArgs {
     const uint16_t* query;        /* [max_tokens, heads, 576] bf16, 16-byte aligned */
     const uint8_t* kv_cache;      /* 16-byte aligned */
@@ -180,7 +183,7 @@ typedef struct KvipTreeAttnArgs {
     void* workspace;              /* kvip_hip_tree_attention_workspace_bytes bytes, 16-byte aligned */
     uint32_t* status;             /* optional */
     int64_t kv_block_stride;      /* bytes, >= 128 * row_stride, multiple of 16 */
-    int32_t row_stride;           /* bytes, >= 656, multiple of 16 */
+    int32_t row_stride;           /* bytes, 656..2^24, multiple of 16 */
     int32_t batch;                /* 1..KVIP_DRAFT_MAX_BATCH */
     int32_t heads;                /* 1..128 */
     int32_t max_nodes;            /* 1..KVIP_DRAFT_MAX_NODES */
@@ -188,7 +191,7 @@ typedef struct KvipTreeAttnArgs {
     int32_t max_blocks;           /* 1..2^17 */
     int32_t num_blocks;
     int32_t output_dtype;         /* KVIP_DTYPE_BF16 or _FP32 */
-    float scale;
+    float scale;                  /* finite */
     int32_t reserved;
 } KvipTreeAttnArgs;
 

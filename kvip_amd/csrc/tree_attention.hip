@@ -923,6 +923,7 @@ extern "C" uint32_t kvip_hip_tree_attention(const KvipTreeAttnArgs* a, void* str
                     a->row_stride <= (1 << 24) && a->row_stride % 16 == 0 && a->kv_block_stride % 16 == 0 &&
                     a->kv_block_stride >= static_cast<int64_t>(kvip::kBlockTokens) * a->row_stride &&
                     (a->output_dtype == KVIP_DTYPE_BF16 || a->output_dtype == KVIP_DTYPE_FP32) &&
+                    a->scale - a->scale == 0.f &&  // finite
                     kvip::ta_most_steps(a->batch, a->heads, a->max_nodes, a->max_blocks) <= 0x7FFFFFFF;
     if (!ok) return KVIP_ERR_INVALID;
     const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -9,6 +9,8 @@ states the arithmetic. The reference has no counterpart (its attention is its en
 """
 from __future__ import annotations
 
+import math
+
 from kvip_amd.runtime import abi
 
 BLOCK_TOKENS = 128
@@ -20,7 +22,7 @@ ROW_BYTES = 656
 class TreeAttention:
     """Output [max_tokens, heads, 512] (bf16 or fp32), log-sum-exp float32 [max_tokens, heads] (lse=True) and status
     allocated once; `bind` validates a call's tensors, `__call__` enqueues it on the current stream
-    (capturable). max_nodes: step tokens of a request (1..64); max_context: its cached rows, the step's
+    (capturable; one object's calls follow one another, as they share its workspace). max_nodes: step tokens of a request (1..64); max_context: its cached rows, the step's
     among them."""
 
     def __init__(self, torch, *, batch, heads, max_nodes, max_tokens, max_context, device, output_dtype=None, lse=False):
@@ -41,6 +43,7 @@ class TreeAttention:
         self.library = abi.load_library()
         # Parts of items that several workgroups share, at most two per workgroup.
         nbytes = int(self.library.kvip_hip_tree_attention_workspace_bytes(batch, heads, max_nodes, self.max_blocks))
+        abi.require(nbytes > 0, "batch * heads * max_nodes * max_context is too large for one call")
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.args = None
 
@@ -69,6 +72,7 @@ class TreeAttention:
                                         visible.is_contiguous()), f"visible must be contiguous int64 [{self.max_tokens}]")
         for x in (query, kv_cache, block_table, seq_lens, cu_seqlens, visible):
             abi.require(x is None or x.device == self.device, f"tree attention tensors must be on {self.device}")
+        abi.require(math.isfinite(scale), "scale must be finite")
         p = abi.ptr
         self.args = abi.TreeAttnArgs(
             query=p(query), kv_cache=p(kv_cache), block_table=p(block_table), seq_lens=p(seq_lens), cu_seqlens=p(cu_seqlens),

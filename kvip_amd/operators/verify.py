@@ -13,7 +13,8 @@ from kvip_amd.runtime import abi
 
 class DraftVerifier:
     """out_tokens int64 [batch, max_nodes], kept int32 [batch], path int32 [batch, max_nodes] and status are allocated
-    once; `bind` validates a call's tensors, `__call__` enqueues it on the current stream."""
+    once; `bind` validates a call's tensors, `__call__` enqueues it on the current stream (one object's calls
+    follow one another, as they share its workspace)."""
 
     def __init__(self, torch, *, batch, max_nodes, vocab, device):
         abi.require(1 <= batch <= abi.DRAFT_MAX_BATCH, f"batch must be in 1..{abi.DRAFT_MAX_BATCH}")

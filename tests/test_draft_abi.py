@@ -103,10 +103,13 @@ def test_tree_attention_rejects_before_launch():
         dict(seq_lens=0), dict(cu_seqlens=0), dict(batch=0), dict(batch=1025), dict(heads=0), dict(heads=129),
         dict(max_nodes=0), dict(max_nodes=65), dict(max_tokens=0), dict(max_blocks=0), dict(max_blocks=(1 << 17) + 1),
         dict(num_blocks=0), dict(row_stride=640), dict(row_stride=664), dict(kv_block_stride=128 * 640),
-        dict(output_dtype=abi.DTYPE_FP16)])
+        dict(output_dtype=abi.DTYPE_FP16), dict(row_stride=(1 << 24) + 16, kv_block_stride=1 << 32),
+        dict(scale=float("inf")), dict(scale=float("nan")),
+        dict(batch=1024, heads=128, max_nodes=64, max_blocks=1 << 17)])  # steps that 32 bits do not count
     size = abi.load_library().kvip_hip_tree_attention_workspace_bytes
     assert size(0, 16, 4, 4) == size(2, 129, 4, 4) == size(2, 16, 65, 4) == size(2, 16, 4, 0) == 0
     assert 0 < size(1, 16, 4, 1) < size(64, 16, 4, 1024)
+    assert size(1024, 128, 64, 1 << 17) == 0
 
 
 def test_verification_rejects_before_launch():

@@ -80,6 +80,24 @@ def test_rotary_matches(torch_gpu, dtype, half, tokens, heads, rotary, dim, skip
     assert torch.all(out[..., dim:] == 7.0) and np.array_equal(host(whole[..., skip:]), x)
 
 
+def test_rotary_and_store_of_more_tokens_than_a_launch(torch_gpu):
+    torch = torch_gpu
+    say("case rotary and store of 2^22 + 5 tokens")
+    n = (1 << 22) + 5
+    rotary = kvip_amd.Rotary(torch, rotary_dim=2, device="cuda")
+    x = torch.randn((1, 2), device="cuda").repeat(n, 1)
+    positions = torch.arange(n, device="cuda") % 1000
+    rotary.bind(positions, x)()
+    assert torch.equal(x[1000:], x[:n - 1000]) and not torch.equal(x[0], x[1])
+    kv = torch.zeros((2, 128, ROW), dtype=torch.uint8, device="cuda")
+    latent = torch.randn((1, 576), device="cuda").to(torch.bfloat16).expand(n, 576)
+    slots = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    slots[0], slots[-1] = 7, 200
+    kvip_amd.KvRowStore(torch, kv_cache=kv).bind(latent[:, :512], latent[:, 512:], slots)()
+    flat = kv.view(256, ROW)
+    assert bool(flat[7].any()) and torch.equal(flat[7], flat[200]) and int(flat.any(1).sum()) == 2
+
+
 def test_rotary_inverse_is_the_gradient(torch_gpu):
     """<turn(x), g> = <x, back(g)> for the turn's gradient, and differences of the turned features."""
     torch = torch_gpu
@@ -416,6 +434,31 @@ def test_tree_attention_matches(torch_gpu, heads, counts, contexts):
     assert int(op.status.item()) == 0
 
 
+@pytest.mark.parametrize("heads,requests,longest", [(2, 400, 5000), (96, 48, 8000), (40, 30, 9000)])
+def test_tree_attention_many_long_requests(torch_gpu, heads, requests, longest):
+    """More steps than workgroups take at a time, of requests with shared pages and of some without tokens:
+    shares that start, end and pass through several requests."""
+    torch = torch_gpu
+    say(f"case tree many heads={heads} requests={requests} longest={longest}")
+    rng = np.random.default_rng(heads)
+    step = Step(torch, rng, [1], [127], heads, spare=149, pad=requests + 4)
+    counts = [int(rng.random() < 0.9) * (1 + int(heads == 40 and rng.random() < 0.7)) for _ in range(requests)]
+    lens = [int(rng.integers(n, longest)) if rng.random() < 0.8 else n for n in counts]
+    step.counts, step.lens, step.contexts = counts, lens, [x - n for x, n in zip(lens, counts)]
+    step.table = rng.integers(0, step.pages, (requests, -(-longest // 128))).astype(np.int32)
+    step.cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    step.tokens = int(step.cu[-1]) + 2
+    step.query = torch.from_numpy(rng.standard_normal((step.tokens, heads, 576)).astype(np.float32)).to(torch.bfloat16)
+    step.bits = np.zeros(step.tokens, np.uint64)
+    for b, n in enumerate(counts):
+        step.bits[step.cu[b]:step.cu[b] + n] = [(1 << (i + 1)) - 1 for i in range(n)]
+    op = step.run()
+    step.check(op)
+    assert int(op.status.item()) == 0
+    first = op.output.clone()
+    assert torch.equal(op(), first)  # joined in one order
+
+
 def test_tree_attention_options(torch_gpu):
     """fp32 output without log-sum-exp, padded rows, another scale, more max_nodes than any request has, a
     chain without bits, and the functional form."""
@@ -559,6 +602,11 @@ def test_tree_attention_refuses(torch_gpu):
         for value in values:
             with pytest.raises(ValueError):
                 op.bind(**{**good, name: value})
+    for scale in (float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            op.bind(**good, scale=scale)
+    with pytest.raises(ValueError):  # more steps than 32 bits count
+        kvip_amd.TreeAttention(torch, batch=1024, heads=128, max_nodes=64, max_tokens=1, max_context=1 << 24, device="cuda")
     assert not op.bind(**good)().any()  # a step without tokens
 
 
