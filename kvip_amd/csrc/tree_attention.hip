@@ -522,7 +522,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     uint32_t nan = 0;
                     const uint32_t at = slot + tn * kValueDim;
                     const uint32_t sc = slot + kNopeSlot + kRopeSlot + tk * 2 * kTaTile * 4 + tn * 4;
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const v4i x = *(LdsV4i)(at + (((16 * tk + i) ^ ta_swz(tn)) << 4));
 #pragma unroll
@@ -538,23 +538,23 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     const uint32_t bad = static_cast<uint32_t>(found | found >> 32);
                     if (t >= t_last) lds_sync();  // the waves of the stream have all looked (or none needs to)
                     if ((bad >> tn & 1) || page < 0 || first + tn >= req.length) {
-#pragma unroll 1
+#pragma unroll 4
                         for (int i = 0; i < 16; ++i) {
                             *(__attribute__((address_space(3))) v4i*)(at + (16 * tk + i) * 16) = v4i{0, 0, 0, 0};
                         }
 #pragma unroll
                         for (int i = 0; i < 2; ++i) *(__attribute__((address_space(3))) float*)(sc + i * kTaTile * 4) = 0.f;
                     }
-                    sees = 0;
+                    // Bit j: the row sees the tile's token j. The step's token 0 is the tile's token -d.
                     const uint64_t seen = s_seen[tn];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int token = 8 * (i >> 2) + 4 * tk + (i & 3), rel = first + token - req.past;
-                        const bool in = page >= 0 && (rel < 0 || (rel < KVIP_DRAFT_MAX_NODES && rel < req.length - req.past &&
-                                                                  (seen >> (rel & 63) & 1) != 0));
-                        sees |= in ? 1u << i : 0u;
-                        if (in && (bad >> token & 1)) l_sum = NAN;
-                    }
+                    const int d = first - req.past, left = req.length - first;
+                    uint32_t row_sees = d >= 64 ? 0u : d >= 0 ? static_cast<uint32_t>(seen >> d) : d > -32 ?
+                        static_cast<uint32_t>(seen) << -d | ((1u << -d) - 1) : ~0u;
+                    if (left < 32) row_sees &= left <= 0 ? 0u : (1u << left) - 1;
+                    if (page < 0) row_sees = 0;
+                    if (row_sees & bad) l_sum = NAN;
+                    row_sees >>= 4 * tk;
+                    sees = (row_sees & 0xF) | (row_sees >> 4 & 0xF0) | (row_sees >> 8 & 0xF00) | (row_sees >> 12 & 0xF000);
                 }
                 const uint32_t ro = slot + kNopeSlot + tn * 128 + ((tk ^ ((tn >> 1) & 7)) << 4);
                 uint32_t ko = slot + tn * kValueDim + ((tk ^ ta_swz(tn)) << 4);
