@@ -62,7 +62,7 @@ constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
 constexpr int kMinSteps = 2;                // steps of a share, at least: 900 cache rows take 20.8 us (1: 22.6, 3: 22.4, 4: 23.3)
 constexpr int kHeadSteps = 6;               // what an item's start costs, in steps (the queries' loads, the first tile's)
-constexpr int kJoinGroups = 2048;            // workgroups of the join, at most, where items allow (8 per CU)
+constexpr int kJoinWaves = 8192;            // waves of the join, at most, where items allow
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kTaMargin = 8.0f * kLog2e;
@@ -873,17 +873,18 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     }
 }
 
-// Joins the parts of items that several shares hold: a workgroup per 32 rows and 32 features, whose waves take
-// every fourth part. A lane holds four features of four quarters for one row, as the parts do; the waves' sums
-// meet in LDS, from where a row's features are stored side by side. It goes on to the features `slices` blocks
-// further, so that many items do not make for many workgroups that find nothing. Few items of many parts (two requests of
-// 131000 tokens, 9 tokens of 32 heads) and many items of few both have enough waves: with all of an item's
-// parts on one wave the join of the former took 44 us, this way 13.
-template <int R>
-__global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAttnArgs p, int shares, int slices) {
-    constexpr int kPitch = 36;
-    __shared__ float s_sums[kTaWaves][kTaRows * kPitch];
-    __shared__ float2 s_state[kTaWaves][kTaRows];  // maximum and sum
+// Joins the parts of items that several shares hold. A workgroup of W waves takes 32 rows and U of the 64 units
+// of 8 features at a time; its waves take every W-th part, and meet in LDS, from where a row's features are stored
+// side by side. A lane holds four features of a row per unit, as the parts do. What bounds it is how many
+// loads are under way and how many waves there are to start: few items have many parts, which go over more
+// waves (2 requests of one token, 32 heads, up to 93000 rows: 43.5 us with 8, 49.5 with 4), many items have few and
+// take more units per workgroup, and go on to the units `slices` further (U = 16 with W = 16 and no such loop took
+// 3584 workgroups for 7 requests of 12 tokens x 20 heads, and 48 us instead of 29).
+template <int R, int U, int W>
+__global__ __launch_bounds__(W * 64) void tree_join_kernel(const KvipTreeAttnArgs p, int shares, int slices) {
+    constexpr int kPitch = 65, kAtOnce = 16 / U;  // parts whose loads are issued together
+    __shared__ f32x4 s_sums[W][U * kPitch];
+    __shared__ float2 s_state[W][kTaRows];  // maximum and sum
     const int tiles = ta_tiles(p.max_nodes * p.heads, R);
     const int slice = blockIdx.x % slices, rg = blockIdx.x / slices % R, item = blockIdx.x / slices / R;
     const int b = item / tiles, rt = item % tiles;
@@ -894,56 +895,83 @@ __global__ __launch_bounds__(kTaThreads) void tree_join_kernel(const KvipTreeAtt
     const int rows = req.nodes * p.heads, first_row = (rt * R + rg) * kTaRows;
     if (first_row >= rows) return;
     if (of.y <= 1) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int n = lane & 31, kg = lane >> 5;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 31;
     auto part = [&](int k) { return (of.x + k) * 2 + (k == 0 ? 1 : 0); };  // of share of.x + k
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int k = w; k < of.y; k += kTaWaves) m = fmaxf(m, work.rows(part(k), rg)[n].x);
-    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
-    const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + first_row + r;
-    for (int f = slice; f < kBlocks; f += slices) {
-        float l = 0.f;
-        f32x4 v[4] = {};
-#pragma unroll 4
-        for (int k = w; k < of.y; k += kTaWaves) {
-            const float2 state = work.rows(part(k), rg)[n];
-            const f32x4* sums = work.group(part(k), rg) + f * 4 * 64 + lane;
-            const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
-            l += weight * state.y;
+    for (int unit = slice * U; unit < kBlocks * 4; unit += slices * U) {
+        if (unit != slice * U) __syncthreads();  // the sums before are read
+        float m = -INFINITY, l = 0.f;
+        f32x4 v[U] = {};
+        for (int k0 = w; k0 < of.y; k0 += W * kAtOnce) {
+            float2 state[kAtOnce];
+            f32x4 x[kAtOnce][U];
+            float most = m;
 #pragma unroll
-            for (int a = 0; a < 4; ++a) v[a] += weight * __builtin_nontemporal_load(sums + a * 64);
+            for (int i = 0; i < kAtOnce; ++i) {
+                const int k = k0 + i * W;
+                state[i] = make_float2(-INFINITY, 0.f);
+                if (k < of.y) {
+                    state[i] = work.rows(part(k), rg)[n];
+                    const f32x4* sums = work.group(part(k), rg) + unit * 64 + lane;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) x[i][u] = __builtin_nontemporal_load(sums + u * 64);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) most = fmaxf(most, state[i].x);
+            const float keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - most);
+            l *= keep;
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] *= keep;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (k0 + i * W >= of.y) break;
+                const float weight = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[i].x - most);
+                l += weight * state[i].y;
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] += weight * x[i][u];
+            }
+            m = most;
         }
-        if (f != slice) __syncthreads();  // the sums before are read
 #pragma unroll
-        for (int a = 0; a < 4; ++a) *reinterpret_cast<f32x4*>(s_sums[w] + n * kPitch + 8 * a + 4 * kg) = v[a];
-        if (kg == 0) s_state[w][n] = make_float2(m, l);
+        for (int u = 0; u < U; ++u) s_sums[w][u * kPitch + lane] = v[u];
+        if (lane < kTaRows) s_state[w][n] = make_float2(m, l);
         __syncthreads();
-        float most = -INFINITY, sum = 0.f;
+        for (int i = threadIdx.x; i < kTaRows * U * 2; i += W * 64) {
+            const int r = i / (U * 2), u = i / 2 % U, kg = i % 2;
+            if (first_row + r >= rows) break;
+            float most = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < kTaWaves; ++i) most = fmaxf(most, s_state[i][r].x);
-        f32x4 out = {};
+            for (int k = 0; k < W; ++k) most = fmaxf(most, s_state[k][r].x);
+            f32x4 out = {};
 #pragma unroll
-        for (int i = 0; i < kTaWaves; ++i) {
-            const float2 state = s_state[i][r];
-            const float weight = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - most);
-            sum += weight * state.y;
-            out += weight * *reinterpret_cast<const f32x4*>(s_sums[i] + r * kPitch + c);
+            for (int k = 0; k < W; ++k) {
+                const float2 state = s_state[k][r];
+                const float weight = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - most);
+                sum += weight * state.y;
+                out += weight * s_sums[k][u * kPitch + kg * kTaRows + r];
+            }
+            const int64_t out_row = static_cast<int64_t>(req.begin) * p.heads + first_row + r;
+            ta_store(p, out_row * kValueDim + (unit + u) * 8 + kg * 4, out * (sum > 0.f || sum != sum ? 1.f / sum : 0.f));
+            if (unit + u == 0 && kg == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(most, sum);
         }
-        if (first_row + r >= rows) continue;
-        ta_store(p, out_row * kValueDim + f * 32 + c, out * (sum > 0.f || sum != sum ? 1.f / sum : 0.f));
-        if (f == 0 && c == 0 && p.lse != nullptr) p.lse[out_row] = ta_lse(most, sum);
     }
+}
+
+template <int R, int U, int W>
+void launch_join(const KvipTreeAttnArgs& a, int shares, int groups, hipStream_t s) {
+    int slices = kBlocks * 4 / U;
+    while (slices > 1 && groups * slices * W > kJoinWaves) slices /= 2;
+    hipLaunchKernelGGL((tree_join_kernel<R, U, W>), dim3(groups * slices), dim3(W * 64), 0, s, a, shares, slices);
 }
 
 template <int R>
 void launch_tree(const KvipTreeAttnArgs& a, hipStream_t s) {
     const int shares = ta_shares(a.batch, a.heads, a.max_nodes, a.max_blocks);
     hipLaunchKernelGGL(tree_attention_kernel<R>, dim3(shares), dim3(kTaThreads), 0, s, a);
-    const int items = a.batch * ta_tiles(a.max_nodes * a.heads, R);
-    int slices = kBlocks;
-    while (slices > 1 && items * R * slices > kJoinGroups) slices /= 2;
-    hipLaunchKernelGGL(tree_join_kernel<R>, dim3(items * R * slices), dim3(kTaThreads), 0, s, a, shares, slices);
+    const int groups = a.batch * ta_tiles(a.max_nodes * a.heads, R) * R;
+    if (groups <= 32) launch_join<R, 4, 8>(a, shares, groups, s);
+    else if (groups <= 128) launch_join<R, 4, 4>(a, shares, groups, s);
+    else launch_join<R, 8, 4>(a, shares, groups, s);
 }
 
 }  // namespace
