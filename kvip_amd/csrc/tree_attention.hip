@@ -878,7 +878,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
 // side by side. A lane holds four features of a row per unit, as the parts do. What bounds it is how many
 // loads are under way and how many waves there are to start: few items have many parts, which go over more
 // waves (2 requests of one token, 32 heads, up to 93000 rows: 43.5 us with 8, 49.5 with 4), many items have few and
-// take more units per workgroup, and go on to the units `slices` further (U = 16 with W = 16 and no such loop took
+// take more units per workgroup, and go on to the units `slices` further (U = 1 with W = 16 and no such loop took
 // 3584 workgroups for 7 requests of 12 tokens x 20 heads, and 48 us instead of 29).
 template <int R, int U, int W>
 __global__ __launch_bounds__(W * 64) void tree_join_kernel(const KvipTreeAttnArgs p, int shares, int slices) {
