@@ -434,7 +434,8 @@ def test_tree_attention_matches(torch_gpu, heads, counts, contexts):
     assert int(op.status.item()) == 0
 
 
-@pytest.mark.parametrize("heads,requests,longest", [(2, 400, 5000), (96, 48, 8000), (40, 30, 9000)])
+@pytest.mark.parametrize("heads,requests,longest", [(2, 400, 5000), (96, 48, 8000), (40, 30, 9000), (2, 700, 900), (3, 1024, 400),
+                                                   (40, 2, 30000)])
 def test_tree_attention_many_long_requests(torch_gpu, heads, requests, longest):
     """More steps than workgroups take at a time, of requests with shared pages and of some without tokens:
     shares that start, end and pass through several requests."""
