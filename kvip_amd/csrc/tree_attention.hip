@@ -796,6 +796,23 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                     for (int a = 0; a < 4; ++a) out[(f * 4 + a) * 64] = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]};
                     return;
                 }
+                if (p.output_dtype == KVIP_DTYPE_BF16) {
+                    // The halves of the wave hold every other four features of a row: swapped, each has eight.
+#pragma unroll
+                    for (int a = 0; a < 4; a += 2) {
+                        v4i v;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const auto pair = __builtin_amdgcn_permlane32_swap(
+                                pack_bf16(x[4 * a + 2 * e] * factor, x[4 * a + 2 * e + 1] * factor),
+                                pack_bf16(x[4 * a + 2 * e + 4] * factor, x[4 * a + 2 * e + 5] * factor), false, false);
+                            v[e] = pair[0];
+                            v[e + 2] = pair[1];
+                        }
+                        if (row < rows) *reinterpret_cast<v4i*>(static_cast<__bf16*>(p.output) + out_row * kValueDim + 32 * f + 8 * a + 8 * hk) = v;
+                    }
+                    return;
+                }
                 if (row >= rows) return;
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
