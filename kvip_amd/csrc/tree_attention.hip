@@ -447,7 +447,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             asm volatile("" : : : "memory");
         };
 
-        __syncthreads();  // the LDS of the item before (at first: the line of work) is free
+        lds_sync();  // the LDS of the item before (at first: the line of work) is free; its stores may be under way
         int page = page_of(t0), page_next = page;
         aim(t0, page);
         into(ring_lds);
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             }
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
             if constexpr (kStreams > 1) {  // the barriers of the merge
-                for (int i = 0; i < 5; ++i) __syncthreads();
+                for (int i = 0; i < 5; ++i) lds_sync();
             }
         } else {
             const uint32_t rope_q_lds = lds_addr(s_mem + L::kQuery) + rg * 4096;                 // + lane * 16
@@ -839,9 +839,9 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 // Merge of the two streams: with the maximum M over them, sums = sum_w 2^(m_w - M) o_w and l likewise. A
                 // wave sums half of the blocks, whose other half it puts into LDS, 8 blocks at a time.
                 float2* s_state = reinterpret_cast<float2*>(s_mem + L::kState);
-                __syncthreads();  // every wave is done with its ring and its rows' bits
+                lds_sync();  // every wave is done with its ring and its rows' bits
                 if (hk == 0) s_state[w * kTaRows + hn] = make_float2(m_all, l_all);
-                __syncthreads();
+                lds_sync();
                 const float2 other = s_state[(w ^ R) * kTaRows + hn];
                 const float top = fmaxf(m_all, other.x);
                 const float mine = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_all - top);
@@ -852,7 +852,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                 const uint32_t in_lds = lds_addr(s_mem) + (w ^ R) * 4 * 4096 + le * 16;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (half > 0) __syncthreads();
+                    if (half > 0) lds_sync();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         if (j / 4 == st) continue;
@@ -863,7 +863,7 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
                             *(LdsF32x4Out)(out_lds + ((j & 3) * 4 + a) * 1024) = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * mine;
                         }
                     }
-                    __syncthreads();
+                    lds_sync();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         if (j / 4 != st) continue;
