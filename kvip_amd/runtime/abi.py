@@ -376,14 +376,20 @@ def stream_handle(torch, device) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(torch, device) -> int:
+    """`stream_handle` without a Stream object, which costs 2 of the 6 us of a small call."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return stream_handle(torch, device) if raw is None else raw(device.index)
+
+
 def launch(torch, device, entry, args, what: str) -> None:
     """Calls a C entry with the current stream of `device`, which is made the current device around the
     call where it is not (a stream handle of 0 names the current device's default stream)."""
     if torch.cuda.current_device() == device.index:
-        check(entry(ctypes.byref(args), stream_handle(torch, device)), what)
+        check(entry(ctypes.byref(args), raw_stream(torch, device)), what)
         return
     with torch.cuda.device(device):
-        check(entry(ctypes.byref(args), stream_handle(torch, device)), what)
+        check(entry(ctypes.byref(args), raw_stream(torch, device)), what)
 
 
 def require(ok, what: str) -> None:

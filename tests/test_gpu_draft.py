@@ -881,6 +881,14 @@ def test_a_captured_round_replays(torch_gpu):
             assert torch.equal(a, b), seed
 
 
+def test_calls_take_the_current_stream(torch_gpu):
+    torch = torch_gpu
+    device, side = torch.device("cuda", torch.cuda.current_device()), torch.cuda.Stream()
+    assert abi.raw_stream(torch, device) == abi.stream_handle(torch, device)
+    with torch.cuda.stream(side):
+        assert abi.raw_stream(torch, device) == abi.stream_handle(torch, device) == side.cuda_stream
+
+
 def test_objects_run_side_by_side(torch_gpu):
     """Two engines on two streams at once do not touch one another's workspaces."""
     torch = torch_gpu
