@@ -325,7 +325,8 @@ bool valid_tables(const KvipPageTableArgs* a) {
 }
 
 int table_groups(int batch, int tokens) {
-    const int by_request = (batch + kTableWaves - 1) / kTableWaves, by_row = (tokens + 1023) / 1024;
+    // 512 rows each: 105000 rows take 12.5 us with truncate (1024: 13.3, 256: 13.7, for the tickets).
+    const int by_request = (batch + kTableWaves - 1) / kTableWaves, by_row = (tokens + 511) / 512;
     return by_request > by_row ? by_request : by_row;
 }
 
