@@ -19,9 +19,7 @@
 namespace kvip {
 namespace {
 
-constexpr int kVerifyThreads = 256;
-constexpr int kPerLane = 16;                              // weights per thread
-constexpr int kPart = kVerifyThreads * kPerLane;          // weights per workgroup
+constexpr int kPart = 4096;                                // weights per workgroup
 constexpr int kMaxParts = (1 << 20) / kPart;
 constexpr int kTicketWords = 32;                          // a line per ticket: atomics on one line queue up, 12 ns each
 
@@ -141,12 +139,15 @@ KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, 
     if (lane == 0) p.kept[b] = kept;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerifyArgs p) {
+// THREADS: 512 where all workgroups are on the card at once with that (a thread's weights are added up one after
+// the other: 16 trees over 32000 take 11.1 us, 11.8 with 256), else 256 (64 chains over 131072: 27.0, 28.1 with 512).
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void verify_kernel(const KvipVerifyArgs p) {
+    constexpr int kPerLane = kPart / THREADS;  // weights per thread
     typedef typename Weights<T>::vec V;
     constexpr int kLoad = 16 / sizeof(T);
     __shared__ Walk s_walk;
-    __shared__ double s_wave[kVerifyThreads / 64], s_before, s_left;
+    __shared__ double s_wave[THREADS / 64], s_before, s_left;
     __shared__ int s_last, s_part, s_found, s_near, s_count, s_gone[KVIP_DRAFT_MAX_NODES];
     const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int begin = min(max(p.cu_seqlens[b], 0), p.max_tokens);
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < kPerLane / kLoad; ++j) {
-        const int at = part * kPart + (j * kVerifyThreads + tid) * kLoad;
+        const int at = part * kPart + (j * THREADS + tid) * kLoad;
         double x[kLoad];
         weights(at, x);
         exclude(at, x, s_count, s_gone);
@@ -223,7 +224,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
     uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<double*>(p.workspace) + static_cast<int64_t>(p.batch) * gridDim.x) +
                        b * kTicketWords;
     if (tid == 0) {
-        const double whole = (s_wave[0] + s_wave[1]) + (s_wave[2] + s_wave[3]);
+        double whole = 0.0;
+#pragma unroll
+        for (int k = 0; k < THREADS / 64; ++k) whole += s_wave[k];
         uint64_t before = __hip_atomic_exchange(reinterpret_cast<uint64_t*>(sums + part), __builtin_bit_cast(uint64_t, whole),
                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("" : "+v"(before));  // the exchange has been done
@@ -234,8 +237,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
     if (!s_last) return;
 
     // The part in which the running sum passes the share, and the sum before it: one part per thread
-    // (at most 256), in order.
-    static_assert(kMaxParts <= kVerifyThreads, "a part per thread");
+    // in order.
+    static_assert(kMaxParts <= THREADS, "a part per thread");
     const double mine = tid < static_cast<int>(gridDim.x)
                             ? __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<uint64_t*>(sums + tid),
                                                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) : 0.0;
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
         __syncthreads();
         double before = 0.0, whole = 0.0;
 #pragma unroll
-        for (int k = 0; k < kVerifyThreads / 64; ++k) {
+        for (int k = 0; k < THREADS / 64; ++k) {
             before += k < wave ? s_wave[k] : 0.0;
             whole += s_wave[k];
         }
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
     if (drawable) {
         gather_gone(chosen);
         if (tid == 0) s_near = -1;
-        // In order: 16 weights in a row per thread.
+        // In order: kPerLane weights in a row per thread.
         const int at = chosen * kPart + tid * kPerLane;
         double x[kPerLane], own = 0.0;
 #pragma unroll
@@ -314,6 +317,18 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const KvipVerify
 
 int verify_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
 
+constexpr int kCardWaves = 256 * 32;  // waves that the card holds
+
+template <typename T>
+void launch_verify(const KvipVerifyArgs& a, hipStream_t s) {
+    const dim3 grid(verify_parts(a.vocab), a.batch);
+    if (static_cast<int64_t>(grid.x) * grid.y * (512 / 64) <= kCardWaves) {
+        hipLaunchKernelGGL((verify_kernel<T, 512>), grid, dim3(512), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((verify_kernel<T, 256>), grid, dim3(256), 0, s, a);
+    }
+}
+
 }  // namespace
 }  // namespace kvip
 
@@ -333,12 +348,11 @@ extern "C" uint32_t kvip_hip_verify_drafts(const KvipVerifyArgs* a, void* stream
                     a->probs_stride >= a->vocab && (a->draft_probs == nullptr || a->draft_stride >= a->vocab) &&
                     (a->dtype == KVIP_DTYPE_FP32 || a->dtype == KVIP_DTYPE_BF16 || a->dtype == KVIP_DTYPE_FP16);
     if (!ok) return KVIP_ERR_INVALID;
-    const dim3 grid(kvip::verify_parts(a->vocab), a->batch), block(kvip::kVerifyThreads);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     switch (a->dtype) {
-        case KVIP_DTYPE_FP32: hipLaunchKernelGGL(kvip::verify_kernel<float>, grid, block, 0, s, *a); break;
-        case KVIP_DTYPE_BF16: hipLaunchKernelGGL(kvip::verify_kernel<__bf16>, grid, block, 0, s, *a); break;
-        default: hipLaunchKernelGGL(kvip::verify_kernel<_Float16>, grid, block, 0, s, *a); break;
+        case KVIP_DTYPE_FP32: kvip::launch_verify<float>(*a, s); break;
+        case KVIP_DTYPE_BF16: kvip::launch_verify<__bf16>(*a, s); break;
+        default: kvip::launch_verify<_Float16>(*a, s); break;
     }
     return static_cast<uint32_t>(hipGetLastError());
 }

@@ -673,7 +673,7 @@ def check_verify(case, op, *, nodes, limit=64):
 @pytest.mark.parametrize("drafted", ["chain", "tree", "draft"])
 @pytest.mark.parametrize("dtype,vocab,counts", [("fp32", 1, [1, 3]), ("fp32", 7, [0, 5, 1, 64]), ("bf16", 500, [9] * 20),
                                                 ("fp16", 4096, [3, 17, 2]), ("fp32", 4097, [12] * 6), ("bf16", 100003, [4, 6]),
-                                                ("fp32", 40000, [33] * 3)])
+                                                ("fp32", 40000, [33] * 3), ("bf16", 9001, [1, 3] * 200)])
 def test_verification_matches(torch_gpu, drafted, dtype, vocab, counts):
     torch = torch_gpu
     say(f"case verify {drafted} {dtype} vocab={vocab} counts={counts[:5]}")
