@@ -8,7 +8,7 @@
 // What bounds it: memory (each feature read and written once), latency for a step's few tokens. The
 // angles cost as much as some 40 features, so a workgroup works them out once for a run of tokens
 // into LDS and every head of these tokens takes them from there. 8192 tokens of 64 query
-// heads and a key of 128 features take 59 us (4.6 TB/s; a large copy reaches 5.1), a step of 256 tokens 6 us.
+// heads and a key of 128 features take 59 us (4.6 TB/s; a large copy reaches 5.1), a step of 256 tokens 4.
 #include "kvip_device.h"
 #include "kvip_hip_draft.h"
 

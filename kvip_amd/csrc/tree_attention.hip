@@ -28,7 +28,7 @@
 // TFLOP/s, 125 us at the rate of a large bf16 product): the instructions between the MFMAs, 10 VALU and 1.4 LDS ones
 // per MFMA, 4 of them conversions that each of the four waves does for itself (MFMA busy 38 % of the
 // cycles, waiting 17 %), at the 2.2 to 2.4 GHz that the card holds under this load. Few rows (64
-// requests x 4 tokens x 16 heads on 1000-16384 rows: 127 us, 2.95 TB/s): the same loop at 2.0 GHz beside the
+// requests x 4 tokens x 16 heads on 1000-16384 rows: 126 us, 2.97 TB/s): the same loop at 2.0 GHz beside the
 // loads. Short contexts: a chain of latencies (lengths, page, tile and queries, two steps, join).
 // Dropped after measuring: two waves per SIMD that split the features (310 us for the first of these,
 // which then took 224), the query as two fp8 terms against the key's bytes (261), touching the next
