@@ -12,9 +12,10 @@
 //     (exact), with the query; a scale group's dot products are summed on their own and added as
 //     fma(group, scale, s) in fp32.
 //   - So a lane holds one row's logits of 16 tokens: the softmax takes one lane swap per tile, and the
-//     probabilities times the group's scale (rounded once to bf16) are the value product's operand
-//     without leaving their registers, as the order of tokens along K is free. The value operand (8
-//     tokens of one feature per lane) comes from the token-major tile by transposing LDS reads.
+//     probabilities times the group's scale (rounded once to bf16) are the value product's operand in the
+//     lane that has them, as the order of tokens along K is free (they wait in LDS, in 32 bits, while the
+//     next tile's logits need the registers). The value operand (8 tokens of one feature per lane)
+//     comes from the token-major tile by transposing LDS reads.
 //   - The running maximum is raised lazily, when a tile exceeds it by kTaMargin.
 //   - One wave per SIMD hides nothing by itself, so the tile loop is one stretch of 68 MFMAs with everything
 //     else in between: the logits of tile t + 1, then the values of tile t with the softmax of tile t + 1
