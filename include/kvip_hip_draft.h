@@ -170,7 +170,7 @@ typedef struct KvipRowStoreArgs {
  * cut to the range, tokens past max_nodes are not computed). Rows of output and lse behind
  * cu_seqlens[batch] are left as they were. The launch counts steps of 32 rows x 128 (token, head) pairs in 32
  * bits: where batch * heads * max_nodes * max_blocks could pass that, workspace_bytes is 0 and the
- * call is refused. A workspace serves one call at a time. */
+ * call is refused. A workspace serves one call at a time, and the lengths stay as they are while it runs. */
 typedef struct KvipTreeAttnArgs {
     const uint16_t* query;        /* [max_tokens, heads, 576] bf16, 16-byte aligned */
     const uint8_t* kv_cache;      /* 16-byte aligned */

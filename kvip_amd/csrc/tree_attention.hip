@@ -361,14 +361,15 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             return static_cast<uint32_t>(ta_tiles(q.nodes * p.heads, R)) * length_of(ta_steps<R>(q.length));
         };
         uint32_t cost = cost_of(req);
-        while (pos >= b_pos + cost) {  // ends at the request that holds pos, as pos < end <= the line's length
+        // Ends at the request that holds pos, as pos < end <= the line's length.
+        while (pos >= b_pos + cost && b + 1 < p.batch) {
             b_pos += cost;
             req = ta_request(p, ++b, &err);
             cost = cost_of(req);
         }
         err = 0;
         const int steps = ta_steps<R>(req.length), length = length_of(steps);
-        const uint32_t within = pos - b_pos;
+        const uint32_t within = min(pos - b_pos, max(cost, 1u) - 1);
         const int rt = __builtin_amdgcn_readfirstlane(within / length);
         const int from_at = __builtin_amdgcn_readfirstlane(within - rt * length);
         const int to_at = __builtin_amdgcn_readfirstlane(min(length, static_cast<int>(from_at + (end - pos))));
@@ -907,7 +908,8 @@ __global__ __launch_bounds__(W * 64) void tree_join_kernel(const KvipTreeAttnArg
     const int slice = blockIdx.x % slices, rg = blockIdx.x / slices % R, item = blockIdx.x / slices / R;
     const int b = item / tiles, rt = item % tiles;
     const TaWork<R> work(p.workspace, shares);
-    const int2 of = work.items[item];  // where the item has rows
+    int2 of = work.items[item];  // where the item has rows
+    of.y = static_cast<unsigned>(of.x) < static_cast<unsigned>(shares) ? min(of.y, shares - of.x) : 0;
     uint32_t err = 0;
     const TaRequest req = ta_request(p, b, &err);
     const int rows = req.nodes * p.heads, first_row = (rt * R + rg) * kTaRows;
