@@ -62,8 +62,8 @@ typedef struct KvipPagedRows {
  *   slots[row]      = page * 128 + position % 128 of the token, -1 for refused requests and for
  *                     rows behind the last token;
  *   positions[row]  = length before + depth in the tree (chain: + place); rows behind: 0;
- *   visible[row]    (with parents) bit i: step token i of the request is this token or one of
- *                     its ancestors; rows behind: 0.
+ *   visible[row]    bit i: step token i of the request is this token or one of its ancestors
+ *                     (chain: bits 0 .. place, at most all 64); rows behind: 0.
  *
  * kvip_hip_page_tables_truncate cuts every request to a shorter length, clears the table entries of the
  * pages that are no longer needed and pushes those, in the order that undoes their popping:
@@ -91,7 +91,7 @@ typedef struct KvipPageTableArgs {
     int32_t* cu_seqlens;          /* extend: [batch + 1] */
     int64_t* positions;           /* extend: [max_tokens] */
     int64_t* slots;               /* extend: [max_tokens] */
-    int64_t* visible;             /* extend: [max_tokens], NULL without parents */
+    int64_t* visible;             /* extend: [max_tokens]; without parents NULL leaves it out */
     uint32_t* status;             /* optional */
     int32_t batch;                /* 1..KVIP_DRAFT_MAX_BATCH */
     int32_t max_blocks;

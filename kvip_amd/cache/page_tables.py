@@ -60,8 +60,9 @@ class PageTables:
         self._args = abi.PageTableArgs(
             block_table=p(self.block_table), lengths=p(self.lengths), free_pages=p(self.free), free_count=p(self.free_count),
             bases=p(self.bases), steps=p(self.steps), ticket=p(self.ticket), rows=p(self.rows), cu_seqlens=p(self.cu_seqlens),
-            positions=p(self.positions), slots=p(self.slots), status=p(self.status), batch=self.batch,
-            max_blocks=self.max_blocks, num_blocks=self.num_blocks, max_tokens=self.max_tokens, row_sets=len(rows))
+            positions=p(self.positions), slots=p(self.slots), visible=p(self.visible), status=p(self.status),
+            batch=self.batch, max_blocks=self.max_blocks, num_blocks=self.num_blocks, max_tokens=self.max_tokens,
+            row_sets=len(rows))
 
     def _rows(self, cache):
         """(base, block stride, row stride, row bytes) of a paged tensor, in bytes."""
@@ -86,12 +87,12 @@ class PageTables:
     def extend(self, counts, parents=None):
         """Appends counts[b] tokens to request b; counts int32 [batch] on the device. parents int32
         [max_tokens] names every row's parent within its request (-1: none) where the tokens are trees of
-        at most 64: positions then follow the depth, and `visible` gets each token's ancestors and itself.
+        at most 64: positions then follow the depth. `visible` gets each token's ancestors and itself: in a chain
+        (no parents) the tokens before it and itself.
         Returns (cu_seqlens, slots, positions)."""
         a = self._args  # copied by the launch
         a.counts = self._ints(counts, (self.batch,), "counts")
         a.parents = 0 if parents is None else self._ints(parents, (self.max_tokens,), "parents")
-        a.visible = 0 if parents is None else self.visible.data_ptr()
         abi.launch(self.torch, self.device, self.library.kvip_hip_page_tables_extend, a, "page tables")
         return self.cu_seqlens, self.slots, self.positions
 

@@ -179,6 +179,7 @@ __global__ __launch_bounds__(kTableThreads) void extend_tables_kernel(const Kvip
     const int first = p.parents == nullptr ? 0 : s.start[p.batch];
     for (int t = first + blockIdx.x * kTableThreads + tid; t < p.max_tokens; t += gridDim.x * kTableThreads) {
         int64_t slot = -1, position = 0;
+        uint64_t seen = 0;
         if (t < s.start[p.batch]) {
             int lo = 0, hi = p.batch - 1;  // the last request that starts at or before t has the row
             while (lo < hi) {
@@ -188,13 +189,14 @@ __global__ __launch_bounds__(kTableThreads) void extend_tables_kernel(const Kvip
             }
             const int within = t - s.start[lo], at = s.length[lo] + within;
             position = at;
+            seen = ~0ull >> (63 - min(within, 63));  // of a chain: every token up to this one
             if (within < s.step[lo]) {
                 slot = static_cast<int64_t>(page_of(p, s, lo, at / kBlockTokens, top)) * kBlockTokens + at % kBlockTokens;
             }
         }
         p.slots[t] = slot;
         p.positions[t] = position;
-        if (p.visible != nullptr) p.visible[t] = 0;
+        if (p.visible != nullptr) p.visible[t] = static_cast<int64_t>(seen);
     }
 }
 

@@ -135,7 +135,7 @@ class Tables:
                 if tree is not None and i >= 64:
                     continue
                 positions[rows + i] = base + (i if tree is None else depth[i])
-                visible[rows + i] = 0 if tree is None else bits[i]
+                visible[rows + i] = (1 << min(i + 1, 64)) - 1 if tree is None else bits[i]
                 if step:
                     slots[rows + i] = self.pages[b][(base + i) // BLOCK] * BLOCK + (base + i) % BLOCK
             rows += n

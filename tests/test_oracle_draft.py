@@ -136,3 +136,10 @@ def test_tables_model_undoes_and_refuses():
     t.max_tokens = 2000
     cu, _, _, _, status = t.extend([1, 200, 500])
     assert status == 8 and t.lengths == [2, 400, 0]
+
+
+def test_tables_model_makes_a_chain_visible():
+    t = draft.Tables(2, 4, 8, 80)
+    visible = t.extend([3, 70])[3]
+    assert visible[:3] == [1, 3, 7] and visible[3:73] == [(1 << min(i, 64)) - 1 for i in range(1, 71)] and not any(visible[73:])
+    assert visible[3:67] == draft.ancestors(range(-1, 63))[0]  # as a tree whose tokens each follow the one before
