@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define KVIP_DRAFT_ABI_VERSION 1u
+#define KVIP_DRAFT_ABI_VERSION 2u
 
 /* Device status bits beside those of kvip_hip.h (BAD_BLOCK 1, HISTOGRAM 2, BAD_TOKEN 4). */
 #define KVIP_STATUS_NO_PAGE 8u      /* a request got no pages: the free list is too short */
@@ -58,7 +58,8 @@ typedef struct KvipPagedRows {
  * than 64 tokens (KVIP_STATUS_BAD_LENGTH), or where it and the requests before it need more pages
  * than there are (KVIP_STATUS_NO_PAGE; one that needs none is not refused for that). Writes
  *   cu_seqlens[b]   = sum of the counts before b (a negative one counts as 0), at most max_tokens;
- *   bases[b]        = the length before; steps[b] = the tokens appended (0: refused);
+ *   bases[b]        = the length before; steps[b] = the tokens appended (0: refused; a refused request
+ *                     keeps its rows in the step, so what reads these needs steps as well);
  *   slots[row]      = page * 128 + position % 128 of the token, -1 for refused requests and for
  *                     rows behind the last token;
  *   positions[row]  = length before + depth in the tree (chain: + place); rows behind: 0;
@@ -167,7 +168,8 @@ typedef struct KvipRowStoreArgs {
  * NaN or a scale that is not finite becomes NaN as a whole. Blocks outside the cache set
  * KVIP_STATUS_BAD_BLOCK and count as not there; lengths outside 0 .. max_blocks * 128, fewer
  * rows than step tokens or more than max_nodes of these set KVIP_STATUS_BAD_LENGTH (the length is
- * cut to the range, tokens past max_nodes are not computed). Rows of output and lse behind
+ * cut to the range, tokens past max_nodes are not computed). With steps, a request with steps[b] <= 0
+ * (one that kvip_hip_page_tables_extend refused) sees nothing: output 0, lse -infinity. Rows of output and lse behind
  * cu_seqlens[batch] are left as they were. The launch counts steps of 32 rows x 128 (token, head) pairs in 32
  * bits: where batch * heads * max_nodes * max_blocks could pass that, workspace_bytes is 0 and the
  * call is refused. A workspace serves one call at a time, and the lengths stay as they are while it runs. */
@@ -193,6 +195,7 @@ typedef struct KvipTreeAttnArgs {
     int32_t output_dtype;         /* KVIP_DTYPE_BF16 or _FP32 */
     float scale;                  /* finite */
     int32_t reserved;
+    const int32_t* steps;         /* [batch], or NULL */
 } KvipTreeAttnArgs;
 
 /* Verification of drafted tokens. probs[row][v] is the target's probability of token v after the
@@ -208,7 +211,8 @@ typedef struct KvipTreeAttnArgs {
  * So a token is distributed as the target says, whatever was drafted.
  *   path[b]          rows (within the request) of the walk, kept[b] of them, then -1;
  *   out_tokens[b]    the walk's tokens after token 0, then the drawn one, then -1.
- * A request without rows gets kept 0. Tokens outside 0 .. vocab - 1 set KVIP_STATUS_BAD_TOKEN and are never
+ * A request without rows gets kept 0, as does, with steps, one with steps[b] <= 0 (which
+ * kvip_hip_page_tables_extend refused). Tokens outside 0 .. vocab - 1 set KVIP_STATUS_BAD_TOKEN and are never
  * taken; parents that do not come before their child set KVIP_STATUS_BAD_TREE and count as -1; a
  * request of more than max_nodes rows sets KVIP_STATUS_BAD_LENGTH (the rest is not looked at);
  * weights without a positive finite sum set KVIP_STATUS_BAD_PROBS and give token -1. Weights that
@@ -233,6 +237,7 @@ typedef struct KvipVerifyArgs {
     int32_t vocab;                /* 1..2^20 */
     int32_t dtype;                /* of probs and draft_probs: KVIP_DTYPE_FP32, _BF16 or _FP16 */
     int32_t reserved;
+    const int32_t* steps;         /* [batch], or NULL */
 } KvipVerifyArgs;
 
 uint32_t kvip_hip_draft_abi_version(void);

@@ -4,7 +4,7 @@ Holds, as device tensors, the block table and length of every request and the st
 of a paged cache, and lays out a step from the request lengths without a host read: `extend(counts)`
 appends tokens (pages, slots, positions, the visibility of a tree's tokens), `commit(kept)` keeps the
 accepted ones and gives the other pages back, `truncate(lengths)` shortens or ends requests. The
-tensors feed the operators of the same step: `cu_seqlens`, `lengths`, `block_table` and `visible` go to
+tensors feed the operators of the same step: `cu_seqlens`, `lengths`, `block_table`, `visible` and `steps` go to
 `kvip_amd.TreeAttention` (`block_table`, `lengths` and `cu_seqlens` also to `kvip_amd.PrefillIndexer`), `slots` and
 `positions` to `kvip_amd.KvRowStore` and `kvip_amd.Rotary`, `slots` to `IndexCacheStorage` as its slot
 mapping. `include/kvip_hip_draft.h` states the rules. Calls only enqueue on the current stream
@@ -28,7 +28,8 @@ class PageTables:
     scales of every layer.
 
     block_table int32 [batch, blocks], lengths int32 [batch], free int32 [num_blocks] and free_count int32
-    [1] are the state; cu_seqlens int32 [batch + 1], positions, slots, visible int64 [max_tokens] the last step's
+    [1] are the state; steps int32 [batch] has the tokens that the last extend appended (0 where it refused a
+    request, whose rows stay in the step: TreeAttention and DraftVerifier take `steps` to leave it out); cu_seqlens int32 [batch + 1], positions, slots, visible int64 [max_tokens] the last step's
     layout; status int32 [1] collects KVIP_STATUS_* bits."""
 
     def __init__(self, torch, *, batch, max_context, num_blocks, max_tokens, device, caches=()):

@@ -192,7 +192,7 @@ struct TaRequest {
     int begin;   // first row of the step
     int nodes;   // its step tokens (at most max_nodes)
     int past;    // position of step token 0 (below 0 where the length is too short)
-    int length;  // cache rows
+    int length;  // cache rows (a refused request's: none, so that its rows get their zeros)
 };
 
 KVIP_DEVICE TaRequest ta_request(const KvipTreeAttnArgs& p, int b, uint32_t* err) {
@@ -200,10 +200,11 @@ KVIP_DEVICE TaRequest ta_request(const KvipTreeAttnArgs& p, int b, uint32_t* err
     q.begin = min(max(p.cu_seqlens[b], 0), p.max_tokens);
     const int all = min(max(p.cu_seqlens[b + 1], q.begin), p.max_tokens) - q.begin;
     const int given = p.seq_lens[b];
+    const bool refused = p.steps != nullptr && p.steps[b] <= 0;
     q.nodes = min(all, p.max_nodes);
-    q.length = min(max(given, 0), p.max_blocks * kBlockTokens);
+    q.length = refused ? 0 : min(max(given, 0), p.max_blocks * kBlockTokens);
     q.past = q.length - all;
-    if (given != q.length || all != q.nodes || (all > 0 && q.past < 0)) *err |= KVIP_STATUS_BAD_LENGTH;
+    if (all != q.nodes || (!refused && (given != q.length || (all > 0 && q.past < 0)))) *err |= KVIP_STATUS_BAD_LENGTH;
     return q;
 }
 

@@ -22,8 +22,8 @@ ROW_BYTES = 656
 class TreeAttention:
     """Output [max_tokens, heads, 512] (bf16 or fp32), log-sum-exp float32 [max_tokens, heads] (lse=True) and status
     allocated once; `bind` validates a call's tensors, `__call__` enqueues it on the current stream
-    (capturable; one object's calls follow one another, as they share its workspace). max_nodes: step tokens of a request (1..64); max_context: its cached rows, the step's
-    among them."""
+    (capturable; one object's calls follow one another, as they share its workspace). max_nodes: step tokens
+    of a request (1..64); max_context: its cached rows, the step's among them."""
 
     def __init__(self, torch, *, batch, heads, max_nodes, max_tokens, max_context, device, output_dtype=None, lse=False):
         abi.require(1 <= batch <= abi.DRAFT_MAX_BATCH, f"batch must be in 1..{abi.DRAFT_MAX_BATCH}")
@@ -47,12 +47,13 @@ class TreeAttention:
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.args = None
 
-    def bind(self, query, kv_cache, block_table, seq_lens, cu_seqlens, visible=None, scale=KEY_DIM ** -0.5):
+    def bind(self, query, kv_cache, block_table, seq_lens, cu_seqlens, visible=None, scale=KEY_DIM ** -0.5, *, steps=None):
         """query bf16 [max_tokens, heads, 576]; kv_cache 1-byte [blocks, 128, row_stride] (or [blocks, 128, 1,
         row_stride]) with rows of 656 bytes; block_table int32 [batch, blocks of max_context or fewer];
         seq_lens int32 [batch]: cached rows, the step's among them; cu_seqlens int32 [batch + 1]; visible int64
-        [max_tokens] as kvip_amd.PageTables.extend writes it (None: a chain). Rows behind the last token are
-        neither read nor written."""
+        [max_tokens] as kvip_amd.PageTables.extend writes it (None: a chain). steps int32 [batch] (PageTables.steps,
+        read before its commit): requests with 0, which extend refused and which have no rows of the step in the
+        cache, get zeros. Rows behind the last token are neither read nor written."""
         t = self.torch
         abi.require(query.dtype == t.bfloat16 and tuple(query.shape) == (self.max_tokens, self.heads, KEY_DIM) and
                     query.is_contiguous(), f"query must be contiguous bfloat16 [{self.max_tokens}, {self.heads}, {KEY_DIM}]")
@@ -70,7 +71,9 @@ class TreeAttention:
                         f"{what} must be contiguous int32 {list(shape)}")
         abi.require(visible is None or (visible.dtype == t.int64 and tuple(visible.shape) == (self.max_tokens,) and
                                         visible.is_contiguous()), f"visible must be contiguous int64 [{self.max_tokens}]")
-        for x in (query, kv_cache, block_table, seq_lens, cu_seqlens, visible):
+        abi.require(steps is None or (steps.dtype == t.int32 and tuple(steps.shape) == (self.batch,) and steps.is_contiguous()),
+                    f"steps must be contiguous int32 [{self.batch}]")
+        for x in (query, kv_cache, block_table, seq_lens, cu_seqlens, visible, steps):
             abi.require(x is None or x.device == self.device, f"tree attention tensors must be on {self.device}")
         abi.require(math.isfinite(scale), "scale must be finite")
         p = abi.ptr
@@ -79,9 +82,9 @@ class TreeAttention:
             visible=p(visible), output=p(self.output), lse=p(self.lse), workspace=p(self.workspace), status=p(self.status),
             kv_block_stride=kv_cache.stride(0), row_stride=kv_cache.stride(1), batch=self.batch, heads=self.heads,
             max_nodes=self.max_nodes, max_tokens=self.max_tokens, max_blocks=int(block_table.shape[1]),
-            num_blocks=int(kv_cache.shape[0]), scale=float(scale),
+            num_blocks=int(kv_cache.shape[0]), scale=float(scale), steps=p(steps),
             output_dtype=abi.DTYPE_FP32 if self.output.dtype == t.float32 else abi.DTYPE_BF16)
-        self._bound = (query, kv_cache, block_table, seq_lens, cu_seqlens, visible)
+        self._bound = (query, kv_cache, block_table, seq_lens, cu_seqlens, visible, steps)
         return self
 
     def __call__(self):
@@ -91,11 +94,11 @@ class TreeAttention:
 
 
 def tree_attention(query, kv_cache, block_table, seq_lens, cu_seqlens, visible=None, scale=KEY_DIM ** -0.5, *,
-                   max_nodes=abi.DRAFT_MAX_NODES, output_dtype=None):
+                   max_nodes=abi.DRAFT_MAX_NODES, output_dtype=None, steps=None):
     """One tree-attention call (arguments as `TreeAttention.bind`); returns [rows, heads, 512]."""
     import torch
 
     op = TreeAttention(torch, batch=int(seq_lens.shape[0]), heads=int(query.shape[1]), max_nodes=max_nodes,
                        max_tokens=int(query.shape[0]), max_context=int(block_table.shape[1]) * BLOCK_TOKENS,
                        device=query.device, output_dtype=output_dtype)
-    return op.bind(query, kv_cache, block_table, seq_lens, cu_seqlens, visible, scale)()
+    return op.bind(query, kv_cache, block_table, seq_lens, cu_seqlens, visible, scale, steps=steps)()

@@ -32,11 +32,12 @@ class DraftVerifier:
         self.workspace = torch.zeros(nbytes // 8, dtype=torch.int64, device=self.device)
         self.args = None
 
-    def bind(self, probs, tokens, cu_seqlens, uniforms, final_uniforms, *, parents=None, draft_probs=None):
+    def bind(self, probs, tokens, cu_seqlens, uniforms, final_uniforms, *, parents=None, draft_probs=None, steps=None):
         """probs [rows, vocab] (fp32, bf16 or fp16; rows at any stride): the target's probabilities after
         each step token; tokens int64 [rows]; cu_seqlens int32 [batch + 1]; uniforms float32 [rows] and
         final_uniforms float32 [batch] in [0, 1). parents int32 [rows]: trees of chosen tokens; draft_probs (as
-        probs): a chain whose next token each row drew; neither: a chain of chosen tokens."""
+        probs): a chain whose next token each row drew; neither: a chain of chosen tokens. steps int32 [batch]
+        (PageTables.steps, read before its commit): requests with 0, which extend refused, keep nothing."""
         t = self.torch
         codes = {t.float32: abi.DTYPE_FP32, t.bfloat16: abi.DTYPE_BF16, t.float16: abi.DTYPE_FP16}
         rows = int(probs.shape[0])
@@ -51,9 +52,9 @@ class DraftVerifier:
         for x, dtype, shape, what in ((tokens, t.int64, (rows,), "tokens"), (uniforms, t.float32, (rows,), "uniforms"),
                                       (cu_seqlens, t.int32, (self.batch + 1,), "cu_seqlens"),
                                       (final_uniforms, t.float32, (self.batch,), "final_uniforms"),
-                                      (parents, t.int32, (rows,), "parents")):
-            abi.require(x is None and what == "parents" or (x.dtype == dtype and tuple(x.shape) == shape and
-                                                            x.is_contiguous() and x.device == self.device),
+                                      (parents, t.int32, (rows,), "parents"), (steps, t.int32, (self.batch,), "steps")):
+            abi.require(x is None and what in ("parents", "steps") or
+                        (x.dtype == dtype and tuple(x.shape) == shape and x.is_contiguous() and x.device == self.device),
                         f"{what} must be contiguous {dtype} {list(shape)} on {self.device}")
         p = abi.ptr
         self.args = abi.VerifyArgs(
@@ -62,8 +63,8 @@ class DraftVerifier:
             path=p(self.path), workspace=p(self.workspace), status=p(self.status),
             probs_stride=max(probs.stride(0), self.vocab), draft_stride=0 if draft_probs is None else
             max(draft_probs.stride(0), self.vocab), batch=self.batch, max_nodes=self.max_nodes, max_tokens=rows,
-            vocab=self.vocab, dtype=codes[probs.dtype])
-        self._bound = (probs, draft_probs, tokens, cu_seqlens, parents, uniforms, final_uniforms)
+            vocab=self.vocab, dtype=codes[probs.dtype], steps=p(steps))
+        self._bound = (probs, draft_probs, tokens, cu_seqlens, parents, uniforms, final_uniforms, steps)
         return self
 
     def __call__(self):

@@ -10,7 +10,7 @@ from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parents[1] / "_lib" / "libkvip_hip.so"
 ABI_VERSION = 15
-DRAFT_ABI_VERSION = 1
+DRAFT_ABI_VERSION = 2
 
 KVIP_OK = 0
 KVIP_ERR_INVALID = 100000
@@ -240,6 +240,7 @@ class TreeAttnArgs(ctypes.Structure):
         ("output", _p), ("lse", _p), ("workspace", _p), ("status", _p), ("kv_block_stride", _i64),
         ("row_stride", _i32), ("batch", _i32), ("heads", _i32), ("max_nodes", _i32), ("max_tokens", _i32),
         ("max_blocks", _i32), ("num_blocks", _i32), ("output_dtype", _i32), ("scale", ctypes.c_float), ("reserved", _i32),
+        ("steps", _p),
     ]
 
 
@@ -248,7 +249,7 @@ class VerifyArgs(ctypes.Structure):
         ("probs", _p), ("draft_probs", _p), ("tokens", _p), ("cu_seqlens", _p), ("parents", _p), ("uniforms", _p),
         ("final_uniforms", _p), ("out_tokens", _p), ("kept", _p), ("path", _p), ("workspace", _p), ("status", _p),
         ("probs_stride", _i64), ("draft_stride", _i64), ("batch", _i32), ("max_nodes", _i32), ("max_tokens", _i32),
-        ("vocab", _i32), ("dtype", _i32), ("reserved", _i32),
+        ("vocab", _i32), ("dtype", _i32), ("reserved", _i32), ("steps", _p),
     ]
 
 

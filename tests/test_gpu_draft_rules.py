@@ -2,12 +2,16 @@
 parents, requests that got no pages, targets whose support was drafted whole, workspaces of several
 shapes, latents and scales at the ends of their range. Against oracle/draft.py, with the bounds of
 tests/test_gpu_draft.py."""
+import math
+
 import numpy as np
 import pytest
 
 import kvip_amd
+from kvip_amd.runtime import abi
 from oracle import draft
-from tests.test_gpu_draft import HALF_STEP, ROW, SCALE, Round, device, host, random_parents, same_tables, say
+from tests.test_gpu_draft import (HALF_STEP, ROW, SCALE, Round, Step, check_verify, device, host, random_parents,
+                                  run_verify, same_tables, say, verify_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +82,105 @@ def test_a_bound_attention_takes_trees_and_chains_in_turn(torch_gpu):
         same_tables(r.tables, model)
     for op in (r.tables, r.store, r.attention):
         assert int(op.status.item()) == 0
+
+
+# --- requests that got no pages --------------------------------------------------------------
+
+
+def random_rows(rng, count):
+    """uint8 [count, 656]: rows of N(0, 1) latents and rotary features."""
+    rows = np.zeros((count, ROW), np.uint8)
+    codes, scales = draft.stored_rows(rng.standard_normal((count, 512)).astype(np.float32))
+    rows[:, :512], rows[:, 640:656] = codes, scales.view(np.uint8)
+    rope = rng.standard_normal((count, 64)).astype(np.float32)
+    rows[:, 512:640] = (rope.view(np.uint32) >> 16).astype("<u2").view(np.uint8)
+    return rows
+
+
+def test_a_refused_request_answers_nothing(torch_gpu):
+    """A request that gets no page keeps its length and its rows of the step; nothing of it is attended or verified,
+    the others go on, and so does it once there are pages."""
+    torch = torch_gpu
+    say("case refused request")
+    r, rng = Round(torch, 21), np.random.default_rng(21)
+    t = r.tables
+    r.attention.bind(r.query, r.kv, t.block_table, t.lengths, t.cu_seqlens, t.visible, steps=t.steps)
+    r.verifier.bind(r.probs, r.tokens, t.cu_seqlens, r.uniforms, r.final, parents=r.parents, steps=t.steps)
+    r.kv.copy_(torch.from_numpy(random_rows(rng, 40 * 128)).view(40, 128, ROW))
+    for counts in [[0, 25, 0]] * 5 + [[21, 0, 0]] * 2 + [[0, 0, 21]] * 2:
+        t.extend(device(torch, counts, torch.int32))
+        t.commit(device(torch, counts, torch.int32))
+    assert t.lengths.tolist() == [42, 125, 42] and int(t.status.item()) == 0
+    counts, pages = [6, 7, 5], t.free_count.clone()
+    for seed, there in ((3, False), (4, True)):
+        t.free_count.copy_(pages if there else torch.zeros_like(pages))  # the other pages are someone else's
+        t.status.zero_()
+        r.inputs(seed, counts)
+        bases = t.lengths.tolist()
+        r.step()
+        table, kept = t.block_table.cpu().numpy(), r.verifier.kept.tolist()
+        assert int(t.status.item()) == (0 if there else abi.STATUS_NO_PAGE)
+        assert t.lengths.tolist() == [n + k for n, k in zip(bases, kept)]
+        at, probs = 0, host(r.probs)
+        for b, n in enumerate(counts):
+            s = slice(at, at + n)
+            at += n
+            if b == 1 and not there:
+                assert kept[b] == 0 and set(r.verifier.out_tokens[b].tolist()) == set(r.verifier.path[b].tolist()) == {-1}
+                assert not r.attention.output[s].any() and t.slots[s].tolist() == [-1] * n
+                continue
+            walk, out = draft.verify(probs[s], r.tokens[s].tolist(), r.parents[s].tolist(), None, r.uniforms[s].tolist(),
+                                     float(r.final[b]))
+            assert r.verifier.path[b].tolist()[:kept[b]] == walk and r.verifier.out_tokens[b].tolist()[:kept[b]] == out
+            # The first token sees the rows before it, which the step leaves where they were, and itself.
+            rows = r.kv.cpu().numpy().reshape(-1, ROW)[[table[b, p // 128] * 128 + p % 128 for p in range(bases[b] + 1)]]
+            want, _, bound, _ = draft.tree_attention(host(r.query)[s][0], rows, np.ones(len(rows), bool), SCALE)
+            assert np.all(np.abs(host(r.attention.output)[s][0] - want) <= bound + np.abs(want) * HALF_STEP["bf16"])
+    for op in (r.store, r.attention, r.verifier):
+        assert int(op.status.item()) == 0
+
+
+@pytest.mark.parametrize("heads,counts,contexts,steps", [
+    (16, [3, 2, 4], [200, 300, 0], [3, 0, 4]), (16, [64, 2], [1000, 40], [0, 2]), (128, [12, 5, 9], [4000, 900, 20], [12, 0, 9]),
+    (40, [7, 1], [20000, 30000], [7, 0]), (8, [1] * 90, [(53 * i) % 900 for i in range(90)], [i % 3 and 1 for i in range(90)])])
+def test_attention_of_refused_requests_is_zero(torch_gpu, heads, counts, contexts, steps):
+    torch = torch_gpu
+    say(f"case refused attention heads={heads} counts={counts[:5]}")
+    step = Step(torch, np.random.default_rng(heads), counts, contexts, heads)
+    op = step.run()
+    query, kv, table, lens, cu, visible = op._bound[:6]
+    op.bind(query, kv, table, lens, cu, visible, steps=device(torch, steps, torch.int32))
+    step.check(op, only=[b for b, n in enumerate(steps) if n])
+    for b, n in enumerate(steps):
+        if n == 0:
+            rows = slice(int(step.cu[b]), int(step.cu[b + 1]))
+            assert not op.output[rows].any() and bool((op.lse[rows] == -math.inf).all()), b
+    assert int(op.status.item()) == 0
+    again = kvip_amd.tree_attention(query, kv, table, lens, cu, visible, max_nodes=max(counts), steps=device(torch, steps, torch.int32))
+    assert torch.equal(again[:int(step.cu[-1])], op.output[:int(step.cu[-1])])
+    for bad in (device(torch, steps, torch.int64), device(torch, steps[:-1], torch.int32), device(torch, steps, torch.int32).cpu()):
+        with pytest.raises(ValueError):
+            op.bind(query, kv, table, lens, cu, visible, steps=bad)
+
+
+@pytest.mark.parametrize("drafted", ["tree", "draft"])
+def test_verification_of_refused_requests_keeps_nothing(torch_gpu, drafted):
+    torch = torch_gpu
+    say(f"case refused verification {drafted}")
+    rng = np.random.default_rng(5)
+    counts, steps = [4, 5, 0, 6], [4, 0, 0, 6]
+    case = verify_case(torch, rng, counts, 9001, drafted, "fp32")
+    op = run_verify(torch, case, nodes=6, vocab=9001)
+    check_verify(case, op, nodes=6)
+    all_tokens, all_kept, all_path = (x.clone() for x in (op.out_tokens, op.kept, op.path))
+    probs, q, tokens, cu, parents, uniforms, final = op._bound[:7]
+    named = dict(parents=parents, draft_probs=q)
+    op.bind(probs, tokens, cu, uniforms, final, steps=device(torch, steps, torch.int32), **named)()
+    assert int(op.kept[1]) == 0 and bool((op.out_tokens[1] == -1).all()) and bool((op.path[1] == -1).all())
+    for b in (0, 2, 3):
+        assert torch.equal(op.out_tokens[b], all_tokens[b]) and torch.equal(op.path[b], all_path[b])
+        assert op.kept[b] == all_kept[b]
+    assert int(op.status.item()) == 0
+    for bad in (device(torch, steps, torch.int64), device(torch, steps[:-1], torch.int32), device(torch, steps, torch.int32).cpu()):
+        with pytest.raises(ValueError):
+            op.bind(probs, tokens, cu, uniforms, final, steps=bad, **named)
