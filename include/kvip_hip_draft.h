@@ -30,7 +30,7 @@ extern "C" {
 #define KVIP_STATUS_NO_PAGE 8u      /* a request got no pages: the free list is too short */
 #define KVIP_STATUS_BAD_LENGTH 16u  /* a length or count outside its range */
 #define KVIP_STATUS_BAD_TREE 32u    /* a parent that does not come before its child, or a path that does not rise */
-#define KVIP_STATUS_BAD_PROBS 64u   /* no token can be drawn: the weights of a row have no positive finite sum */
+#define KVIP_STATUS_BAD_PROBS 64u   /* no token can be drawn: a row without a weight, or whose weights have no finite sum */
 
 #define KVIP_DTYPE_FP16 3           /* beside the KVIP_DTYPE_* of kvip_hip.h */
 
@@ -208,15 +208,17 @@ typedef struct KvipTreeAttnArgs {
  * Where the walk ends, one more token is drawn, the first v at which the running sum of the weights
  * passes final_uniforms[b] times their whole: weights max(probs - draft_probs, 0) after a
  * refused child of a chain with draft_probs, else probs without the children's tokens. Sums in 64 bits.
- * So a token is distributed as the target says, whatever was drafted.
+ * So a token is distributed as the target says, whatever was drafted. Probabilities of few bits need not sum to
+ * 1: where nothing has a weight, probs are drawn from after a refused child of a chain with draft_probs, and
+ * else the last child that has a probability is the token drawn.
  *   path[b]          rows (within the request) of the walk, kept[b] of them, then -1;
  *   out_tokens[b]    the walk's tokens after token 0, then the drawn one, then -1.
  * A request without rows gets kept 0, as does, with steps, one with steps[b] <= 0 (which
  * kvip_hip_page_tables_extend refused). Tokens outside 0 .. vocab - 1 set KVIP_STATUS_BAD_TOKEN and are never
  * taken; parents that do not come before their child set KVIP_STATUS_BAD_TREE and count as -1; a
  * request of more than max_nodes rows sets KVIP_STATUS_BAD_LENGTH (the rest is not looked at);
- * weights without a positive finite sum set KVIP_STATUS_BAD_PROBS and give token -1. Weights that
- * are negative or NaN count as 0. */
+ * a row in which no token has a weight, or the weights no finite sum, sets KVIP_STATUS_BAD_PROBS and
+ * gives token -1. Weights that are negative or NaN count as 0. */
 typedef struct KvipVerifyArgs {
     const void* probs;            /* [max_tokens, vocab], rows probs_stride elements apart */
     const void* draft_probs;      /* the same, draft_stride; or NULL */

@@ -57,6 +57,7 @@ struct Walk {
     int kept;                             // its rows
     int residual;                         // weights are max(probs - draft_probs, 0)
     int excluded;                         // tokens whose weight is 0
+    int last;                             // the last chosen child with a weight where the walk ends, -1: none
     int tokens[KVIP_DRAFT_MAX_NODES];
 };
 
@@ -86,8 +87,10 @@ KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, 
     int at = 0, kept = 1, residual = 0;
     int place = lane == 0 ? 0 : -1;  // lane i: row of the walk's i-th token
     unsigned long long tried;
+    int last = -1;
     for (;;) {  // at most n rounds: a child comes after its parent
         tried = __ballot(child && up == at);
+        last = -1;
         const double u = lane_double(uniform, at);
         int next = -1;
         if (draft != nullptr) {
@@ -105,11 +108,12 @@ KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, 
                 const int c = __ffsll(left) - 1;
                 const int64_t name = __builtin_amdgcn_readlane(static_cast<int>(token), c);  // named: below 2^20
                 left &= ~__ballot(child && up == at && token == name);  // named again: nothing left
-                const double high = low + lane_double(mine, c);
+                const double weight = lane_double(mine, c), high = low + weight;
                 if (low <= u && u < high) {
                     next = c;
                     break;
                 }
+                if (weight > 0.0) last = static_cast<int>(name);
                 low = high;
             }
         }
@@ -123,6 +127,7 @@ KVIP_DEVICE void walk_request(const KvipVerifyArgs& p, int b, int begin, int n, 
         w->kept = kept;
         w->residual = residual;
         w->excluded = draft != nullptr ? 0 : __popcll(tried);
+        w->last = last;
     }
     if (draft == nullptr && (tried >> lane & 1)) {
         w->tokens[__popcll(tried & ((1ull << lane) - 1))] = static_cast<int>(token);
@@ -240,9 +245,9 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const KvipVerifyArgs p)
     // The part in which the running sum passes the share, and the sum before it: one part per thread
     // in order.
     static_assert(kMaxParts <= THREADS, "a part per thread");
-    const double mine = tid < static_cast<int>(gridDim.x)
-                            ? __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<uint64_t*>(sums + tid),
-                                                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) : 0.0;
+    double mine = tid < static_cast<int>(gridDim.x)
+                      ? __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<uint64_t*>(sums + tid),
+                                                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) : 0.0;
     // Runs a block-wide inclusive sum of v; returns it, and the whole to *total.
     auto running = [&](double v, double* total) {
         const double in_wave = wave_running(v);
@@ -259,7 +264,25 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const KvipVerifyArgs p)
         return before + in_wave;
     };
     double whole;
-    const double upto = running(mine, &whole);
+    double upto = running(mine, &whole);
+    if (whole == 0.0 && draft != nullptr) {
+        // A target that is nowhere above its draft (the refused token was a rounding step below): drawn from itself,
+        // by this workgroup alone, as it is rare.
+        draft = nullptr;
+        for (int k = 0; k < static_cast<int>(gridDim.x); ++k) {
+            double of_part = 0.0, part_sum;
+#pragma unroll
+            for (int j = 0; j < kPerLane / kLoad; ++j) {
+                double x[kLoad];
+                weights(k * kPart + (j * THREADS + tid) * kLoad, x);
+#pragma unroll
+                for (int e = 0; e < kLoad; ++e) of_part += x[e];
+            }
+            running(of_part, &part_sum);
+            if (tid == k) mine = part_sum;
+        }
+        upto = running(mine, &whole);
+    }
     const double target = static_cast<double>(p.final_uniforms[b]) * whole;
     if (tid == 0) {
         s_part = kMaxParts;
@@ -309,9 +332,11 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const KvipVerifyArgs p)
         if (last >= 0) atomicMax(&s_near, last);
         __syncthreads();
         drawn = s_found < 1 << 30 ? s_found : s_near;
+    } else if (whole == 0.0) {
+        drawn = s_walk.last;  // children that are the whole target, whose probabilities fall short of 1 by a rounding
     }
     if (tid == 0) {
-        if (!drawable) report(p.status, KVIP_STATUS_BAD_PROBS);
+        if (drawn < 0) report(p.status, KVIP_STATUS_BAD_PROBS);
         p.out_tokens[static_cast<int64_t>(b) * p.max_nodes + s_walk.kept - 1] = drawn;
     }
 }

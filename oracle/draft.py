@@ -172,7 +172,7 @@ def verify(probs, tokens, parents, draft, uniforms, final):
     at, path = 0, [0]
     while True:
         children = [i for i in range(at + 1, n) if up[i] == at and named[i]]
-        u, taken = float(uniforms[at]), None
+        u, taken, weighty = float(uniforms[at]), None, -1
         if draft is not None:
             if children and u * float(draft[at, int(tokens[at + 1])]) < weight(probs, at, at + 1):
                 taken = at + 1
@@ -186,6 +186,7 @@ def verify(probs, tokens, parents, draft, uniforms, final):
                 if low <= u < high:
                     taken = i
                     break
+                weighty = int(tokens[i]) if weight(probs, at, i) > 0 else weighty
                 low = high
         if taken is None:
             break
@@ -199,7 +200,10 @@ def verify(probs, tokens, parents, draft, uniforms, final):
         rest[[int(tokens[i]) for i in children]] = 0.0
     rest = np.where(rest > 0, rest, 0.0)
     whole = rest.sum()
-    last = -1
+    if whole == 0 and draft is not None:  # a target that is nowhere above its draft
+        rest = np.where(probs[at] > 0, probs[at], 0.0)
+        whole = rest.sum()
+    last = weighty if whole == 0 else -1  # children that are the whole target
     if 0 < whole < math.inf:
         passed = np.flatnonzero((np.cumsum(rest) > float(final) * whole) & (rest > 0))
         last = int(passed[0]) if len(passed) else int(np.flatnonzero(rest)[-1])

@@ -10,8 +10,8 @@ import pytest
 import kvip_amd
 from kvip_amd.runtime import abi
 from oracle import draft
-from tests.test_gpu_draft import (HALF_STEP, ROW, SCALE, Round, Step, check_verify, device, host, random_parents,
-                                  run_verify, same_tables, say, verify_case)
+from tests.test_gpu_draft import (HALF_STEP, ROW, SCALE, Round, Step, check_verify, device, dtype_of, host,
+                                  random_parents, run_verify, same_tables, say, softmax_rows, verify_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,90 @@ def test_verification_of_refused_requests_keeps_nothing(torch_gpu, drafted):
     for bad in (device(torch, steps, torch.int64), device(torch, steps[:-1], torch.int32), device(torch, steps, torch.int32).cpu()):
         with pytest.raises(ValueError):
             op.bind(probs, tokens, cu, uniforms, final, steps=bad, **named)
+
+
+# --- targets whose support was drafted whole --------------------------------------------------
+
+
+def one_row(torch, weights, tokens, parents, dtype, vocab, u, final, draft_row=None):
+    """A case of one request per entry of `u` whose rows all have the same target."""
+    t, n = dtype_of(torch, dtype), len(tokens)
+    probs = torch.zeros((len(u) * n, vocab), dtype=t, device="cuda")
+    for v, x in weights.items():
+        probs[:, v] = x
+    q = None
+    if draft_row is not None:
+        q = torch.zeros_like(probs)
+        for v, x in draft_row.items():
+            q[:, v] = x
+    uniforms = np.zeros((len(u), n), np.float32)
+    uniforms[:, 0] = u
+    return dict(probs=probs, tokens=np.tile(tokens, len(u)), parents=None if parents is None else np.tile(np.int32(parents), len(u)),
+                draft=q, cu=np.arange(len(u) + 1) * n, uniforms=uniforms.reshape(-1), final=np.float32(final))
+
+
+@pytest.mark.parametrize("dtype,vocab", [("bf16", 2), ("bf16", 5000), ("fp32", 40000), ("fp16", 9001)])
+def test_children_that_are_the_whole_support(torch_gpu, dtype, vocab):
+    """bf16(0.1) + bf16(0.9) is 0.9985: a number above it falls to the last child with a weight, not to no token."""
+    torch = torch_gpu
+    say(f"case whole support {dtype} {vocab}")
+    last = vocab - 1
+    u = [0.0, 0.05, 0.1005, 0.5, 0.99, 0.999, 1 - 2.0 ** -24]
+    for tokens, parents in (([0, 0, last], [-1, 0, 0]), ([0, last, 0], [-1, 0, 0]), ([0, 0, last, 0], [-1, 0, 0, 0])):
+        case = one_row(torch, {0: 0.1, last: 0.9}, tokens, parents, dtype, vocab, u, np.linspace(0, 0.99, len(u)))
+        case["probs"] *= 0.995  # fp32 and fp16 come short too
+        op = run_verify(torch, case, nodes=len(tokens), vocab=vocab)
+        check_verify(case, op, nodes=len(tokens))
+        assert int(op.status.item()) == 0 and bool((op.out_tokens[:, 0] >= 0).all())
+        first = op.out_tokens[:, 0].tolist()
+        assert first[-1] == (last if tokens[1] == 0 else 0) and set(first) == {0, last}
+    # A chain's only child is the whole target; a child without a weight is not drawn either.
+    case = one_row(torch, {last: 0.998}, [0, last], None, dtype, vocab, u, np.linspace(0, 0.99, len(u)))
+    op = run_verify(torch, case, nodes=2, vocab=vocab)
+    check_verify(case, op, nodes=2)
+    assert op.out_tokens[:, 0].tolist() == [last] * len(u) and op.kept.tolist() == [2] * 5 + [1, 1]
+    if vocab > 2:
+        case = one_row(torch, {last: 0.998}, [0, last, 1], [-1, 0, 0], dtype, vocab, u, np.linspace(0, 0.99, len(u)))
+        op = run_verify(torch, case, nodes=3, vocab=vocab)
+        check_verify(case, op, nodes=3)
+        assert op.out_tokens[:, 0].tolist() == [last] * len(u) and int(op.status.item()) == 0
+
+
+@pytest.mark.parametrize("dtype,vocab", [("bf16", 2), ("bf16", 5000), ("fp32", 40000), ("fp16", 9001)])
+def test_a_refusal_that_leaves_no_residual(torch_gpu, dtype, vocab):
+    """A drafted token whose target is a rounding step below its draft is refused now and then, and
+    max(p - q, 0) is 0 everywhere: the target itself is drawn from."""
+    torch = torch_gpu
+    say(f"case no residual {dtype} {vocab}")
+    last, final = vocab - 1, [0.0, 0.1, 0.4, 0.6, 0.9, 1 - 2.0 ** -24]
+    u = [1 - 2.0 ** -24] * len(final)
+    case = one_row(torch, {0: 0.5, last: 0.5 - 2.0 ** -9}, [0, last], None, dtype, vocab, u, final, {0: 0.5, last: 0.5})
+    op = run_verify(torch, case, nodes=2, vocab=vocab)
+    for _ in range(2):
+        check_verify(case, op, nodes=2)
+        assert op.kept.tolist() == [1] * len(final) and op.out_tokens[:, 0].tolist() == [0] * 3 + [last] * 3
+    assert int(op.status.item()) == 0
+    if vocab < 4:
+        return
+    rng = np.random.default_rng(vocab)  # a target of many tokens, each at most its draft
+    p = softmax_rows(rng, 2, vocab, sharp=1.0)[:1]
+    case["probs"].copy_(torch.from_numpy(p))
+    case["draft"].copy_(case["probs"])
+    token = int(p.argmax())
+    case["tokens"][1::2] = token
+    case["draft"][:, token] *= 1.25
+    op = run_verify(torch, case, nodes=2, vocab=vocab)
+    check_verify(case, op, nodes=2)
+    assert op.kept.tolist() == [1] * len(final) and int(op.status.item()) == 0
+
+
+def test_rows_without_any_weight_still_have_no_token(torch_gpu):
+    torch = torch_gpu
+    say("case no weight at all")
+    for weights, draft_row in (({}, None), ({}, {0: 1.0}), ({0: -1.0, 7: float("nan")}, None), ({0: -1.0}, {0: 1.0, 7: 0.5}),
+                               ({0: float("inf")}, {0: 1.0, 3: 1.0})):
+        tokens, parents = ([0, 3], None) if draft_row else ([0, 3, 7], [-1, 0, 0])
+        case = one_row(torch, weights, tokens, parents, "fp32", 5000, [0.0, 0.7], [0.0, 0.7], draft_row)
+        op = run_verify(torch, case, nodes=len(tokens), vocab=5000)
+        check_verify(case, op, nodes=len(tokens))
+        assert op.out_tokens[:, 0].tolist() == [-1, -1] and int(op.status.item()) == abi.STATUS_BAD_PROBS

@@ -143,3 +143,28 @@ def test_tables_model_makes_a_chain_visible():
     visible = t.extend([3, 70])[3]
     assert visible[:3] == [1, 3, 7] and visible[3:73] == [(1 << min(i, 64)) - 1 for i in range(1, 71)] and not any(visible[73:])
     assert visible[3:67] == draft.ancestors(range(-1, 63))[0]  # as a tree whose tokens each follow the one before
+
+
+def test_a_target_that_falls_short_of_one_still_gives_a_token():
+    bf16 = [0.10009765625, 0.8984375]  # bf16(0.1) and bf16(0.9)
+    p = np.asarray([bf16 + [0.0]] * 4)
+    for u, last in ((0.0, 0), (0.999, 1), (1 - 2.0 ** -24, 1)):
+        path, out = draft.verify(p, [9, 0, 1, 0], [-1, 0, 0, 0], None, [u, 0, 0, 0], 0.5)
+        assert out[0] == last and len(path) == (2 if u < 0.9 else 1)
+    assert draft.verify(p, [9, 1, 0, 2], [-1, 0, 0, 0], None, [0.999, 0, 0, 0], 0.5) == ([0], [0])
+    # A refused token one step of bf16 below its draft, the rest equal: max(p - q, 0) is 0.
+    p, q = np.asarray([[0.5, 0.498046875]] * 2), np.asarray([[0.5, 0.5]] * 2)
+    assert draft.verify(p, [0, 1], None, q, [0.9999, 0], 0.4) == ([0], [0])
+    assert draft.verify(p, [0, 1], None, q, [0.9999, 0], 0.6) == ([0], [1])
+    assert draft.verify(np.zeros((2, 2)), [0, 1], None, q, [0.9, 0], 0.6) == ([0], [-1])
+    assert draft.verify(np.zeros((2, 2)), [0, 1], None, None, [0.9, 0], 0.6) == ([0], [-1])
+
+
+def test_tokens_of_a_target_drafted_whole_are_distributed_as_it():
+    """All of the target's tokens drafted as children, probabilities that sum to 1 - 2^-7: no token is missing, and
+    none has more than its probability and the missing part."""
+    p, grid = np.asarray([0.25, 0.5, 0.2421875]), 4096
+    got = np.zeros(3)
+    for u in (np.arange(grid) + 0.5) / grid:
+        got[draft.verify(np.stack([p] * 4), [0, 2, 0, 1], [-1, 0, 0, 0], None, [u, 0, 0, 0], 0.0)[1][0]] += 1 / grid
+    assert math.isclose(got.sum(), 1.0) and np.all(np.abs(got - p) <= (1 - p.sum()) + 1 / grid) and np.all(got >= p - 1 / grid)
