@@ -230,7 +230,8 @@ typedef struct KvipVerifyArgs {
     int64_t* out_tokens;          /* [batch, max_nodes] */
     int32_t* kept;                /* [batch] */
     int32_t* path;                /* [batch, max_nodes] */
-    void* workspace;              /* kvip_hip_verify_drafts_workspace_bytes bytes, 8-byte aligned, zero at first */
+    void* workspace;              /* kvip_hip_verify_drafts_workspace_bytes bytes, 8-byte aligned, zero before its first call;
+                                     calls of other shapes may follow in it, one at a time */
     uint32_t* status;             /* optional */
     int64_t probs_stride, draft_stride;
     int32_t batch;                /* 1..KVIP_DRAFT_MAX_BATCH */

@@ -226,9 +226,10 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const KvipVerifyArgs p)
     sum = wave_running(sum);
     if (lane == 63) s_wave[wave] = sum;
     __syncthreads();
-    double* sums = static_cast<double*>(p.workspace) + static_cast<int64_t>(b) * gridDim.x;
-    uint32_t* ticket = reinterpret_cast<uint32_t*>(static_cast<double*>(p.workspace) + static_cast<int64_t>(p.batch) * gridDim.x) +
-                       b * kTicketWords;
+    // The tickets first, at the same place for every shape: they are 0 between calls, whatever the sums behind hold.
+    uint32_t* ticket = static_cast<uint32_t*>(p.workspace) + b * kTicketWords;
+    double* sums = reinterpret_cast<double*>(static_cast<uint32_t*>(p.workspace) + KVIP_DRAFT_MAX_BATCH * kTicketWords) +
+                   static_cast<int64_t>(b) * gridDim.x;
     if (tid == 0) {
         double whole = 0.0;
 #pragma unroll
@@ -360,8 +361,8 @@ void launch_verify(const KvipVerifyArgs& a, hipStream_t s) {
 
 extern "C" uint64_t kvip_hip_verify_drafts_workspace_bytes(int32_t batch, int32_t vocab) {
     if (batch < 1 || vocab < 1) return 0;
-    return static_cast<uint64_t>(batch) * kvip::verify_parts(vocab) * sizeof(double) +
-           static_cast<uint64_t>(batch) * kvip::kTicketWords * sizeof(uint32_t);
+    return static_cast<uint64_t>(KVIP_DRAFT_MAX_BATCH) * kvip::kTicketWords * sizeof(uint32_t) +
+           static_cast<uint64_t>(batch) * kvip::verify_parts(vocab) * sizeof(double);
 }
 
 extern "C" uint32_t kvip_hip_verify_drafts(const KvipVerifyArgs* a, void* stream) {

@@ -271,3 +271,27 @@ def test_rows_without_any_weight_still_have_no_token(torch_gpu):
         op = run_verify(torch, case, nodes=len(tokens), vocab=5000)
         check_verify(case, op, nodes=len(tokens))
         assert op.out_tokens[:, 0].tolist() == [-1, -1] and int(op.status.item()) == abi.STATUS_BAD_PROBS
+
+
+# --- one workspace, several shapes ------------------------------------------------------------
+
+
+def test_a_workspace_serves_calls_of_other_shapes(torch_gpu):
+    """One buffer, cleared once and large enough for each, under calls of different batches and vocabularies."""
+    torch = torch_gpu
+    say("case shared workspace")
+    rng = np.random.default_rng(31)
+    shapes = [(3, 40000), (40, 300), (20, 9001), (1, 100003), (200, 5000)]
+    made = []
+    for batch, vocab in shapes:
+        case = verify_case(torch, rng, [3] * batch, vocab, "chain", "bf16")
+        made.append((case, run_verify(torch, case, nodes=3, vocab=vocab)))
+    words = max(op.workspace.numel() for _, op in made)
+    shared = torch.zeros(words, dtype=torch.int64, device="cuda")
+    for _, op in made:
+        op.args.workspace = shared.data_ptr()
+    for k in (0, 1, 2, 1, 3, 4, 0, 2, 4, 1):
+        case, op = made[k]
+        op.out_tokens.fill_(-9)
+        check_verify(case, op, nodes=3)
+        assert int(op.status.item()) == 0
