@@ -135,8 +135,9 @@ typedef struct KvipRotaryArgs {
 
 /* Rows of the paged KV cache (656 bytes: 512 fp8 e4m3 features, 64 bf16 rotary features, four fp32
  * scales). Token t's row goes to slot slots[t] (negative: none; past the cache: KVIP_STATUS_BAD_TOKEN
- * and none): for each 128 latent features scale = largest magnitude / 448 (1 where that is 0) and
- * features rounded from latent / scale; the rotary features turned as above (positions given) or
+ * and none): for each 128 latent features scale = largest magnitude / 448 (1 where that quotient is 0) and
+ * features rounded from latent / scale. A NaN stays one and does not count for the scale; an infinity makes its
+ * group's scale infinite and itself a NaN. The rotary features turned as above (positions given) or
  * as they are (NULL). Slots of one call differ. */
 typedef struct KvipRowStoreArgs {
     const void* latent;           /* [tokens, 512], rows latent_stride elements apart */

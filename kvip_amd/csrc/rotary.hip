@@ -155,7 +155,8 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(const Kvip
         largest = fmaxf(largest, fabsf(x[e]));
     }
     largest = row16_max(largest);
-    const float scale = largest > 0.f ? largest / 448.f : 1.f;
+    const float quotient = largest / 448.f;  // 0 for the smallest magnitudes too, below 3.2e-43
+    const float scale = quotient > 0.f ? quotient : 1.f;
     int packed[2] = {0, 0};
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {

@@ -40,21 +40,22 @@ _CODES = np.asarray([fp8_e4m3_decode(np.asarray([c], np.uint8))[0] for c in rang
 
 
 def e4m3_bytes(values):
-    """float32 within +-448 -> e4m3 bytes, to the nearest code, halves to the even one."""
+    """float32 within +-448 or NaN -> e4m3 bytes, to the nearest code, halves to the even one."""
     x = np.abs(np.asarray(values, np.float64))
     hi = np.clip(np.searchsorted(_CODES, x), 1, 126)
     lo = hi - 1
     below, above = x - _CODES[lo], _CODES[hi] - x
     code = np.where((below < above) | ((below == above) & (lo % 2 == 0)), lo, hi)
-    return (code | (np.signbit(values) * 128)).astype(np.uint8)
+    return (np.where(np.isnan(x), 127, code) | (np.signbit(values) * 128)).astype(np.uint8)
 
 
 def stored_rows(latent):
     """(codes uint8 [n, 512], scales float32 [n, 4]) of latents [n, 512]."""
     x = np.asarray(latent, np.float32).reshape(-1, 4, 128)
-    largest = np.abs(x).max(2)
-    scales = np.where(largest > 0, largest / np.float32(448), np.float32(1)).astype(np.float32)
-    return e4m3_bytes(np.clip(x / scales[:, :, None], -448, 448)).reshape(-1, 512), scales
+    scales = np.fmax.reduce(np.abs(x), axis=2) / np.float32(448)  # of the numbers among them
+    scales = np.where(scales > 0, scales, np.float32(1)).astype(np.float32)
+    with np.errstate(invalid="ignore"):  # an infinity over its own scale
+        return e4m3_bytes(np.clip(x / scales[:, :, None], -448, 448)).reshape(-1, 512), scales
 
 
 def row_parts(rows):

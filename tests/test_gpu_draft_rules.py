@@ -295,3 +295,39 @@ def test_a_workspace_serves_calls_of_other_shapes(torch_gpu):
         op.out_tokens.fill_(-9)
         check_verify(case, op, nodes=3)
         assert int(op.status.item()) == 0
+
+
+# --- latents at the ends of their range -------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_latents_below_and_past_the_range(torch_gpu, dtype):
+    """Groups whose largest magnitude over 448 is 0 in 32 bits are zeros with scale 1, not 0 / 0; a NaN stays in its
+    feature, an infinity makes its scale infinite and itself a NaN; all as the restatement has them."""
+    torch = torch_gpu
+    say(f"case latents at the ends {dtype}")
+    rng = np.random.default_rng(7)
+    t = dtype_of(torch, dtype)
+    tops = [1e-45, 1e-43, 3.1e-43, 3.2e-43, 1e-41, 1e-38, 1e-30, 6e-8, 1e-7, 1.0, 6e4, 3e38]
+    x = rng.uniform(-1, 1, (len(tops) + 3, 512)).astype(np.float32)
+    for i, top in enumerate(tops):
+        x[i] *= np.float32(0.5 * top)
+        x[i, ::128] = np.float32(top)
+        x[i, 1::128] = 0.0
+    x[-3, 5], x[-3, 200:384] = np.nan, np.nan
+    x[-2, 130], x[-2, 131] = np.inf, np.nan
+    x[-1, 400] = -np.inf
+    latent = torch.from_numpy(x).to(t).cuda()
+    rope = torch.zeros((len(x), 64), dtype=t, device="cuda")
+    kv = torch.zeros((1, 128, ROW), dtype=torch.uint8, device="cuda")
+    op = kvip_amd.KvRowStore(torch, kv_cache=kv)
+    op.bind(latent, rope, torch.arange(len(x), device="cuda"))()
+    values = latent.float().cpu().numpy()
+    codes, scales = draft.stored_rows(values)
+    got = kv[0, :len(x)].cpu().numpy()
+    assert np.array_equal(got[:, 640:656].copy().view("<f4"), scales)
+    none = (codes & 127) == 127
+    assert np.array_equal((got[:, :512] & 127) == 127, none) and np.array_equal(got[:, :512][~none], codes[~none])
+    finite = np.isfinite(values).all(1)
+    assert not none[finite].any() and none[~finite].any(1).all()
+    assert int(op.status.item()) == 0

@@ -168,3 +168,17 @@ def test_tokens_of_a_target_drafted_whole_are_distributed_as_it():
     for u in (np.arange(grid) + 0.5) / grid:
         got[draft.verify(np.stack([p] * 4), [0, 2, 0, 1], [-1, 0, 0, 0], None, [u, 0, 0, 0], 0.0)[1][0]] += 1 / grid
     assert math.isclose(got.sum(), 1.0) and np.all(np.abs(got - p) <= (1 - p.sum()) + 1 / grid) and np.all(got >= p - 1 / grid)
+
+
+def test_rows_of_the_smallest_and_largest_latents():
+    latent = np.zeros((4, 512), np.float32)
+    latent[0, ::128], latent[0, 5] = 3.1e-43, -1e-45  # over 448: 0 in 32 bits
+    latent[1, ::128] = 3.2e-43                        # over 448: the least number there is
+    latent[2, 3], latent[2, 4], latent[2, 128:256] = np.nan, 2.0, np.nan
+    latent[3, 300], latent[3, 301] = -np.inf, 1.0
+    bytes_, scales = draft.stored_rows(latent)
+    assert np.all(scales[0] == 1) and not (bytes_[0] & 127).any()
+    assert np.all(scales[1] == np.float32(1e-45)) and (bytes_[1] & 127).max() < 127
+    assert scales[2].tolist() == [np.float32(2 / 448), 1, 1, 1] and np.all(bytes_[2, 128:256] & 127 == 127)
+    assert bytes_[2, 3] & 127 == 127 and bytes_[2, 4] == 126
+    assert np.isinf(scales[3, 2]) and bytes_[3, 300] & 127 == 127 and not (np.delete(bytes_[3], 300) & 127).any()
