@@ -785,6 +785,13 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
             }
             values(slot, std::false_type{});
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
+            // A seen scale that is not finite: where it made a logit -infinity, the probability 0 times the scale left
+            // NaN in all of the scale group's features, but in no other.
+#pragma unroll
+            for (int gr = 0; gr < kScaleGroups; ++gr) {
+                hold(o[4 * gr]);
+                if (o[4 * gr][0] != o[4 * gr][0]) l_sum = NAN;
+            }
 
             const int le = fresh(lane), hn = le & 31, hk = le >> 5;  // not held over the tiles
             const int row = first_row + hn;

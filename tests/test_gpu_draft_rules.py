@@ -331,3 +331,26 @@ def test_latents_below_and_past_the_range(torch_gpu, dtype):
     finite = np.isfinite(values).all(1)
     assert not none[finite].any() and none[~finite].any(1).all()
     assert int(op.status.item()) == 0
+
+
+# --- scales that are not finite ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,counts,contexts,at", [
+    (16, [3, 2, 1], [300, 200, 90], [10, 40]), (128, [2, 1, 3], [700, 500, 40], [600, 3]), (16, [1, 1, 1], [127, 64, 31], [0, 40]),
+    (40, [7, 5, 2], [20000, 9000, 300], [12000, 8900]), (8, [4] * 60, [400] * 60, [100, 399])])
+def test_a_seen_scale_that_is_not_finite(torch_gpu, heads, counts, contexts, at):
+    """Rows before the step, which every token sees: the first request holds an infinite scale, the second a
+    negative one, and each token and head of theirs is NaN as a whole, whatever sign its products have."""
+    say(f"case infinite scale heads={heads} counts={counts[:3]} contexts={contexts[:3]}")
+    step = Step(torch_gpu, np.random.default_rng(heads + contexts[0]), counts, contexts, heads)
+    scales = step.rows[:, 640:656].copy().view("<f4")
+    scales[step.slot(0, at[0]), 1] = np.inf
+    scales[step.slot(1, at[1]), 3] = -np.inf
+    step.rows[:, 640:656] = scales.view(np.uint8)
+    for output in ("bf16", "fp32"):
+        op = step.run(output=output)
+        step.check(op, output=output, only=range(2, len(counts)))
+        bad = slice(0, int(step.cu[2]))
+        assert bool(op.output[bad].isnan().all()) and bool(op.lse[bad].isnan().all())
+        assert int(op.status.item()) == 0
