@@ -39,7 +39,8 @@ extern "C" {
 #define KVIP_DRAFT_MAX_TOKENS (1 << 20)
 
 /* A paged cache whose rows kvip_hip_page_tables_move copies: row of slot s (block s / 128, s % 128)
- * at base + (s / 128) * block_stride + (s % 128) * row_stride. All in bytes, multiples of 4. */
+ * at base + (s / 128) * block_stride + (s % 128) * row_stride. All in bytes, multiples of 4; no row
+ * lies over another. */
 typedef struct KvipPagedRows {
     int64_t base;
     int64_t block_stride;

@@ -24,13 +24,14 @@ class PageTables:
     """batch: requests (1..1024, a request that is not there has length 0); max_context: positions of a
     request; num_blocks: pages of the cache, all free at first and taken from 0 up; max_tokens: rows
     of a step; caches: the paged tensors [num_blocks, 128, ...] (rows contiguous, a multiple of 4
-    bytes) whose rows `commit(kept, path)` copies together: the KV rows, index keys and
+    bytes, none over another) whose rows `commit(kept, path)` copies together: the KV rows, index keys and
     scales of every layer.
 
     block_table int32 [batch, blocks], lengths int32 [batch], free int32 [num_blocks] and free_count int32
     [1] are the state; steps int32 [batch] has the tokens that the last extend appended (0 where it refused a
-    request, whose rows stay in the step: TreeAttention and DraftVerifier take `steps` to leave it out); cu_seqlens int32 [batch + 1], positions, slots, visible int64 [max_tokens] the last step's
-    layout; status int32 [1] collects KVIP_STATUS_* bits."""
+    request, whose rows stay in the step: TreeAttention and DraftVerifier take `steps` to leave it out); cu_seqlens
+    int32 [batch + 1], positions, slots, visible int64 [max_tokens] the last step's layout; status int32 [1] collects
+    KVIP_STATUS_* bits."""
 
     def __init__(self, torch, *, batch, max_context, num_blocks, max_tokens, device, caches=()):
         abi.require(1 <= batch <= abi.DRAFT_MAX_BATCH, f"batch must be in 1..{abi.DRAFT_MAX_BATCH}")
@@ -42,6 +43,7 @@ class PageTables:
         self.batch, self.num_blocks, self.max_tokens = int(batch), int(num_blocks), int(max_tokens)
         self.max_blocks = (int(max_context) + BLOCK_TOKENS - 1) // BLOCK_TOKENS
         rows = [self._rows(c) for c in caches]
+        abi.require(len({base for base, *_ in rows}) == len(rows), "a cache must not be named twice")
         self.caches = tuple(caches)
 
         def ints(*shape, dtype=torch.int32):
@@ -76,8 +78,12 @@ class PageTables:
             abi.require(n == 1 or stride == width, "a cache's rows must be contiguous")
             width *= n
         found = (cache.data_ptr(), cache.stride(0) * size, cache.stride(1) * size, width * size)
-        abi.require(all(v % 4 == 0 for v in found) and found[2] >= found[3] and width >= 1,
+        abi.require(all(v % 4 == 0 for v in found) and width >= 1,
                     "a cache's address, strides and rows must be multiples of 4 bytes")
+        _, block, row, size = found
+        places, pages = row * (BLOCK_TOKENS - 1), block * (self.num_blocks - 1)  # from the first to the last
+        apart = row >= size and (self.num_blocks == 1 or block >= places + size or (block >= size and row >= pages + size))
+        abi.require(apart, "a cache's rows must not overlap")
         return found
 
     def _ints(self, x, shape, what):

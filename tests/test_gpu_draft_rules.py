@@ -354,3 +354,39 @@ def test_a_seen_scale_that_is_not_finite(torch_gpu, heads, counts, contexts, at)
         bad = slice(0, int(step.cu[2]))
         assert bool(op.output[bad].isnan().all()) and bool(op.lse[bad].isnan().all())
         assert int(op.status.item()) == 0
+
+
+# --- rows of the tables' caches ---------------------------------------------------------------
+
+
+def test_caches_whose_rows_overlap_are_refused(torch_gpu):
+    torch = torch_gpu
+    make = dict(batch=2, max_context=512, num_blocks=4, max_tokens=16, device="cuda")
+    flat = torch.zeros(8 * 128 * 16, dtype=torch.uint8, device="cuda")
+    one = flat[:128 * 16].view(1, 128, 16)
+    for cache in (one.expand(4, 128, 16), flat.as_strided((4, 128, 16), (64 * 16, 16, 1)), flat.as_strided((4, 128, 16), (127 * 16, 16, 1)),
+                  flat.as_strided((4, 128, 16), (8, 64, 1)), flat[:16].expand(4, 128, 16)):
+        with pytest.raises(ValueError):
+            kvip_amd.PageTables(torch, **make, caches=[cache])
+    # Places first, pages in between, one page, rows with room behind them: no row overlaps another.
+    good = [flat[:128 * 4 * 16].view(128, 4, 16).transpose(0, 1), flat.view(4, 2, 128, 16)[:, 1], flat.as_strided((4, 128, 16), (128 * 20, 20, 1)),
+            flat.as_strided((4, 128, 16), (127 * 20 + 16, 20, 1))]
+    for cache in good:
+        kvip_amd.PageTables(torch, **make, caches=[cache])
+    kvip_amd.PageTables(torch, **{**make, "num_blocks": 1}, caches=[one])
+    kvip_amd.PageTables(torch, **make, caches=[good[0][..., :8], good[0][..., 8:]])
+    for twice in ([good[0], good[0]], [good[0], good[1], good[0][..., :4]]):
+        with pytest.raises(ValueError):
+            kvip_amd.PageTables(torch, **make, caches=twice)
+
+
+def test_rows_move_in_a_cache_of_places_first(torch_gpu):
+    torch = torch_gpu
+    say("case places first")
+    data = (torch.arange(128 * 4 * 16, device="cuda") % 251).to(torch.uint8).view(128, 4, 16)
+    want = data.clone()
+    op = kvip_amd.PageTables(torch, batch=1, max_context=512, num_blocks=4, max_tokens=16, device="cuda", caches=[data.transpose(0, 1)])
+    op.extend(device(torch, [6], torch.int32))
+    op.commit(device(torch, [3], torch.int32), device(torch, [[0, 2, 5]], torch.int32))
+    want[1, 0], want[2, 0] = want[2, 0].clone(), want[5, 0].clone()
+    assert torch.equal(data, want) and int(op.status.item()) == 0
