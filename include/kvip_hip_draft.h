@@ -76,7 +76,8 @@ typedef struct KvipPagedRows {
  * kvip_hip_page_tables_move copies the rows of the kept tokens together, before a truncate with
  * `kept`: for i < targets[b], position bases[b] + i gets the rows of position bases[b] +
  * path[b][i], in `row_sets` caches. A path rises strictly and stays below steps[b], else the
- * copying of that request stops there and KVIP_STATUS_BAD_TREE is set. */
+ * copying of that request stops there and KVIP_STATUS_BAD_TREE is set. A target above path_stride
+ * sets KVIP_STATUS_BAD_LENGTH: rows past the path's places stay where they are. */
 typedef struct KvipPageTableArgs {
     int32_t* block_table;         /* [batch, max_blocks] */
     int32_t* lengths;             /* [batch] */

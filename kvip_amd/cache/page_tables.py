@@ -107,7 +107,7 @@ class PageTables:
         """Keeps kept[b] tokens of the last step (int32 [batch], at most those appended) and gives back
         the pages of the rest. path int32 [batch, places], as kvip_amd.DraftVerifier returns it, names the
         kept tokens of trees: their rows in `caches` are copied together first (without it the first
-        kept[b] are kept). Returns lengths."""
+        kept[b] are kept; more kept than places set a status bit). Returns lengths."""
         a = self._args  # copied by the launch
         a.targets, a.kept = self._ints(kept, (self.batch,), "kept"), 1
         if path is not None:

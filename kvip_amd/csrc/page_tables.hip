@@ -267,56 +267,67 @@ __global__ __launch_bounds__(kTableThreads) void truncate_tables_kernel(const Kv
 
 // One workgroup per (request, cache). A thread takes the same 4 bytes of every row, so the rows that it
 // still has to read are never ones that it has written: rows are read 8 at a time, and the row at
-// place i comes from a place >= i.
+// place i comes from a place >= i. A path is looked up 64 places at a time.
 constexpr int kMoveAhead = 8;
+constexpr int kMovePlaces = 64;
 __global__ __launch_bounds__(256) void move_rows_kernel(const KvipPageTableArgs p) {
-    __shared__ int64_t s_from[KVIP_DRAFT_MAX_NODES], s_to[KVIP_DRAFT_MAX_NODES];  // slots
+    __shared__ int64_t s_from[kMovePlaces], s_to[kMovePlaces];  // slots
     __shared__ int s_count;
     const int b = blockIdx.x, tid = threadIdx.x;
     const int capacity = p.max_blocks * kBlockTokens;
     const int base = clamp_int(p.bases[b], 0, capacity);
     const int step = min(p.steps[b], capacity - base);
-    const int want = clamp_int(p.targets[b], 0, min(min(max(step, 0), p.path_stride), KVIP_DRAFT_MAX_NODES));
-    if (tid < 64) {
-        const int32_t* table = p.block_table + static_cast<int64_t>(b) * p.max_blocks;
-        const int node = tid < want ? p.path[static_cast<int64_t>(b) * p.path_stride + tid] : -1;
-        const int before = __shfl_up(node, 1);
-        bool ok = tid < want && node >= 0 && node < step && (tid == 0 || node > before);
-        int64_t from = 0, to = 0;
-        uint32_t err = tid < want && !ok ? KVIP_STATUS_BAD_TREE : 0u;
-        if (ok) {
-            const int src = base + node, dst = base + tid;
-            const int src_page = table[src / kBlockTokens], dst_page = table[dst / kBlockTokens];
-            ok = static_cast<unsigned>(src_page) < static_cast<unsigned>(p.num_blocks) &&
-                 static_cast<unsigned>(dst_page) < static_cast<unsigned>(p.num_blocks);
-            if (!ok) err = KVIP_STATUS_BAD_BLOCK;
-            from = static_cast<int64_t>(src_page) * kBlockTokens + src % kBlockTokens;
-            to = static_cast<int64_t>(dst_page) * kBlockTokens + dst % kBlockTokens;
-        }
-        s_from[tid] = from;
-        s_to[tid] = to;
-        const unsigned long long bad = __ballot(tid < want && !ok);
-        if (tid == 0) s_count = bad != 0 ? __ffsll(bad) - 1 : want;  // the rows before the first bad one
-        if (blockIdx.y == 0) report(p.status, err);
-    }
-    __syncthreads();
+    const int kept = clamp_int(p.targets[b], 0, max(step, 0));
+    const int want = min(kept, p.path_stride);
+    if (tid == 0 && blockIdx.y == 0 && want < kept) report(p.status, KVIP_STATUS_BAD_LENGTH);
+    const int32_t* table = p.block_table + static_cast<int64_t>(b) * p.max_blocks;
+    const int32_t* path = p.path + static_cast<int64_t>(b) * p.path_stride;
     const KvipPagedRows c = p.rows[blockIdx.y];
-    const int count = s_count;
     auto at = [&](int64_t slot) {
         return reinterpret_cast<uint32_t*>(c.base + slot / kBlockTokens * c.block_stride + slot % kBlockTokens * c.row_stride);
     };
-    for (int64_t w = tid; w < c.row_bytes / 4; w += 256) {
-        for (int i = 0; i < count; i += kMoveAhead) {
-            uint32_t v[kMoveAhead];
-#pragma unroll
-            for (int k = 0; k < kMoveAhead; ++k) {
-                if (i + k < count) v[k] = at(s_from[i + k])[w];
+    for (int first = 0; first < want; first += kMovePlaces) {
+        if (tid < kMovePlaces) {
+            const int place = first + tid;
+            const bool named = place < want;
+            const int node = named ? path[place] : -1;
+            const int before = named && place > 0 ? path[place - 1] : -1;
+            bool ok = named && node >= 0 && node < step && node > before;
+            int64_t from = 0, to = 0;
+            uint32_t err = named && !ok ? KVIP_STATUS_BAD_TREE : 0u;
+            if (ok) {
+                const int src = base + node, dst = base + place;
+                const int src_page = table[src / kBlockTokens], dst_page = table[dst / kBlockTokens];
+                ok = static_cast<unsigned>(src_page) < static_cast<unsigned>(p.num_blocks) &&
+                     static_cast<unsigned>(dst_page) < static_cast<unsigned>(p.num_blocks);
+                if (!ok) err = KVIP_STATUS_BAD_BLOCK;
+                from = static_cast<int64_t>(src_page) * kBlockTokens + src % kBlockTokens;
+                to = static_cast<int64_t>(dst_page) * kBlockTokens + dst % kBlockTokens;
             }
+            s_from[tid] = from;
+            s_to[tid] = to;
+            const unsigned long long bad = __ballot(named && !ok);
+            // The rows before the first bad one.
+            if (tid == 0) s_count = bad != 0 ? __ffsll(bad) - 1 : min(want - first, kMovePlaces);
+            if (blockIdx.y == 0) report(p.status, err);
+        }
+        __syncthreads();
+        const int count = s_count;
+        for (int64_t w = tid; w < c.row_bytes / 4; w += 256) {
+            for (int i = 0; i < count; i += kMoveAhead) {
+                uint32_t v[kMoveAhead];
 #pragma unroll
-            for (int k = 0; k < kMoveAhead; ++k) {
-                if (i + k < count) at(s_to[i + k])[w] = v[k];
+                for (int k = 0; k < kMoveAhead; ++k) {
+                    if (i + k < count) v[k] = at(s_from[i + k])[w];
+                }
+#pragma unroll
+                for (int k = 0; k < kMoveAhead; ++k) {
+                    if (i + k < count) at(s_to[i + k])[w] = v[k];
+                }
             }
         }
+        if (count < kMovePlaces) break;  // uniform: the path's end, or a bad place
+        __syncthreads();
     }
 }
 

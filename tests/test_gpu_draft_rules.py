@@ -390,3 +390,37 @@ def test_rows_move_in_a_cache_of_places_first(torch_gpu):
     op.commit(device(torch, [3], torch.int32), device(torch, [[0, 2, 5]], torch.int32))
     want[1, 0], want[2, 0] = want[2, 0].clone(), want[5, 0].clone()
     assert torch.equal(data, want) and int(op.status.item()) == 0
+
+
+# --- paths of many places ---------------------------------------------------------------------
+
+
+def test_paths_longer_than_a_tree_move_every_row(torch_gpu):
+    """A chain has no limit of 64 tokens, nor has the path that names those kept; a path that falls behind place 64
+    stops there, and a count above the path's places is reported."""
+    torch = torch_gpu
+    say("case long paths")
+    rng = np.random.default_rng(17)
+    kept, steps, places = [150, 64, 65, 200, 129], [300, 200, 66, 201, 140], 150
+    cache = torch.from_numpy(rng.integers(0, 256, (30, 128, 656))).to(torch.uint8).cuda()
+    op = kvip_amd.PageTables(torch, batch=5, max_context=512, num_blocks=30, max_tokens=1000, device="cuda", caches=[cache])
+    op.extend(device(torch, [100, 0, 127, 5, 90], torch.int32))
+    op.commit(op.steps.clone())
+    op.extend(device(torch, steps, torch.int32))
+    path = np.full((5, places), -1, np.int32)
+    for b in range(5):
+        n = min(kept[b], places)
+        path[b, :n] = np.sort(rng.choice(steps[b], n, replace=False))
+    path[4, 100] = path[4, 99]  # does not rise
+    table, bases = op.block_table.cpu().numpy().copy(), op.bases.tolist()
+    rows = cache.cpu().numpy().copy().reshape(-1, 656)
+    assert int(op.status.item()) == 0
+    op.commit(device(torch, kept, torch.int32), device(torch, path, torch.int32))
+    assert int(op.status.item()) == abi.STATUS_BAD_TREE | abi.STATUS_BAD_LENGTH
+    assert op.lengths.tolist() == [n + k for n, k in zip(bases, kept)]
+    want = rows.copy()
+    for b, n in enumerate((150, 64, 65, 150, 100)):
+        for i in range(n):
+            src, dst = bases[b] + path[b, i], bases[b] + i
+            want[table[b, dst // 128] * 128 + dst % 128] = rows[table[b, src // 128] * 128 + src % 128]
+    assert np.array_equal(cache.cpu().numpy().reshape(want.shape), want)
