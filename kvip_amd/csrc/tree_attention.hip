@@ -197,13 +197,15 @@ struct TaRequest {
 
 KVIP_DEVICE TaRequest ta_request(const KvipTreeAttnArgs& p, int b, uint32_t* err) {
     TaRequest q;
-    q.begin = min(max(p.cu_seqlens[b], 0), p.max_tokens);
-    const int all = min(max(p.cu_seqlens[b + 1], q.begin), p.max_tokens) - q.begin;
+    const int first = p.cu_seqlens[b], behind = p.cu_seqlens[b + 1];
+    q.begin = min(max(first, 0), p.max_tokens);
+    const int all = min(max(behind, q.begin), p.max_tokens) - q.begin;
     const int given = p.seq_lens[b];
     const bool refused = p.steps != nullptr && p.steps[b] <= 0;
     q.nodes = min(all, p.max_nodes);
     q.length = refused ? 0 : min(max(given, 0), p.max_blocks * kBlockTokens);
     q.past = q.length - all;
+    if (first != q.begin || behind != q.begin + all) *err |= KVIP_STATUS_BAD_LENGTH;
     if (all != q.nodes || (!refused && (given != q.length || (all > 0 && q.past < 0)))) *err |= KVIP_STATUS_BAD_LENGTH;
     return q;
 }

@@ -155,11 +155,12 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const KvipVerifyArgs p)
     __shared__ double s_wave[THREADS / 64], s_before, s_left;
     __shared__ int s_last, s_part, s_found, s_near, s_count, s_gone[KVIP_DRAFT_MAX_NODES];
     const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int begin = min(max(p.cu_seqlens[b], 0), p.max_tokens);
+    const int first = p.cu_seqlens[b], behind = p.cu_seqlens[b + 1];
+    const int begin = min(max(first, 0), p.max_tokens), end = min(max(behind, begin), p.max_tokens);
     const bool refused = p.steps != nullptr && p.steps[b] <= 0;
-    const int all = refused ? 0 : min(max(p.cu_seqlens[b + 1], begin), p.max_tokens) - begin;
+    const int all = refused ? 0 : end - begin;
     const int n = min(all, p.max_nodes);
-    if (part == 0 && tid == 0 && all > n) report(p.status, KVIP_STATUS_BAD_LENGTH);
+    if (part == 0 && tid == 0 && (all > n || begin != first || end != behind)) report(p.status, KVIP_STATUS_BAD_LENGTH);
     if (n == 0) {  // uniform over the request's workgroups: its ticket is not used
         if (part == 0 && tid < p.max_nodes) {
             p.path[static_cast<int64_t>(b) * p.max_nodes + tid] = -1;

@@ -424,3 +424,37 @@ def test_paths_longer_than_a_tree_move_every_row(torch_gpu):
             src, dst = bases[b] + path[b, i], bases[b] + i
             want[table[b, dst // 128] * 128 + dst % 128] = rows[table[b, src // 128] * 128 + src % 128]
     assert np.array_equal(cache.cpu().numpy().reshape(want.shape), want)
+
+
+# --- row counts that leave the arrays ---------------------------------------------------------
+
+
+def test_rows_past_the_arrays_are_reported(torch_gpu):
+    """cu_seqlens that go past the rows of the query or the probabilities, or fall: reported, and the requests that
+    lie in the arrays as ever."""
+    torch = torch_gpu
+    say("case rows past the arrays")
+    step = Step(torch, np.random.default_rng(3), [3, 4, 2], [100, 200, 50], 16)
+    op = step.run(nodes=4)
+    query, kv, table, lens, cu, visible = op._bound[:6]
+    for ends in ([0, 3, 7, step.tokens + 1], [0, 3, 7, 6], [0, 3, 7, 1 << 30]):
+        op.status.zero_()
+        op.bind(query, kv, table, lens, device(torch, ends, torch.int32), visible)
+        q, got = step.query.double().numpy(), host(op())
+        for b in (0, 1):
+            rows = step.rows[[step.slot(b, p) for p in range(step.lens[b])]]
+            for i in range(step.counts[b]):
+                at, sees = step.cu[b] + i, np.ones(step.lens[b], bool)
+                sees[step.contexts[b]:] = [bool(int(step.bits[at]) >> j & 1) for j in range(step.counts[b])]
+                want, _, bound, _ = draft.tree_attention(q[at], rows, sees, SCALE)
+                assert np.all(np.abs(got[at] - want) <= bound + np.abs(want) * HALF_STEP["bf16"])
+        assert int(op.status.item()) == abi.STATUS_BAD_LENGTH, ends
+    case = verify_case(torch, np.random.default_rng(4), [3, 4, 2], 500, "chain", "fp32")
+    for ends in ([0, 3, 7, 12], [0, 3, 7, 6], [0, 3, 7, 1 << 30]):
+        op = run_verify(torch, {**case, "cu": np.asarray(ends)}, nodes=5, vocab=500)
+        op()
+        assert int(op.status.item()) & abi.STATUS_BAD_LENGTH, ends
+        first = run_verify(torch, case, nodes=5, vocab=500)
+        first()
+        assert int(first.status.item()) == 0
+        assert torch.equal(op.out_tokens[:2], first.out_tokens[:2]) and torch.equal(op.path[:2], first.path[:2])
