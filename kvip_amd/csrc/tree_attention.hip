@@ -350,9 +350,9 @@ __global__ __launch_bounds__(kTaThreads, 1) void tree_attention_kernel(const Kvi
     const TaWork<R> work(p.workspace, shares);
     const uint32_t ring_lds = lds_addr(s_mem) + st * kTaSlot;
     // Logits are kept as they come and scaled on their way into the exponential. A negative scale turns the
-    // query's signs; one of 0 becomes 2^-100, which no logit shows.
+    // query's signs; one of 0 becomes 2^-126, which no logit below 10^32 shows.
     const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(
-        __float_as_int(fmaxf(fabsf(p.scale * kLog2e), 0x1p-100f))));
+        __float_as_int(fmaxf(fabsf(p.scale * kLog2e), 0x1p-126f))));
     const int flip = p.scale < 0.f ? static_cast<int>(0x80008000u) : 0;
     const int row_stride = p.row_stride;
 

@@ -458,3 +458,18 @@ def test_rows_past_the_arrays_are_reported(torch_gpu):
         first()
         assert int(first.status.item()) == 0
         assert torch.equal(op.out_tokens[:2], first.out_tokens[:2]) and torch.equal(op.path[:2], first.path[:2])
+
+
+# --- a scale of zero --------------------------------------------------------------------------
+
+
+def test_a_zero_scale_weighs_all_rows_alike(torch_gpu):
+    """Also where the products that it is applied to are 10^31."""
+    say("case zero scale")
+    step = Step(torch_gpu, np.random.default_rng(23), [3, 2], [260, 70], 16)
+    scales = step.rows[:, 640:656].copy().view("<f4")
+    step.rows[:, 640:656] = (scales * np.float32(1e30)).view(np.uint8)
+    for scale in (0.0, -0.0):
+        op = step.run(scale=scale)
+        step.check(op, scale=scale)
+        assert int(op.status.item()) == 0
