@@ -5,9 +5,10 @@ of a paged cache, and lays out a step from the request lengths without a host re
 appends tokens (pages, slots, positions, the visibility of a tree's tokens), `commit(kept)` keeps the
 accepted ones and gives the other pages back, `truncate(lengths)` shortens or ends requests. The
 tensors feed the operators of the same step: `cu_seqlens`, `lengths`, `block_table`, `visible` and `steps` go to
-`kvip_amd.TreeAttention` (`block_table`, `lengths` and `cu_seqlens` also to `kvip_amd.PrefillIndexer`), `slots` and
-`positions` to `kvip_amd.KvRowStore` and `kvip_amd.Rotary`, `slots` to `IndexCacheStorage` as its slot
-mapping. `include/kvip_hip_draft.h` states the rules. Calls only enqueue on the current stream
+`kvip_amd.TreeAttention`, `slots` and `positions` to `kvip_amd.KvRowStore` and `kvip_amd.Rotary`. Steps of chains (and
+prompt chunks) also feed the selection: `block_table`, `lengths` and `cu_seqlens` go to `kvip_amd.PrefillIndexer`, `slots` to
+`kvip_amd.IndexCacheStorage` as its slot mapping. Trees do not: that indexer lets a row see every row of the step before
+it, siblings among them, and siblings share a position. `include/kvip_hip_draft.h` states the rules. Calls only enqueue on the current stream
 and allocate nothing, so they can be captured; one object's calls follow one another (they share its
 state). There is no CPU path and no counterpart in the reference, whose engine does this on the host.
 """

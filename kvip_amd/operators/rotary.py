@@ -108,7 +108,8 @@ class Rotary:
         """positions int64 [tokens]; query (and key) [tokens, heads, dim] or [tokens, dim] of one type (bf16,
         fp16, fp32), dim >= rotary_dim, strided as long as the last dimension is contiguous. Without an
         output the array is turned in place; with one, features behind rotary_dim are copied. An output
-        does not overlap another array. inverse: turned back (also the gradient of a turn)."""
+        does not overlap another array. inverse: turned by the negative angle, times the same magnitude: the gradient
+        of a turn, and what undoes it where the magnitude is 1 (else up to the magnitude's square)."""
         t = self.torch
         abi.require(positions.dtype == t.int64 and positions.dim() == 1 and positions.is_contiguous() and
                     positions.device == self.device, f"positions must be contiguous int64 [tokens] on {self.device}")

@@ -473,3 +473,53 @@ def test_a_zero_scale_weighs_all_rows_alike(torch_gpu):
         op = step.run(scale=scale)
         step.check(op, scale=scale)
         assert int(op.status.item()) == 0
+
+
+# --- the tables' tensors in the framework's indexer -------------------------------------------
+
+
+def test_the_indexer_selects_by_the_tables(torch_gpu):
+    """A step of chains: kvip_amd.PrefillIndexer on the tables' cu_seqlens, lengths and block_table selects what it
+    selects with the same made on the host, and a row sees the context and the step's rows up to its own."""
+    torch = torch_gpu
+    say("case indexer by the tables")
+    rng = np.random.default_rng(29)
+    before, counts = [700, 3000, 0, 130], [5, 12, 3, 1]
+    op = kvip_amd.PageTables(torch, batch=4, max_context=4096, num_blocks=60, max_tokens=4000, device="cuda")
+    model = draft.Tables(4, 32, 60, 4000)
+    for step in (before, counts):
+        op.extend(device(torch, step, torch.int32))
+        model.extend(step)
+        if step is before:
+            op.commit(op.steps.clone())
+            model.commit(before)
+    rows = sum(counts)
+    query = torch.randn((rows, 64, 128), device="cuda").to(torch.float8_e4m3fn)
+    key = torch.randn((60, 128, 128), device="cuda").to(torch.float8_e4m3fn)
+    weights = torch.randn((rows, 64), device="cuda")
+    table = np.zeros((4, 32), np.int32)
+    for b, pages in enumerate(model.pages):
+        table[b, :len(pages)] = pages
+    indexer = kvip_amd.PrefillIndexer(torch, max_rows=rows, max_context=4096, max_sequences=4, device="cuda")
+    host_made = (device(torch, np.concatenate([[0], np.cumsum(counts)]), torch.int32), device(torch, model.lengths, torch.int32),
+                 device(torch, table, torch.int32))
+    want = indexer(query, weights, None, key, None, *host_made).clone()
+    got = indexer(query, weights, None, key, None, op.cu_seqlens, op.lengths, op.block_table)
+    assert torch.equal(got, want) and int(indexer.status.item()) == 0 and int(op.status.item()) == 0
+    at = 0
+    for b, n in enumerate(counts):
+        for i in range(n):
+            chosen = [x for x in got[at].tolist() if x >= 0]
+            assert len(set(chosen)) == len(chosen) == min(before[b] + i + 1, 2048) and max(chosen) <= before[b] + i
+            at += 1
+
+
+# --- the most rows a request can have ---------------------------------------------------------
+
+
+def test_all_heads_and_all_step_tokens(torch_gpu):
+    say("case 128 heads of 64 tokens")
+    step = Step(torch_gpu, np.random.default_rng(41), [64, 64, 1], [300, 10, 1000], 128)
+    op = step.run()
+    step.check(op)
+    assert int(op.status.item()) == 0
