@@ -5,9 +5,9 @@
 // With need_b = ceil((len_b + count_b) / 128) - ceil(len_b / 128), request b's block j past its old ones is
 // page free[top - 1 - (sum of the needs before b) - (j - old blocks)], so once the two prefix sums
 // over the batch (tokens, pages) are known, every table entry and slot is independent of the others.
-// What bounds it: latency (a few loads, two scans, one launch), then the 16 to 24 bytes written per token.
-// Extend takes 5.6 us for 64 requests with trees of 1-9 tokens, 8.4 for 300 requests of 1-700 tokens (105000
-// rows, 1.7 MB); truncate 3.9 and 4.2.
+// What bounds it: latency (a few loads, two scans, one launch), then the 24 bytes written per token.
+// Extend takes 5.5 us for 64 requests with trees of 1-9 tokens, 8.6 for 300 requests of 1-700 tokens (105000
+// rows, 2.5 MB); truncate 3.9 and 4.2.
 // Every workgroup does both scans itself (4 requests per thread, at most 1024) instead of a launch before
 // it, counts itself on a ticket when it has read the state, and writes the entries of the requests and rows that
 // it takes in turn; the last one on the ticket moves the lengths and the stack's top on. Nothing that one

@@ -28,7 +28,7 @@
 // What bounds it. Many rows per cache row (8 requests x 12 tokens x 128 heads on 2000-8192 rows: 190 us, 795
 // TFLOP/s, 125 us at the rate of a large bf16 product): the instructions between the MFMAs, 10 VALU and 1.4 LDS ones
 // per MFMA, 4 of them conversions that each of the four waves does for itself (MFMA busy 38 % of the
-// cycles, waiting 17 %), at the 2.2 to 2.4 GHz that the card holds under this load. Few rows (64
+// cycles, waiting 18 %), at the 2.2 to 2.4 GHz that the card holds under this load. Few rows (64
 // requests x 4 tokens x 16 heads on 1000-16384 rows: 126 us, 2.97 TB/s): the same loop at 2.0 GHz beside the
 // loads. Short contexts: a chain of latencies (lengths, page, tile and queries, two steps, join).
 // Dropped after measuring: two waves per SIMD that split the features (310 us for the first of these,
@@ -62,8 +62,13 @@ constexpr int kScaleGroups = 4;
 constexpr int kBlocks = kValueDim / 32;     // accumulator blocks of 32 features
 constexpr int kTaGroups = 256;              // shares: one workgroup per CU
 constexpr int kMinSteps = 2;                // steps of a share, at least: 900 cache rows take 20.8 us (1: 22.6, 3: 22.4, 4: 23.3)
-constexpr int kHeadSteps = 6;               // what an item's start costs, in steps (the queries' loads, the first tile's)
-constexpr int kJoinWaves = 8192;            // waves of the join, at most, where items allow
+// What an item's start costs, in steps (the queries' loads, the first tile's). 200 requests of 4 tokens x 16 heads on
+// 100-1500 rows take 67.5 us (3: 73.9, 4: 71.3, 8: 71.0), 40 of 8 tokens x 128 heads on 100-600 rows 94.6 (109, 98, 95);
+// long contexts move by 1 %.
+constexpr int kHeadSteps = 6;
+// Waves of the join, at most, where items allow. 80 requests of 4 tokens x 16 heads on 2000-8000 rows take 101.7 us
+// (4096: 104.0, 16384: 103.8); most other batches move by 1 %.
+constexpr int kJoinWaves = 8192;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kTaMargin = 8.0f * kLog2e;
@@ -998,6 +1003,9 @@ template <int R>
 void launch_tree(const KvipTreeAttnArgs& a, hipStream_t s) {
     const int shares = ta_shares(a.batch, a.heads, a.max_nodes, a.max_blocks);
     hipLaunchKernelGGL(tree_attention_kernel<R>, dim3(shares), dim3(kTaThreads), 0, s, a);
+    // Few groups of 32 rows have many parts each, many have few (batches of 4 tokens x 16 heads on 2000-8000 rows with
+    // 4 units and 8 waves / 4 and 4 / 8 and 4: 2 requests 29.1 / 29.4 / 32.5 us, 16 requests (32 groups) 40.8 / 41.1 /
+    // 41.4, 64 (128 groups) 84.8 / 83.5 / 84.0; 1000 requests on 50-400 rows with 4 and 4 / 8 and 4: 149.6 / 145).
     const int groups = a.batch * ta_tiles(a.max_nodes * a.heads, R) * R;
     if (groups <= 32) launch_join<R, 4, 8>(a, shares, groups, s);
     else if (groups <= 128) launch_join<R, 4, 4>(a, shares, groups, s);

@@ -7,8 +7,9 @@
 // walk (one wave, a lane per token: one gather, then register work) instead of a launch before it,
 // sums its weights in 64 bits and counts itself on the request's ticket; the last one adds up the
 // sums in order, finds the part that holds the place and goes through it again (from the cache).
-// 64 chains of 5 tokens over 131072 fp32 weights take 27 us, of which reading the 67 MB is 13; the rest is the
-// walk before it (four dependent loads) and the last workgroup's round after it. 16 trees over 32000: 11 us.
+// Where a refusal leaves no weight, that last workgroup goes through the whole row alone (rare).
+// 64 chains of 5 tokens over 131072 fp32 weights take 27-28 us, of which reading the 67 MB is 13; the rest is the
+// walk before it (four dependent loads) and the last workgroup's round after it. 16 trees over 32000: 11.3 us.
 // The sums cross workgroups as atomics of agent scope, which are carried out where all XCDs see them: an
 // exchange whose answer is waited for before the ticket is drawn, and loads after the last ticket. (A
 // release and an acquire around the ticket write back and invalidate the XCD's L2 in every workgroup: 72 us
