@@ -171,11 +171,12 @@ typedef struct KvipRowStoreArgs {
  * NaN or a scale that is not finite becomes NaN as a whole. Blocks outside the cache set
  * KVIP_STATUS_BAD_BLOCK and count as not there; lengths outside 0 .. max_blocks * 128, fewer
  * rows than step tokens, more than max_nodes of these, or cu_seqlens that fall or leave 0 .. max_tokens
- * set KVIP_STATUS_BAD_LENGTH (lengths and rows are cut to the range, tokens past max_nodes are not computed). With steps, a request with steps[b] <= 0
- * (one that kvip_hip_page_tables_extend refused) sees nothing: output 0, lse -infinity. Rows of output and lse behind
- * cu_seqlens[batch] are left as they were. The launch counts steps of 32 rows x 128 (token, head) pairs in 32
- * bits: where batch * heads * max_nodes * max_blocks could pass that, workspace_bytes is 0 and the
- * call is refused. A workspace serves one call at a time, and the lengths stay as they are while it runs. */
+ * set KVIP_STATUS_BAD_LENGTH (lengths and rows are cut to the range, tokens past max_nodes are not
+ * computed). With steps, a request with steps[b] <= 0 (one that kvip_hip_page_tables_extend refused) sees
+ * nothing: output 0, lse -infinity. Rows of output and lse behind cu_seqlens[batch] are left as they were.
+ * The launch counts steps of 32 rows x 128 (token, head) pairs in 32 bits: where batch * heads *
+ * max_nodes * max_blocks could pass that, workspace_bytes is 0 and the call is refused. A workspace serves
+ * one call at a time, and the lengths stay as they are while it runs. */
 typedef struct KvipTreeAttnArgs {
     const uint16_t* query;        /* [max_tokens, heads, 576] bf16, 16-byte aligned */
     const uint8_t* kv_cache;      /* 16-byte aligned */
@@ -220,9 +221,9 @@ typedef struct KvipTreeAttnArgs {
  * kvip_hip_page_tables_extend refused). Tokens outside 0 .. vocab - 1 set KVIP_STATUS_BAD_TOKEN and are never
  * taken; parents that do not come before their child set KVIP_STATUS_BAD_TREE and count as -1; a
  * request of more than max_nodes rows (the rest is not looked at) and cu_seqlens that fall or leave
- * 0 .. max_tokens (cut to it) set KVIP_STATUS_BAD_LENGTH;
- * a row in which no token has a weight, or the weights no finite sum, sets KVIP_STATUS_BAD_PROBS and
- * gives token -1. Weights that are negative or NaN count as 0. */
+ * 0 .. max_tokens (cut to it) set KVIP_STATUS_BAD_LENGTH; a row in which no token has a weight, or the
+ * weights no finite sum, sets KVIP_STATUS_BAD_PROBS and gives token -1. Weights that are negative or NaN
+ * count as 0. */
 typedef struct KvipVerifyArgs {
     const void* probs;            /* [max_tokens, vocab], rows probs_stride elements apart */
     const void* draft_probs;      /* the same, draft_stride; or NULL */

@@ -8,9 +8,9 @@ tensors feed the operators of the same step: `cu_seqlens`, `lengths`, `block_tab
 `kvip_amd.TreeAttention`, `slots` and `positions` to `kvip_amd.KvRowStore` and `kvip_amd.Rotary`. Steps of chains (and
 prompt chunks) also feed the selection: `block_table`, `lengths` and `cu_seqlens` go to `kvip_amd.PrefillIndexer`, `slots` to
 `kvip_amd.IndexCacheStorage` as its slot mapping. Trees do not: that indexer lets a row see every row of the step before
-it, siblings among them, and siblings share a position. `include/kvip_hip_draft.h` states the rules. Calls only enqueue on the current stream
-and allocate nothing, so they can be captured; one object's calls follow one another (they share its
-state). There is no CPU path and no counterpart in the reference, whose engine does this on the host.
+it, siblings among them, and siblings share a position. `include/kvip_hip_draft.h` states the rules. Calls only
+enqueue on the current stream and allocate nothing, so they can be captured; one object's calls follow one
+another (they share its state). There is no CPU path and no counterpart in the reference, whose engine does this on the host.
 """
 from __future__ import annotations
 

@@ -186,6 +186,56 @@ def test_verification_of_refused_requests_keeps_nothing(torch_gpu, drafted):
             op.bind(probs, tokens, cu, uniforms, final, steps=bad, **named)
 
 
+def test_a_captured_round_with_refusals_replays(torch_gpu):
+    """A captured round whose pages run out on some replays, against a second engine that runs every round eagerly."""
+    torch = torch_gpu
+    say("case captured refusals")
+    engines = [Round(torch, 25), Round(torch, 25)]
+    for r in engines:
+        t = r.tables
+        r.attention.bind(r.query, r.kv, t.block_table, t.lengths, t.cu_seqlens, t.visible, steps=t.steps)
+        r.verifier.bind(r.probs, r.tokens, t.cu_seqlens, r.uniforms, r.final, parents=r.parents, steps=t.steps)
+    eager, graphed = engines
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for r in engines:
+            for _ in range(5):
+                r.tables.extend(device(torch, [0, 25, 0], torch.int32))
+                r.tables.commit(device(torch, [0, 25, 0], torch.int32))
+            r.inputs(0, [3, 2, 4])
+            r.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        graphed.step()
+    refused = 0
+    for seed in range(1, 9):
+        counts = [int(x) for x in np.random.default_rng(seed).integers(1, 8, 3)]
+        pages = eager.tables.free_count.clone()
+        for r in engines:
+            r.inputs(seed, counts)
+            if seed % 3:
+                r.tables.free_count.zero_()
+            r.tables.status.zero_()
+        bases = eager.tables.lengths.tolist()
+        eager.step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager.state(), graphed.state()):
+            assert torch.equal(a, b), seed
+        refused += sum(k == 0 for k in graphed.verifier.kept.tolist())
+        assert graphed.tables.lengths.tolist() == [n + k for n, k in zip(bases, graphed.verifier.kept.tolist())]
+        if seed % 3:
+            for r in engines:
+                r.tables.free_count.add_(pages)
+        if seed == 4:  # back to the edge of a page, to be refused again
+            for r in engines:
+                r.tables.truncate(device(torch, [0, 127, 0], torch.int32))
+    assert refused > 0
+
+
 # --- targets whose support was drafted whole --------------------------------------------------
 
 
