@@ -22,10 +22,15 @@ __all__ = [
     "sparse_attention",
     "TreeAttention",
     "tree_attention",
+    "ChunkAttention",
+    "chunk_attention",
     "DraftVerifier",
+    "LogitProcessor",
+    "TokenHistory",
     "Rotary",
     "rotary_frequencies",
     "KvRowStore",
+    "NormRotary",
     "PageTables",
     "VllmIndexSelector",
     "PagedIndexer",
@@ -58,10 +63,15 @@ _EXPORTS = {
     "sparse_attention": ("operators.sfa", "sparse_attention"),
     "TreeAttention": ("operators.tree", "TreeAttention"),
     "tree_attention": ("operators.tree", "tree_attention"),
+    "ChunkAttention": ("operators.chunk", "ChunkAttention"),
+    "chunk_attention": ("operators.chunk", "chunk_attention"),
     "DraftVerifier": ("operators.verify", "DraftVerifier"),
+    "LogitProcessor": ("operators.logits", "LogitProcessor"),
+    "TokenHistory": ("operators.logits", "TokenHistory"),
     "Rotary": ("operators.rotary", "Rotary"),
     "rotary_frequencies": ("operators.rotary", "rotary_frequencies"),
     "KvRowStore": ("operators.rotary", "KvRowStore"),
+    "NormRotary": ("operators.norm", "NormRotary"),
     "PageTables": ("cache.page_tables", "PageTables"),
     "VllmIndexSelector": ("adapters.vllm.selector", "VllmIndexSelector"),
     "PagedIndexer": ("adapters.vllm.selector", "PagedIndexer"),

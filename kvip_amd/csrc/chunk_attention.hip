@@ -1,0 +1,682 @@
+// Attention of chunks of new tokens over the paged KV rows (kvip_hip_prompt.h).
+//
+// The rows of the problem are a request's (chunk token, head) pairs. There are many per cached row, so a cached row
+// is read by many workgroups, and converting its fp8 features in every one of them costs more than the products
+// (attention of a few step tokens over the same rows spends 10 vector instructions per MFMA that way). So the rows
+// are laid out once, as bf16, in the order in which the tile loop wants them in LDS (expand): a tile of 32 rows is an
+// image of 72 pieces x 32 rows x 16 bytes that direct-to-LDS loads copy as it stands.
+//
+// A workgroup of 4 waves takes 128 rows of the problem, 32 per wave; a wave keeps its queries (144 registers) and its
+// 32 x 512 sums (the 256 accumulation registers). Logits are computed transposed (cached rows x rows of the problem), so
+// that a lane holds one row's logits of 16 cached rows: the softmax takes one lane swap per tile, and the
+// probabilities, rounded to bf16, are the value product's operand in the lane that has them, as the order of cached
+// rows along K is free. The value operand is read transposed from the same image. The running maximum is raised
+// lazily, when a tile exceeds it by kCaMargin.
+//
+// Few row tiles over long contexts are cut along the context into segments, whose parts a third launch joins.
+#include <type_traits>
+
+#include "kvip_hip_prompt.h"
+#include "lds_async.h"
+
+namespace kvip {
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* LdsS16x4;
+
+constexpr int kCaThreads = 256;
+constexpr int kCaWaves = 4;
+constexpr int kCaRows = 32;                       // rows of the problem per wave (MFMA N)
+constexpr int kCaTileRows = kCaRows * kCaWaves;   // ... per workgroup
+constexpr int kCaTile = 32;                       // cached rows of a tile (MFMA M of the logits)
+constexpr int kCaKey = 576, kCaValue = 512;
+constexpr int kCaBlocks = kCaValue / 32;          // accumulator blocks of 32 features
+constexpr int kCaFrags = kCaKey / 16;             // MFMAs of a tile's logits
+constexpr int kCaPieces = kCaKey / 8;
+constexpr int kCaImage = kCaPieces * kCaTile * 16;
+constexpr int kCaSlots = 4;                       // images in LDS
+constexpr int kCaLoads = kCaImage / 1024 / kCaWaves;
+constexpr int kCaUnits = 512;                     // workgroups of a launch whose row tiles are cut, at most
+constexpr int kCaCutTiles = 256;                  // row tiles that are cut, at most
+constexpr int kCaMostCuts = 32;
+constexpr int kCaPartSteps = 10;                  // what storing and joining a part costs, in tiles
+constexpr int kCaCus = 256;
+constexpr float kCaLog2e = 1.44269504088896341f;
+constexpr float kCaLn2 = 0.693147180559945309f;
+constexpr float kCaMargin = 8.0f * kCaLog2e;
+static_assert(kCaLoads * 1024 * kCaWaves == kCaImage, "whole loads");
+static_assert(kCaSlots * kCaImage <= 160 * 1024, "LDS of a CU");
+
+// Place of piece j (8 features) of a tile's row t in its image, in 16-byte units. A key read takes one piece of 32
+// consecutive rows; a value read takes four pieces of 4 rows at a time, which the XOR spreads over all banks.
+KVIP_DEVICE int ca_place(int piece, int t) { return piece * kCaTile + (t ^ ((piece & 3) << 2)); }
+
+// What the expanding launch leaves for the others.
+struct ChunkPlan {
+    int units;                                // workgroups with work
+    int cut;                                  // tiles of a segment
+    int cut_tiles;                            // row tiles, where they are cut; else 0
+    int reserved;
+    int units_before[KVIP_DRAFT_MAX_BATCH + 1];
+    int tiles_before[KVIP_DRAFT_MAX_BATCH + 1];  // row tiles
+    int images_before[KVIP_DRAFT_MAX_BATCH + 1];
+};
+
+// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there), then the
+// images, then the parts: 32 rows x 512 sums per wave as its lanes hold them ([block][quarter][lane] 16 bytes),
+// then their (maximum, sum) pairs.
+struct ChunkWork {
+    ChunkPlan* plan;
+    uint2* flags;
+    uint8_t* images;
+    f32x4* sums;
+    float2* states;
+};
+__host__ __device__ inline int64_t ca_images(int64_t max_rows, int batch) { return (max_rows + kCaTile - 1) / kCaTile + batch; }
+__host__ __device__ inline size_t ca_align(size_t n) { return (n + 1023) / 1024 * 1024; }
+__host__ __device__ inline ChunkWork ca_work(void* base, int64_t images, size_t* bytes) {
+    uint8_t* p = static_cast<uint8_t*>(base);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        uint8_t* q = p + at;
+        at = ca_align(at + n);
+        return q;
+    };
+    ChunkWork w;
+    w.plan = reinterpret_cast<ChunkPlan*>(take(sizeof(ChunkPlan)));
+    w.flags = reinterpret_cast<uint2*>(take(static_cast<size_t>(images + 64) * sizeof(uint2)));  // read 64 at a time
+    w.images = take(static_cast<size_t>(images) * kCaImage);
+    w.sums = reinterpret_cast<f32x4*>(take(static_cast<size_t>(kCaUnits) * kCaWaves * kCaBlocks * 4 * 64 * sizeof(f32x4)));
+    w.states = reinterpret_cast<float2*>(take(static_cast<size_t>(kCaUnits) * kCaTileRows * sizeof(float2)));
+    if (bytes != nullptr) *bytes = at;
+    return w;
+}
+
+// A request as the kernels take it.
+struct ChunkRequest {
+    int begin;   // first token
+    int tokens;
+    int length;  // cached rows
+    KVIP_DEVICE int past() const { return length - tokens; }
+};
+KVIP_DEVICE ChunkRequest ca_request(const KvipChunkAttnArgs& p, int b, uint32_t* err) {
+    ChunkRequest q;
+    const int first = p.cu_seqlens[b], behind = p.cu_seqlens[b + 1], given = p.seq_lens[b];
+    const bool refused = p.steps != nullptr && p.steps[b] <= 0;
+    q.begin = min(max(first, 0), p.max_tokens);
+    q.tokens = min(max(behind, q.begin), p.max_tokens) - q.begin;
+    q.length = refused ? 0 : min(max(given, 0), p.max_blocks * kBlockTokens);
+    if (first != q.begin || behind != q.begin + q.tokens || (!refused && (given != q.length || (q.tokens > 0 && given < q.tokens)))) {
+        *err |= KVIP_STATUS_BAD_LENGTH;
+    }
+    return q;
+}
+KVIP_DEVICE int ca_row_tiles(const ChunkRequest& q, int heads) { return (q.tokens * heads + kCaTileRows - 1) / kCaTileRows; }
+KVIP_DEVICE int ca_steps(const ChunkRequest& q) { return q.tokens > 0 ? (q.length + kCaTile - 1) / kCaTile : 0; }
+
+KVIP_DEVICE uint32_t ca_pack(float a, float b) {  // hardware round to nearest even
+    const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// Plan and images. Every workgroup sums the requests' tiles for itself and takes images in turn; the first one also
+// leaves the plan. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8 rotary features.
+__global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChunkAttnArgs p) {
+    __shared__ __align__(16) uint8_t s_image[kCaImage];
+    __shared__ int s_before[KVIP_DRAFT_MAX_BATCH + 1];
+    __shared__ uint32_t s_sums[kCaWaves];
+    __shared__ uint2 s_flags[kCaWaves];
+    constexpr int kPer = KVIP_DRAFT_MAX_BATCH / kCaThreads;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int64_t most = ca_images(p.max_rows, p.batch);
+    const ChunkWork work = ca_work(p.workspace, most, nullptr);
+    uint32_t err = 0;
+    int steps[kPer], tiles[kPer];
+    uint32_t sum = 0, sum_tiles = 0, total, total_tiles;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int b = tid * kPer + i;
+        steps[i] = tiles[i] = 0;
+        if (b < p.batch) {
+            const ChunkRequest q = ca_request(p, b, &err);
+            steps[i] = ca_steps(q);
+            tiles[i] = ca_row_tiles(q, p.heads);
+        }
+        sum += steps[i];
+        sum_tiles += tiles[i];
+    }
+    uint32_t before = block_exclusive_scan(sum, s_sums, &total);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int b = tid * kPer + i;
+        if (b <= p.batch) s_before[b] = before;
+        before += steps[i];
+    }
+    if (tid == 0) s_before[p.batch] = total;
+    __syncthreads();
+
+    if (blockIdx.x == 0) {
+        // Where the row tiles would leave CUs without work, the context is cut into k segments of the longest request's:
+        // the k whose rounds of workgroups (one per CU) times their tiles are the fewest.
+        ChunkPlan* plan = work.plan;
+        uint32_t tiles_before = block_exclusive_scan(sum_tiles, s_sums, &total_tiles);
+        __shared__ int s_longest, s_units[kCaMostCuts];
+        if (tid == 0) s_longest = 1;
+        if (tid < kCaMostCuts) s_units[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (steps[i] > 0) atomicMax(&s_longest, steps[i]);
+        }
+        __syncthreads();
+        const int longest = s_longest;
+        for (int k = 0; k < kCaMostCuts; ++k) {
+            const int cut = (longest + k) / (k + 1);
+            int units = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) units += tiles[i] * max((steps[i] + cut - 1) / cut, 1);
+            if (total_tiles <= kCaCutTiles) atomicAdd(&s_units[k], units);
+        }
+        __syncthreads();
+        int cut = longest, best = 0x7FFFFFFF;
+        bool is_cut = false;
+        if (total_tiles <= kCaCutTiles) {
+            for (int k = 0; k < kCaMostCuts; ++k) {
+                const int c = (longest + k) / (k + 1), units = s_units[k];
+                const int cost = (units + kCaCus - 1) / kCaCus * (c + (k > 0 ? kCaPartSteps : 0));
+                if (units <= kCaUnits && cost < best) {
+                    best = cost;
+                    cut = c;
+                    is_cut = k > 0;
+                }
+            }
+        }
+        uint32_t mine = 0, total_units;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mine += tiles[i] * max((steps[i] + cut - 1) / cut, 1);
+        uint32_t units_before = block_exclusive_scan(mine, s_sums, &total_units);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int b = tid * kPer + i;
+            if (b >= p.batch) break;
+            plan->units_before[b] = units_before;
+            plan->tiles_before[b] = tiles_before;
+            // No images: none that would fit.
+            const bool fits = s_before[b + 1] <= most;
+            plan->images_before[b] = fits ? s_before[b] : -1;
+            if (!fits && steps[i] > 0) err |= KVIP_STATUS_BAD_LENGTH;
+            units_before += tiles[i] * max((steps[i] + cut - 1) / cut, 1);
+            tiles_before += tiles[i];
+        }
+        if (tid == 0) {
+            plan->units = total_units;
+            plan->cut = cut;
+            plan->cut_tiles = is_cut ? total_tiles : 0;
+            plan->units_before[p.batch] = total_units;
+            plan->tiles_before[p.batch] = total_tiles;
+        }
+        report(p.status, err);
+    }
+
+    int b = 0;
+    for (int image = blockIdx.x; image < static_cast<int>(total) && image < most; image += gridDim.x) {
+        // The request: the last one whose images begin at or before this one (empty ones share its beginning).
+        int lo = b, hi = p.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (s_before[mid] <= image) lo = mid;
+            else hi = mid - 1;
+        }
+        b = lo;
+        if (s_before[b + 1] > most) continue;  // its request does not fit
+        uint32_t none = 0;
+        const ChunkRequest q = ca_request(p, b, &none);
+        const int first = (image - s_before[b]) * kCaTile, t = tid >> 3, piece = tid & 7;
+        const int page = p.block_table[static_cast<int64_t>(b) * p.max_blocks + first / kBlockTokens];
+        const bool in_cache = static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks);
+        if (!in_cache && tid == 0) report(p.status, KVIP_STATUS_BAD_BLOCK);
+        const bool there = in_cache && first + t < q.length;
+        v4i raw[4] = {}, rope = {};
+        f32x4 scale = {};
+        if (there) {
+            const uint8_t* row = p.kv_cache + page * p.kv_block_stride + static_cast<int64_t>(first % kBlockTokens + t) * p.row_stride;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) raw[k] = *reinterpret_cast<const v4i*>(row + k * 128 + piece * 16);
+            rope = *reinterpret_cast<const v4i*>(row + kCaValue + piece * 16);
+            scale = *reinterpret_cast<const f32x4*>(row + kCaValue + 128);
+        }
+        v4i out[8];
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x0 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 0), x1 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 1);
+                const float x2 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 2), x3 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 3);
+                const uint32_t lo2 = ca_pack(x0 * scale[k], x1 * scale[k]), hi2 = ca_pack(x2 * scale[k], x3 * scale[k]);
+                odd |= (((lo2 & 0x7F807F80u) + 0x00800080u) | ((hi2 & 0x7F807F80u) + 0x00800080u)) & 0x80008000u;
+                out[2 * k + i / 2][2 * (i & 1)] = static_cast<int>(lo2);
+                out[2 * k + i / 2][2 * (i & 1) + 1] = static_cast<int>(hi2);
+            }
+        }
+        // A row's 8 threads lie side by side: bit t of the flags of the whole tile.
+        const uint64_t odd_lanes = __ballot(odd != 0), gone_lanes = __ballot(!there);
+        const bool zero = odd_lanes >> (lane & 56) & 0xFF;
+        uint32_t odd_rows = 0, gone_rows = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            odd_rows |= ((odd_lanes >> (8 * i) & 0xFF) != 0 ? 1u : 0u) << i;
+            gone_rows |= static_cast<uint32_t>(gone_lanes >> (8 * i) & 1) << i;
+        }
+        __syncthreads();  // the image before is copied
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                *reinterpret_cast<v4i*>(s_image + 16 * ca_place(k * 16 + piece * 2 + i, t)) = zero ? v4i{0, 0, 0, 0} : out[2 * k + i];
+            }
+        }
+        *reinterpret_cast<v4i*>(s_image + 16 * ca_place(kCaValue / 8 + piece, t)) = rope;
+        if (lane == 0) s_flags[w] = make_uint2(odd_rows, gone_rows);
+        __syncthreads();
+        v4i* to = reinterpret_cast<v4i*>(work.images + static_cast<int64_t>(image) * kCaImage);
+#pragma unroll
+        for (int i = 0; i < kCaImage / 16 / kCaThreads; ++i) to[tid + i * kCaThreads] = *reinterpret_cast<const v4i*>(s_image + 16 * (tid + i * kCaThreads));
+        if (tid == 0) {
+            uint2 flags = make_uint2(0, 0);
+#pragma unroll
+            for (int i = 0; i < kCaWaves; ++i) {
+                flags.x |= s_flags[i].x << (8 * i);
+                flags.y |= s_flags[i].y << (8 * i);
+            }
+            work.flags[image] = flags;
+        }
+    }
+}
+
+KVIP_DEVICE float ca_half_max(float x) {  // over lanes l and l ^ 32
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+KVIP_DEVICE float ca_half_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+KVIP_DEVICE float ca_share(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
+KVIP_DEVICE float ca_lse(float m, float l) {  // maximum in log2 units, sum (0 where the row sees nothing)
+    return l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * kCaLn2 : -INFINITY;
+}
+KVIP_DEVICE void ca_store(const KvipChunkAttnArgs& p, int64_t at, f32x4 v) {
+    if (p.output_dtype == KVIP_DTYPE_FP32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.output) + at) = v;
+    } else {
+        *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.output) + at) = __builtin_convertvector(v, bf16x4);
+    }
+}
+
+// Direct-to-LDS load from a wave-uniform address and a lane's offset below 2^32 (see lds_async.h).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+KVIP_DEVICE void ca_dma16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Keeps an accumulator in accumulation registers from here to the next hold.
+KVIP_DEVICE void ca_hold(v16f& acc) { asm volatile("" : "+a"(acc)); }
+
+// A unit of the plan: request b, row tile rt, segment seg.
+struct ChunkUnit {
+    int b, rt, seg;
+};
+KVIP_DEVICE bool ca_unit(const ChunkPlan* plan, int batch, int unit, int* s_found, ChunkUnit* u) {
+    if (unit >= plan->units) return false;
+    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
+        if (plan->units_before[b] <= unit && unit < plan->units_before[b + 1]) {
+            const int tiles = plan->tiles_before[b + 1] - plan->tiles_before[b];
+            const int segs = (plan->units_before[b + 1] - plan->units_before[b]) / tiles, at = unit - plan->units_before[b];
+            s_found[0] = b;
+            s_found[1] = tiles - 1 - at / segs;  // the tiles that see most first
+            s_found[2] = at % segs;
+        }
+    }
+    __syncthreads();
+    u->b = __builtin_amdgcn_readfirstlane(s_found[0]);
+    u->rt = __builtin_amdgcn_readfirstlane(s_found[1]);
+    u->seg = __builtin_amdgcn_readfirstlane(s_found[2]);
+    return true;
+}
+
+// Tiles that a row tile's rows see.
+KVIP_DEVICE int ca_reach(const ChunkRequest& q, int rt, int heads) {
+    const int last = min((rt + 1) * kCaTileRows, q.tokens * heads) - 1;
+    const int end = min(max(q.past() + last / heads + 1, 0), q.length);
+    return (end + kCaTile - 1) / kCaTile;
+}
+
+__global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const KvipChunkAttnArgs p) {
+    __shared__ __align__(1024) uint8_t s_ring[kCaSlots * kCaImage];
+    __shared__ int s_found[4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const ChunkWork work = ca_work(p.workspace, ca_images(p.max_rows, p.batch), nullptr);
+    ChunkUnit unit;
+    if (!ca_unit(work.plan, p.batch, blockIdx.x, s_found, &unit)) return;
+    uint32_t none = 0;
+    const ChunkRequest q = ca_request(p, unit.b, &none);
+    const int image0 = __builtin_amdgcn_readfirstlane(work.plan->images_before[unit.b]);
+    const int cut = __builtin_amdgcn_readfirstlane(work.plan->cut);
+    const int rows = q.tokens * p.heads, first_row = unit.rt * kCaTileRows + w * kCaRows;
+    const int reach = image0 < 0 ? 0 : ca_reach(q, unit.rt, p.heads);
+    const int t0 = unit.seg * cut, t1 = min(t0 + cut, reach);
+    const bool whole = reach <= cut;
+    const int hn = lane & 31, hk = lane >> 5;
+    const int row = first_row + hn, node = min(row, rows - 1) / p.heads;
+    const int64_t out_row = static_cast<int64_t>(q.begin) * p.heads + row;
+    if (t0 >= t1) {
+        if (unit.seg != 0 || reach > 0) return;  // nothing of the row tile is here
+        for (int i = tid; i < kCaTileRows * (kCaValue / 4); i += kCaThreads) {  // rows that see nothing
+            const int r = unit.rt * kCaTileRows + i / (kCaValue / 4);
+            if (r < rows) ca_store(p, (static_cast<int64_t>(q.begin) * p.heads + r) * kCaValue + i % (kCaValue / 4) * 4, f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+        if (p.lse != nullptr && hk == 0 && row < rows) p.lse[out_row] = -INFINITY;
+        return;
+    }
+    const int sees = min(max(q.past() + node + 1, 0), q.length);  // cached rows that the lane's row sees
+    // The first tile that some row of the wave does not see whole.
+    const int t_mask = min(max(q.past() + min(first_row, rows - 1) / p.heads + 1, 0), q.length) / kCaTile;
+    const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(fabsf(p.scale * kCaLog2e), 0x1p-126f))));
+    const int flip = p.scale < 0.f ? static_cast<int>(0x80008000u) : 0;
+
+    const uint32_t ring = lds_addr(s_ring);
+    const uint8_t* from = work.images + static_cast<int64_t>(image0 + t0) * kCaImage + w * (kCaLoads * 1024);
+    auto fetch = [&](int t, int i) {  // load i of tile t's image (past the last tile: the last one again)
+        ca_dma16(from + static_cast<int64_t>(min(t, t1 - 1) - t0) * kCaImage + i * 1024, lane * 16,
+                 ring + (t - t0) % kCaSlots * kCaImage + w * (kCaLoads * 1024) + i * 1024);
+    };
+#pragma unroll
+    for (int t = 0; t < kCaSlots - 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < kCaLoads; ++i) fetch(t0 + t, i);
+    }
+    // Queries of the wave's rows (rows past the last read it again; their outputs are not written): fragment i holds
+    // features 16 i + 8 (lane / 32) .. + 7.
+    const uint16_t* query = p.query + (static_cast<int64_t>(q.begin) * p.heads + min(row, rows - 1)) * kCaKey + hk * 8;
+    v4i qf[kCaFrags];
+#pragma unroll
+    for (int i = 0; i < kCaFrags; ++i) qf[i] = *reinterpret_cast<const v4i*>(query + i * 16);
+    v16f o[kCaBlocks];
+#pragma unroll
+    for (int f = 0; f < kCaBlocks; ++f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
+        ca_hold(o[f]);
+    }
+#pragma unroll
+    for (int i = 0; i < kCaFrags; ++i) {
+        qf[i] ^= flip;
+        asm volatile("" : "+v"(qf[i]));  // waited for here, not in the tile loop
+    }
+    float m_run = -INFINITY, l_sum = 0.f;
+    v16f s;
+    v4i pb[2];  // probabilities of the tile whose values come next
+
+    // The flags of 64 tiles, which the lanes hold.
+    int held_first = t0;
+    uint2 held = work.flags[image0 + min(t0 + lane, reach - 1)];
+    auto flags_of = [&](int t) {
+        if (t >= held_first + 64) {
+            held_first = t;
+            held = work.flags[image0 + min(t + lane, reach - 1)];
+        }
+        return make_uint2(__builtin_amdgcn_readlane(held.x, t - held_first), __builtin_amdgcn_readlane(held.y, t - held_first));
+    };
+    auto slot_of = [&](int t) { return ring + (t - t0) % kCaSlots * kCaImage; };
+    const uint32_t key_at[2] = {static_cast<uint32_t>(16 * ca_place(hk, hn)), static_cast<uint32_t>(16 * (ca_place(2 + hk, hn) - 2 * kCaTile))};
+    constexpr int kAhead = 4;  // operands are read from LDS so many products before their use
+    auto key = [&](uint32_t slot, int i) { return *(LdsV4i)(slot + key_at[i & 1] + i * 1024); };
+    // Logits of tile t; the loads of the tile `ahead` stand between the products.
+    auto logits = [&](int t, int ahead) {
+        const uint32_t slot = slot_of(t);
+        v4i kb[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) kb[i] = key(slot, i);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kCaFrags; ++i) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kb[i % kAhead]), __builtin_bit_cast(bf16x8, qf[i]), s, 0, 0, 0);
+            if (i + kAhead < kCaFrags) kb[i % kAhead] = key(slot, i + kAhead);
+            if (i % 4 == 0) fetch(ahead, i / 4);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const uint2 flags = flags_of(t);
+        if (t >= t_mask || flags.x != 0 || flags.y != 0) {
+            const int left = sees - t * kCaTile;
+            uint32_t seen = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+            seen &= ~flags.y;
+            if (seen & flags.x) l_sum = NAN;
+            seen >>= 4 * hk;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (!(seen >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
+            }
+        }
+    };
+    // Softmax of the logits, p = 2^(scale2 (logit - m)), in 18 pieces. Its factor for what came before (alpha) counts
+    // once the values of the tile before are in.
+    float mx, bias, alpha, fresh_sum;
+    bool raise;
+    auto softmax = [&](int piece) {
+        if (piece == 0) {
+            mx = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+            mx = ca_half_max(mx);
+            fresh_sum = 0.f;
+        } else if (piece == 1) {
+            raise = (mx - m_run) * scale2 > kCaMargin;  // also the first finite maximum
+            const float m_new = raise ? mx : m_run;
+            alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * scale2) : raise ? 0.f : 1.f;
+            m_run = m_new;
+            bias = m_new == -INFINITY ? 0.f : -m_new * scale2;
+        } else {
+            s[piece - 2] = __builtin_amdgcn_exp2f(fmaf(s[piece - 2], scale2, bias));
+            fresh_sum += s[piece - 2];
+        }
+    };
+    auto take = [&] {  // the softmax's results become those of the tile whose values come next
+        l_sum = l_sum * alpha + fresh_sum;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pb[i >> 2][i & 3] = static_cast<int>(ca_pack(s[2 * i], s[2 * i + 1]));
+    };
+    const int vp = (lane >> 4 & 1) * 2 + (lane >> 1 & 1), vt = 4 * hk + (lane >> 2 & 3);  // piece of a block, row of eight
+    const uint32_t value_at[2] = {static_cast<uint32_t>(16 * ca_place(vp, vt) + 8 * (lane & 1)),
+                                  static_cast<uint32_t>(16 * ca_place(vp, vt + 8) + 8 * (lane & 1))};
+    auto value = [&](uint32_t slot, int i) {  // operand of product i: block i / 2, cached rows 16 (i % 2) .. + 15
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4)(slot + value_at[0] + (i >> 1) * 2048 + (i & 1) * 256));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4)(slot + value_at[1] + (i >> 1) * 2048 + (i & 1) * 256));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    // Values of tile t, the softmax of the next one beside them.
+    auto values = [&](int t, auto with_softmax) {
+        constexpr bool kSoftmax = decltype(with_softmax)::value;
+        const uint32_t slot = slot_of(t);
+        bf16x8 vb[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) vb[i] = value(slot, i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2 * kCaBlocks; ++i) {
+            if ((i & 1) == 0) ca_hold(o[i >> 1]);
+            o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i % kAhead], __builtin_bit_cast(bf16x8, pb[i & 1]), o[i >> 1], 0, 0, 0);
+            if ((i & 1) == 1) ca_hold(o[i >> 1]);
+            if (i + kAhead < 2 * kCaBlocks) vb[i % kAhead] = value(slot, i + kAhead);
+            if (kSoftmax && i < 18) softmax(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Tile t has landed, and the image of the tile before last is free for the one that comes three later.
+    auto arrive = [&] {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((kCaSlots - 3) * kCaLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" : : : "memory");
+    };
+    arrive();
+    logits(t0, t0 + kCaSlots - 2);
+#pragma unroll
+    for (int i = 0; i < 18; ++i) softmax(i);
+    take();
+#pragma unroll 1
+    for (int t = t0; t + 1 < t1; ++t) {
+        arrive();
+        logits(t + 1, t + kCaSlots - 1);
+        values(t, std::true_type{});
+        if (__ballot(raise) != 0ull) {
+#pragma unroll
+            for (int f = 0; f < kCaBlocks; ++f) {
+                ca_hold(o[f]);
+                o[f] *= alpha;
+                ca_hold(o[f]);
+            }
+        }
+        take();
+    }
+    values(t1 - 1, std::false_type{});
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
+
+    const float l_all = ca_half_sum(l_sum), m_all = m_run * scale2;  // log2 units from here on
+    const float factor = whole ? ca_share(l_all) : 1.f;
+    f32x4* part = work.sums + (static_cast<int64_t>(blockIdx.x) * kCaWaves + w) * (kCaBlocks * 4 * 64) + lane;
+#pragma unroll
+    for (int f = 0; f < kCaBlocks; ++f) {
+        ca_hold(o[f]);
+        const v16f x = o[f];
+        if (!whole) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) part[(f * 4 + a) * 64] = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]};
+        } else if (p.output_dtype == KVIP_DTYPE_BF16) {
+            // The halves of the wave hold every other four features of a row: swapped, each has eight.
+#pragma unroll
+            for (int a = 0; a < 4; a += 2) {
+                v4i v;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const auto pair = __builtin_amdgcn_permlane32_swap(
+                        ca_pack(x[4 * a + 2 * e] * factor, x[4 * a + 2 * e + 1] * factor),
+                        ca_pack(x[4 * a + 2 * e + 4] * factor, x[4 * a + 2 * e + 5] * factor), false, false);
+                    v[e] = pair[0];
+                    v[e + 2] = pair[1];
+                }
+                if (row < rows) *reinterpret_cast<v4i*>(static_cast<__bf16*>(p.output) + out_row * kCaValue + 32 * f + 8 * a + 8 * hk) = v;
+            }
+        } else if (row < rows) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                ca_store(p, out_row * kCaValue + 32 * f + 8 * a + 4 * hk, f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * factor);
+            }
+        }
+    }
+    if (hk == 0) {
+        if (!whole) work.states[static_cast<int64_t>(blockIdx.x) * kCaTileRows + w * kCaRows + hn] = make_float2(m_all, l_all);
+        else if (p.lse != nullptr && row < rows) p.lse[out_row] = ca_lse(m_all, l_all);
+    }
+}
+
+// Joins the parts of row tiles that were cut. A workgroup takes one wave's 32 rows and a quarter of the features.
+__global__ __launch_bounds__(kCaThreads) void chunk_join_kernel(const KvipChunkAttnArgs p) {
+    __shared__ int s_found[4];
+    const ChunkWork work = ca_work(p.workspace, ca_images(p.max_rows, p.batch), nullptr);
+    const ChunkPlan* plan = work.plan;
+    const int slice = blockIdx.x % 4, rg = blockIdx.x / 4 % kCaWaves, tile = blockIdx.x / 4 / kCaWaves;
+    if (tile >= plan->cut_tiles) return;
+    for (int b = threadIdx.x; b < p.batch; b += kCaThreads) {
+        const int first = plan->tiles_before[b], behind = plan->tiles_before[b + 1];
+        if (first <= tile && tile < behind) {
+            s_found[0] = b;
+            s_found[1] = tile - first;
+            s_found[2] = (plan->units_before[b + 1] - plan->units_before[b]) / (behind - first);
+            s_found[3] = plan->units_before[b] + (behind - 1 - tile) * s_found[2];
+        }
+    }
+    __syncthreads();
+    const int b = s_found[0], rt = s_found[1], unit = s_found[3], cut = plan->cut;
+    uint32_t none = 0;
+    const ChunkRequest q = ca_request(p, b, &none);
+    const int reach = plan->images_before[b] < 0 ? 0 : ca_reach(q, rt, p.heads);
+    if (reach <= cut) return;  // whole
+    const int parts = min((reach + cut - 1) / cut, s_found[2]);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hn = lane & 31;
+    const int row = rt * kCaTileRows + rg * kCaRows + hn, rows = q.tokens * p.heads;
+    const float2* states = work.states + static_cast<int64_t>(unit) * kCaTileRows + rg * kCaRows + hn;
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, states[i * kCaTileRows].x);
+    for (int i = 0; i < parts; ++i) {
+        const float2 state = states[i * kCaTileRows];
+        l += state.x == -INFINITY ? state.y : state.y * __builtin_amdgcn_exp2f(state.x - m);
+    }
+    const float factor = ca_share(l);
+    const int64_t out_row = static_cast<int64_t>(q.begin) * p.heads + row;
+    constexpr int kRun = kCaBlocks / 4;  // fours of features of a wave
+    const int at = (slice * kCaWaves + w) * kRun;
+    f32x4 x[kRun] = {};
+    for (int i = 0; i < parts; ++i) {
+        const float mi = states[i * kCaTileRows].x;
+        const float weight = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
+        const f32x4* part = work.sums + (static_cast<int64_t>(unit + i) * kCaWaves + rg) * (kCaBlocks * 4 * 64) + lane;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) x[j] += part[(at + j) * 64] * weight;
+    }
+    if (row >= rows) return;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+        ca_store(p, out_row * kCaValue + (at + j) / 4 * 32 + (at + j) % 4 * 8 + (lane >> 5) * 4, x[j] * factor);
+    }
+    if (slice == 0 && threadIdx.x < kCaRows && p.lse != nullptr) p.lse[out_row] = ca_lse(m, l);
+}
+
+int64_t ca_row_tiles_most(int batch, int heads, int max_tokens) {
+    return (static_cast<int64_t>(max_tokens) * heads + kCaTileRows - 1) / kCaTileRows + batch;
+}
+
+bool ca_sizes(int32_t batch, int32_t heads, int32_t max_tokens, int64_t max_rows) {
+    return batch >= 1 && batch <= KVIP_DRAFT_MAX_BATCH && heads >= 1 && heads <= 128 && max_tokens >= 1 &&
+           max_tokens <= KVIP_DRAFT_MAX_TOKENS && max_rows >= 1 && max_rows <= (1ll << 31);
+}
+
+}  // namespace
+}  // namespace kvip
+
+extern "C" uint64_t kvip_hip_chunk_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t max_tokens, int64_t max_rows) {
+    if (!kvip::ca_sizes(batch, heads, max_tokens, max_rows)) return 0;
+    size_t bytes;
+    kvip::ca_work(nullptr, kvip::ca_images(max_rows, batch), &bytes);
+    return bytes;
+}
+
+extern "C" uint32_t kvip_hip_chunk_attention(const KvipChunkAttnArgs* a, void* stream) {
+    if (a == nullptr) return KVIP_ERR_INVALID;
+    auto aligned = [](const void* x, unsigned n) { return (reinterpret_cast<uintptr_t>(x) & (n - 1)) == 0; };
+    const bool ok = a->query && a->kv_cache && a->block_table && a->seq_lens && a->cu_seqlens && a->output && a->workspace &&
+                    aligned(a->query, 16) && aligned(a->kv_cache, 16) && aligned(a->output, 16) && aligned(a->workspace, 16) &&
+                    kvip::ca_sizes(a->batch, a->heads, a->max_tokens, a->max_rows) && a->max_blocks >= 1 &&
+                    a->max_blocks <= (1 << 17) && a->num_blocks >= 1 && a->num_blocks < (1 << 24) &&
+                    a->row_stride >= KVIP_KV_ROW_BYTES && a->row_stride <= (1 << 24) && a->row_stride % 16 == 0 &&
+                    a->kv_block_stride % 16 == 0 && a->kv_block_stride >= static_cast<int64_t>(kvip::kBlockTokens) * a->row_stride &&
+                    (a->output_dtype == KVIP_DTYPE_BF16 || a->output_dtype == KVIP_DTYPE_FP32) && a->scale - a->scale == 0.f;
+    if (!ok) return KVIP_ERR_INVALID;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t images = kvip::ca_images(a->max_rows, a->batch), tiles = kvip::ca_row_tiles_most(a->batch, a->heads, a->max_tokens);
+    const int64_t units = tiles < kvip::kCaUnits ? kvip::kCaUnits : tiles;
+    hipLaunchKernelGGL(kvip::chunk_expand_kernel, dim3(static_cast<unsigned>(images < 1024 ? images : 1024)), dim3(kvip::kCaThreads), 0, s, *a);
+    hipLaunchKernelGGL(kvip::chunk_attention_kernel, dim3(static_cast<unsigned>(units)), dim3(kvip::kCaThreads), 0, s, *a);
+    const int64_t joined = tiles < kvip::kCaCutTiles ? tiles : kvip::kCaCutTiles;
+    hipLaunchKernelGGL(kvip::chunk_join_kernel, dim3(static_cast<unsigned>(joined * kvip::kCaWaves * 4)), dim3(kvip::kCaThreads), 0, s, *a);
+    return static_cast<uint32_t>(hipGetLastError());
+}

@@ -1,0 +1,424 @@
+// Logits to probabilities (penalties, biases, grammar masks, temperature) and the histories that the penalties
+// read (kvip_hip_prompt.h).
+//
+// Nearly all of a row is alike: a logit, a bit whether the request holds the token, for those it holds a count, a
+// bit whether the grammar allows it. Only the row's drafted ancestors and the request's biases (some hundred
+// tokens of a vocabulary) need more, and each of these is worked out by one thread on its own: a bit in LDS takes
+// the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing, and a
+// token named several times gets the same sum, in the list's order, whichever thread has it.
+#include "kvip_device.h"
+#include "kvip_hip_prompt.h"
+
+namespace kvip {
+namespace {
+
+constexpr int kLgThreads = 512;
+constexpr int kLgWaves = kLgThreads / 64;
+constexpr int kLgVec = 8;                      // tokens of a thread at a time: a byte of the bit masks
+constexpr int kLgRun = kLgThreads * kLgVec;
+constexpr int kLgMaxPart = 1 << 17;            // tokens of a workgroup (16 KB of bits)
+constexpr float kLgLog2e = 1.44269504088896341f;
+constexpr float kLgLargest = 3.402823466e38f;
+
+template <typename T> struct Logits { typedef T vec __attribute__((ext_vector_type(kLgVec), aligned(sizeof(T)))); };
+
+struct LogitStat {
+    float m, l;  // largest x, sum of exp((x - m) / temperature)
+    int first;   // first token of the largest x
+    int reserved;
+};
+
+struct LogitRow {
+    float repetition, inverse, presence, frequency;
+    float c;      // log2(e) / temperature
+    bool greedy;
+    bool plain;   // c is an ordinary number, so that exp2((x - m) c) needs no care but for an m of infinity
+};
+
+KVIP_DEVICE float penalised(float x, const LogitRow& r, bool held, int n) {
+    if (held) x *= x > 0.f ? r.inverse : r.repetition;
+    return n > 0 ? x - fmaf(r.frequency, static_cast<float>(n), r.presence) : x;
+}
+
+KVIP_DEVICE float weight_of(float x, float m, const LogitRow& r) {
+    if (r.plain && m < INFINITY) return __builtin_amdgcn_exp2f((x - m) * r.c);
+    return x == m ? 1.f : x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaxf(x - m, -kLgLargest) * r.c);
+}
+
+KVIP_DEVICE void merge(LogitStat& a, float m, float l, int first, const LogitRow& r) {
+    if (m > a.m) {
+        a.l = a.m == -INFINITY ? l : a.l * weight_of(a.m, m, r) + l;
+        a.m = m;
+        a.first = first;
+    } else if (m == a.m) {
+        a.l += l;
+        a.first = min(a.first, first);
+    } else if (m != -INFINITY) {
+        a.l += l * weight_of(m, a.m, r);
+    }
+}
+
+KVIP_DEVICE void merge_block(LogitStat& a, LogitStat* s_stats, const LogitRow& r) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        merge(a, __shfl_xor(a.m, d), __shfl_xor(a.l, d), __shfl_xor(a.first, d), r);
+    }
+    if ((threadIdx.x & 63) == 0) s_stats[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = s_stats[0];
+#pragma unroll
+    for (int w = 1; w < kLgWaves; ++w) merge(a, s_stats[w].m, s_stats[w].l, s_stats[w].first, r);
+}
+
+// A row's part [begin, end) of the vocabulary.
+template <typename T>
+struct LogitPart {
+    const KvipLogitArgs& p;
+    const T* logits;
+    const int32_t* counts;    // of the request, or null
+    const uint8_t* seen;
+    const uint8_t* allowed;   // or null
+    const uint32_t* special;  // LDS: tokens that are not the dense pass's
+    int begin, end;
+    LogitRow row;
+    uint32_t err;
+
+    KVIP_DEVICE float allowed_or_none(float x, bool may) {
+        if (!may) return -INFINITY;
+        if (x != x) {
+            err |= KVIP_STATUS_BAD_PROBS;
+            return -INFINITY;
+        }
+        return x;
+    }
+
+    // The tokens v .. v + 7 (v a multiple of 8), -infinity for those past the end or not the dense pass's.
+    KVIP_DEVICE void load(int v, float (&x)[kLgVec]) {
+        const int there = min(end - v, kLgVec);
+        if (there == kLgVec) {
+            const auto raw = *reinterpret_cast<const typename Logits<T>::vec*>(logits + v);
+#pragma unroll
+            for (int i = 0; i < kLgVec; ++i) x[i] = static_cast<float>(raw[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLgVec; ++i) x[i] = i < there ? static_cast<float>(logits[v + i]) : 0.f;
+        }
+        uint32_t may = (1u << there) - 1;
+        if (special != nullptr) may &= ~(special[(v - begin) >> 5] >> (v & 31));
+        if (allowed != nullptr) may &= allowed[v >> 3];
+        const uint32_t held = seen != nullptr ? seen[v >> 3] & may : 0u;
+        if (held != 0) {
+#pragma unroll
+            for (int i = 0; i < kLgVec; ++i) {
+                if (held >> i & 1) x[i] = penalised(x[i], row, true, counts[v + i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLgVec; ++i) x[i] = allowed_or_none(x[i], may >> i & 1);
+    }
+
+    // Token v with its biases and the row's ancestors.
+    KVIP_DEVICE float one(int v, int b, const int* way, int ways) {
+        int n = seen != nullptr ? counts[v] : 0;
+        bool held = seen != nullptr && (seen[v >> 3] >> (v & 7) & 1);
+        for (int i = 0; i < ways; ++i) {
+            n += way[i] == v;
+            held = held || way[i] == v;
+        }
+        float x = penalised(static_cast<float>(logits[v]), row, held, n);
+        const int32_t* names = p.bias_tokens + static_cast<int64_t>(b) * p.biases;
+        const float* values = p.bias_values + static_cast<int64_t>(b) * p.biases;
+        for (int i = 0; i < p.biases; ++i) {
+            if (names[i] == v) x += values[i];
+        }
+        return allowed_or_none(x, allowed == nullptr || (allowed[v >> 3] >> (v & 7) & 1));
+    }
+};
+
+enum { kLgStats = 1, kLgWrite = 2 };  // both: a row is one part
+
+template <typename T, typename O, int MODE>
+__global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs p, int parts, int part_size) {
+    __shared__ uint32_t s_special[kLgMaxPart / 32];
+    __shared__ LogitStat s_stats[kLgWaves];
+    __shared__ int s_way[64];
+    __shared__ int s_ways, s_request;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int row = blockIdx.x / parts, part = blockIdx.x % parts;
+    uint32_t err = 0;
+
+    if (tid == 0) s_request = p.batch;
+    __syncthreads();
+    for (int b = tid; b < p.batch; b += kLgThreads) {
+        const int from = p.cu_seqlens[b], to = p.cu_seqlens[b + 1];
+        if (from <= row && row < to) atomicMin(&s_request, b);
+        if (from < 0 || to < from || to > p.max_tokens) err |= KVIP_STATUS_BAD_LENGTH;
+    }
+    if (blockIdx.x != 0 || (MODE & kLgStats) == 0) err = 0;
+    __syncthreads();
+    const int b = s_request;
+    if (b >= p.batch) {
+        report(p.status, err);
+        return;
+    }
+    const int words = (p.vocab + 31) / 32;
+    LogitPart<T> at = {p, static_cast<const T*>(p.logits) + row * p.logits_stride,
+                       p.counts == nullptr ? nullptr : p.counts + static_cast<int64_t>(b) * p.vocab,
+                       p.seen == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.seen + static_cast<int64_t>(b) * words),
+                       p.allowed == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.allowed + static_cast<int64_t>(row) * words),
+                       nullptr, part * part_size, min((part + 1) * part_size, p.vocab), {}, 0};
+    const float temperature = p.temperature == nullptr ? 1.f : p.temperature[b];
+    at.row.repetition = p.repetition == nullptr ? 1.f : p.repetition[b];
+    at.row.inverse = 1.f / at.row.repetition;
+    at.row.presence = p.presence == nullptr ? 0.f : p.presence[b];
+    at.row.frequency = p.frequency == nullptr ? 0.f : p.frequency[b];
+    at.row.greedy = !(temperature > 0.f);
+    at.row.c = at.row.greedy ? 1.f : kLgLog2e / temperature;
+    at.row.plain = at.row.c > 0.f && at.row.c < INFINITY;
+
+    // The row's ancestors, and which tokens of this part are not the dense pass's.
+    uint64_t mine = 0;  // bit k: this thread has the token that entry tid + 512 k names
+    const int listed = (p.visible == nullptr ? 0 : 63) + p.biases;
+    if (listed > 0) {
+        if (tid < 64) {
+            const int begin = min(max(p.cu_seqlens[b], 0), p.max_tokens), behind = min(max(p.cu_seqlens[b + 1], begin), p.max_tokens);
+            bool on = p.visible != nullptr && lane > 0 && begin + lane < behind &&
+                      (static_cast<uint64_t>(p.visible[row]) >> lane & 1);
+            const int64_t token = on ? p.tokens[begin + lane] : 0;
+            if (on && (token < 0 || token >= p.vocab)) {
+                err |= KVIP_STATUS_BAD_TOKEN;
+                on = false;
+            }
+            const uint64_t all = __ballot(on);
+            if (on) s_way[__popcll(all & ((1ull << lane) - 1))] = static_cast<int>(token);
+            if (lane == 0) s_ways = __popcll(all);
+        }
+        for (int i = tid; i < (at.end - at.begin + 31) / 32; i += kLgThreads) s_special[i] = 0;
+        __syncthreads();
+        const int ways = s_ways;
+        for (int e = tid, k = 0; e < ways + p.biases; e += kLgThreads, ++k) {
+            const int v = e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
+            if (v >= p.vocab) err |= KVIP_STATUS_BAD_TOKEN;
+            if (v < at.begin || v >= at.end) continue;
+            const uint32_t bit = 1u << (v & 31);
+            if (!(atomicOr(&s_special[(v - at.begin) >> 5], bit) & bit)) mine |= 1ull << k;
+        }
+        __syncthreads();
+        at.special = s_special;
+    }
+    auto named = [&](int k) {
+        const int e = tid + k * kLgThreads, ways = s_ways;
+        return e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
+    };
+
+    LogitStat stat = {-INFINITY, 0.f, p.vocab, 0};
+    LogitStat* stats = static_cast<LogitStat*>(p.workspace) + static_cast<int64_t>(row) * parts;
+    if constexpr ((MODE & kLgStats) != 0) {
+        for (int v = at.begin + tid * kLgVec; v < at.end; v += kLgRun) {
+            float x[kLgVec], most;
+            at.load(v, x);
+            most = x[0];
+#pragma unroll
+            for (int i = 1; i < kLgVec; ++i) most = fmaxf(most, x[i]);
+            if (most > stat.m) {
+                stat.l *= weight_of(stat.m, most, at.row);
+                stat.m = most;
+#pragma unroll
+                for (int i = kLgVec - 1; i >= 0; --i) stat.first = x[i] == most ? v + i : stat.first;
+            }
+            if (!at.row.greedy && stat.m != -INFINITY) {
+#pragma unroll
+                for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
+            }
+        }
+        for (uint64_t left = mine; left != 0; left &= left - 1) {
+            const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
+            merge(stat, at.one(v, b, s_way, s_ways), 1.f, v, at.row);
+        }
+        merge_block(stat, s_stats, at.row);
+        if constexpr (MODE == kLgStats) {
+            if (tid == 0) stats[part] = stat;
+        }
+        err |= at.err;
+    } else {
+        if (tid < parts) stat = stats[tid];
+        merge_block(stat, s_stats, at.row);
+    }
+    if constexpr ((MODE & kLgWrite) != 0) {
+        if (part == 0 && tid == 0 && stat.m == -INFINITY) err |= KVIP_STATUS_BAD_PROBS;
+        const float share = stat.m == -INFINITY ? 0.f : 1.f / stat.l;
+        auto prob = [&](float x, int v) {
+            if (stat.m == -INFINITY) return 0.f;
+            return at.row.greedy ? (v == stat.first ? 1.f : 0.f) : weight_of(x, stat.m, at.row) * share;
+        };
+        O* out = static_cast<O*>(p.probs) + row * p.probs_stride;
+        for (int v = at.begin + tid * kLgVec; v < at.end; v += kLgRun) {
+            float x[kLgVec];
+            at.load(v, x);
+            typename Logits<O>::vec y;
+#pragma unroll
+            for (int i = 0; i < kLgVec; ++i) y[i] = static_cast<O>(prob(x[i], v + i));
+            if (at.end - v >= kLgVec) {
+                *reinterpret_cast<typename Logits<O>::vec*>(out + v) = y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLgVec; ++i) {
+                    if (v + i < at.end) out[v + i] = y[i];
+                }
+            }
+        }
+        if (listed > 0) {
+            __syncthreads();  // the dense pass's zeros are in place
+            for (uint64_t left = mine; left != 0; left &= left - 1) {
+                const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
+                out[v] = static_cast<O>(prob(at.one(v, b, s_way, s_ways), v));
+            }
+        }
+    }
+    report(p.status, err);
+}
+
+// A launch has fewer than 2^32 threads.
+bool logits_fit(int rows, int parts) { return static_cast<int64_t>(rows) * parts * kLgThreads < (1ll << 32); }
+
+// Parts of a row: enough workgroups for 4 per CU, of whole runs.
+void logit_parts(int rows, int vocab, int* parts, int* size) {
+    const int64_t runs = (vocab + kLgRun - 1) / kLgRun, most = kLgMaxPart / kLgRun;
+    int64_t want = (1024 + rows - 1) / rows;
+    want = want < (runs + most - 1) / most ? (runs + most - 1) / most : want > runs ? runs : want;
+    const int64_t per = (runs + want - 1) / want;
+    *parts = static_cast<int>((runs + per - 1) / per);
+    *size = static_cast<int>(per * kLgRun);
+}
+
+template <typename T, typename O>
+void launch_logits(const KvipLogitArgs& a, hipStream_t s) {
+    int parts, size;
+    logit_parts(a.max_tokens, a.vocab, &parts, &size);
+    const dim3 grid(static_cast<unsigned>(parts) * static_cast<unsigned>(a.max_tokens)), block(kLgThreads);
+    if (parts == 1) {
+        hipLaunchKernelGGL((logits_kernel<T, O, kLgStats | kLgWrite>), grid, block, 0, s, a, parts, size);
+    } else {
+        hipLaunchKernelGGL((logits_kernel<T, O, kLgStats>), grid, block, 0, s, a, parts, size);
+        hipLaunchKernelGGL((logits_kernel<T, O, kLgWrite>), grid, block, 0, s, a, parts, size);
+    }
+}
+
+template <typename T>
+void launch_logits(const KvipLogitArgs& a, hipStream_t s) {
+    switch (a.probs_dtype) {
+        case KVIP_DTYPE_BF16: launch_logits<T, __bf16>(a, s); break;
+        case KVIP_DTYPE_FP16: launch_logits<T, _Float16>(a, s); break;
+        default: launch_logits<T, float>(a, s); break;
+    }
+}
+
+// A request's counts over one part of the vocabulary, counted in LDS and written whole, so that nothing has to be
+// cleared before.
+constexpr int kHistThreads = 1024;
+constexpr int kHistPart = 1 << 14;  // 64 KB of counts
+
+__global__ __launch_bounds__(kHistThreads) void history_load_kernel(const KvipHistoryArgs p, int parts) {
+    __shared__ int s_counts[kHistPart];
+    __shared__ uint32_t s_seen[kHistPart / 32];
+    const int tid = threadIdx.x, i = blockIdx.x / parts, part = blockIdx.x % parts;
+    const int request = p.requests[i], first = p.cu_seqlens[i], behind = p.cu_seqlens[i + 1];
+    const int most = static_cast<int>(p.max_tokens);
+    const int from = min(max(first, 0), most), to = min(max(behind, from), most);
+    uint32_t err = from != first || to != behind || request >= p.batch ? KVIP_STATUS_BAD_LENGTH : 0;
+    if (part == 0 && tid == 0) report(p.status, err);
+    if (request < 0 || request >= p.batch) return;
+    const int begin = part * kHistPart, size = min(kHistPart, p.vocab - begin), words = (size + 31) / 32;
+    for (int v = tid; v < size; v += kHistThreads) s_counts[v] = 0;
+    for (int w = tid; w < words; w += kHistThreads) s_seen[w] = 0;
+    __syncthreads();
+    const int64_t written = static_cast<int64_t>(from) + max(p.prompt_lens[i], 0);
+    err = 0;
+    for (int64_t t = from + tid; t < to; t += kHistThreads) {
+        const int64_t v = p.tokens[t];
+        if (v < 0 || v >= p.vocab) err = KVIP_STATUS_BAD_TOKEN;
+        if (v < begin || v >= begin + size) continue;
+        const int at = static_cast<int>(v) - begin;
+        atomicOr(&s_seen[at >> 5], 1u << (at & 31));
+        if (t >= written) atomicAdd(&s_counts[at], 1);
+    }
+    if (part == 0) report(p.status, err);
+    __syncthreads();
+    int32_t* counts = p.counts + static_cast<int64_t>(request) * p.vocab + begin;
+    uint32_t* seen = p.seen + static_cast<int64_t>(request) * ((p.vocab + 31) / 32) + begin / 32;
+    for (int v = tid; v < size; v += kHistThreads) counts[v] = s_counts[v];
+    for (int w = tid; w < words; w += kHistThreads) seen[w] = s_seen[w];
+}
+
+__global__ __launch_bounds__(256) void history_append_kernel(const KvipHistoryArgs p) {
+    const int at = blockIdx.x * 256 + threadIdx.x, b = at / p.token_stride, i = at % p.token_stride;
+    if (b >= p.batch) return;
+    const int kept = p.kept[b];
+    if (i == 0 && (kept < 0 || kept > p.token_stride)) report(p.status, KVIP_STATUS_BAD_LENGTH);
+    if (i >= kept) return;
+    const int64_t v = p.tokens[at];
+    if (v < 0 || v >= p.vocab) {
+        report(p.status, KVIP_STATUS_BAD_TOKEN);
+        return;
+    }
+    atomicAdd(&p.counts[static_cast<int64_t>(b) * p.vocab + v], 1);
+    atomicOr(&p.seen[static_cast<int64_t>(b) * ((p.vocab + 31) / 32) + v / 32], 1u << (v % 32));
+}
+
+bool valid_history(const KvipHistoryArgs* a) {
+    return a != nullptr && a->counts && a->seen && a->tokens && a->batch >= 1 && a->batch <= KVIP_DRAFT_MAX_BATCH &&
+           a->vocab >= 1 && a->vocab <= (1 << 20);
+}
+
+bool logit_dtype(int32_t t) { return t == KVIP_DTYPE_FP32 || t == KVIP_DTYPE_BF16 || t == KVIP_DTYPE_FP16; }
+
+}  // namespace
+}  // namespace kvip
+
+extern "C" uint32_t kvip_hip_prompt_abi_version(void) { return KVIP_PROMPT_ABI_VERSION; }
+
+extern "C" uint32_t kvip_hip_history_load(const KvipHistoryArgs* a, void* stream) {
+    if (!kvip::valid_history(a) || !a->requests || !a->cu_seqlens || !a->prompt_lens || a->count < 1 ||
+        a->count > KVIP_DRAFT_MAX_BATCH || a->max_tokens < 0 || a->max_tokens > 0x7FFFFFFF) {
+        return KVIP_ERR_INVALID;
+    }
+    const int parts = (a->vocab + kvip::kHistPart - 1) / kvip::kHistPart;
+    hipLaunchKernelGGL(kvip::history_load_kernel, dim3(a->count * parts), dim3(kvip::kHistThreads), 0,
+                       static_cast<hipStream_t>(stream), *a, parts);
+    return static_cast<uint32_t>(hipGetLastError());
+}
+
+extern "C" uint32_t kvip_hip_history_append(const KvipHistoryArgs* a, void* stream) {
+    if (!kvip::valid_history(a) || !a->kept || a->token_stride < 1 || a->token_stride > KVIP_DRAFT_MAX_NODES) return KVIP_ERR_INVALID;
+    hipLaunchKernelGGL(kvip::history_append_kernel, dim3((a->batch * a->token_stride + 255) / 256), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), *a);
+    return static_cast<uint32_t>(hipGetLastError());
+}
+
+extern "C" uint64_t kvip_hip_process_logits_workspace_bytes(int32_t max_tokens, int32_t vocab) {
+    if (max_tokens < 1 || max_tokens > KVIP_DRAFT_MAX_TOKENS || vocab < 1 || vocab > (1 << 20)) return 0;
+    int parts, size;
+    kvip::logit_parts(max_tokens, vocab, &parts, &size);
+    if (!kvip::logits_fit(max_tokens, parts)) return 0;
+    return static_cast<uint64_t>(max_tokens) * parts * sizeof(kvip::LogitStat);
+}
+
+extern "C" uint32_t kvip_hip_process_logits(const KvipLogitArgs* a, void* stream) {
+    if (a == nullptr) return KVIP_ERR_INVALID;
+    const bool ok = a->logits && a->probs && a->cu_seqlens && a->workspace &&
+                    (reinterpret_cast<uintptr_t>(a->workspace) & 15u) == 0 && (a->counts == nullptr) == (a->seen == nullptr) &&
+                    (a->tokens == nullptr) == (a->visible == nullptr) && a->biases >= 0 && a->biases <= KVIP_LOGIT_MAX_BIASES &&
+                    (a->biases == 0 || (a->bias_tokens && a->bias_values)) && a->batch >= 1 &&
+                    a->batch <= KVIP_DRAFT_MAX_BATCH && a->max_tokens >= 1 && a->max_tokens <= KVIP_DRAFT_MAX_TOKENS &&
+                    a->vocab >= 1 && a->vocab <= (1 << 20) && a->logits_stride >= a->vocab && a->probs_stride >= a->vocab &&
+                    kvip::logit_dtype(a->dtype) && kvip::logit_dtype(a->probs_dtype) &&
+                    kvip_hip_process_logits_workspace_bytes(a->max_tokens, a->vocab) != 0;
+    if (!ok) return KVIP_ERR_INVALID;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (a->dtype) {
+        case KVIP_DTYPE_BF16: kvip::launch_logits<__bf16>(*a, s); break;
+        case KVIP_DTYPE_FP16: kvip::launch_logits<_Float16>(*a, s); break;
+        default: kvip::launch_logits<float>(*a, s); break;
+    }
+    return static_cast<uint32_t>(hipGetLastError());
+}

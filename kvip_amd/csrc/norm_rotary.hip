@@ -1,0 +1,332 @@
+// Norm of every head of queries and keys and its turn by the token's position in one pass, and for the indexer the
+// fp8 features and scale of each head, keys into their paged cache (kvip_hip_prompt.h).
+//
+// A head is held by G lanes (8 features each, as two runs of four, so that both features of a pair are in one lane in
+// either layout); its sums and its largest magnitude are taken over those lanes by DPP and lane swaps. Mean and
+// variance are two passes over registers, in 32 bits. Heads of other sizes go through LDS, a wave per head.
+// A workgroup takes a run of tokens and works their angles out once; a thread holds its features' weights.
+#include "kvip_hip_prompt.h"
+#include "turn.h"
+
+namespace kvip {
+namespace {
+
+constexpr int kNrThreads = 256;
+constexpr int kNrWaves = kNrThreads / 64;
+constexpr int kNrPairs = 1024;  // pairs of a workgroup's run of tokens (8 KB of LDS)
+constexpr int kNrLane = 8;      // features of a lane
+
+template <typename T> struct Four { typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
+
+template <int CTRL>
+KVIP_DEVICE float dpp_all(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+
+// x of all G lanes of a group put together, in every lane of it; G lanes lie side by side.
+template <int G, typename F>
+KVIP_DEVICE float over_group(float x, F f) {
+    x = f(x, dpp_all<0xB1>(x));   // lane ^ 1
+    x = f(x, dpp_all<0x4E>(x));   // lane ^ 2
+    x = f(x, dpp_all<0x141>(x));  // mirrored in 8
+    if constexpr (G >= 16) x = f(x, dpp_all<0x140>(x));  // mirrored in 16
+    if constexpr (G >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    return x;
+}
+template <int G> KVIP_DEVICE float group_sum(float x) { return over_group<G>(x, [](float a, float b) { return a + b; }); }
+template <int G> KVIP_DEVICE float group_max(float x) { return over_group<G>(x, [](float a, float b) { return fmaxf(a, b); }); }
+
+// Scale of a head whose largest magnitude is given, and a feature under it: as in the rows of the KV cache.
+KVIP_DEVICE float head_scale(float largest) {
+    const float quotient = largest / 448.f;
+    return quotient > 0.f ? quotient : 1.f;
+}
+KVIP_DEVICE float under_scale(float x, float scale) {
+    x /= scale;
+    return x > 448.f ? 448.f : x < -448.f ? -448.f : x;
+}
+
+// Where a head of queries or a key goes: false where nowhere.
+struct HeadPlace {
+    int64_t out, scale;  // elements
+};
+KVIP_DEVICE bool head_place(const KvipNormRotaryArgs& p, const KvipNormTensor& t, bool paged, int64_t token, int head, HeadPlace* at,
+                            uint32_t* err) {
+    if (!paged) {
+        at->out = token * t.out_token + head * t.out_head;
+        at->scale = token * t.heads + head;
+        return true;
+    }
+    const int64_t slot = p.slots[token];
+    if (slot >= static_cast<int64_t>(p.num_blocks) * kBlockTokens) *err |= KVIP_STATUS_BAD_TOKEN;
+    if (slot < 0 || slot >= static_cast<int64_t>(p.num_blocks) * kBlockTokens) return false;
+    at->out = slot / kBlockTokens * t.out_token + slot % kBlockTokens * kIndexDim;
+    at->scale = slot / kBlockTokens * t.out_head + slot % kBlockTokens;
+    return true;
+}
+
+template <typename T, bool HALF, int G, bool QUANT>
+__global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormRotaryArgs p, int run) {
+    typedef typename Four<T>::vec V;
+    __shared__ __align__(16) float2 s_turn[kNrPairs];
+    const int tid = threadIdx.x, pairs = p.rotary_dim / 2;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * run;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(run), p.tokens - first));
+    for (int i = tid; i < tokens * pairs; i += kNrThreads) {
+        s_turn[i] = turn_of(p.positions[first + i / pairs], p.frequencies[i % pairs], p.magnitude, false);
+    }
+    __syncthreads();
+    const int j = tid % G;
+    const bool live = j * kNrLane < p.dim, turned = j * kNrLane < p.rotary_dim;
+    const int at[2] = {HALF && turned ? 4 * j : 8 * j, HALF && turned ? pairs + 4 * j : 8 * j + 4};
+    const float share = 1.f / static_cast<float>(p.dim);
+    uint32_t err = 0;
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+        const KvipNormTensor& t = p.tensors[k];
+        if (t.x == nullptr) continue;
+        float weight[kNrLane], bias[kNrLane];
+#pragma unroll
+        for (int i = 0; i < kNrLane; ++i) {
+            weight[i] = live && t.weight != nullptr ? t.weight[at[i / 4] + i % 4] : 1.f;
+            bias[i] = live && t.bias != nullptr ? t.bias[at[i / 4] + i % 4] : 0.f;
+        }
+        for (int u = tid / G; u < tokens * t.heads; u += kNrThreads / G) {
+            const int token = u / t.heads, head = u % t.heads;
+            const T* in = static_cast<const T*>(t.x) + (first + token) * t.x_token + head * t.x_head;
+            float x[kNrLane];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                V raw = {};
+                if (live) raw = *reinterpret_cast<const V*>(in + at[r]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[4 * r + i] = static_cast<float>(raw[i]);
+            }
+            if (t.norm != KVIP_NORM_NONE) {
+                float sum = 0.f;
+                if (t.norm == KVIP_NORM_LAYER) {
+#pragma unroll
+                    for (int i = 0; i < kNrLane; ++i) sum += x[i];
+                    const float mean = group_sum<G>(sum) * share;
+#pragma unroll
+                    for (int i = 0; i < kNrLane; ++i) x[i] -= mean;
+                    sum = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < kNrLane; ++i) sum = fmaf(x[i], x[i], sum);
+                const float factor = 1.f / sqrtf(group_sum<G>(live ? sum : 0.f) * share + p.epsilon);
+#pragma unroll
+                for (int i = 0; i < kNrLane; ++i) x[i] = fmaf(x[i] * factor, weight[i], bias[i]);
+            } else if (t.weight != nullptr || t.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < kNrLane; ++i) x[i] = fmaf(x[i], weight[i], bias[i]);
+            }
+            if (turned) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 turn = s_turn[token * pairs + 4 * j + i];
+                    float& a = x[HALF ? i : 2 * i];
+                    float& b = x[HALF ? 4 + i : 2 * i + 1];
+                    const float c = a * turn.x - b * turn.y;
+                    b = b * turn.x + a * turn.y;
+                    a = c;
+                }
+            }
+            HeadPlace place;
+            if (!head_place(p, t, QUANT && k == 1, first + token, head, &place, &err) || !live) continue;
+            if constexpr (QUANT) {
+                float largest = 0.f;
+#pragma unroll
+                for (int i = 0; i < kNrLane; ++i) largest = fmaxf(largest, fabsf(x[i]));
+                const float scale = head_scale(group_max<G>(largest));
+                uint8_t* out = static_cast<uint8_t*>(t.out) + place.out;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    int packed = 0;
+                    packed = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[4 * r], scale), under_scale(x[4 * r + 1], scale), packed, false);
+                    packed = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[4 * r + 2], scale), under_scale(x[4 * r + 3], scale), packed, true);
+                    *reinterpret_cast<int*>(out + at[r]) = packed;
+                }
+                if (j == 0) t.scales[place.scale] = scale;
+            } else {
+                T* out = static_cast<T*>(t.out) + place.out;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    V y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = static_cast<T>(x[4 * r + i]);
+                    *reinterpret_cast<V*>(out + at[r]) = y;
+                }
+            }
+        }
+    }
+    report(p.status, err);
+}
+
+// Heads whose features do not come in eights: a wave per head, feature lane + 64 i in register i, pairs met in LDS.
+template <typename T>
+__global__ __launch_bounds__(kNrThreads) void norm_rotary_any_kernel(const KvipNormRotaryArgs p) {
+    constexpr int kPer = KVIP_NORM_MAX_DIM / 64;
+    __shared__ float s_head[kNrWaves][KVIP_NORM_MAX_DIM];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, pairs = p.rotary_dim / 2;
+    const int heads = p.tensors[0].heads + (p.tensors[1].x != nullptr ? p.tensors[1].heads : 0);
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kNrWaves + w;
+    const int64_t token = unit / heads;
+    if (token >= p.tokens) return;  // the whole wave, which meets no other
+    int head = static_cast<int>(unit % heads);
+    const int k = head >= p.tensors[0].heads;
+    if (k == 1) head -= p.tensors[0].heads;
+    const KvipNormTensor& t = p.tensors[k];
+    const T* in = static_cast<const T*>(t.x) + token * t.x_token + head * t.x_head;
+    const float share = 1.f / static_cast<float>(p.dim);
+    float x[kPer], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        x[i] = lane + 64 * i < p.dim ? static_cast<float>(in[lane + 64 * i]) : 0.f;
+        sum += x[i];
+    }
+    float factor = 1.f, mean = 0.f;
+    if (t.norm == KVIP_NORM_LAYER) mean = group_sum<64>(sum) * share;
+    if (t.norm != KVIP_NORM_NONE) {
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            x[i] -= mean;
+            if (lane + 64 * i < p.dim) sum = fmaf(x[i], x[i], sum);
+        }
+        factor = 1.f / sqrtf(group_sum<64>(sum) * share + p.epsilon);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int f = lane + 64 * i;
+        if (f >= p.dim) continue;
+        x[i] *= factor;
+        if (t.weight != nullptr || t.bias != nullptr) {
+            x[i] = fmaf(x[i], t.weight != nullptr ? t.weight[f] : 1.f, t.bias != nullptr ? t.bias[f] : 0.f);
+        }
+        s_head[w][f] = x[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int f = lane + 64 * i;
+        if (f >= p.dim) continue;
+        if (f < p.rotary_dim) {
+            const int pair = p.half ? f % pairs : f / 2;
+            const bool second = p.half ? f >= pairs : (f & 1) != 0;
+            const float other = s_head[w][p.half ? (second ? f - pairs : f + pairs) : f ^ 1];
+            const float2 turn = turn_of(p.positions[token], p.frequencies[pair], p.magnitude, false);
+            x[i] = x[i] * turn.x + (second ? other : -other) * turn.y;
+        }
+        largest = fmaxf(largest, fabsf(x[i]));
+    }
+    HeadPlace place;
+    uint32_t err = 0;
+    const bool there = head_place(p, t, p.quantised != 0 && k == 1, token, head, &place, &err);
+    if (lane == 0) report(p.status, err);
+    if (!there) return;
+    const float scale = p.quantised != 0 ? head_scale(group_max<64>(largest)) : 1.f;
+    if (p.quantised != 0 && lane == 0) t.scales[place.scale] = scale;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int f = lane + 64 * i;
+        if (f >= p.dim) continue;
+        if (p.quantised != 0) {
+            const int code = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[i], scale), 0.f, 0, false);
+            static_cast<uint8_t*>(t.out)[place.out + f] = static_cast<uint8_t>(code & 0xFF);
+        } else {
+            static_cast<T*>(t.out)[place.out + f] = static_cast<T>(x[i]);
+        }
+    }
+}
+
+template <typename T, int G, bool QUANT>
+void launch_group(const KvipNormRotaryArgs& a, int run, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>((a.tokens + run - 1) / run)), block(kNrThreads);
+    if (a.half) {
+        hipLaunchKernelGGL((norm_rotary_kernel<T, true, G, QUANT>), grid, block, 0, s, a, run);
+    } else {
+        hipLaunchKernelGGL((norm_rotary_kernel<T, false, G, QUANT>), grid, block, 0, s, a, run);
+    }
+}
+
+template <typename T>
+void launch_norm_rotary(const KvipNormRotaryArgs& a, hipStream_t s) {
+    const int heads = a.tensors[0].heads + (a.tensors[1].x != nullptr ? a.tensors[1].heads : 0);
+    if (a.dim % kNrLane != 0 || a.rotary_dim % kNrLane != 0) {
+        const int64_t units = a.tokens * heads;
+        hipLaunchKernelGGL(norm_rotary_any_kernel<T>, dim3(static_cast<unsigned>((units + kNrWaves - 1) / kNrWaves)), dim3(kNrThreads),
+                           0, s, a);
+        return;
+    }
+    // Lanes of a head, and tokens of a workgroup: enough for each group of lanes to have a head, as many as there is LDS
+    // for, and few enough that 1024 workgroups (4 per CU) have some.
+    const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : a.dim <= 256 ? 32 : 64;
+    const int64_t fill = (kNrThreads / lanes + heads - 1) / heads, share = (a.tokens + 1023) / 1024;
+    const int64_t room = kNrPairs / (a.rotary_dim / 2), want = fill < share ? fill : share;
+    const int run = static_cast<int>(want < 1 ? 1 : want > room ? room : want);
+    if (a.quantised) launch_group<T, 16, true>(a, run, s);
+    else if (lanes == 8) launch_group<T, 8, false>(a, run, s);
+    else if (lanes == 16) launch_group<T, 16, false>(a, run, s);
+    else if (lanes == 32) launch_group<T, 32, false>(a, run, s);
+    else launch_group<T, 64, false>(a, run, s);
+}
+
+bool valid_norm(const KvipNormRotaryArgs& a, int k) {
+    const KvipNormTensor& t = a.tensors[k];
+    if (t.x == nullptr) return k == 1;
+    if (!t.out || t.heads < 1 || t.heads > 65536 || t.norm < KVIP_NORM_NONE || t.norm > KVIP_NORM_LAYER) return false;
+    if (!a.quantised) return true;
+    // A lane stores four bytes at a time.
+    if (!t.scales || (reinterpret_cast<uintptr_t>(t.out) & 3u) != 0 || t.out_token % 4 != 0) return false;
+    if (k == 0) return t.out_head % 4 == 0;
+    return a.slots && t.heads == 1 && a.num_blocks >= 1 && t.out_token >= kBlockTokens * kIndexDim && t.out_head >= kBlockTokens;
+}
+
+// A launch has fewer than 2^32 threads: longer calls are made in runs of tokens.
+constexpr int64_t kNrLaunchUnits = 1 << 25;
+
+}  // namespace
+}  // namespace kvip
+
+extern "C" uint32_t kvip_hip_norm_rotary(const KvipNormRotaryArgs* a, void* stream) {
+    if (a == nullptr) return KVIP_ERR_INVALID;
+    const bool ok = a->positions && a->frequencies && a->tokens >= 0 && a->tokens <= (1ll << 31) && a->rotary_dim >= 2 &&
+                    a->rotary_dim % 2 == 0 && a->rotary_dim <= a->dim && a->dim <= KVIP_NORM_MAX_DIM &&
+                    (!a->quantised || a->dim == KVIP_INDEX_DIM) && a->epsilon >= 0.f && a->epsilon - a->epsilon == 0.f &&
+                    kvip::valid_norm(*a, 0) && kvip::valid_norm(*a, 1) &&
+                    (a->dtype == KVIP_DTYPE_BF16 || a->dtype == KVIP_DTYPE_FP16 || a->dtype == KVIP_DTYPE_FP32);
+    if (!ok) return KVIP_ERR_INVALID;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t size = a->dtype == KVIP_DTYPE_FP32 ? 4 : 2;
+    const int64_t heads = a->tensors[0].heads + (a->tensors[1].x != nullptr ? a->tensors[1].heads : 0);
+    const int64_t most = heads > kvip::kNrLaunchUnits ? 1 : kvip::kNrLaunchUnits / heads;
+    for (int64_t first = 0; first < a->tokens; first += most) {
+        KvipNormRotaryArgs part = *a;
+        part.positions += first;
+        if (part.slots != nullptr) part.slots += first;
+        part.tokens = a->tokens - first < most ? a->tokens - first : most;
+        for (int k = 0; k < 2; ++k) {
+            KvipNormTensor& t = part.tensors[k];
+            if (t.x == nullptr) continue;
+            t.x = static_cast<const char*>(t.x) + first * t.x_token * size;
+            if (a->quantised && k == 1) continue;  // by slots
+            t.out = static_cast<char*>(t.out) + first * t.out_token * (a->quantised ? 1 : size);
+            if (a->quantised) t.scales += first * t.heads;
+        }
+        switch (a->dtype) {
+            case KVIP_DTYPE_BF16: kvip::launch_norm_rotary<__bf16>(part, s); break;
+            case KVIP_DTYPE_FP16: kvip::launch_norm_rotary<_Float16>(part, s); break;
+            default: kvip::launch_norm_rotary<float>(part, s); break;
+        }
+    }
+    return static_cast<uint32_t>(hipGetLastError());
+}

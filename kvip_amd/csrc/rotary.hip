@@ -9,8 +9,8 @@
 // angles cost as much as some 40 features, so a workgroup works them out once for a run of tokens
 // into LDS and every head of these tokens takes them from there. 8192 tokens of 64 query
 // heads and a key of 128 features take 59 us (4.6 TB/s; a large copy reaches 5.1), a step of 256 tokens 4.
-#include "kvip_device.h"
 #include "kvip_hip_draft.h"
+#include "turn.h"
 
 namespace kvip {
 namespace {
@@ -26,14 +26,6 @@ template <typename T> struct Feature;
 template <> struct Feature<__bf16> { typedef __bf16 vec __attribute__((ext_vector_type(kVec), aligned(2))); };
 template <> struct Feature<_Float16> { typedef _Float16 vec __attribute__((ext_vector_type(kVec), aligned(2))); };
 template <> struct Feature<float> { typedef float vec __attribute__((ext_vector_type(kVec), aligned(4))); };
-
-KVIP_DEVICE float2 turn_of(int64_t position, double frequency, float magnitude, bool inverse) {
-    const double turns = static_cast<double>(position) * frequency * 0.15915494309189533577;  // 1 / (2 pi)
-    const float fraction = static_cast<float>(turns - rint(turns));
-    float s, c;
-    sincospif(2.0f * fraction, &s, &c);
-    return make_float2(c * magnitude, (inverse ? -s : s) * magnitude);
-}
 
 template <typename T>
 KVIP_DEVICE void turn_pair(T a, T b, float2 t, T* x, T* y) {

@@ -11,6 +11,7 @@ from pathlib import Path
 LIBRARY = Path(__file__).resolve().parents[1] / "_lib" / "libkvip_hip.so"
 ABI_VERSION = 15
 DRAFT_ABI_VERSION = 2
+PROMPT_ABI_VERSION = 1
 
 KVIP_OK = 0
 KVIP_ERR_INVALID = 100000
@@ -253,6 +254,52 @@ class VerifyArgs(ctypes.Structure):
     ]
 
 
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2  # this and the following: include/kvip_hip_prompt.h
+NORM_MAX_DIM = 512
+LOGIT_MAX_BIASES = 4096
+
+
+class ChunkAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", _p), ("kv_cache", _p), ("block_table", _p), ("seq_lens", _p), ("cu_seqlens", _p), ("steps", _p),
+        ("output", _p), ("lse", _p), ("workspace", _p), ("status", _p), ("kv_block_stride", _i64), ("max_rows", _i64),
+        ("row_stride", _i32), ("batch", _i32), ("heads", _i32), ("max_tokens", _i32), ("max_blocks", _i32),
+        ("num_blocks", _i32), ("output_dtype", _i32), ("scale", ctypes.c_float),
+    ]
+
+
+class NormTensor(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("out", _p), ("weight", _p), ("bias", _p), ("scales", _p), ("x_token", _i64), ("x_head", _i64),
+        ("out_token", _i64), ("out_head", _i64), ("heads", _i32), ("norm", _i32),
+    ]
+
+
+class NormRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("tensors", NormTensor * 2), ("positions", _p), ("frequencies", _p), ("slots", _p), ("status", _p), ("tokens", _i64),
+        ("dim", _i32), ("rotary_dim", _i32), ("half", _i32), ("dtype", _i32), ("quantised", _i32), ("num_blocks", _i32),
+        ("epsilon", ctypes.c_float), ("magnitude", ctypes.c_float),
+    ]
+
+
+class HistoryArgs(ctypes.Structure):
+    _fields_ = [
+        ("counts", _p), ("seen", _p), ("tokens", _p), ("requests", _p), ("cu_seqlens", _p), ("prompt_lens", _p), ("kept", _p),
+        ("status", _p), ("max_tokens", _i64), ("count", _i32), ("batch", _i32), ("vocab", _i32), ("token_stride", _i32),
+    ]
+
+
+class LogitArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", _p), ("probs", _p), ("cu_seqlens", _p), ("temperature", _p), ("repetition", _p), ("presence", _p),
+        ("frequency", _p), ("counts", _p), ("seen", _p), ("tokens", _p), ("visible", _p), ("bias_tokens", _p),
+        ("bias_values", _p), ("allowed", _p), ("workspace", _p), ("status", _p), ("logits_stride", _i64),
+        ("probs_stride", _i64), ("batch", _i32), ("max_tokens", _i32), ("vocab", _i32), ("biases", _i32), ("dtype", _i32),
+        ("probs_dtype", _i32),
+    ]
+
+
 # name -> (argtypes, restype); must list every function declared in include/kvip_hip.h.
 PROTOTYPES = {
     "kvip_hip_abi_version": ([], ctypes.c_uint32),
@@ -319,6 +366,18 @@ DRAFT_PROTOTYPES = {
     "kvip_hip_verify_drafts_workspace_bytes": ([_i32, _i32], ctypes.c_uint64),
 }
 
+# The same for include/kvip_hip_prompt.h.
+PROMPT_PROTOTYPES = {
+    "kvip_hip_prompt_abi_version": ([], ctypes.c_uint32),
+    "kvip_hip_chunk_attention": ([ctypes.POINTER(ChunkAttnArgs), _p], ctypes.c_uint32),
+    "kvip_hip_chunk_attention_workspace_bytes": ([_i32, _i32, _i32, _i64], ctypes.c_uint64),
+    "kvip_hip_norm_rotary": ([ctypes.POINTER(NormRotaryArgs), _p], ctypes.c_uint32),
+    "kvip_hip_history_load": ([ctypes.POINTER(HistoryArgs), _p], ctypes.c_uint32),
+    "kvip_hip_history_append": ([ctypes.POINTER(HistoryArgs), _p], ctypes.c_uint32),
+    "kvip_hip_process_logits": ([ctypes.POINTER(LogitArgs), _p], ctypes.c_uint32),
+    "kvip_hip_process_logits_workspace_bytes": ([_i32, _i32], ctypes.c_uint64),
+}
+
 _LIB = None
 
 
@@ -339,7 +398,7 @@ def load_library(path: Path | None = None):
             "(kvip_amd has no CPU fallback)"
         )
     lib = ctypes.CDLL(str(path))
-    for name, (argtypes, restype) in (*PROTOTYPES.items(), *DRAFT_PROTOTYPES.items()):
+    for name, (argtypes, restype) in (*PROTOTYPES.items(), *DRAFT_PROTOTYPES.items(), *PROMPT_PROTOTYPES.items()):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = argtypes, restype
     version = lib.kvip_hip_abi_version()
@@ -348,6 +407,9 @@ def load_library(path: Path | None = None):
     version = lib.kvip_hip_draft_abi_version()
     if version != DRAFT_ABI_VERSION:
         raise RuntimeError(f"libkvip_hip.so draft ABI {version} != expected {DRAFT_ABI_VERSION}; rebuild")
+    version = lib.kvip_hip_prompt_abi_version()
+    if version != PROMPT_ABI_VERSION:
+        raise RuntimeError(f"libkvip_hip.so prompt ABI {version} != expected {PROMPT_ABI_VERSION}; rebuild")
     if path == LIBRARY:
         _LIB = lib
     return lib
