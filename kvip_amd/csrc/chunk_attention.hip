@@ -15,6 +15,7 @@
 //
 // Few row tiles over long contexts are cut along the context into segments, whose parts a third launch joins.
 #include <type_traits>
+#include <utility>
 
 #include "kvip_hip_prompt.h"
 #include "lds_async.h"
@@ -41,8 +42,8 @@ constexpr int kCaPieces = kCaKey / 8;
 constexpr int kCaImage = kCaPieces * kCaTile * 16;
 constexpr int kCaSlots = 4;                       // images in LDS
 constexpr int kCaLoads = kCaImage / 1024 / kCaWaves;
-constexpr int kCaUnits = 512;                     // workgroups of a launch whose row tiles are cut, at most
-constexpr int kCaCutTiles = 256;                  // row tiles that are cut, at most
+constexpr int kCaUnits = 1024;                    // workgroups of a launch whose row tiles are cut, at most
+constexpr int kCaCutTiles = 512;                  // row tiles that are cut, at most
 constexpr int kCaMostCuts = 32;
 constexpr int kCaPartSteps = 10;                  // what storing and joining a part costs, in tiles
 constexpr int kCaCus = 256;
@@ -62,9 +63,10 @@ struct ChunkPlan {
     int cut;                                  // tiles of a segment
     int cut_tiles;                            // row tiles, where they are cut; else 0
     int reserved;
-    int units_before[KVIP_DRAFT_MAX_BATCH + 1];
-    int tiles_before[KVIP_DRAFT_MAX_BATCH + 1];  // row tiles
-    int images_before[KVIP_DRAFT_MAX_BATCH + 1];
+    int request[KVIP_DRAFT_MAX_BATCH];           // in the order of the work
+    int units_before[KVIP_DRAFT_MAX_BATCH + 1];  // in that order
+    int tiles_before[KVIP_DRAFT_MAX_BATCH + 1];  // row tiles, in that order
+    int images_before[KVIP_DRAFT_MAX_BATCH];     // of request b, -1: none
 };
 
 // Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there), then the
@@ -136,19 +138,18 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
     const int64_t most = ca_images(p.max_rows, p.batch);
     const ChunkWork work = ca_work(p.workspace, most, nullptr);
     uint32_t err = 0;
-    int steps[kPer], tiles[kPer];
+    int steps[kPer];
     uint32_t sum = 0, sum_tiles = 0, total, total_tiles;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = tid * kPer + i;
-        steps[i] = tiles[i] = 0;
+        steps[i] = 0;
         if (b < p.batch) {
             const ChunkRequest q = ca_request(p, b, &err);
             steps[i] = ca_steps(q);
-            tiles[i] = ca_row_tiles(q, p.heads);
+            sum_tiles += ca_row_tiles(q, p.heads);
         }
         sum += steps[i];
-        sum_tiles += tiles[i];
     }
     uint32_t before = block_exclusive_scan(sum, s_sums, &total);
 #pragma unroll
@@ -161,62 +162,81 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
     __syncthreads();
 
     if (blockIdx.x == 0) {
-        // Where the row tiles would leave CUs without work, the context is cut into k segments of the longest request's:
-        // the k whose rounds of workgroups (one per CU) times their tiles are the fewest.
+        __shared__ int s_longest, s_steps[KVIP_DRAFT_MAX_BATCH], s_tiles[KVIP_DRAFT_MAX_BATCH + 1], s_units[kCaMostCuts];
+        __shared__ unsigned long long s_work;  // tiles of all row tiles
         ChunkPlan* plan = work.plan;
-        uint32_t tiles_before = block_exclusive_scan(sum_tiles, s_sums, &total_tiles);
-        __shared__ int s_longest, s_units[kCaMostCuts];
-        if (tid == 0) s_longest = 1;
+        if (tid == 0) {
+            s_longest = 1;
+            s_work = 0;
+        }
         if (tid < kCaMostCuts) s_units[tid] = 0;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (steps[i] > 0) atomicMax(&s_longest, steps[i]);
+        block_exclusive_scan(sum_tiles, s_sums, &total_tiles);
+        // Requests by their context, the longest first, so that what is left at the end is short.
+        for (int b = tid; b < p.batch; b += kCaThreads) {
+            uint32_t none = 0;
+            const ChunkRequest q = ca_request(p, b, &none);
+            const int steps_b = ca_steps(q);
+            int rank = 0;
+            for (int i = 0; i < p.batch; ++i) {
+                const int other = s_before[i + 1] - s_before[i];
+                rank += other > steps_b || (other == steps_b && i < b);
+            }
+            plan->request[rank] = b;
+            s_steps[rank] = steps_b;
+            s_tiles[rank] = ca_row_tiles(q, p.heads);
+            atomicMax(&s_longest, steps_b);
+            // Half of the chunk's own rows is not seen.
+            atomicAdd(&s_work, static_cast<unsigned long long>(s_tiles[rank]) * max(steps_b - q.tokens / (2 * kCaTile), 1));
         }
         __syncthreads();
         const int longest = s_longest;
-        for (int k = 0; k < kCaMostCuts; ++k) {
-            const int cut = (longest + k) / (k + 1);
-            int units = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) units += tiles[i] * max((steps[i] + cut - 1) / cut, 1);
-            if (total_tiles <= kCaCutTiles) atomicAdd(&s_units[k], units);
+        for (int b = tid / kCaMostCuts; b < p.batch && total_tiles <= kCaCutTiles; b += kCaThreads / kCaMostCuts) {
+            const int k = tid % kCaMostCuts, c = (longest + k) / (k + 1);
+            atomicAdd(&s_units[k], s_tiles[b] * max((s_steps[b] + c - 1) / c, 1));
         }
         __syncthreads();
-        int cut = longest, best = 0x7FFFFFFF;
-        bool is_cut = false;
-        if (total_tiles <= kCaCutTiles) {
-            for (int k = 0; k < kCaMostCuts; ++k) {
-                const int c = (longest + k) / (k + 1), units = s_units[k];
-                const int cost = (units + kCaCus - 1) / kCaCus * (c + (k > 0 ? kCaPartSteps : 0));
-                if (units <= kCaUnits && cost < best) {
-                    best = cost;
-                    cut = c;
-                    is_cut = k > 0;
-                }
+        // The context is cut into k + 1 segments of the longest request's where that ends earlier: the workgroups come in
+        // rounds of one per CU, or, where they are unequal, keep every CU busy but for half of one of them.
+        int cut = longest;
+        float best = 0.f;
+        for (int k = 0; k < (total_tiles <= kCaCutTiles ? kCaMostCuts : 0); ++k) {
+            const int c = (longest + k) / (k + 1), units = s_units[k];
+            const float rounds = static_cast<float>((units + kCaCus - 1) / kCaCus * c), spread = static_cast<float>(s_work) / kCaCus + 0.5f * c;
+            const float cost = fmaxf(fminf(rounds, spread), c) + (k > 0 ? kCaPartSteps * (1.f + static_cast<float>(units) / kCaCus) : 0.f);
+            if (k == 0 || (units <= kCaUnits && cost < best)) {
+                best = cost;
+                cut = c;
             }
         }
-        uint32_t mine = 0, total_units;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) mine += tiles[i] * max((steps[i] + cut - 1) / cut, 1);
-        uint32_t units_before = block_exclusive_scan(mine, s_sums, &total_units);
+        uint32_t mine = 0, mine_tiles = 0, total_units;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int b = tid * kPer + i;
-            if (b >= p.batch) break;
-            plan->units_before[b] = units_before;
-            plan->tiles_before[b] = tiles_before;
+            const int r = tid * kPer + i;
+            if (r >= p.batch) break;
+            mine += s_tiles[r] * max((s_steps[r] + cut - 1) / cut, 1);
+            mine_tiles += s_tiles[r];
+        }
+        uint32_t units_before = block_exclusive_scan(mine, s_sums, &total_units);
+        uint32_t tiles_before = block_exclusive_scan(mine_tiles, s_sums, &total_tiles);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int r = tid * kPer + i;
+            if (r >= p.batch) break;
+            plan->units_before[r] = units_before;
+            plan->tiles_before[r] = tiles_before;
+            units_before += s_tiles[r] * max((s_steps[r] + cut - 1) / cut, 1);
+            tiles_before += s_tiles[r];
             // No images: none that would fit.
+            const int b = r;
             const bool fits = s_before[b + 1] <= most;
             plan->images_before[b] = fits ? s_before[b] : -1;
-            if (!fits && steps[i] > 0) err |= KVIP_STATUS_BAD_LENGTH;
-            units_before += tiles[i] * max((steps[i] + cut - 1) / cut, 1);
-            tiles_before += tiles[i];
+            if (!fits && s_before[b + 1] > s_before[b]) err |= KVIP_STATUS_BAD_LENGTH;
         }
         if (tid == 0) {
             plan->units = total_units;
             plan->cut = cut;
-            plan->cut_tiles = is_cut ? total_tiles : 0;
+            plan->cut_tiles = cut < longest ? total_tiles : 0;
             plan->units_before[p.batch] = total_units;
             plan->tiles_before[p.batch] = total_tiles;
         }
@@ -322,13 +342,21 @@ KVIP_DEVICE void ca_store(const KvipChunkAttnArgs& p, int64_t at, f32x4 v) {
 // Direct-to-LDS load from a wave-uniform address and a lane's offset below 2^32 (see lds_async.h).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+// OFFSET moves both sides.
+template <int OFFSET>
 KVIP_DEVICE void ca_dma16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" : : "s"(lds), "v"(offset), "s"(base), "n"(OFFSET) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
 // Keeps an accumulator in accumulation registers from here to the next hold.
 KVIP_DEVICE void ca_hold(v16f& acc) { asm volatile("" : "+a"(acc)); }
+
+// f(0), f(1), ... of compile-time indices.
+template <typename F, int... I>
+KVIP_DEVICE void for_all(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
 
 // A unit of the plan: request b, row tile rt, segment seg.
 struct ChunkUnit {
@@ -340,7 +368,7 @@ KVIP_DEVICE bool ca_unit(const ChunkPlan* plan, int batch, int unit, int* s_foun
         if (plan->units_before[b] <= unit && unit < plan->units_before[b + 1]) {
             const int tiles = plan->tiles_before[b + 1] - plan->tiles_before[b];
             const int segs = (plan->units_before[b + 1] - plan->units_before[b]) / tiles, at = unit - plan->units_before[b];
-            s_found[0] = b;
+            s_found[0] = plan->request[b];
             s_found[1] = tiles - 1 - at / segs;  // the tiles that see most first
             s_found[2] = at % segs;
         }
@@ -394,15 +422,22 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     const int flip = p.scale < 0.f ? static_cast<int>(0x80008000u) : 0;
 
     const uint32_t ring = lds_addr(s_ring);
-    const uint8_t* from = work.images + static_cast<int64_t>(image0 + t0) * kCaImage + w * (kCaLoads * 1024);
-    auto fetch = [&](int t, int i) {  // load i of tile t's image (past the last tile: the last one again)
-        ca_dma16(from + static_cast<int64_t>(min(t, t1 - 1) - t0) * kCaImage + i * 1024, lane * 16,
-                 ring + (t - t0) % kCaSlots * kCaImage + w * (kCaLoads * 1024) + i * 1024);
+    auto slot_of = [&](int t) { return ring + ((t - t0) & (kCaSlots - 1)) * kCaImage; };
+    // The wave's share of tile t's image (past the last tile: the last one again), in kCaLoads loads.
+    const uint8_t* from;
+    uint32_t to;
+    auto aim = [&](int t) {
+        from = work.images + static_cast<int64_t>(image0 + min(t, t1 - 1)) * kCaImage + w * (kCaLoads * 1024);
+        to = slot_of(t) + w * (kCaLoads * 1024);
+    };
+    auto fetch = [&](auto which) {
+        constexpr int i = decltype(which)::value;
+        ca_dma16<i % 4 * 1024>(from + i / 4 * 4096, lane * 16, to + i / 4 * 4096);
     };
 #pragma unroll
     for (int t = 0; t < kCaSlots - 2; ++t) {
-#pragma unroll
-        for (int i = 0; i < kCaLoads; ++i) fetch(t0 + t, i);
+        aim(t0 + t);
+        for_all(fetch, std::make_integer_sequence<int, kCaLoads>{});
     }
     // Queries of the wave's rows (rows past the last read it again; their outputs are not written): fragment i holds
     // features 16 i + 8 (lane / 32) .. + 7.
@@ -433,29 +468,54 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         if (t >= held_first + 64) {
             held_first = t;
             held = work.flags[image0 + min(t + lane, reach - 1)];
+            asm volatile("" : "+v"(held.x), "+v"(held.y));  // waited for here, not at every use
         }
         return make_uint2(__builtin_amdgcn_readlane(held.x, t - held_first), __builtin_amdgcn_readlane(held.y, t - held_first));
     };
-    auto slot_of = [&](int t) { return ring + (t - t0) % kCaSlots * kCaImage; };
+    asm volatile("" : "+v"(held.x), "+v"(held.y));
+
+    // Operands are read from LDS kAhead products before their use, across the borders of logits and values too.
+    constexpr int kAhead = 4;
+    v4i ring_of[kAhead];
     const uint32_t key_at[2] = {static_cast<uint32_t>(16 * ca_place(hk, hn)), static_cast<uint32_t>(16 * (ca_place(2 + hk, hn) - 2 * kCaTile))};
-    constexpr int kAhead = 4;  // operands are read from LDS so many products before their use
-    auto key = [&](uint32_t slot, int i) { return *(LdsV4i)(slot + key_at[i & 1] + i * 1024); };
-    // Logits of tile t; the loads of the tile `ahead` stand between the products.
-    auto logits = [&](int t, int ahead) {
-        const uint32_t slot = slot_of(t);
-        v4i kb[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) kb[i] = key(slot, i);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.f;
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < kCaFrags; ++i) {
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kb[i % kAhead]), __builtin_bit_cast(bf16x8, qf[i]), s, 0, 0, 0);
-            if (i + kAhead < kCaFrags) kb[i % kAhead] = key(slot, i + kAhead);
-            if (i % 4 == 0) fetch(ahead, i / 4);
+    const int vp = (lane >> 4 & 1) * 2 + (lane >> 1 & 1), vt = 4 * hk + (lane >> 2 & 3);  // piece of a block, row of eight
+    const uint32_t value_at[2] = {static_cast<uint32_t>(16 * ca_place(vp, vt) + 8 * (lane & 1)),
+                                  static_cast<uint32_t>(16 * ca_place(vp, vt + 8) + 8 * (lane & 1))};
+    // Addresses of a tile's keys or values; opaque, so that the reads take their places as offsets.
+    struct Base {
+        uint32_t at[2];
+    };
+    auto base_of = [&](int t, const uint32_t (&at)[2]) {
+        Base base = {{slot_of(t) + at[0], slot_of(t) + at[1]}};
+        asm volatile("" : "+v"(base.at[0]), "+v"(base.at[1]));
+        return base;
+    };
+    auto key = [&](const Base& base, int i) { ring_of[i % kAhead] = *(LdsV4i)(base.at[i & 1] + i * 1024); };
+    auto value = [&](const Base& base, int i) {  // of product i: block i / 2, cached rows 16 (i % 2) .. + 15
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4)(base.at[0] + (i >> 1) * 2048 + (i & 1) * 256));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4)(base.at[1] + (i >> 1) * 2048 + (i & 1) * 256));
+        ring_of[i % kAhead] = __builtin_bit_cast(v4i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    static_assert(kCaFrags % kAhead == 0 && 2 * kCaBlocks % kAhead == 0, "the operand ring goes on at its start");
+    // Logits of a tile, whose first operands are under way; the loads that are aimed at stand between the products, the
+    // first value operands of the tile at `next` behind them.
+    auto logits = [&](const Base& base, const Base& next) {
+        for_all([&](auto which) {
+            constexpr int i = decltype(which)::value;
+            if constexpr (i == 0) {
+                const v16f zero = {};
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ring_of[i % kAhead]), __builtin_bit_cast(bf16x8, qf[i]), zero, 0, 0, 0);
+            } else {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ring_of[i % kAhead]), __builtin_bit_cast(bf16x8, qf[i]), s, 0, 0, 0);
+            }
+            if constexpr (i + kAhead < kCaFrags) key(base, i + kAhead);
+            else value(next, i + kAhead - kCaFrags);
+            if constexpr (i % 4 == 0) fetch(std::integral_constant<int, i / 4>{});
             __builtin_amdgcn_sched_barrier(0);
-        }
+        }, std::make_integer_sequence<int, kCaFrags>{});
+    };
+    static_assert(kCaLoads * 4 == kCaFrags, "a load every four products");
+    auto mask = [&](int t) {
         const uint2 flags = flags_of(t);
         if (t >= t_mask || flags.x != 0 || flags.y != 0) {
             const int left = sees - t * kCaTile;
@@ -486,9 +546,12 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
             alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * scale2) : raise ? 0.f : 1.f;
             m_run = m_new;
             bias = m_new == -INFINITY ? 0.f : -m_new * scale2;
+            asm volatile("" : "+v"(bias));
         } else {
-            s[piece - 2] = __builtin_amdgcn_exp2f(fmaf(s[piece - 2], scale2, bias));
-            fresh_sum += s[piece - 2];
+            float p1 = __builtin_amdgcn_exp2f(fmaf(s[piece - 2], scale2, bias));
+            fresh_sum += p1;
+            asm volatile("" : "+v"(p1), "+v"(fresh_sum));  // here, not behind the products
+            s[piece - 2] = p1;
         }
     };
     auto take = [&] {  // the softmax's results become those of the tile whose values come next
@@ -496,48 +559,55 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
 #pragma unroll
         for (int i = 0; i < 8; ++i) pb[i >> 2][i & 3] = static_cast<int>(ca_pack(s[2 * i], s[2 * i + 1]));
     };
-    const int vp = (lane >> 4 & 1) * 2 + (lane >> 1 & 1), vt = 4 * hk + (lane >> 2 & 3);  // piece of a block, row of eight
-    const uint32_t value_at[2] = {static_cast<uint32_t>(16 * ca_place(vp, vt) + 8 * (lane & 1)),
-                                  static_cast<uint32_t>(16 * ca_place(vp, vt + 8) + 8 * (lane & 1))};
-    auto value = [&](uint32_t slot, int i) {  // operand of product i: block i / 2, cached rows 16 (i % 2) .. + 15
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4)(slot + value_at[0] + (i >> 1) * 2048 + (i & 1) * 256));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4)(slot + value_at[1] + (i >> 1) * 2048 + (i & 1) * 256));
-        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-    // Values of tile t, the softmax of the next one beside them.
-    auto values = [&](int t, auto with_softmax) {
-        constexpr bool kSoftmax = decltype(with_softmax)::value;
-        const uint32_t slot = slot_of(t);
-        bf16x8 vb[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) vb[i] = value(slot, i);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 2 * kCaBlocks; ++i) {
-            if ((i & 1) == 0) ca_hold(o[i >> 1]);
-            o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i % kAhead], __builtin_bit_cast(bf16x8, pb[i & 1]), o[i >> 1], 0, 0, 0);
-            if ((i & 1) == 1) ca_hold(o[i >> 1]);
-            if (i + kAhead < 2 * kCaBlocks) vb[i % kAhead] = value(slot, i + kAhead);
-            if (kSoftmax && i < 18) softmax(i);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    // Tile t has landed, and the image of the tile before last is free for the one that comes three later.
+    // Every load of the tile after next has landed but the last kCaLoads of this wave, and all reads of this wave are done;
+    // then those of all waves.
     auto arrive = [&] {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((kCaSlots - 3) * kCaLoads) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" : : : "memory");
     };
+    // Values of a tile, whose first operands are under way, with the softmax of the next one beside them and the first key
+    // operands of the one after that (at `next`) behind them: when the last reads are done, so is the tile.
+    auto values = [&](const Base& base, const Base& next, auto with_softmax) {
+        constexpr bool kSoftmax = decltype(with_softmax)::value;
+        for_all([&](auto which) {
+            constexpr int i = decltype(which)::value;
+            if constexpr (i % 2 == 0) ca_hold(o[i / 2]);
+            o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ring_of[i % kAhead]), __builtin_bit_cast(bf16x8, pb[i % 2]), o[i / 2], 0, 0, 0);
+            if constexpr (i % 2 == 1) ca_hold(o[i / 2]);
+            if constexpr (i + kAhead < 2 * kCaBlocks) value(base, i + kAhead);
+            else if constexpr (kSoftmax) {
+                if constexpr (i + kAhead == 2 * kCaBlocks) arrive();
+                key(next, i + kAhead - 2 * kCaBlocks);
+            }
+            if constexpr (kSoftmax && i < 18) softmax(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }, std::make_integer_sequence<int, 2 * kCaBlocks>{});
+    };
     arrive();
-    logits(t0, t0 + kCaSlots - 2);
+    Base values_base = base_of(t0, value_at), keys_base = base_of(t0, key_at);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) key(keys_base, i);
+    aim(t0 + kCaSlots - 2);
+    logits(keys_base, values_base);
+    mask(t0);
 #pragma unroll
     for (int i = 0; i < 18; ++i) softmax(i);
     take();
+    if (t0 + 1 < t1) {
+        arrive();
+        keys_base = base_of(t0 + 1, key_at);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) key(keys_base, i);
+    }
 #pragma unroll 1
     for (int t = t0; t + 1 < t1; ++t) {
-        arrive();
-        logits(t + 1, t + kCaSlots - 1);
-        values(t, std::true_type{});
+        aim(t + kCaSlots - 1);
+        const Base here = base_of(t, value_at), keys_next = base_of(t + 2, key_at);
+        logits(keys_base, here);
+        mask(t + 1);
+        values(here, keys_next, std::true_type{});
+        keys_base = keys_next;
         if (__ballot(raise) != 0ull) {
 #pragma unroll
             for (int f = 0; f < kCaBlocks; ++f) {
@@ -548,7 +618,11 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         }
         take();
     }
-    values(t1 - 1, std::false_type{});
+    values_base = base_of(t1 - 1, value_at);
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) value(values_base, i);
+    values(values_base, values_base, std::false_type{});
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
 
     const float l_all = ca_half_sum(l_sum), m_all = m_run * scale2;  // log2 units from here on
@@ -599,7 +673,7 @@ __global__ __launch_bounds__(kCaThreads) void chunk_join_kernel(const KvipChunkA
     for (int b = threadIdx.x; b < p.batch; b += kCaThreads) {
         const int first = plan->tiles_before[b], behind = plan->tiles_before[b + 1];
         if (first <= tile && tile < behind) {
-            s_found[0] = b;
+            s_found[0] = plan->request[b];
             s_found[1] = tile - first;
             s_found[2] = (plan->units_before[b + 1] - plan->units_before[b]) / (behind - first);
             s_found[3] = plan->units_before[b] + (behind - 1 - tile) * s_found[2];
@@ -615,24 +689,43 @@ __global__ __launch_bounds__(kCaThreads) void chunk_join_kernel(const KvipChunkA
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hn = lane & 31;
     const int row = rt * kCaTileRows + rg * kCaRows + hn, rows = q.tokens * p.heads;
     const float2* states = work.states + static_cast<int64_t>(unit) * kCaTileRows + rg * kCaRows + hn;
+    constexpr int kRun = kCaBlocks / 4;  // fours of features of a wave
+    constexpr int kAtOnce = 4;           // parts whose loads are issued together
+    const int at = (slice * kCaWaves + w) * kRun;
+    const f32x4* sums = work.sums + (static_cast<int64_t>(unit) * kCaWaves + rg) * (kCaBlocks * 4 * 64) + at * 64 + lane;
     float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, states[i * kCaTileRows].x);
-    for (int i = 0; i < parts; ++i) {
-        const float2 state = states[i * kCaTileRows];
-        l += state.x == -INFINITY ? state.y : state.y * __builtin_amdgcn_exp2f(state.x - m);
+    f32x4 x[kRun] = {};
+    for (int first = 0; first < parts; first += kAtOnce) {
+        float2 state[kAtOnce];
+        f32x4 y[kAtOnce][kRun];
+        float most = m;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            state[i] = make_float2(-INFINITY, 0.f);
+            if (first + i >= parts) continue;
+            state[i] = states[(first + i) * kCaTileRows];
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) y[i][j] = __builtin_nontemporal_load(sums + (static_cast<int64_t>(first + i) * kCaWaves * (kCaBlocks * 4) + j) * 64);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) most = fmaxf(most, state[i].x);
+        const float keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - most);
+        l *= keep;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) x[j] *= keep;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (first + i >= parts) break;
+            // A part without a maximum has no sums, but may be NaN as a whole.
+            const float weight = state[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[i].x - most);
+            l += state[i].x == -INFINITY ? state[i].y : state[i].y * weight;
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) x[j] += y[i][j] * weight;
+        }
+        m = most;
     }
     const float factor = ca_share(l);
     const int64_t out_row = static_cast<int64_t>(q.begin) * p.heads + row;
-    constexpr int kRun = kCaBlocks / 4;  // fours of features of a wave
-    const int at = (slice * kCaWaves + w) * kRun;
-    f32x4 x[kRun] = {};
-    for (int i = 0; i < parts; ++i) {
-        const float mi = states[i * kCaTileRows].x;
-        const float weight = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
-        const f32x4* part = work.sums + (static_cast<int64_t>(unit + i) * kCaWaves + rg) * (kCaBlocks * 4 * 64) + lane;
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) x[j] += part[(at + j) * 64] * weight;
-    }
     if (row >= rows) return;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
