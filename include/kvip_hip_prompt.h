@@ -43,7 +43,9 @@ extern "C" {
  * to 32 plus 32 * batch: it sees nothing. With steps, a request with steps[b] <= 0 (one that
  * kvip_hip_page_tables_extend refused) sees nothing: output 0, lse -infinity. Rows of output and lse behind
  * cu_seqlens[batch] are left as they were. A workspace serves one call at a time, and the lengths stay as
- * they are while it runs. */
+ * they are while it runs.
+ * Where max_tokens is at most 64 and max_tokens * heads at most 512 * batch, kvip_hip_tree_attention does the work
+ * (without visible): it rounds probabilities times scales, not features, and max_rows does not count. */
 typedef struct KvipChunkAttnArgs {
     const uint16_t* query;        /* [max_tokens, heads, 576] bf16, 16-byte aligned */
     const uint8_t* kv_cache;      /* 16-byte aligned */
@@ -61,7 +63,7 @@ typedef struct KvipChunkAttnArgs {
     int32_t batch;                /* 1..KVIP_DRAFT_MAX_BATCH */
     int32_t heads;                /* 1..128 */
     int32_t max_tokens;           /* 1..KVIP_DRAFT_MAX_TOKENS */
-    int32_t max_blocks;           /* 1..2^17 */
+    int32_t max_blocks;           /* 1..2^17, as the workspace's */
     int32_t num_blocks;           /* 1..2^24 - 1 */
     int32_t output_dtype;         /* KVIP_DTYPE_BF16 or _FP32 */
     float scale;                  /* finite */
@@ -175,7 +177,7 @@ typedef struct KvipLogitArgs {
 
 uint32_t kvip_hip_prompt_abi_version(void);
 uint32_t kvip_hip_chunk_attention(const KvipChunkAttnArgs* args, void* stream);
-uint64_t kvip_hip_chunk_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t max_tokens, int64_t max_rows);
+uint64_t kvip_hip_chunk_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t max_tokens, int32_t max_blocks, int64_t max_rows);
 uint32_t kvip_hip_norm_rotary(const KvipNormRotaryArgs* args, void* stream);
 uint32_t kvip_hip_history_load(const KvipHistoryArgs* args, void* stream);
 uint32_t kvip_hip_history_append(const KvipHistoryArgs* args, void* stream);

@@ -126,8 +126,8 @@ KVIP_DEVICE uint32_t ca_pack(float a, float b) {  // hardware round to nearest e
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// Plan and images. Every workgroup sums the requests' tiles for itself and takes images in turn; the first one also
-// leaves the plan. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8 rotary features.
+// Plan and images. Every workgroup sums the requests' tiles for itself; the first one leaves the plan, the others take
+// images in turn. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8 rotary features.
 __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChunkAttnArgs p) {
     __shared__ __align__(16) uint8_t s_image[kCaImage];
     __shared__ int s_before[KVIP_DRAFT_MAX_BATCH + 1];
@@ -241,10 +241,11 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
             plan->tiles_before[p.batch] = total_tiles;
         }
         report(p.status, err);
+        return;
     }
 
     int b = 0;
-    for (int image = blockIdx.x; image < static_cast<int>(total) && image < most; image += gridDim.x) {
+    for (int image = blockIdx.x - 1; image < static_cast<int>(total) && image < most; image += gridDim.x - 1) {
         // The request: the last one whose images begin at or before this one (empty ones share its beginning).
         int lo = b, hi = p.batch - 1;
         while (lo < hi) {
@@ -743,11 +744,24 @@ bool ca_sizes(int32_t batch, int32_t heads, int32_t max_tokens, int64_t max_rows
            max_tokens <= KVIP_DRAFT_MAX_TOKENS && max_rows >= 1 && max_rows <= (1ll << 31);
 }
 
+// Few rows of the problem per request are the business of kvip_hip_tree_attention, which reads the cache as it is: here
+// the images cost 1808 bytes of traffic per cached row. One request of 16 heads on 16000 rows, 1 / 16 / 64 tokens: 25.6 / 46.9 /
+// 69.7 us there, 52.3 / 55.1 / 69.8 here; of 128 heads, 4 / 16 / 64 tokens: 50.3 / 105 / 318 and 56.5 / 95.9 / 258; 8
+// requests of 16 heads x 8 tokens on 8000 rows: 55.0 and 80.4, of 128 heads: 190 and 166.
+bool ca_few(int32_t batch, int32_t heads, int32_t max_tokens, int32_t max_blocks) {
+    return max_tokens <= KVIP_DRAFT_MAX_NODES && static_cast<int64_t>(max_tokens) * heads <= 512ll * batch &&
+           kvip_hip_tree_attention_workspace_bytes(batch, heads, max_tokens, max_blocks) != 0;
+}
+
 }  // namespace
 }  // namespace kvip
 
-extern "C" uint64_t kvip_hip_chunk_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t max_tokens, int64_t max_rows) {
-    if (!kvip::ca_sizes(batch, heads, max_tokens, max_rows)) return 0;
+extern "C" uint64_t kvip_hip_chunk_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t max_tokens, int32_t max_blocks,
+                                                             int64_t max_rows) {
+    if (!kvip::ca_sizes(batch, heads, max_tokens, max_rows) || max_blocks < 1 || max_blocks > (1 << 17)) return 0;
+    if (kvip::ca_few(batch, heads, max_tokens, max_blocks)) {
+        return kvip_hip_tree_attention_workspace_bytes(batch, heads, max_tokens, max_blocks);
+    }
     size_t bytes;
     kvip::ca_work(nullptr, kvip::ca_images(max_rows, batch), &bytes);
     return bytes;
@@ -764,10 +778,34 @@ extern "C" uint32_t kvip_hip_chunk_attention(const KvipChunkAttnArgs* a, void* s
                     a->kv_block_stride % 16 == 0 && a->kv_block_stride >= static_cast<int64_t>(kvip::kBlockTokens) * a->row_stride &&
                     (a->output_dtype == KVIP_DTYPE_BF16 || a->output_dtype == KVIP_DTYPE_FP32) && a->scale - a->scale == 0.f;
     if (!ok) return KVIP_ERR_INVALID;
+    if (kvip::ca_few(a->batch, a->heads, a->max_tokens, a->max_blocks)) {
+        KvipTreeAttnArgs t = {};
+        t.query = a->query;
+        t.kv_cache = a->kv_cache;
+        t.block_table = a->block_table;
+        t.seq_lens = a->seq_lens;
+        t.cu_seqlens = a->cu_seqlens;
+        t.steps = a->steps;
+        t.output = a->output;
+        t.lse = a->lse;
+        t.workspace = a->workspace;
+        t.status = a->status;
+        t.kv_block_stride = a->kv_block_stride;
+        t.row_stride = a->row_stride;
+        t.batch = a->batch;
+        t.heads = a->heads;
+        t.max_nodes = a->max_tokens;
+        t.max_tokens = a->max_tokens;
+        t.max_blocks = a->max_blocks;
+        t.num_blocks = a->num_blocks;
+        t.output_dtype = a->output_dtype;
+        t.scale = a->scale;
+        return kvip_hip_tree_attention(&t, stream);
+    }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t images = kvip::ca_images(a->max_rows, a->batch), tiles = kvip::ca_row_tiles_most(a->batch, a->heads, a->max_tokens);
     const int64_t units = tiles < kvip::kCaUnits ? kvip::kCaUnits : tiles;
-    hipLaunchKernelGGL(kvip::chunk_expand_kernel, dim3(static_cast<unsigned>(images < 1024 ? images : 1024)), dim3(kvip::kCaThreads), 0, s, *a);
+    hipLaunchKernelGGL(kvip::chunk_expand_kernel, dim3(static_cast<unsigned>(images < 1024 ? images : 1024) + 1), dim3(kvip::kCaThreads), 0, s, *a);
     hipLaunchKernelGGL(kvip::chunk_attention_kernel, dim3(static_cast<unsigned>(units)), dim3(kvip::kCaThreads), 0, s, *a);
     const int64_t joined = tiles < kvip::kCaCutTiles ? tiles : kvip::kCaCutTiles;
     hipLaunchKernelGGL(kvip::chunk_join_kernel, dim3(static_cast<unsigned>(joined * kvip::kCaWaves * 4)), dim3(kvip::kCaThreads), 0, s, *a);

@@ -42,7 +42,7 @@ class ChunkAttention:
         abi.require(self.device.type == "cuda", "chunk attention runs on the GPU (kvip_amd has no CPU path)")
         self.batch, self.heads, self.max_tokens, self.max_rows = int(batch), int(heads), int(max_tokens), max_rows
         self.library = abi.load_library()
-        nbytes = int(self.library.kvip_hip_chunk_attention_workspace_bytes(batch, heads, max_tokens, max_rows))
+        nbytes = int(self.library.kvip_hip_chunk_attention_workspace_bytes(batch, heads, max_tokens, self.max_blocks, max_rows))
         abi.require(nbytes > 0, "the sizes are too large for one call")
         self.output = torch.zeros((max_tokens, heads, VALUE_DIM), dtype=output_dtype, device=self.device)
         self.lse = torch.zeros((max_tokens, heads), dtype=torch.float32, device=self.device) if lse else None

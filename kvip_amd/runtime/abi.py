@@ -370,7 +370,7 @@ DRAFT_PROTOTYPES = {
 PROMPT_PROTOTYPES = {
     "kvip_hip_prompt_abi_version": ([], ctypes.c_uint32),
     "kvip_hip_chunk_attention": ([ctypes.POINTER(ChunkAttnArgs), _p], ctypes.c_uint32),
-    "kvip_hip_chunk_attention_workspace_bytes": ([_i32, _i32, _i32, _i64], ctypes.c_uint64),
+    "kvip_hip_chunk_attention_workspace_bytes": ([_i32, _i32, _i32, _i32, _i64], ctypes.c_uint64),
     "kvip_hip_norm_rotary": ([ctypes.POINTER(NormRotaryArgs), _p], ctypes.c_uint32),
     "kvip_hip_history_load": ([ctypes.POINTER(HistoryArgs), _p], ctypes.c_uint32),
     "kvip_hip_history_append": ([ctypes.POINTER(HistoryArgs), _p], ctypes.c_uint32),

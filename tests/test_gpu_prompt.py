@@ -21,9 +21,10 @@ LOWEST = {"fp32": 2.0 ** -149, "bf16": 2.0 ** -133, "fp16": 2.0 ** -24}  # step 
 
 
 class Chunks:
-    """Packed chunks over a shuffled cache: counts[b] new tokens, contexts[b] rows before them."""
+    """Packed chunks over a shuffled cache: counts[b] new tokens, contexts[b] rows before them, `pad` rows behind the last
+    token (more than 64 rows in all: not the business of tree attention)."""
 
-    def __init__(self, torch, rng, counts, contexts, heads, *, stride=ROW, spare=2, pad=2):
+    def __init__(self, torch, rng, counts, contexts, heads, *, stride=ROW, spare=2, pad=70):
         self.torch, self.counts, self.heads = torch, counts, heads
         self.lens = [c + n for c, n in zip(contexts, counts)]
         blocks = [-(-x // 128) for x in self.lens]
@@ -110,7 +111,7 @@ def test_chunk_attention_of_many_requests(torch_gpu, heads, requests, most, long
     step.lens = [n + int(rng.integers(0, longest)) if rng.random() < 0.7 else n for n in step.counts]
     step.table = rng.integers(0, step.pages, (requests, -(-max(step.lens) // 128))).astype(np.int32)
     step.cu = np.concatenate([[0], np.cumsum(step.counts)]).astype(np.int32)
-    step.tokens = int(step.cu[-1]) + 2
+    step.tokens = int(step.cu[-1]) + 70
     step.query = torch.randn((step.tokens, heads, 576), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
     op = step.run()
     step.check(op, every=41)
@@ -125,6 +126,29 @@ def test_chunk_attention_cut_along_the_context(torch_gpu, heads, counts, context
     step.check(op, every=7)
     first = op.output.clone()
     assert torch_gpu.equal(op(), first)
+
+
+@pytest.mark.parametrize("heads,counts,contexts", [(16, [1], [0]), (16, [30], [700]), (5, [40, 3, 0], [100, 129, 4]), (128, [2], [300]),
+                                                   (16, [1] * 40, list(range(0, 200, 5)))])
+def test_chunk_attention_of_few_rows(torch_gpu, heads, counts, contexts):
+    """What tree attention carries out: its roundings, and its status bits."""
+    torch = torch_gpu
+    say(f"case chunk few heads={heads} counts={counts[:6]}")
+    step = Chunks(torch, np.random.default_rng(heads), counts, contexts, heads, pad=2)
+    op = step.run(max_rows=1)
+    got, lse, q = host(op()), host(op.lse), step.query.double().numpy()
+    for b, n in enumerate(counts):
+        rows = step.rows[[step.slot(b, p) for p in range(step.lens[b])]]
+        for i in range(n):
+            sees = np.arange(len(rows)) <= step.lens[b] - n + i
+            want, want_lse, bound, lse_bound = draft.tree_attention(q[step.cu[b] + i], rows, sees, SCALE)
+            assert np.all(np.abs(got[step.cu[b] + i] - want) <= bound + np.abs(want) * 2.0 ** -8), (b, i)
+            assert np.all(np.abs(lse[step.cu[b] + i] - want_lse) <= lse_bound), (b, i)
+    assert np.all(got[step.cu[-1]:] == 3.0) and int(op.status.item()) == 0
+    step.table[0, 0] = step.pages
+    op = step.run(steps=[1] + [0] * (len(counts) - 1))
+    op()
+    assert int(op.status.item()) == abi.STATUS_BAD_BLOCK and not op.output[counts[0]:step.cu[-1]].any()
 
 
 def test_chunk_attention_options(torch_gpu):
@@ -260,10 +284,10 @@ def test_chunk_attention_long_cache(torch_gpu):
     long = 1 << 22
     table = torch.zeros((2, long // 128), dtype=torch.int32, device="cuda")
     table[1, :step.table.shape[1]] = device(torch, np.maximum(step.table[1], 0), torch.int32)
-    op = kvip_amd.ChunkAttention(torch, batch=2, heads=16, max_tokens=41, max_context=long, max_rows=long + 1024, device="cuda")
-    op.bind(step.query[4:45].cuda().contiguous(), step.kv, table, device(torch, [long, step.lens[1]], torch.int32),
+    op = kvip_amd.ChunkAttention(torch, batch=2, heads=16, max_tokens=101, max_context=long, max_rows=long + 1024, device="cuda")
+    op.bind(step.query[4:105].cuda().contiguous(), step.kv, table, device(torch, [long, step.lens[1]], torch.int32),
             device(torch, [0, 1, 41], torch.int32))
-    got, q = host(op()), step.query.double().numpy()[4:45]
+    got, q = host(op()), step.query.double().numpy()[4:105]
     key, value, _ = prompt.features(step.rows[[step.slot(1, p) for p in range(step.lens[1])]])
     for i in (0, 17, 39):
         want, _, bound, _ = prompt.attention(q[1 + i], key[:701 + i], value[:701 + i], SCALE)

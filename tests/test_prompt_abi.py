@@ -64,8 +64,13 @@ def test_chunk_attention_rejects_before_launch():
         dict(output_dtype=abi.DTYPE_FP16), dict(row_stride=(1 << 24) + 16, kv_block_stride=1 << 32),
         dict(scale=float("inf")), dict(scale=float("nan"))])
     size = abi.load_library().kvip_hip_chunk_attention_workspace_bytes
-    assert size(0, 16, 4, 4) == size(2, 129, 4, 4) == size(2, 16, 0, 4) == size(2, 16, 4, 0) == size(2, 16, 4, (1 << 31) + 1) == 0
-    assert 1152 * 32 < size(1, 16, 4, 1) < size(64, 16, 4, 1 << 20) and size(64, 16, 4, 1 << 20) > (1 << 20) * 1152
+    assert size(0, 16, 4, 4, 4) == size(2, 129, 4, 4, 4) == size(2, 16, 0, 4, 4) == size(2, 16, 4, 0, 4) == 0
+    assert size(2, 16, 4, 4, 0) == size(2, 16, 4, 4, (1 << 31) + 1) == size(2, 16, 4, (1 << 17) + 1, 4) == 0
+    assert 1152 * 32 < size(1, 16, 65, 4, 1) < size(64, 16, 65, 4, 1 << 20) and size(64, 16, 65, 4, 1 << 20) > (1 << 20) * 1152
+    # Few rows of the problem per request: tree attention's.
+    tree = abi.load_library().kvip_hip_tree_attention_workspace_bytes
+    assert size(1, 16, 32, 40, 1 << 20) == tree(1, 16, 32, 40) and size(1, 16, 33, 40, 1 << 20) > (1 << 20) * 1152
+    assert size(2, 16, 64, 40, 1 << 20) == tree(2, 16, 64, 40) and size(2, 16, 65, 40, 1 << 20) > (1 << 20) * 1152
 
 
 def test_norm_rotary_rejects_before_launch():
