@@ -6,8 +6,8 @@
 // tokens of a vocabulary) need more, and each of these is worked out by one thread on its own: a bit in LDS takes
 // the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing, and a
 // token named several times gets the same sum, in the list's order, whichever thread has it.
-#include "kvip_device.h"
 #include "kvip_hip_prompt.h"
+#include "lane_groups.h"
 
 namespace kvip {
 namespace {
@@ -21,6 +21,7 @@ constexpr float kLgLog2e = 1.44269504088896341f;
 constexpr float kLgLargest = 3.402823466e38f;
 
 template <typename T> struct Logits { typedef T vec __attribute__((ext_vector_type(kLgVec), aligned(sizeof(T)))); };
+typedef int LogitCounts __attribute__((ext_vector_type(kLgVec), aligned(4)));
 
 struct LogitStat {
     float m, l;  // largest x, sum of exp((x - m) / temperature)
@@ -45,29 +46,30 @@ KVIP_DEVICE float weight_of(float x, float m, const LogitRow& r) {
     return x == m ? 1.f : x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaxf(x - m, -kLgLargest) * r.c);
 }
 
-KVIP_DEVICE void merge(LogitStat& a, float m, float l, int first, const LogitRow& r) {
-    if (m > a.m) {
-        a.l = a.m == -INFINITY ? l : a.l * weight_of(a.m, m, r) + l;
-        a.m = m;
-        a.first = first;
-    } else if (m == a.m) {
-        a.l += l;
-        a.first = min(a.first, first);
-    } else if (m != -INFINITY) {
-        a.l += l * weight_of(m, a.m, r);
-    }
-}
-
+// All threads' statistics put together, in every thread: largest first, then sums and places under it.
 KVIP_DEVICE void merge_block(LogitStat& a, LogitStat* s_stats, const LogitRow& r) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        merge(a, __shfl_xor(a.m, d), __shfl_xor(a.l, d), __shfl_xor(a.first, d), r);
-    }
-    if ((threadIdx.x & 63) == 0) s_stats[threadIdx.x >> 6] = a;
+    const int w = threadIdx.x >> 6;
+    const float most = group_max<64>(a.m);
+    if ((threadIdx.x & 63) == 0) s_stats[w].m = most;
     __syncthreads();
-    a = s_stats[0];
+    float all = s_stats[0].m;
 #pragma unroll
-    for (int w = 1; w < kLgWaves; ++w) merge(a, s_stats[w].m, s_stats[w].l, s_stats[w].first, r);
+    for (int i = 1; i < kLgWaves; ++i) all = fmaxf(all, s_stats[i].m);
+    const float l = group_sum<64>(a.m == -INFINITY ? 0.f : a.l * weight_of(a.m, all, r));
+    int first = a.m == all ? a.first : 0x7FFFFFFF;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) first = min(first, __shfl_xor(first, d));
+    if ((threadIdx.x & 63) == 0) {
+        s_stats[w].l = l;
+        s_stats[w].first = first;
+    }
+    __syncthreads();
+    a = {all, s_stats[0].l, s_stats[0].first, 0};
+#pragma unroll
+    for (int i = 1; i < kLgWaves; ++i) {
+        a.l += s_stats[i].l;
+        a.first = min(a.first, s_stats[i].first);
+    }
 }
 
 // A row's part [begin, end) of the vocabulary.
@@ -83,38 +85,58 @@ struct LogitPart {
     LogitRow row;
     uint32_t err;
 
-    KVIP_DEVICE float allowed_or_none(float x, bool may) {
-        if (!may) return -INFINITY;
-        if (x != x) {
-            err |= KVIP_STATUS_BAD_PROBS;
-            return -INFINITY;
-        }
-        return x;
-    }
-
-    // The tokens v .. v + 7 (v a multiple of 8), -infinity for those past the end or not the dense pass's.
-    KVIP_DEVICE void load(int v, float (&x)[kLgVec]) {
+    // Eight tokens from v on (a multiple of 8) as they lie in memory, and which of them the grammar allows.
+    struct Raw {
+        typename Logits<T>::vec x;
+        uint32_t may;
+    };
+    KVIP_DEVICE Raw fetch(int v) const {
+        Raw raw;
+        raw.may = 0;
         const int there = min(end - v, kLgVec);
+        if (there <= 0) return raw;
+        raw.may = (1u << there) - 1;
+        if (allowed != nullptr) raw.may &= allowed[v >> 3];
         if (there == kLgVec) {
-            const auto raw = *reinterpret_cast<const typename Logits<T>::vec*>(logits + v);
-#pragma unroll
-            for (int i = 0; i < kLgVec; ++i) x[i] = static_cast<float>(raw[i]);
+            raw.x = *reinterpret_cast<const typename Logits<T>::vec*>(logits + v);
         } else {
 #pragma unroll
-            for (int i = 0; i < kLgVec; ++i) x[i] = i < there ? static_cast<float>(logits[v + i]) : 0.f;
+            for (int i = 0; i < kLgVec; ++i) raw.x[i] = i < there ? logits[v + i] : static_cast<T>(0.f);
         }
-        uint32_t may = (1u << there) - 1;
-        if (special != nullptr) may &= ~(special[(v - begin) >> 5] >> (v & 31));
-        if (allowed != nullptr) may &= allowed[v >> 3];
-        const uint32_t held = seen != nullptr ? seen[v >> 3] & may : 0u;
+        return raw;
+    }
+
+    // Their x, -infinity for those that are not the dense pass's.
+    KVIP_DEVICE void adjust(int v, Raw raw, float (&x)[kLgVec]) {
+#pragma unroll
+        for (int i = 0; i < kLgVec; ++i) x[i] = static_cast<float>(raw.x[i]);
+        if (special != nullptr) raw.may &= ~(special[(v - begin) >> 5] >> (v & 31));
+        const uint32_t held = seen != nullptr ? seen[v >> 3] & raw.may : 0u;
         if (held != 0) {
+            LogitCounts n;
+            if (end - v >= kLgVec) {
+                n = *reinterpret_cast<const LogitCounts*>(counts + v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLgVec; ++i) n[i] = v + i < end ? counts[v + i] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kLgVec; ++i) x[i] = held >> i & 1 ? penalised(x[i], row, true, n[i]) : x[i];
+        }
+        float sum = x[0];
+#pragma unroll
+        for (int i = 1; i < kLgVec; ++i) sum += x[i];
+        if (raw.may != 0xFFu || sum != sum) {  // tokens left out, a NaN, or infinities of both signs
 #pragma unroll
             for (int i = 0; i < kLgVec; ++i) {
-                if (held >> i & 1) x[i] = penalised(x[i], row, true, counts[v + i]);
+                if (!(raw.may >> i & 1)) {
+                    x[i] = -INFINITY;
+                } else if (x[i] != x[i]) {
+                    err |= KVIP_STATUS_BAD_PROBS;
+                    x[i] = -INFINITY;
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kLgVec; ++i) x[i] = allowed_or_none(x[i], may >> i & 1);
     }
 
     // Token v with its biases and the row's ancestors.
@@ -131,7 +153,10 @@ struct LogitPart {
         for (int i = 0; i < p.biases; ++i) {
             if (names[i] == v) x += values[i];
         }
-        return allowed_or_none(x, allowed == nullptr || (allowed[v >> 3] >> (v & 7) & 1));
+        if (allowed != nullptr && !(allowed[v >> 3] >> (v & 7) & 1)) return -INFINITY;
+        if (x == x) return x;
+        err |= KVIP_STATUS_BAD_PROBS;
+        return -INFINITY;
     }
 };
 
@@ -145,9 +170,24 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     __shared__ int s_ways, s_request;
     const int tid = threadIdx.x, lane = tid & 63;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
+    const int words = (p.vocab + 31) / 32;
     uint32_t err = 0;
+    LogitPart<T> at = {p, static_cast<const T*>(p.logits) + row * p.logits_stride, nullptr, nullptr,
+                       p.allowed == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.allowed + static_cast<int64_t>(row) * words),
+                       nullptr, part * part_size, min((part + 1) * part_size, p.vocab), {}, 0};
+    const int first = at.begin + tid * kLgVec;
+    // What does not need the request is under way before it is known.
+    typename LogitPart<T>::Raw next = at.fetch(first);
+    const uint64_t seen_by = p.visible != nullptr ? static_cast<uint64_t>(p.visible[row]) : 0;
+    LogitStat* stats = static_cast<LogitStat*>(p.workspace) + static_cast<int64_t>(row) * parts;
+    LogitStat stat = {-INFINITY, 0.f, p.vocab, 0};
+    if (MODE == kLgWrite && tid < parts) stat = stats[tid];
 
     if (tid == 0) s_request = p.batch;
+    const int listed = (p.visible == nullptr ? 0 : 63) + p.biases;
+    if (listed > 0) {
+        for (int i = tid; i < (at.end - at.begin + 31) / 32; i += kLgThreads) s_special[i] = 0;
+    }
     __syncthreads();
     for (int b = tid; b < p.batch; b += kLgThreads) {
         const int from = p.cu_seqlens[b], to = p.cu_seqlens[b + 1];
@@ -161,12 +201,10 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
         report(p.status, err);
         return;
     }
-    const int words = (p.vocab + 31) / 32;
-    LogitPart<T> at = {p, static_cast<const T*>(p.logits) + row * p.logits_stride,
-                       p.counts == nullptr ? nullptr : p.counts + static_cast<int64_t>(b) * p.vocab,
-                       p.seen == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.seen + static_cast<int64_t>(b) * words),
-                       p.allowed == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.allowed + static_cast<int64_t>(row) * words),
-                       nullptr, part * part_size, min((part + 1) * part_size, p.vocab), {}, 0};
+    if (p.seen != nullptr) {
+        at.counts = p.counts + static_cast<int64_t>(b) * p.vocab;
+        at.seen = reinterpret_cast<const uint8_t*>(p.seen + static_cast<int64_t>(b) * words);
+    }
     const float temperature = p.temperature == nullptr ? 1.f : p.temperature[b];
     at.row.repetition = p.repetition == nullptr ? 1.f : p.repetition[b];
     at.row.inverse = 1.f / at.row.repetition;
@@ -178,12 +216,10 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
 
     // The row's ancestors, and which tokens of this part are not the dense pass's.
     uint64_t mine = 0;  // bit k: this thread has the token that entry tid + 512 k names
-    const int listed = (p.visible == nullptr ? 0 : 63) + p.biases;
     if (listed > 0) {
         if (tid < 64) {
             const int begin = min(max(p.cu_seqlens[b], 0), p.max_tokens), behind = min(max(p.cu_seqlens[b + 1], begin), p.max_tokens);
-            bool on = p.visible != nullptr && lane > 0 && begin + lane < behind &&
-                      (static_cast<uint64_t>(p.visible[row]) >> lane & 1);
+            bool on = lane > 0 && begin + lane < behind && (seen_by >> lane & 1);
             const int64_t token = on ? p.tokens[begin + lane] : 0;
             if (on && (token < 0 || token >= p.vocab)) {
                 err |= KVIP_STATUS_BAD_TOKEN;
@@ -193,7 +229,6 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
             if (on) s_way[__popcll(all & ((1ull << lane) - 1))] = static_cast<int>(token);
             if (lane == 0) s_ways = __popcll(all);
         }
-        for (int i = tid; i < (at.end - at.begin + 31) / 32; i += kLgThreads) s_special[i] = 0;
         __syncthreads();
         const int ways = s_ways;
         for (int e = tid, k = 0; e < ways + p.biases; e += kLgThreads, ++k) {
@@ -211,12 +246,12 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
         return e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
     };
 
-    LogitStat stat = {-INFINITY, 0.f, p.vocab, 0};
-    LogitStat* stats = static_cast<LogitStat*>(p.workspace) + static_cast<int64_t>(row) * parts;
     if constexpr ((MODE & kLgStats) != 0) {
-        for (int v = at.begin + tid * kLgVec; v < at.end; v += kLgRun) {
+        for (int v = first; v < at.end; v += kLgRun) {
+            const auto raw = next;
+            next = at.fetch(v + kLgRun);
             float x[kLgVec], most;
-            at.load(v, x);
+            at.adjust(v, raw, x);
             most = x[0];
 #pragma unroll
             for (int i = 1; i < kLgVec; ++i) most = fmaxf(most, x[i]);
@@ -226,22 +261,28 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
 #pragma unroll
                 for (int i = kLgVec - 1; i >= 0; --i) stat.first = x[i] == most ? v + i : stat.first;
             }
-            if (!at.row.greedy && stat.m != -INFINITY) {
+            if (at.row.greedy || stat.m == -INFINITY) continue;
 #pragma unroll
-                for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
-            }
+            for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
         }
         for (uint64_t left = mine; left != 0; left &= left - 1) {
             const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
-            merge(stat, at.one(v, b, s_way, s_ways), 1.f, v, at.row);
+            const float x = at.one(v, b, s_way, s_ways);
+            if (x > stat.m) {
+                stat = {x, (stat.m == -INFINITY ? 0.f : stat.l * weight_of(stat.m, x, at.row)) + 1.f, v, 0};
+            } else if (x != -INFINITY) {
+                stat.l += weight_of(x, stat.m, at.row);
+                if (x == stat.m) stat.first = min(stat.first, v);
+            }
         }
         merge_block(stat, s_stats, at.row);
         if constexpr (MODE == kLgStats) {
             if (tid == 0) stats[part] = stat;
+        } else {
+            next = at.fetch(first);
         }
         err |= at.err;
     } else {
-        if (tid < parts) stat = stats[tid];
         merge_block(stat, s_stats, at.row);
     }
     if constexpr ((MODE & kLgWrite) != 0) {
@@ -252,9 +293,11 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
             return at.row.greedy ? (v == stat.first ? 1.f : 0.f) : weight_of(x, stat.m, at.row) * share;
         };
         O* out = static_cast<O*>(p.probs) + row * p.probs_stride;
-        for (int v = at.begin + tid * kLgVec; v < at.end; v += kLgRun) {
+        for (int v = first; v < at.end; v += kLgRun) {
+            const auto raw = next;
+            next = at.fetch(v + kLgRun);
             float x[kLgVec];
-            at.load(v, x);
+            at.adjust(v, raw, x);
             typename Logits<O>::vec y;
 #pragma unroll
             for (int i = 0; i < kLgVec; ++i) y[i] = static_cast<O>(prob(x[i], v + i));

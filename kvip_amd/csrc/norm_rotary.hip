@@ -6,6 +6,7 @@
 // variance are two passes over registers, in 32 bits. Heads of other sizes go through LDS, a wave per head.
 // A workgroup takes a run of tokens and works their angles out once; a thread holds its features' weights.
 #include "kvip_hip_prompt.h"
+#include "lane_groups.h"
 #include "turn.h"
 
 namespace kvip {
@@ -17,31 +18,6 @@ constexpr int kNrPairs = 1024;  // pairs of a workgroup's run of tokens (8 KB of
 constexpr int kNrLane = 8;      // features of a lane
 
 template <typename T> struct Four { typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
-
-template <int CTRL>
-KVIP_DEVICE float dpp_all(float x) {
-    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xF, 0xF, true));
-}
-
-// x of all G lanes of a group put together, in every lane of it; G lanes lie side by side.
-template <int G, typename F>
-KVIP_DEVICE float over_group(float x, F f) {
-    x = f(x, dpp_all<0xB1>(x));   // lane ^ 1
-    x = f(x, dpp_all<0x4E>(x));   // lane ^ 2
-    x = f(x, dpp_all<0x141>(x));  // mirrored in 8
-    if constexpr (G >= 16) x = f(x, dpp_all<0x140>(x));  // mirrored in 16
-    if constexpr (G >= 32) {
-        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    }
-    if constexpr (G >= 64) {
-        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    }
-    return x;
-}
-template <int G> KVIP_DEVICE float group_sum(float x) { return over_group<G>(x, [](float a, float b) { return a + b; }); }
-template <int G> KVIP_DEVICE float group_max(float x) { return over_group<G>(x, [](float a, float b) { return fmaxf(a, b); }); }
 
 // Scale of a head whose largest magnitude is given, and a feature under it: as in the rows of the KV cache.
 KVIP_DEVICE float head_scale(float largest) {
