@@ -6,6 +6,8 @@
 // tokens of a vocabulary) need more, and each of these is worked out by one thread on its own: a bit in LDS takes
 // the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing, and a
 // token named several times gets the same sum, in the list's order, whichever thread has it.
+#include <type_traits>
+
 #include "kvip_hip_prompt.h"
 #include "lane_groups.h"
 
@@ -16,6 +18,7 @@ constexpr int kLgThreads = 512;
 constexpr int kLgWaves = kLgThreads / 64;
 constexpr int kLgVec = 8;                      // tokens of a thread at a time: a byte of the bit masks
 constexpr int kLgRun = kLgThreads * kLgVec;
+constexpr int kLgListed = 16;                  // biases looked at together
 constexpr int kLgMaxPart = 1 << 17;            // tokens of a workgroup (16 KB of bits)
 constexpr float kLgLog2e = 1.44269504088896341f;
 constexpr float kLgLargest = 3.402823466e38f;
@@ -106,7 +109,8 @@ struct LogitPart {
         return raw;
     }
 
-    // Their x, -infinity for those that are not the dense pass's.
+    // Their x, -infinity for those that are not the dense pass's; CAREFUL: and for NaN, which is noted.
+    template <bool CAREFUL>
     KVIP_DEVICE void adjust(int v, Raw raw, float (&x)[kLgVec]) {
 #pragma unroll
         for (int i = 0; i < kLgVec; ++i) x[i] = static_cast<float>(raw.x[i]);
@@ -123,18 +127,19 @@ struct LogitPart {
 #pragma unroll
             for (int i = 0; i < kLgVec; ++i) x[i] = held >> i & 1 ? penalised(x[i], row, true, n[i]) : x[i];
         }
-        float sum = x[0];
-#pragma unroll
-        for (int i = 1; i < kLgVec; ++i) sum += x[i];
-        if (raw.may != 0xFFu || sum != sum) {  // tokens left out, a NaN, or infinities of both signs
+        if (raw.may != 0xFFu) {
 #pragma unroll
             for (int i = 0; i < kLgVec; ++i) {
-                if (!(raw.may >> i & 1)) {
-                    x[i] = -INFINITY;
-                } else if (x[i] != x[i]) {
-                    err |= KVIP_STATUS_BAD_PROBS;
-                    x[i] = -INFINITY;
-                }
+                const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(raw.may), i, 1));
+                x[i] = __uint_as_float((__float_as_uint(x[i]) & keep) | (0xFF800000u & ~keep));
+            }
+        }
+        if constexpr (CAREFUL) {
+#pragma unroll
+            for (int i = 0; i < kLgVec; ++i) {
+                if (x[i] == x[i]) continue;
+                err |= KVIP_STATUS_BAD_PROBS;
+                x[i] = -INFINITY;
             }
         }
     }
@@ -150,9 +155,19 @@ struct LogitPart {
         float x = penalised(static_cast<float>(logits[v]), row, held, n);
         const int32_t* names = p.bias_tokens + static_cast<int64_t>(b) * p.biases;
         const float* values = p.bias_values + static_cast<int64_t>(b) * p.biases;
-        for (int i = 0; i < p.biases; ++i) {
-            if (names[i] == v) x += values[i];
+        int i = 0;
+        for (; i + kLgListed <= p.biases; i += kLgListed) {  // in one go, as each load is waited for
+            int name[kLgListed];
+            float value[kLgListed];
+#pragma unroll
+            for (int j = 0; j < kLgListed; ++j) {
+                name[j] = names[i + j];
+                value[j] = values[i + j];
+            }
+#pragma unroll
+            for (int j = 0; j < kLgListed; ++j) x = name[j] == v ? x + value[j] : x;
         }
+        for (; i < p.biases; ++i) x = names[i] == v ? x + values[i] : x;
         if (allowed != nullptr && !(allowed[v >> 3] >> (v & 7) & 1)) return -INFINITY;
         if (x == x) return x;
         err |= KVIP_STATUS_BAD_PROBS;
@@ -247,23 +262,37 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     };
 
     if constexpr ((MODE & kLgStats) != 0) {
-        for (int v = first; v < at.end; v += kLgRun) {
-            const auto raw = next;
-            next = at.fetch(v + kLgRun);
-            float x[kLgVec], most;
-            at.adjust(v, raw, x);
-            most = x[0];
+        auto pass = [&](auto careful) {
+            for (int v = first; v < at.end; v += kLgRun) {
+                const auto raw = next;
+                next = at.fetch(v + kLgRun);
+                float x[kLgVec], most;
+                at.template adjust<decltype(careful)::value>(v, raw, x);
+                most = x[0];
 #pragma unroll
-            for (int i = 1; i < kLgVec; ++i) most = fmaxf(most, x[i]);
-            if (most > stat.m) {
-                stat.l *= weight_of(stat.m, most, at.row);
-                stat.m = most;
+                for (int i = 1; i < kLgVec; ++i) most = fmaxf(most, x[i]);
+                if (most > stat.m) {
+                    stat.l *= weight_of(stat.m, most, at.row);
+                    stat.m = most;
 #pragma unroll
-                for (int i = kLgVec - 1; i >= 0; --i) stat.first = x[i] == most ? v + i : stat.first;
+                    for (int i = kLgVec - 1; i >= 0; --i) stat.first = x[i] == most ? v + i : stat.first;
+                }
+                if (at.row.greedy || stat.m == -INFINITY) continue;
+                if (at.row.plain && stat.m < INFINITY) {
+#pragma unroll
+                    for (int i = 0; i < kLgVec; ++i) stat.l += __builtin_amdgcn_exp2f((x[i] - stat.m) * at.row.c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
+                }
             }
-            if (at.row.greedy || stat.m == -INFINITY) continue;
-#pragma unroll
-            for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
+        };
+        // A NaN makes the sum one: looked for only then.
+        if (!at.row.greedy && at.row.plain) pass(std::false_type{});
+        if (at.row.greedy || !at.row.plain || stat.l != stat.l) {
+            stat = {-INFINITY, 0.f, p.vocab, 0};
+            next = at.fetch(first);
+            pass(std::true_type{});
         }
         for (uint64_t left = mine; left != 0; left &= left - 1) {
             const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
@@ -290,17 +319,23 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
         const float share = stat.m == -INFINITY ? 0.f : 1.f / stat.l;
         auto prob = [&](float x, int v) {
             if (stat.m == -INFINITY) return 0.f;
-            return at.row.greedy ? (v == stat.first ? 1.f : 0.f) : weight_of(x, stat.m, at.row) * share;
+            return at.row.greedy ? (v == stat.first ? 1.f : 0.f) : fmaxf(weight_of(x, stat.m, at.row) * share, 0.f);
         };
+        const bool fast = !at.row.greedy && at.row.plain && stat.m != -INFINITY && stat.m < INFINITY;
         O* out = static_cast<O*>(p.probs) + row * p.probs_stride;
         for (int v = first; v < at.end; v += kLgRun) {
             const auto raw = next;
             next = at.fetch(v + kLgRun);
             float x[kLgVec];
-            at.adjust(v, raw, x);
+            at.template adjust<false>(v, raw, x);
             typename Logits<O>::vec y;
+            if (fast) {  // a NaN gets 0 from the maximum
 #pragma unroll
-            for (int i = 0; i < kLgVec; ++i) y[i] = static_cast<O>(prob(x[i], v + i));
+                for (int i = 0; i < kLgVec; ++i) y[i] = static_cast<O>(fmaxf(__builtin_amdgcn_exp2f((x[i] - stat.m) * at.row.c) * share, 0.f));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLgVec; ++i) y[i] = static_cast<O>(prob(x[i], v + i));
+            }
             if (at.end - v >= kLgVec) {
                 *reinterpret_cast<typename Logits<O>::vec*>(out + v) = y;
             } else {
