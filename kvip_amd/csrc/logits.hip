@@ -91,15 +91,16 @@ struct LogitPart {
     // Eight tokens from v on (a multiple of 8) as they lie in memory, and which of them the grammar allows.
     struct Raw {
         typename Logits<T>::vec x;
-        uint32_t may;
+        uint32_t may, held;  // held: by the request, where that is known
     };
     KVIP_DEVICE Raw fetch(int v) const {
         Raw raw;
-        raw.may = 0;
+        raw.may = raw.held = 0;
         const int there = min(end - v, kLgVec);
         if (there <= 0) return raw;
         raw.may = (1u << there) - 1;
         if (allowed != nullptr) raw.may &= allowed[v >> 3];
+        if (seen != nullptr) raw.held = seen[v >> 3];
         if (there == kLgVec) {
             raw.x = *reinterpret_cast<const typename Logits<T>::vec*>(logits + v);
         } else {
@@ -115,7 +116,7 @@ struct LogitPart {
 #pragma unroll
         for (int i = 0; i < kLgVec; ++i) x[i] = static_cast<float>(raw.x[i]);
         if (special != nullptr) raw.may &= ~(special[(v - begin) >> 5] >> (v & 31));
-        const uint32_t held = seen != nullptr ? seen[v >> 3] & raw.may : 0u;
+        const uint32_t held = raw.held & raw.may;
         if (held != 0) {
             LogitCounts n;
             if (end - v >= kLgVec) {
@@ -219,6 +220,7 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     if (p.seen != nullptr) {
         at.counts = p.counts + static_cast<int64_t>(b) * p.vocab;
         at.seen = reinterpret_cast<const uint8_t*>(p.seen + static_cast<int64_t>(b) * words);
+        if (first < at.end) next.held = at.seen[first >> 3];
     }
     const float temperature = p.temperature == nullptr ? 1.f : p.temperature[b];
     at.row.repetition = p.repetition == nullptr ? 1.f : p.repetition[b];
