@@ -6,8 +6,6 @@
 // tokens of a vocabulary) need more, and each of these is worked out by one thread on its own: a bit in LDS takes
 // the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing, and a
 // token named several times gets the same sum, in the list's order, whichever thread has it.
-#include <type_traits>
-
 #include "kvip_hip_prompt.h"
 #include "lane_groups.h"
 
@@ -39,10 +37,9 @@ struct LogitRow {
     bool plain;   // c is an ordinary number, so that exp2((x - m) c) needs no care but for an m of infinity
 };
 
-KVIP_DEVICE float penalised(float x, const LogitRow& r, bool held, int n) {
-    if (held) x *= x > 0.f ? r.inverse : r.repetition;
-    return n > 0 ? x - fmaf(r.frequency, static_cast<float>(n), r.presence) : x;
-}
+// All bits where bit i of x is set, else none; and a where `on` has bits, b where it has none.
+KVIP_DEVICE uint32_t bit_mask(uint32_t x, int i) { return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(x), i, 1)); }
+KVIP_DEVICE uint32_t pick(uint32_t on, uint32_t a, uint32_t b) { return (a & on) | (b & ~on); }
 
 KVIP_DEVICE float weight_of(float x, float m, const LogitRow& r) {
     if (r.plain && m < INFINITY) return __builtin_amdgcn_exp2f((x - m) * r.c);
@@ -126,13 +123,17 @@ struct LogitPart {
                 for (int i = 0; i < kLgVec; ++i) n[i] = v + i < end ? counts[v + i] : 0;
             }
 #pragma unroll
-            for (int i = 0; i < kLgVec; ++i) x[i] = held >> i & 1 ? penalised(x[i], row, true, n[i]) : x[i];
+            for (int i = 0; i < kLgVec; ++i) {  // a token that is not held has a count of 0
+                const uint32_t on = bit_mask(held, i);
+                const float factor = __uint_as_float(pick(on, __float_as_uint(x[i] > 0.f ? row.inverse : row.repetition), 0x3F800000u));
+                const float less = fmaf(row.frequency, static_cast<float>(n[i]), row.presence);
+                x[i] = fmaf(x[i], factor, n[i] > 0 ? -less : -0.f);
+            }
         }
         if (raw.may != 0xFFu) {
 #pragma unroll
             for (int i = 0; i < kLgVec; ++i) {
-                const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(raw.may), i, 1));
-                x[i] = __uint_as_float((__float_as_uint(x[i]) & keep) | (0xFF800000u & ~keep));
+                x[i] = __uint_as_float(pick(bit_mask(raw.may, i), __float_as_uint(x[i]), 0xFF800000u));
             }
         }
         if constexpr (CAREFUL) {
@@ -147,13 +148,15 @@ struct LogitPart {
 
     // Token v with its biases and the row's ancestors.
     KVIP_DEVICE float one(int v, int b, const int* way, int ways) {
-        int n = seen != nullptr ? counts[v] : 0;
         bool held = seen != nullptr && (seen[v >> 3] >> (v & 7) & 1);
+        int n = held ? counts[v] : 0;
         for (int i = 0; i < ways; ++i) {
             n += way[i] == v;
             held = held || way[i] == v;
         }
-        float x = penalised(static_cast<float>(logits[v]), row, held, n);
+        float x = static_cast<float>(logits[v]);
+        if (held) x *= x > 0.f ? row.inverse : row.repetition;
+        if (n > 0) x -= fmaf(row.frequency, static_cast<float>(n), row.presence);
         const int32_t* names = p.bias_tokens + static_cast<int64_t>(b) * p.biases;
         const float* values = p.bias_values + static_cast<int64_t>(b) * p.biases;
         int i = 0;
@@ -264,12 +267,34 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     };
 
     if constexpr ((MODE & kLgStats) != 0) {
-        auto pass = [&](auto careful) {
+        const bool ordinary = !at.row.greedy && at.row.plain;
+        if (ordinary) {
+            // The largest so far starts as the lowest number, so that every difference is one. Infinities and NaN come out as
+            // a sum that is none.
+            float top = -kLgLargest, l = 0.f;
+            for (int v = first; v < at.end; v += kLgRun) {
+                const auto raw = next;
+                next = at.fetch(v + kLgRun);
+                float x[kLgVec], most = top;
+                at.template adjust<false>(v, raw, x);
+#pragma unroll
+                for (int i = 0; i < kLgVec; ++i) most = fmaxf(most, x[i]);
+                l *= __builtin_amdgcn_exp2f((top - most) * at.row.c);
+                top = most;
+#pragma unroll
+                for (int i = 0; i < kLgVec; ++i) l += __builtin_amdgcn_exp2f((x[i] - top) * at.row.c);
+            }
+            stat.l = l;
+            if (l > 0.f) stat.m = top;
+        }
+        if (!ordinary || stat.l != stat.l) {
+            stat = {-INFINITY, 0.f, p.vocab, 0};
+            next = at.fetch(first);
             for (int v = first; v < at.end; v += kLgRun) {
                 const auto raw = next;
                 next = at.fetch(v + kLgRun);
                 float x[kLgVec], most;
-                at.template adjust<decltype(careful)::value>(v, raw, x);
+                at.template adjust<true>(v, raw, x);
                 most = x[0];
 #pragma unroll
                 for (int i = 1; i < kLgVec; ++i) most = fmaxf(most, x[i]);
@@ -280,21 +305,9 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
                     for (int i = kLgVec - 1; i >= 0; --i) stat.first = x[i] == most ? v + i : stat.first;
                 }
                 if (at.row.greedy || stat.m == -INFINITY) continue;
-                if (at.row.plain && stat.m < INFINITY) {
 #pragma unroll
-                    for (int i = 0; i < kLgVec; ++i) stat.l += __builtin_amdgcn_exp2f((x[i] - stat.m) * at.row.c);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
-                }
+                for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
             }
-        };
-        // A NaN makes the sum one: looked for only then.
-        if (!at.row.greedy && at.row.plain) pass(std::false_type{});
-        if (at.row.greedy || !at.row.plain || stat.l != stat.l) {
-            stat = {-INFINITY, 0.f, p.vocab, 0};
-            next = at.fetch(first);
-            pass(std::true_type{});
         }
         for (uint64_t left = mine; left != 0; left &= left - 1) {
             const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
