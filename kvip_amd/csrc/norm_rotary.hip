@@ -24,9 +24,21 @@ KVIP_DEVICE float head_scale(float largest) {
     const float quotient = largest / 448.f;
     return quotient > 0.f ? quotient : 1.f;
 }
-KVIP_DEVICE float under_scale(float x, float scale) {
+KVIP_DEVICE float under_scale(float x, float scale) {  // for any scale
     x /= scale;
     return x > 448.f ? 448.f : x < -448.f ? -448.f : x;
+}
+// Four features' codes. Times the scale's reciprocal a feature is off by two roundings of 2^-24, far less than what
+// its code can hold, and at most 448 but for those, which the conversion rounds away; a scale below the normal
+// range has no exact enough reciprocal.
+KVIP_DEVICE int head_codes(const float (&x)[4], float scale, float reciprocal) {
+    int packed = 0;
+    if (scale >= 0x1p-126f && scale < INFINITY) {
+        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * reciprocal, x[1] * reciprocal, packed, false);
+        return __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * reciprocal, x[3] * reciprocal, packed, true);
+    }
+    packed = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[0], scale), under_scale(x[1], scale), packed, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[2], scale), under_scale(x[3], scale), packed, true);
 }
 
 // Where a head of queries or a key goes: false where nowhere.
@@ -51,6 +63,7 @@ KVIP_DEVICE bool head_place(const KvipNormRotaryArgs& p, const KvipNormTensor& t
 template <typename T, bool HALF, int G, bool QUANT>
 __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormRotaryArgs p, int run) {
     typedef typename Four<T>::vec V;
+    constexpr int kGroups = kNrThreads / G;
     __shared__ __align__(16) float2 s_turn[kNrPairs];
     const int tid = threadIdx.x, pairs = p.rotary_dim / 2;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * run;
@@ -58,39 +71,55 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
     for (int i = tid; i < tokens * pairs; i += kNrThreads) {
         s_turn[i] = turn_of(p.positions[first + i / pairs], p.frequencies[i % pairs], p.magnitude, false);
     }
-    __syncthreads();
     const int j = tid % G;
     const bool live = j * kNrLane < p.dim, turned = j * kNrLane < p.rotary_dim;
     const int at[2] = {HALF && turned ? 4 * j : 8 * j, HALF && turned ? pairs + 4 * j : 8 * j + 4};
     const float share = 1.f / static_cast<float>(p.dim);
     uint32_t err = 0;
+    bool ready = false;  // the angles
 #pragma unroll 1
     for (int k = 0; k < 2; ++k) {
         const KvipNormTensor& t = p.tensors[k];
         if (t.x == nullptr) continue;
+        // This slice's heads of the run, counted along tokens and heads (the last slice takes the keys' first ones).
+        const int slice = k == 0 ? blockIdx.y : gridDim.y - 1 - blockIdx.y, step = kGroups * gridDim.y;
+        const int by_token = step / t.heads, by_head = step % t.heads;
+        int token = (tid / G + slice * kGroups) / t.heads, head = (tid / G + slice * kGroups) % t.heads;
+        const T* in = static_cast<const T*>(t.x) + first * t.x_token;
+        V raw[2] = {};
+        auto fetch = [&] {
+            if (token >= tokens || !live) return;
+            const T* x = in + token * t.x_token + head * t.x_head;
+            raw[0] = *reinterpret_cast<const V*>(x + at[0]);
+            raw[1] = *reinterpret_cast<const V*>(x + at[1]);
+        };
+        fetch();
         float weight[kNrLane], bias[kNrLane];
 #pragma unroll
         for (int i = 0; i < kNrLane; ++i) {
             weight[i] = live && t.weight != nullptr ? t.weight[at[i / 4] + i % 4] : 1.f;
             bias[i] = live && t.bias != nullptr ? t.bias[at[i / 4] + i % 4] : 0.f;
         }
-        for (int u = tid / G; u < tokens * t.heads; u += kNrThreads / G) {
-            const int token = u / t.heads, head = u % t.heads;
-            const T* in = static_cast<const T*>(t.x) + (first + token) * t.x_token + head * t.x_head;
+        if (!ready) __syncthreads();
+        ready = true;
+        while (token < tokens) {
+            const int token_now = token, head_now = head;
             float x[kNrLane];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                V raw = {};
-                if (live) raw = *reinterpret_cast<const V*>(in + at[r]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * r + i] = static_cast<float>(raw[i]);
+            for (int i = 0; i < kNrLane; ++i) x[i] = static_cast<float>(raw[i / 4][i % 4]);
+            token += by_token;
+            head += by_head;
+            if (head >= t.heads) {
+                head -= t.heads;
+                ++token;
             }
+            fetch();
             if (t.norm != KVIP_NORM_NONE) {
                 float sum = 0.f;
                 if (t.norm == KVIP_NORM_LAYER) {
 #pragma unroll
                     for (int i = 0; i < kNrLane; ++i) sum += x[i];
-                    const float mean = group_sum<G>(sum) * share;
+                    const float mean = group_sum<G>(live ? sum : 0.f) * share;
 #pragma unroll
                     for (int i = 0; i < kNrLane; ++i) x[i] -= mean;
                     sum = 0.f;
@@ -107,7 +136,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
             if (turned) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 turn = s_turn[token * pairs + 4 * j + i];
+                    const float2 turn = s_turn[token_now * pairs + 4 * j + i];
                     float& a = x[HALF ? i : 2 * i];
                     float& b = x[HALF ? 4 + i : 2 * i + 1];
                     const float c = a * turn.x - b * turn.y;
@@ -116,19 +145,17 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
                 }
             }
             HeadPlace place;
-            if (!head_place(p, t, QUANT && k == 1, first + token, head, &place, &err) || !live) continue;
+            if (!head_place(p, t, QUANT && k == 1, first + token_now, head_now, &place, &err) || !live) continue;
             if constexpr (QUANT) {
                 float largest = 0.f;
 #pragma unroll
                 for (int i = 0; i < kNrLane; ++i) largest = fmaxf(largest, fabsf(x[i]));
-                const float scale = head_scale(group_max<G>(largest));
+                const float scale = head_scale(group_max<G>(largest)), reciprocal = 1.f / scale;
                 uint8_t* out = static_cast<uint8_t*>(t.out) + place.out;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    int packed = 0;
-                    packed = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[4 * r], scale), under_scale(x[4 * r + 1], scale), packed, false);
-                    packed = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[4 * r + 2], scale), under_scale(x[4 * r + 3], scale), packed, true);
-                    *reinterpret_cast<int*>(out + at[r]) = packed;
+                    const float four[4] = {x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]};
+                    *reinterpret_cast<int*>(out + at[r]) = head_codes(four, scale, reciprocal);
                 }
                 if (j == 0) t.scales[place.scale] = scale;
             } else {
@@ -225,8 +252,8 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_any_kernel(const KvipN
 }
 
 template <typename T, int G, bool QUANT>
-void launch_group(const KvipNormRotaryArgs& a, int run, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.tokens + run - 1) / run)), block(kNrThreads);
+void launch_group(const KvipNormRotaryArgs& a, int run, int slices, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>((a.tokens + run - 1) / run), static_cast<unsigned>(slices)), block(kNrThreads);
     if (a.half) {
         hipLaunchKernelGGL((norm_rotary_kernel<T, true, G, QUANT>), grid, block, 0, s, a, run);
     } else {
@@ -243,17 +270,22 @@ void launch_norm_rotary(const KvipNormRotaryArgs& a, hipStream_t s) {
                            0, s, a);
         return;
     }
-    // Lanes of a head, and tokens of a workgroup: enough for each group of lanes to have a head, as many as there is LDS
-    // for, and few enough that 1024 workgroups (4 per CU) have some.
+    // Lanes of a head, and tokens of a workgroup: enough for each group of lanes to have a head of either array, as many as
+    // there is LDS for, and few enough that 1024 workgroups (4 per CU) have some. Few tokens' heads go over more workgroups.
     const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : a.dim <= 256 ? 32 : 64;
-    const int64_t fill = (kNrThreads / lanes + heads - 1) / heads, share = (a.tokens + 1023) / 1024;
+    const int groups = kNrThreads / lanes;
+    const int least = a.tensors[1].x != nullptr && a.tensors[1].heads < a.tensors[0].heads ? a.tensors[1].heads : a.tensors[0].heads;
+    const int64_t fill = (groups + least - 1) / least, share = (a.tokens + 1023) / 1024;
     const int64_t room = kNrPairs / (a.rotary_dim / 2), want = fill < share ? fill : share;
     const int run = static_cast<int>(want < 1 ? 1 : want > room ? room : want);
-    if (a.quantised) launch_group<T, 16, true>(a, run, s);
-    else if (lanes == 8) launch_group<T, 8, false>(a, run, s);
-    else if (lanes == 16) launch_group<T, 16, false>(a, run, s);
-    else if (lanes == 32) launch_group<T, 32, false>(a, run, s);
-    else launch_group<T, 64, false>(a, run, s);
+    const int64_t runs = (a.tokens + run - 1) / run, rounds = (static_cast<int64_t>(run) * a.tensors[0].heads + groups - 1) / groups;
+    const int64_t spread = 1024 / runs;
+    const int slices = static_cast<int>(spread < 1 ? 1 : spread > rounds ? rounds : spread);
+    if (a.quantised) launch_group<T, 16, true>(a, run, slices, s);
+    else if (lanes == 8) launch_group<T, 8, false>(a, run, slices, s);
+    else if (lanes == 16) launch_group<T, 16, false>(a, run, slices, s);
+    else if (lanes == 32) launch_group<T, 32, false>(a, run, slices, s);
+    else launch_group<T, 64, false>(a, run, slices, s);
 }
 
 bool valid_norm(const KvipNormRotaryArgs& a, int k) {
