@@ -61,8 +61,9 @@ KVIP_DEVICE bool head_place(const KvipNormRotaryArgs& p, const KvipNormTensor& t
 }
 
 template <typename T, bool HALF, int G, bool QUANT>
-__global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormRotaryArgs p, int run) {
+__global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormRotaryArgs p, int run, int slices) {
     typedef typename Four<T>::vec V;
+    typedef Four<float>::vec W;
     constexpr int kGroups = kNrThreads / G;
     __shared__ __align__(16) float2 s_turn[kNrPairs];
     const int tid = threadIdx.x, pairs = p.rotary_dim / 2;
@@ -81,8 +82,10 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
     for (int k = 0; k < 2; ++k) {
         const KvipNormTensor& t = p.tensors[k];
         if (t.x == nullptr) continue;
-        // This slice's heads of the run, counted along tokens and heads (the last slice takes the keys' first ones).
-        const int slice = k == 0 ? blockIdx.y : gridDim.y - 1 - blockIdx.y, step = kGroups * gridDim.y;
+        // This slice's heads of the run, counted along tokens and heads. Where the queries have several slices, the keys have one
+        // of their own.
+        if (slices > 1 && (k == 0) == (blockIdx.y == slices)) continue;
+        const int slice = k == 0 ? blockIdx.y : 0, step = k == 0 ? kGroups * slices : kGroups;
         const int by_token = step / t.heads, by_head = step % t.heads;
         int token = (tid / G + slice * kGroups) / t.heads, head = (tid / G + slice * kGroups) % t.heads;
         const T* in = static_cast<const T*>(t.x) + first * t.x_token;
@@ -94,11 +97,14 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
             raw[1] = *reinterpret_cast<const V*>(x + at[1]);
         };
         fetch();
-        float weight[kNrLane], bias[kNrLane];
-#pragma unroll
-        for (int i = 0; i < kNrLane; ++i) {
-            weight[i] = live && t.weight != nullptr ? t.weight[at[i / 4] + i % 4] : 1.f;
-            bias[i] = live && t.bias != nullptr ? t.bias[at[i / 4] + i % 4] : 0.f;
+        W weight[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}}, bias[2] = {};
+        if (t.weight != nullptr && live) {
+            weight[0] = *reinterpret_cast<const W*>(t.weight + at[0]);
+            weight[1] = *reinterpret_cast<const W*>(t.weight + at[1]);
+        }
+        if (t.bias != nullptr && live) {
+            bias[0] = *reinterpret_cast<const W*>(t.bias + at[0]);
+            bias[1] = *reinterpret_cast<const W*>(t.bias + at[1]);
         }
         if (!ready) __syncthreads();
         ready = true;
@@ -128,10 +134,10 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
                 for (int i = 0; i < kNrLane; ++i) sum = fmaf(x[i], x[i], sum);
                 const float factor = 1.f / sqrtf(group_sum<G>(live ? sum : 0.f) * share + p.epsilon);
 #pragma unroll
-                for (int i = 0; i < kNrLane; ++i) x[i] = fmaf(x[i] * factor, weight[i], bias[i]);
+                for (int i = 0; i < kNrLane; ++i) x[i] = fmaf(x[i] * factor, weight[i / 4][i % 4], bias[i / 4][i % 4]);
             } else if (t.weight != nullptr || t.bias != nullptr) {
 #pragma unroll
-                for (int i = 0; i < kNrLane; ++i) x[i] = fmaf(x[i], weight[i], bias[i]);
+                for (int i = 0; i < kNrLane; ++i) x[i] = fmaf(x[i], weight[i / 4][i % 4], bias[i / 4][i % 4]);
             }
             if (turned) {
 #pragma unroll
@@ -253,11 +259,11 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_any_kernel(const KvipN
 
 template <typename T, int G, bool QUANT>
 void launch_group(const KvipNormRotaryArgs& a, int run, int slices, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.tokens + run - 1) / run), static_cast<unsigned>(slices)), block(kNrThreads);
+    const dim3 grid(static_cast<unsigned>((a.tokens + run - 1) / run), static_cast<unsigned>(slices > 1 && a.tensors[1].x != nullptr ? slices + 1 : slices)), block(kNrThreads);
     if (a.half) {
-        hipLaunchKernelGGL((norm_rotary_kernel<T, true, G, QUANT>), grid, block, 0, s, a, run);
+        hipLaunchKernelGGL((norm_rotary_kernel<T, true, G, QUANT>), grid, block, 0, s, a, run, slices);
     } else {
-        hipLaunchKernelGGL((norm_rotary_kernel<T, false, G, QUANT>), grid, block, 0, s, a, run);
+        hipLaunchKernelGGL((norm_rotary_kernel<T, false, G, QUANT>), grid, block, 0, s, a, run, slices);
     }
 }
 
