@@ -410,6 +410,7 @@ void launch_logits(const KvipLogitArgs& a, hipStream_t s) {
 // cleared before.
 constexpr int kHistThreads = 1024;
 constexpr int kHistPart = 1 << 14;  // 64 KB of counts
+constexpr int kHistAtOnce = 8;      // tokens of a thread whose loads are issued together
 
 __global__ __launch_bounds__(kHistThreads) void history_load_kernel(const KvipHistoryArgs p, int parts) {
     __shared__ int s_counts[kHistPart];
@@ -427,13 +428,22 @@ __global__ __launch_bounds__(kHistThreads) void history_load_kernel(const KvipHi
     __syncthreads();
     const int64_t written = static_cast<int64_t>(from) + max(p.prompt_lens[i], 0);
     err = 0;
-    for (int64_t t = from + tid; t < to; t += kHistThreads) {
-        const int64_t v = p.tokens[t];
-        if (v < 0 || v >= p.vocab) err = KVIP_STATUS_BAD_TOKEN;
-        if (v < begin || v >= begin + size) continue;
-        const int at = static_cast<int>(v) - begin;
-        atomicOr(&s_seen[at >> 5], 1u << (at & 31));
-        if (t >= written) atomicAdd(&s_counts[at], 1);
+    for (int64_t t0 = from + tid; t0 < to; t0 += kHistThreads * kHistAtOnce) {
+        int64_t token[kHistAtOnce];
+#pragma unroll
+        for (int i = 0; i < kHistAtOnce; ++i) {
+            const int64_t t = t0 + i * kHistThreads;
+            token[i] = t < to ? p.tokens[t] : begin + size;  // no token of this part
+        }
+#pragma unroll
+        for (int i = 0; i < kHistAtOnce; ++i) {
+            const int64_t v = token[i], t = t0 + i * kHistThreads;
+            if (t < to && (v < 0 || v >= p.vocab)) err = KVIP_STATUS_BAD_TOKEN;
+            if (v < begin || v >= begin + size) continue;
+            const int at = static_cast<int>(v) - begin;
+            atomicOr(&s_seen[at >> 5], 1u << (at & 31));
+            if (t >= written) atomicAdd(&s_counts[at], 1);
+        }
     }
     if (part == 0) report(p.status, err);
     __syncthreads();
