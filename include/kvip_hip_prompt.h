@@ -33,9 +33,12 @@ extern "C" {
  * 0 .. seq_lens[b] - n + i. Keys and values as for kvip_hip_sparse_attention; per token and head
  *   output = sum_j p_j value_j / sum_j p_j, p_j = exp(s_j - max s), s_j = scale <query, key_j>
  * over the rows it sees (0 where it sees none), lse = log sum_j exp(s_j) (-infinity).
- * Features times their scales, and probabilities, are rounded once to bf16; the rest is in 32 bits.
+ * Features times their scales (products in 32 bits) are rounded once to fp16 under an exponent that the rows of 32
+ * positions share, their largest feature being 2^14 .. 2^15 there: by 2^-11 of themselves, or 2^-39 of that largest;
+ * query features likewise, which only those below 2^-28 of the largest of their (token, head) feel; probabilities by
+ * 2^-11 of themselves, or 2^-29 of the largest's. The rest is in 32 bits.
  * Rows that a token does not see do not reach its output, whatever they hold; a token that sees a row with
- * a feature that is no finite bf16 becomes NaN as a whole (a rotary feature that is not finite reaches the
+ * a value that is no finite 32-bit number becomes NaN as a whole (a rotary feature that is not finite reaches the
  * logits as it is). Blocks outside the cache set KVIP_STATUS_BAD_BLOCK and
  * count as not there; lengths outside 0 .. max_blocks * 128, fewer rows than chunk tokens, or cu_seqlens that
  * fall or leave 0 .. max_tokens set KVIP_STATUS_BAD_LENGTH (they are cut to the range). So does a request

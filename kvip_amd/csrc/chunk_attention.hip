@@ -18,16 +18,20 @@
 #include <utility>
 
 #include "kvip_hip_prompt.h"
+#include "lane_groups.h"
 #include "lds_async.h"
 
 namespace kvip {
 namespace {
 
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* LdsS16x4;
 
 constexpr int kCaThreads = 256;
@@ -50,6 +54,10 @@ constexpr int kCaCus = 256;
 constexpr float kCaLog2e = 1.44269504088896341f;
 constexpr float kCaLn2 = 0.693147180559945309f;
 constexpr float kCaMargin = 8.0f * kCaLog2e;
+constexpr int kCaTop = 14;                        // exponent of the largest feature in an image, and of a row's largest query
+constexpr int kCaSpread = 12;                     // rows of a tile whose exponents differ by more keep their own
+constexpr int kCaSoftmax = 19;                    // pieces of a tile's softmax
+constexpr int kCaLift = 4;                        // exponent that probabilities are lifted by: 2^(kCaMargin + kCaLift) fits fp16
 static_assert(kCaLoads * 1024 * kCaWaves == kCaImage, "whole loads");
 static_assert(kCaSlots * kCaImage <= 160 * 1024, "LDS of a CU");
 
@@ -69,12 +77,13 @@ struct ChunkPlan {
     int images_before[KVIP_DRAFT_MAX_BATCH];     // of request b, -1: none
 };
 
-// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there), then the
-// images, then the parts: 32 rows x 512 sums per wave as its lanes hold them ([block][quarter][lane] 16 bytes),
+// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, exponent and
+// whether its rows have their own) and the rows' exponents, then the images, then the parts: 32 rows x 512 sums per wave as its lanes hold them ([block][quarter][lane] 16 bytes),
 // then their (maximum, sum) pairs.
 struct ChunkWork {
     ChunkPlan* plan;
-    uint2* flags;
+    uint4* flags;
+    int16_t* exponents;
     uint8_t* images;
     f32x4* sums;
     float2* states;
@@ -91,7 +100,8 @@ __host__ __device__ inline ChunkWork ca_work(void* base, int64_t images, size_t*
     };
     ChunkWork w;
     w.plan = reinterpret_cast<ChunkPlan*>(take(sizeof(ChunkPlan)));
-    w.flags = reinterpret_cast<uint2*>(take(static_cast<size_t>(images + 64) * sizeof(uint2)));  // read 64 at a time
+    w.flags = reinterpret_cast<uint4*>(take(static_cast<size_t>(images) * sizeof(uint4)));
+    w.exponents = reinterpret_cast<int16_t*>(take(static_cast<size_t>(images) * kCaTile * sizeof(int16_t)));
     w.images = take(static_cast<size_t>(images) * kCaImage);
     w.sums = reinterpret_cast<f32x4*>(take(static_cast<size_t>(kCaUnits) * kCaWaves * kCaBlocks * 4 * 64 * sizeof(f32x4)));
     w.states = reinterpret_cast<float2*>(take(static_cast<size_t>(kCaUnits) * kCaTileRows * sizeof(float2)));
@@ -121,10 +131,17 @@ KVIP_DEVICE ChunkRequest ca_request(const KvipChunkAttnArgs& p, int b, uint32_t*
 KVIP_DEVICE int ca_row_tiles(const ChunkRequest& q, int heads) { return (q.tokens * heads + kCaTileRows - 1) / kCaTileRows; }
 KVIP_DEVICE int ca_steps(const ChunkRequest& q) { return q.tokens > 0 ? (q.length + kCaTile - 1) / kCaTile : 0; }
 
-KVIP_DEVICE uint32_t ca_pack(float a, float b) {  // hardware round to nearest even
+// Hardware round to nearest even.
+KVIP_DEVICE uint32_t ca_pack(float a, float b) {
     const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
     return __builtin_bit_cast(uint32_t, v);
 }
+KVIP_DEVICE uint32_t ca_pack_half(float a, float b) {
+    const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+// Exponent that takes the largest magnitude (of bits `most`, below infinity's) to 2^kCaTop .. 2^(kCaTop + 1).
+KVIP_DEVICE int ca_exponent(uint32_t most) { return static_cast<int>(most >> 23) - 127 - kCaTop; }
 
 // Plan and images. Every workgroup sums the requests' tiles for itself; the first one leaves the plan, the others take
 // images in turn. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8 rotary features.
@@ -132,7 +149,7 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
     __shared__ __align__(16) uint8_t s_image[kCaImage];
     __shared__ int s_before[KVIP_DRAFT_MAX_BATCH + 1];
     __shared__ uint32_t s_sums[kCaWaves];
-    __shared__ uint2 s_flags[kCaWaves];
+    __shared__ uint4 s_flags[kCaWaves];
     constexpr int kPer = KVIP_DRAFT_MAX_BATCH / kCaThreads;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t most = ca_images(p.max_rows, p.batch);
@@ -271,52 +288,74 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
             rope = *reinterpret_cast<const v4i*>(row + kCaValue + piece * 16);
             scale = *reinterpret_cast<const f32x4*>(row + kCaValue + 128);
         }
-        v4i out[8];
-        uint32_t odd = 0;
+        float x[64];
+        uint32_t most_bits = 0;
+        bool odd = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x0 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 0), x1 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 1);
-                const float x2 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 2), x3 = __builtin_amdgcn_cvt_f32_fp8(raw[k][i], 3);
-                const uint32_t lo2 = ca_pack(x0 * scale[k], x1 * scale[k]), hi2 = ca_pack(x2 * scale[k], x3 * scale[k]);
-                odd |= (((lo2 & 0x7F807F80u) + 0x00800080u) | ((hi2 & 0x7F807F80u) + 0x00800080u)) & 0x80008000u;
-                out[2 * k + i / 2][2 * (i & 1)] = static_cast<int>(lo2);
-                out[2 * k + i / 2][2 * (i & 1) + 1] = static_cast<int>(hi2);
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int bytes = raw[i / 4][i % 4];
+            x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(bytes, 0) * scale[i / 4];
+            x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(bytes, 1) * scale[i / 4];
+            x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(bytes, 2) * scale[i / 4];
+            x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(bytes, 3) * scale[i / 4];
         }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) most_bits = max(most_bits, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        odd = most_bits >= 0x7F800000u;
         // A row's 8 threads lie side by side: bit t of the flags of the whole tile.
-        const uint64_t odd_lanes = __ballot(odd != 0), gone_lanes = __ballot(!there);
+        const uint64_t odd_lanes = __ballot(odd), gone_lanes = __ballot(!there);
         const bool zero = odd_lanes >> (lane & 56) & 0xFF;
+        if (zero) most_bits = 0;
+        float turned[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            turned[i] = bf16_to_float(static_cast<uint16_t>(static_cast<uint32_t>(rope[i / 2]) >> (16 * (i & 1))));
+            const uint32_t bits = __float_as_uint(turned[i]) & 0x7FFFFFFFu;
+            most_bits = max(most_bits, bits < 0x7F800000u ? bits : 0u);
+        }
+        const float most_row = group_max<8>(__uint_as_float(most_bits));  // of rows without a feature: 0
+        const float most_wave = group_max<64>(most_row);
+        const float least_wave = -group_max<64>(most_row > 0.f ? -most_row : -INFINITY);
         uint32_t odd_rows = 0, gone_rows = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             odd_rows |= ((odd_lanes >> (8 * i) & 0xFF) != 0 ? 1u : 0u) << i;
             gone_rows |= static_cast<uint32_t>(gone_lanes >> (8 * i) & 1) << i;
         }
-        __syncthreads();  // the image before is copied
+        if (lane == 0) s_flags[w] = make_uint4(odd_rows, gone_rows, __float_as_uint(most_wave), __float_as_uint(least_wave));
+        __syncthreads();  // and the image before is copied
+        uint4 flags = make_uint4(0, 0, 0, 0x7F800000u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                *reinterpret_cast<v4i*>(s_image + 16 * ca_place(k * 16 + piece * 2 + i, t)) = zero ? v4i{0, 0, 0, 0} : out[2 * k + i];
-            }
+        for (int i = 0; i < kCaWaves; ++i) {
+            flags.x |= s_flags[i].x << (8 * i);
+            flags.y |= s_flags[i].y << (8 * i);
+            flags.z = max(flags.z, s_flags[i].z);
+            flags.w = min(flags.w, s_flags[i].w);
         }
-        *reinterpret_cast<v4i*>(s_image + 16 * ca_place(kCaValue / 8 + piece, t)) = rope;
-        if (lane == 0) s_flags[w] = make_uint2(odd_rows, gone_rows);
+        // One exponent for all rows, unless that would cost the smaller ones their bits: what a token sees must not
+        // depend on rows that it does not.
+        const int tile_exponent = ca_exponent(flags.z);
+        const bool spread = flags.z != 0 && tile_exponent - ca_exponent(flags.w) > kCaSpread;
+        const int exponent = !spread ? tile_exponent : most_row > 0.f ? ca_exponent(__float_as_uint(most_row)) : -200;
+        if (spread && piece == 0) work.exponents[static_cast<int64_t>(image) * kCaTile + t] = static_cast<int16_t>(exponent);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v4i out;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                out[i] = static_cast<int>(ca_pack_half(ldexpf(x[8 * k + 2 * i], -exponent), ldexpf(x[8 * k + 2 * i + 1], -exponent)));
+            }
+            *reinterpret_cast<v4i*>(s_image + 16 * ca_place(k / 2 * 16 + piece * 2 + k % 2, t)) = zero ? v4i{0, 0, 0, 0} : out;
+        }
+        v4i out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = static_cast<int>(ca_pack_half(ldexpf(turned[2 * i], -exponent), ldexpf(turned[2 * i + 1], -exponent)));
+        *reinterpret_cast<v4i*>(s_image + 16 * ca_place(kCaValue / 8 + piece, t)) = out;
         __syncthreads();
         v4i* to = reinterpret_cast<v4i*>(work.images + static_cast<int64_t>(image) * kCaImage);
 #pragma unroll
         for (int i = 0; i < kCaImage / 16 / kCaThreads; ++i) to[tid + i * kCaThreads] = *reinterpret_cast<const v4i*>(s_image + 16 * (tid + i * kCaThreads));
-        if (tid == 0) {
-            uint2 flags = make_uint2(0, 0);
-#pragma unroll
-            for (int i = 0; i < kCaWaves; ++i) {
-                flags.x |= s_flags[i].x << (8 * i);
-                flags.y |= s_flags[i].y << (8 * i);
-            }
-            work.flags[image] = flags;
-        }
+        if (tid == 0) work.flags[image] = make_uint4(flags.x, flags.y, static_cast<uint32_t>(tile_exponent * 2 + (spread ? 1 : 0)), 0);
     }
 }
 
@@ -419,9 +458,6 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     const int sees = min(max(q.past() + node + 1, 0), q.length);  // cached rows that the lane's row sees
     // The first tile that some row of the wave does not see whole.
     const int t_mask = min(max(q.past() + min(first_row, rows - 1) / p.heads + 1, 0), q.length) / kCaTile;
-    const float scale2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(fabsf(p.scale * kCaLog2e), 0x1p-126f))));
-    const int flip = p.scale < 0.f ? static_cast<int>(0x80008000u) : 0;
-
     const uint32_t ring = lds_addr(s_ring);
     auto slot_of = [&](int t) { return ring + ((t - t0) & (kCaSlots - 1)) * kCaImage; };
     // The wave's share of tile t's image (past the last tile: the last one again), in kCaLoads loads.
@@ -453,27 +489,51 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
         ca_hold(o[f]);
     }
+    // They become fp16 under an exponent of their row's, exactly but for features below 2^-28 of its largest. A negative
+    // scale turns their signs.
+    u16x2 most_q = {};
 #pragma unroll
     for (int i = 0; i < kCaFrags; ++i) {
-        qf[i] ^= flip;
-        asm volatile("" : "+v"(qf[i]));  // waited for here, not in the tile loop
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most_q = __builtin_elementwise_max(most_q, __builtin_bit_cast(u16x2, qf[i][j] & 0x7FFF7FFF));
     }
+    uint32_t most_bits = static_cast<uint32_t>(max(most_q[0], most_q[1])) << 16;
+    most_bits = __float_as_uint(ca_half_max(__uint_as_float(most_bits < 0x7F800000u ? most_bits : 0u)));
+    const int q_exponent = max(ca_exponent(most_bits), -126);
+    const float q_factor = __uint_as_float(static_cast<uint32_t>(127 - q_exponent) << 23 | (p.scale < 0.f ? 0x80000000u : 0u));
+#pragma unroll
+    for (int i = 0; i < kCaFrags; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t pair = static_cast<uint32_t>(qf[i][j]);
+            qf[i][j] = static_cast<int>(ca_pack_half(__uint_as_float(pair << 16) * q_factor, __uint_as_float(pair & 0xFFFF0000u) * q_factor));
+        }
+        asm volatile("" : "+v"(qf[i]));  // worked out here, not in the tile loop
+    }
+    const float scale2 = fabsf(p.scale * kCaLog2e);
     float m_run = -INFINITY, l_sum = 0.f;
     v16f s;
     v4i pb[2];  // probabilities of the tile whose values come next
 
     // The flags of 64 tiles, which the lanes hold.
     int held_first = t0;
-    uint2 held = work.flags[image0 + min(t0 + lane, reach - 1)];
+    uint4 held = work.flags[image0 + min(t0 + lane, reach - 1)];
+    asm volatile("" : "+v"(held.x), "+v"(held.y), "+v"(held.z));
+    struct Flags {
+        uint32_t odd, gone;
+        int exponent;
+        bool spread;
+    };
     auto flags_of = [&](int t) {
         if (t >= held_first + 64) {
             held_first = t;
             held = work.flags[image0 + min(t + lane, reach - 1)];
-            asm volatile("" : "+v"(held.x), "+v"(held.y));  // waited for here, not at every use
+            asm volatile("" : "+v"(held.x), "+v"(held.y), "+v"(held.z));  // waited for here, not at every use
         }
-        return make_uint2(__builtin_amdgcn_readlane(held.x, t - held_first), __builtin_amdgcn_readlane(held.y, t - held_first));
+        const int at = t - held_first, last = __builtin_amdgcn_readlane(static_cast<int>(held.z), at);
+        return Flags{static_cast<uint32_t>(__builtin_amdgcn_readlane(held.x, at)), static_cast<uint32_t>(__builtin_amdgcn_readlane(held.y, at)),
+                     last >> 1, (last & 1) != 0};
     };
-    asm volatile("" : "+v"(held.x), "+v"(held.y));
 
     // Operands are read from LDS kAhead products before their use, across the borders of logits and values too.
     constexpr int kAhead = 4;
@@ -498,67 +558,106 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         ring_of[i % kAhead] = __builtin_bit_cast(v4i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     static_assert(kCaFrags % kAhead == 0 && 2 * kCaBlocks % kAhead == 0, "the operand ring goes on at its start");
+    // What the tile's flags and its place say. Features of a tile stand under its exponent, a row's sums under the largest
+    // of the exponents that it has seen: a tile's probabilities take the difference, their sum gives it back.
+    int exponent = -300, shift, lower;  // of the sums; by how much it has just risen; what the tile's is below it
+    float factor;                       // from logits as they come to those in log2 units
+    bool spread;                        // the tile's rows have exponents of their own
+    auto row_exponent = [&](int t, int i) {
+        return static_cast<int>(work.exponents[static_cast<int64_t>(image0 + t) * kCaTile + 8 * (i >> 2) + 4 * hk + (i & 3)]);
+    };
+    Flags flags;
+    int of_tile;
+    auto look = [&](int t) {  // does not need the logits
+        flags = flags_of(t);
+        of_tile = flags.exponent;
+        spread = flags.spread;
+    };
     // Logits of a tile, whose first operands are under way; the loads that are aimed at stand between the products, the
     // first value operands of the tile at `next` behind them.
-    auto logits = [&](const Base& base, const Base& next) {
+    auto logits = [&](int t, const Base& base, const Base& next) {
         for_all([&](auto which) {
             constexpr int i = decltype(which)::value;
             if constexpr (i == 0) {
                 const v16f zero = {};
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ring_of[i % kAhead]), __builtin_bit_cast(bf16x8, qf[i]), zero, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, ring_of[i % kAhead]), __builtin_bit_cast(f16x8, qf[i]), zero, 0, 0, 0);
             } else {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ring_of[i % kAhead]), __builtin_bit_cast(bf16x8, qf[i]), s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, ring_of[i % kAhead]), __builtin_bit_cast(f16x8, qf[i]), s, 0, 0, 0);
             }
             if constexpr (i + kAhead < kCaFrags) key(base, i + kAhead);
             else value(next, i + kAhead - kCaFrags);
             if constexpr (i % 4 == 0) fetch(std::integral_constant<int, i / 4>{});
+            if constexpr (i == kCaFrags / 2) look(t);
             __builtin_amdgcn_sched_barrier(0);
         }, std::make_integer_sequence<int, kCaFrags>{});
     };
     static_assert(kCaLoads * 4 == kCaFrags, "a load every four products");
     auto mask = [&](int t) {
-        const uint2 flags = flags_of(t);
-        if (t >= t_mask || flags.x != 0 || flags.y != 0) {
+        if (t >= t_mask || flags.odd != 0 || flags.gone != 0 || spread) {
             const int left = sees - t * kCaTile;
             uint32_t seen = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-            seen &= ~flags.y;
-            if (seen & flags.x) l_sum = NAN;
+            seen &= ~flags.gone;
+            if (seen & flags.odd) l_sum = NAN;
+            if (seen == 0) of_tile = exponent;
             seen >>= 4 * hk;
+            if (spread) {
+                int top = -300;
+                for (int i = 0; i < 16; ++i) {
+                    if (seen >> (8 * (i >> 2) + (i & 3)) & 1) top = max(top, row_exponent(t, i));
+                }
+                top = static_cast<int>(ca_half_max(static_cast<float>(top)));
+                of_tile = top;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = ldexpf(s[i], min(row_exponent(t, i) - top, 0));
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 if (!(seen >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
             }
         }
     };
-    // Softmax of the logits, p = 2^(scale2 (logit - m)), in 18 pieces. Its factor for what came before (alpha) counts
-    // once the values of the tile before are in.
+    // Softmax of the logits, p = 2^(factor logit - m + kCaLift + lower), in kCaSoftmax pieces. Its factor for what came before
+    // (alpha) counts once the values of the tile before are in.
     float mx, bias, alpha, fresh_sum;
     bool raise;
     auto softmax = [&](int piece) {
         if (piece == 0) {
+            shift = max(of_tile - exponent, 0);
+            exponent += shift;
+            lower = max(of_tile - exponent, -100);
+            // A scale so small that the logits vanish still leaves a number, which what is masked stays below.
+            factor = fmaxf(ldexpf(scale2, q_exponent + of_tile), 0x1p-126f);
+            asm volatile("" : "+v"(factor), "+v"(lower));
+        } else if (piece == 1) {
             mx = s[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-            mx = ca_half_max(mx);
+            mx = ca_half_max(mx) * factor;
             fresh_sum = 0.f;
-        } else if (piece == 1) {
-            raise = (mx - m_run) * scale2 > kCaMargin;  // also the first finite maximum
+        } else if (piece == 2) {
+            raise = mx - m_run > kCaMargin;  // also the first finite maximum
             const float m_new = raise ? mx : m_run;
-            alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_new) * scale2) : raise ? 0.f : 1.f;
+            alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : raise ? 0.f : 1.f;
             m_run = m_new;
-            bias = m_new == -INFINITY ? 0.f : -m_new * scale2;
+            bias = (m_new == -INFINITY ? 0.f : -m_new) + static_cast<float>(kCaLift + lower);
             asm volatile("" : "+v"(bias));
         } else {
-            float p1 = __builtin_amdgcn_exp2f(fmaf(s[piece - 2], scale2, bias));
+            float p1 = s[piece - 3] * factor;  // rounded as the maximum was, however large the logits are
+            asm volatile("" : "+v"(p1));
+            p1 = __builtin_amdgcn_exp2f(p1 + bias);
             fresh_sum += p1;
             asm volatile("" : "+v"(p1), "+v"(fresh_sum));  // here, not behind the products
-            s[piece - 2] = p1;
+            s[piece - 3] = p1;
         }
     };
-    auto take = [&] {  // the softmax's results become those of the tile whose values come next
-        l_sum = l_sum * alpha + fresh_sum;
+    auto take = [&](int t) {  // the softmax's results become those of tile t, whose values come next
+        l_sum = l_sum * alpha + ldexpf(fresh_sum, -lower);
+        if (spread) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pb[i >> 2][i & 3] = static_cast<int>(ca_pack(s[2 * i], s[2 * i + 1]));
+            for (int i = 0; i < 16; ++i) s[i] = ldexpf(s[i], min(row_exponent(t, i) - (exponent + lower), 0));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pb[i >> 2][i & 3] = static_cast<int>(ca_pack_half(s[2 * i], s[2 * i + 1]));
     };
     // Every load of the tile after next has landed but the last kCaLoads of this wave, and all reads of this wave are done;
     // then those of all waves.
@@ -574,14 +673,17 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         for_all([&](auto which) {
             constexpr int i = decltype(which)::value;
             if constexpr (i % 2 == 0) ca_hold(o[i / 2]);
-            o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ring_of[i % kAhead]), __builtin_bit_cast(bf16x8, pb[i % 2]), o[i / 2], 0, 0, 0);
+            o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, ring_of[i % kAhead]), __builtin_bit_cast(f16x8, pb[i % 2]), o[i / 2], 0, 0, 0);
             if constexpr (i % 2 == 1) ca_hold(o[i / 2]);
             if constexpr (i + kAhead < 2 * kCaBlocks) value(base, i + kAhead);
             else if constexpr (kSoftmax) {
                 if constexpr (i + kAhead == 2 * kCaBlocks) arrive();
                 key(next, i + kAhead - 2 * kCaBlocks);
             }
-            if constexpr (kSoftmax && i < 18) softmax(i);
+            if constexpr (kSoftmax) {  // over all products, once the logits are there
+                constexpr int from = i * kCaSoftmax / (2 * kCaBlocks), to = (i + 1) * kCaSoftmax / (2 * kCaBlocks);
+                if constexpr (to > from) softmax(from);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }, std::make_integer_sequence<int, 2 * kCaBlocks>{});
     };
@@ -590,11 +692,11 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) key(keys_base, i);
     aim(t0 + kCaSlots - 2);
-    logits(keys_base, values_base);
+    logits(t0, keys_base, values_base);
     mask(t0);
 #pragma unroll
-    for (int i = 0; i < 18; ++i) softmax(i);
-    take();
+    for (int i = 0; i < kCaSoftmax; ++i) softmax(i);
+    take(t0);
     if (t0 + 1 < t1) {
         arrive();
         keys_base = base_of(t0 + 1, key_at);
@@ -605,19 +707,20 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     for (int t = t0; t + 1 < t1; ++t) {
         aim(t + kCaSlots - 1);
         const Base here = base_of(t, value_at), keys_next = base_of(t + 2, key_at);
-        logits(keys_base, here);
+        logits(t + 1, keys_base, here);
         mask(t + 1);
         values(here, keys_next, std::true_type{});
         keys_base = keys_next;
-        if (__ballot(raise) != 0ull) {
+        if (__ballot(raise || shift != 0) != 0ull) {
+            const float to_new = ldexpf(alpha, -shift);
 #pragma unroll
             for (int f = 0; f < kCaBlocks; ++f) {
                 ca_hold(o[f]);
-                o[f] *= alpha;
+                o[f] *= to_new;
                 ca_hold(o[f]);
             }
         }
-        take();
+        take(t + 1);
     }
     values_base = base_of(t1 - 1, value_at);
     asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
@@ -626,13 +729,13 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     values(values_base, values_base, std::false_type{});
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
 
-    const float l_all = ca_half_sum(l_sum), m_all = m_run * scale2;  // log2 units from here on
-    const float factor = whole ? ca_share(l_all) : 1.f;
+    const float l_all = ldexpf(ca_half_sum(l_sum), -kCaLift);
+    const float share = ldexpf(whole ? ca_share(l_all) : 1.f, exponent - kCaLift);
     f32x4* part = work.sums + (static_cast<int64_t>(blockIdx.x) * kCaWaves + w) * (kCaBlocks * 4 * 64) + lane;
 #pragma unroll
     for (int f = 0; f < kCaBlocks; ++f) {
         ca_hold(o[f]);
-        const v16f x = o[f];
+        const v16f x = o[f] * share;
         if (!whole) {
 #pragma unroll
             for (int a = 0; a < 4; ++a) part[(f * 4 + a) * 64] = f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]};
@@ -644,8 +747,7 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const auto pair = __builtin_amdgcn_permlane32_swap(
-                        ca_pack(x[4 * a + 2 * e] * factor, x[4 * a + 2 * e + 1] * factor),
-                        ca_pack(x[4 * a + 2 * e + 4] * factor, x[4 * a + 2 * e + 5] * factor), false, false);
+                        ca_pack(x[4 * a + 2 * e], x[4 * a + 2 * e + 1]), ca_pack(x[4 * a + 2 * e + 4], x[4 * a + 2 * e + 5]), false, false);
                     v[e] = pair[0];
                     v[e + 2] = pair[1];
                 }
@@ -654,13 +756,13 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         } else if (row < rows) {
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                ca_store(p, out_row * kCaValue + 32 * f + 8 * a + 4 * hk, f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]} * factor);
+                ca_store(p, out_row * kCaValue + 32 * f + 8 * a + 4 * hk, f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]});
             }
         }
     }
     if (hk == 0) {
-        if (!whole) work.states[static_cast<int64_t>(blockIdx.x) * kCaTileRows + w * kCaRows + hn] = make_float2(m_all, l_all);
-        else if (p.lse != nullptr && row < rows) p.lse[out_row] = ca_lse(m_all, l_all);
+        if (!whole) work.states[static_cast<int64_t>(blockIdx.x) * kCaTileRows + w * kCaRows + hn] = make_float2(m_run, l_all);
+        else if (p.lse != nullptr && row < rows) p.lse[out_row] = ca_lse(m_run, l_all);
     }
 }
 

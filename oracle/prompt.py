@@ -1,7 +1,7 @@
 """CPU restatement in 64 bits of the operators on either side of a prompt chunk's layers
 (include/kvip_hip_prompt.h). TEST INFRASTRUCTURE ONLY (see oracle/__init__.py).
 
-features         - keys and values of cached rows as chunk attention takes them (features rounded once to bf16)
+features         - keys and values of cached rows as chunk attention takes them (rounded once to fp16 under an exponent)
 attention        - softmax attention of one token, with a bound for the kernel's roundings
 normed           - norm, weight and bias of heads, with a bound
 turned           - oracle.draft's turn, with a bound
@@ -20,30 +20,38 @@ import numpy as np
 from oracle import draft
 
 BLOCK = 128
-FP32 = 2.0 ** -24  # half a step of 32 bits, of the value; so BF16 below
-BF16 = 2.0 ** -8
+FP32 = 2.0 ** -24  # half a step of 32 bits, of the value; so FP16 below
+FP16 = 2.0 ** -11
 
 
-def to_bf16(x):
-    """float32 values rounded to the nearest bf16, halves to even, as float64."""
-    bits = np.ascontiguousarray(x, np.float32).view(np.uint32).astype(np.uint64)
-    bits = ((bits + 0x7FFF + ((bits >> 16) & 1)) >> 16).astype(np.uint32) << 16
-    return np.where(np.isnan(x), np.nan, bits.view(np.float32)).astype(np.float64)
-
-
-def features(rows):
-    """rows uint8 [n, >= 656] -> (key [n, 576], value [n, 512], odd [n]: a feature is no finite bf16)."""
+def features(rows, positions=None):
+    """rows uint8 [n, >= 656] of one request, at positions 0, 1, ... or as given -> (key [n, 576], value [n, 512], odd [n]: a
+    value is no finite number). Products in 32 bits, rounded to fp16 under the exponent that takes the largest finite
+    feature of the 32 positions' rows (those that are odd left out) to 2^14 .. 2^15, or, where the rows' own exponents
+    differ by more than 12, each under its own."""
+    positions = np.arange(len(rows)) if positions is None else np.asarray(positions)
     with np.errstate(over="ignore", invalid="ignore"):
         nope, rope, scales = draft.row_parts(rows)
         product = nope.astype(np.float32) * np.repeat(scales.astype(np.float32), 128, axis=1)
-        value = to_bf16(product)
-    return np.concatenate([value, rope], axis=1), value, ~np.isfinite(value).all(1)
+        odd = ~np.isfinite(product).all(1)
+        product[odd] = 0
+        key = np.concatenate([product, rope.astype(np.float32)], axis=1)
+        for tile in np.unique(positions // 32):
+            at = np.flatnonzero(positions // 32 == tile)
+            sizes = np.abs(np.where(np.isfinite(key[at]), key[at], 0)).max(1)
+            exponents = np.where(sizes >= 2.0 ** -126, np.frexp(sizes)[1] - 1, -127) - 14
+            if np.any(sizes > 0) and exponents.max() - exponents[sizes > 0].min() <= 12:
+                exponents[:] = exponents.max()
+            for i, exponent in zip(at, exponents):
+                key[i] = np.ldexp(np.ldexp(key[i].astype(np.float64), -exponent).astype(np.float16).astype(np.float64), exponent)
+    return key.astype(np.float64), key[:, :512].astype(np.float64), odd
 
 
 def attention(query, key, value, scale):
     """query [heads, 576] of one token over the rows it sees. Returns (output [heads, 512], lse [heads], bound
-    [heads, 512], lse bound [heads]): the bounds hold for probabilities rounded to bf16, dot products of 576 terms,
-    exponentials and sums of n terms in 32 bits."""
+    [heads, 512], lse bound [heads]): the bounds hold for probabilities rounded to fp16 (2^-11; the smallest, of tiles whose
+    exponent is up to 2 below others', 2^-27 of the maximum's), dot products of 576 terms, exponentials and sums of n
+    terms in 32 bits."""
     q, n = np.asarray(query, np.float64), len(key)
     if n == 0:
         zero = np.zeros((len(q), value.shape[1]))
@@ -55,7 +63,7 @@ def attention(query, key, value, scale):
     p /= whole
     slip = abs(scale) * (np.abs(q) @ np.abs(key).T).max(1) * (576 + 8) * FP32 + np.abs(logits).max(1) * 8 * FP32
     sums = n * 2 * FP32 + 16 * FP32
-    bound = (p @ np.abs(value)) * (BF16 + 2 * slip + sums)[:, None]
+    bound = (p @ np.abs(value)) * (FP16 + 2 * slip + sums)[:, None] + 2.0 ** -27 * np.abs(value).sum(0) / whole
     return p @ value, top[:, 0] + np.log(whole[:, 0]), bound, slip + sums + np.abs(top[:, 0]) * 4 * FP32
 
 

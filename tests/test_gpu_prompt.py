@@ -177,9 +177,9 @@ def test_chunk_attention_equals_tree_attention_of_chains(torch_gpu):
     tree.bind(step.query.cuda(), step.kv, device(torch, step.table, torch.int32), device(torch, step.lens, torch.int32),
               device(torch, step.cu, torch.int32))
     a, b = op()[:70], tree()[:70]
-    # Keys rounded to bf16 move a logit by at most 2^-8 scale sum |q k| (below 2^-8 * 25 here, as sum |q k| <= 576 *
-    # E|q k| + noise < 600); probabilities by twice that, values by 2^-8, each side's probabilities by 2^-8.
-    most = 2 ** -8 * (2 * 600 * SCALE + 3)
+    # Keys rounded to 2^-11 move a logit by at most 2^-11 scale sum |q k| (sum |q k| < 600 here, as 576 E|q k| is 367);
+    # probabilities by twice that, values by 2^-11, this side's probabilities by 2^-11, the tree's by 2^-8.
+    most = 2 ** -11 * (2 * 600 * SCALE + 3) + 2 ** -8
     key = [prompt.features(step.rows[[step.slot(i, p) for p in range(step.lens[i])]])[1] for i in range(3)]
     size = max(float(np.abs(k).max()) for k in key)
     assert float((a - b).abs().max()) <= most * size
@@ -214,6 +214,37 @@ def test_chunk_attention_hidden_rows_hold_anything(torch_gpu, heads):
     assert int(op.status.item()) == 0
 
 
+@pytest.mark.parametrize("heads,counts,contexts", [(16, [70, 9], [100, 700]), (4, [40, 300], [0, 33])])
+def test_chunk_attention_of_rows_of_other_sizes(torch_gpu, heads, counts, contexts):
+    """Rows of a tile that are many orders of magnitude apart, those that a token sees and those that it does not, rows of
+    zeros among them, and whole tiles that are larger or smaller than the others."""
+    torch = torch_gpu
+    say(f"case chunk sizes heads={heads}")
+    rng = np.random.default_rng(heads)
+    step = Chunks(torch, rng, counts, contexts, heads)
+    scales = step.rows[:, 640:656].copy().view("<f4")
+    for b, n in enumerate(counts):
+        for p in range(step.lens[b]):
+            at = step.slot(b, p)
+            scales[at] *= 2.0 ** float(rng.integers(-30, 1) if p % 100 < 50 else -(p // 32 % 5) * 8)
+            if p % 19 == 3:
+                step.rows[at, :640] = 0
+        for p in range(step.lens[b] - 5, step.lens[b]):
+            scales[step.slot(b, p)] = 2.0 ** 60  # the last few: huge
+    step.rows[:, 640:656] = scales.astype("<f4").view(np.uint8)
+    op = step.run(output="fp32")
+    got, q = host(op()), step.query.double().numpy()
+    for b, n in enumerate(counts):
+        key, value, odd = prompt.features(step.rows[[step.slot(b, p) for p in range(step.lens[b])]])
+        assert not odd.any()
+        for i in sorted({0, 1, 7, n // 2, n - 7, n - 6}):
+            row, sees = step.cu[b] + i, step.lens[b] - n + i + 1
+            want, _, bound, _ = prompt.attention(q[row], key[:sees], value[:sees], SCALE)
+            # The probabilities' floor, under the largest exponent that a token has seen: 2^-29 of the largest value.
+            floor = 2.0 ** -28 * sees * np.abs(value[:sees]).max()
+            assert np.all(np.abs(got[row] - want) <= bound + np.abs(want) * 2.0 ** -24 + floor), (b, i)
+
+
 def test_chunk_attention_bad_tables_and_lengths(torch_gpu):
     torch = torch_gpu
     say("case chunk bad tables")
@@ -224,7 +255,7 @@ def test_chunk_attention_bad_tables_and_lengths(torch_gpu):
     assert int(op.status.item()) == abi.STATUS_BAD_BLOCK
     q, got = step.query.double().numpy(), host(op.output)
     there = [p for p in range(510) if p // 128 not in (1, 2)]
-    key, value, _ = prompt.features(step.rows[[step.slot(0, p) for p in there]])
+    key, value, _ = prompt.features(step.rows[[step.slot(0, p) for p in there]], there)
     for i in (0, 39):
         n = sum(p <= 470 + i for p in there)
         want, _, bound, _ = prompt.attention(q[i], key[:n], value[:n], SCALE)
@@ -239,7 +270,7 @@ def test_chunk_attention_bad_tables_and_lengths(torch_gpu):
     assert int(op.status.item()) == abi.STATUS_BAD_LENGTH
     assert not op.output[2].any() and bool((op.lse[2] == -math.inf).all())  # comes before the only row
     key, value, _ = prompt.features(step.rows[[step.slot(1, 0)]])
-    assert np.all(np.abs(host(op.output[3]) - value) <= np.abs(value) * 2 * 2.0 ** -8)
+    assert np.all(np.abs(host(op.output[3]) - value) <= np.abs(value) * (2.0 ** -8 + 2.0 ** -10))
     assert not op.output[4:7].any()
     # cu_seqlens that fall and leave the rows.
     step = Chunks(torch, np.random.default_rng(12), [20, 30, 5], [100, 60, 7], 4)

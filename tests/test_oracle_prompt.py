@@ -8,9 +8,19 @@ import pytest
 from oracle import draft, prompt
 
 
-def test_bf16_rounds_to_the_nearest():
-    x = np.asarray([1.0, 1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8, 1 + 2.0 ** -7, -1 - 2.0 ** -9, 0.0, 3.4e38, np.inf], np.float32)
-    assert prompt.to_bf16(x).tolist() == [1.0, 1.0, 1 + 2.0 ** -6, 1 + 2.0 ** -7, -1.0, 0.0, np.inf, np.inf]
+def test_features_round_to_eleven_bits():
+    rows = np.zeros((40, 656), np.uint8)
+    rows[:, 640:656] = np.asarray([1, 1, 1, 1], "<f4").view(np.uint8)
+    rows[0, 640:644] = np.asarray([1 + 2.0 ** -11 + 2.0 ** -20], "<f4").view(np.uint8)  # rounds up
+    rows[1, 640:644] = np.asarray([1 + 2.0 ** -11], "<f4").view(np.uint8)               # halves to the even step
+    rows[:, :512] = draft.e4m3_bytes(np.ones((40, 512), np.float32))
+    rows[35, 640:644] = np.asarray([3e38], "<f4").view(np.uint8)                        # another tile's exponent
+    rows[36, 0:1] = draft.e4m3_bytes(np.asarray([2.0 ** -9], np.float32))
+    key, value, odd = prompt.features(rows)
+    assert value[0, 0] == 1 + 2.0 ** -10 and value[1, 0] == 1.0 and value[2, 0] == 1.0 and not odd.any()
+    assert value[35, 0] == float(np.float32(3e38).astype(np.float64)) or abs(value[35, 0] / 3e38 - 1) <= 2.0 ** -11
+    assert value[36, 0] == 0.0 and value[36, 200] == 0.0  # far below the largest of their 32 rows
+    assert np.array_equal(key[:, :512], value) and np.array_equal(prompt.features(rows[:32])[1], value[:32])
 
 
 def test_attention_over_equal_logits_is_the_mean():
