@@ -71,10 +71,10 @@ struct ChunkPlan {
     int cut;                                  // tiles of a segment
     int cut_tiles;                            // row tiles, where they are cut; else 0
     int reserved;
-    int request[KVIP_DRAFT_MAX_BATCH];           // in the order of the work
-    int units_before[KVIP_DRAFT_MAX_BATCH + 1];  // in that order
-    int tiles_before[KVIP_DRAFT_MAX_BATCH + 1];  // row tiles, in that order
-    int images_before[KVIP_DRAFT_MAX_BATCH];     // of request b, -1: none
+    // In the order of the work, the longest contexts first:
+    int units_before[KVIP_DRAFT_MAX_BATCH + 1];
+    int tiles_before[KVIP_DRAFT_MAX_BATCH + 1];  // row tiles
+    int4 request[KVIP_DRAFT_MAX_BATCH];          // first token, tokens, cached rows, first image (-1: none)
 };
 
 // Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, exponent and
@@ -199,7 +199,10 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
                 const int other = s_before[i + 1] - s_before[i];
                 rank += other > steps_b || (other == steps_b && i < b);
             }
-            plan->request[rank] = b;
+            // No images: none that would fit.
+            const bool fits = s_before[b + 1] <= most;
+            plan->request[rank] = make_int4(q.begin, q.tokens, q.length, fits ? s_before[b] : -1);
+            if (!fits && steps_b > 0) err |= KVIP_STATUS_BAD_LENGTH;
             s_steps[rank] = steps_b;
             s_tiles[rank] = ca_row_tiles(q, p.heads);
             atomicMax(&s_longest, steps_b);
@@ -244,11 +247,6 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
             plan->tiles_before[r] = tiles_before;
             units_before += s_tiles[r] * max((s_steps[r] + cut - 1) / cut, 1);
             tiles_before += s_tiles[r];
-            // No images: none that would fit.
-            const int b = r;
-            const bool fits = s_before[b + 1] <= most;
-            plan->images_before[b] = fits ? s_before[b] : -1;
-            if (!fits && s_before[b + 1] > s_before[b]) err |= KVIP_STATUS_BAD_LENGTH;
         }
         if (tid == 0) {
             plan->units = total_units;
@@ -398,25 +396,48 @@ KVIP_DEVICE void for_all(F&& f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>{}), ...);
 }
 
-// A unit of the plan: request b, row tile rt, segment seg.
+// What a workgroup has of the plan: unit `at` (row tiles and their segments) or, for the join, row tile `at`. All of it is
+// loaded at once, by the thread that finds it.
 struct ChunkUnit {
-    int b, rt, seg;
+    ChunkRequest q;
+    int image0;     // -1: the request has none
+    int rt, seg;
+    int unit0;      // of the row tile's segment 0
+    int segs;
+    int cut;
 };
-KVIP_DEVICE bool ca_unit(const ChunkPlan* plan, int batch, int unit, int* s_found, ChunkUnit* u) {
-    if (unit >= plan->units) return false;
-    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
-        if (plan->units_before[b] <= unit && unit < plan->units_before[b + 1]) {
-            const int tiles = plan->tiles_before[b + 1] - plan->tiles_before[b];
-            const int segs = (plan->units_before[b + 1] - plan->units_before[b]) / tiles, at = unit - plan->units_before[b];
-            s_found[0] = plan->request[b];
-            s_found[1] = tiles - 1 - at / segs;  // the tiles that see most first
-            s_found[2] = at % segs;
+KVIP_DEVICE bool ca_unit(const ChunkPlan* plan, int batch, int at, bool of_join, int* s_found, ChunkUnit* u) {
+    const int4 head = *reinterpret_cast<const int4*>(plan);
+    for (int r = threadIdx.x; r < batch; r += blockDim.x) {
+        const int units0 = plan->units_before[r], units1 = plan->units_before[r + 1];
+        const int tiles0 = plan->tiles_before[r], tiles1 = plan->tiles_before[r + 1];
+        const int4 request = plan->request[r];
+        const int first = of_join ? tiles0 : units0, behind = of_join ? tiles1 : units1;
+        if (first <= at && at < behind) {
+            const int tiles = tiles1 - tiles0, segs = (units1 - units0) / tiles;
+            const int tile = of_join ? tiles - 1 - (at - tiles0) : (at - units0) / segs;  // in the order of the units
+            s_found[0] = request.x;
+            s_found[1] = request.y;
+            s_found[2] = request.z;
+            s_found[3] = request.w;
+            s_found[4] = tiles - 1 - tile;  // the tiles that see most first
+            s_found[5] = (at - units0) % segs;
+            s_found[6] = units0 + tile * segs;
+            s_found[7] = segs;
         }
     }
+    if (at >= (of_join ? head.z : head.x)) return false;
     __syncthreads();
-    u->b = __builtin_amdgcn_readfirstlane(s_found[0]);
-    u->rt = __builtin_amdgcn_readfirstlane(s_found[1]);
-    u->seg = __builtin_amdgcn_readfirstlane(s_found[2]);
+    auto found = [&](int i) { return __builtin_amdgcn_readfirstlane(s_found[i]); };
+    u->q.begin = found(0);
+    u->q.tokens = found(1);
+    u->q.length = found(2);
+    u->image0 = found(3);
+    u->rt = found(4);
+    u->seg = found(5);
+    u->unit0 = found(6);
+    u->segs = found(7);
+    u->cut = __builtin_amdgcn_readfirstlane(head.y);
     return true;
 }
 
@@ -429,16 +450,14 @@ KVIP_DEVICE int ca_reach(const ChunkRequest& q, int rt, int heads) {
 
 __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const KvipChunkAttnArgs p) {
     __shared__ __align__(1024) uint8_t s_ring[kCaSlots * kCaImage];
-    __shared__ int s_found[4];
+    __shared__ int s_found[8];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const ChunkWork work = ca_work(p.workspace, ca_images(p.max_rows, p.batch), nullptr);
     ChunkUnit unit;
-    if (!ca_unit(work.plan, p.batch, blockIdx.x, s_found, &unit)) return;
-    uint32_t none = 0;
-    const ChunkRequest q = ca_request(p, unit.b, &none);
-    const int image0 = __builtin_amdgcn_readfirstlane(work.plan->images_before[unit.b]);
-    const int cut = __builtin_amdgcn_readfirstlane(work.plan->cut);
+    if (!ca_unit(work.plan, p.batch, blockIdx.x, false, s_found, &unit)) return;
+    const ChunkRequest& q = unit.q;
+    const int image0 = unit.image0, cut = unit.cut;
     const int rows = q.tokens * p.heads, first_row = unit.rt * kCaTileRows + w * kCaRows;
     const int reach = image0 < 0 ? 0 : ca_reach(q, unit.rt, p.heads);
     const int t0 = unit.seg * cut, t1 = min(t0 + cut, reach);
@@ -768,27 +787,16 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
 
 // Joins the parts of row tiles that were cut. A workgroup takes one wave's 32 rows and a quarter of the features.
 __global__ __launch_bounds__(kCaThreads) void chunk_join_kernel(const KvipChunkAttnArgs p) {
-    __shared__ int s_found[4];
+    __shared__ int s_found[8];
     const ChunkWork work = ca_work(p.workspace, ca_images(p.max_rows, p.batch), nullptr);
-    const ChunkPlan* plan = work.plan;
-    const int slice = blockIdx.x % 4, rg = blockIdx.x / 4 % kCaWaves, tile = blockIdx.x / 4 / kCaWaves;
-    if (tile >= plan->cut_tiles) return;
-    for (int b = threadIdx.x; b < p.batch; b += kCaThreads) {
-        const int first = plan->tiles_before[b], behind = plan->tiles_before[b + 1];
-        if (first <= tile && tile < behind) {
-            s_found[0] = plan->request[b];
-            s_found[1] = tile - first;
-            s_found[2] = (plan->units_before[b + 1] - plan->units_before[b]) / (behind - first);
-            s_found[3] = plan->units_before[b] + (behind - 1 - tile) * s_found[2];
-        }
-    }
-    __syncthreads();
-    const int b = s_found[0], rt = s_found[1], unit = s_found[3], cut = plan->cut;
-    uint32_t none = 0;
-    const ChunkRequest q = ca_request(p, b, &none);
-    const int reach = plan->images_before[b] < 0 ? 0 : ca_reach(q, rt, p.heads);
+    const int slice = blockIdx.x % 4, rg = blockIdx.x / 4 % kCaWaves;
+    ChunkUnit u;
+    if (!ca_unit(work.plan, p.batch, blockIdx.x / 4 / kCaWaves, true, s_found, &u)) return;
+    const ChunkRequest& q = u.q;
+    const int rt = u.rt, unit = u.unit0, cut = u.cut;
+    const int reach = u.image0 < 0 ? 0 : ca_reach(q, rt, p.heads);
     if (reach <= cut) return;  // whole
-    const int parts = min((reach + cut - 1) / cut, s_found[2]);
+    const int parts = min((reach + cut - 1) / cut, u.segs);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hn = lane & 31;
     const int row = rt * kCaTileRows + rg * kCaRows + hn, rows = q.tokens * p.heads;
     const float2* states = work.states + static_cast<int64_t>(unit) * kCaTileRows + rg * kCaRows + hn;
