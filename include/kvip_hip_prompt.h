@@ -35,8 +35,9 @@ extern "C" {
  * over the rows it sees (0 where it sees none), lse = log sum_j exp(s_j) (-infinity).
  * Features times their scales (products in 32 bits) are rounded once to fp16 under an exponent that the rows of 32
  * positions share, their largest feature being 2^14 .. 2^15 there: by 2^-11 of themselves, or 2^-39 of that largest;
- * query features likewise, which only those below 2^-28 of the largest of their (token, head) feel; probabilities by
- * 2^-11 of themselves, or 2^-29 of the largest's. The rest is in 32 bits.
+ * rows whose largest features are more than 2^12 apart stand under exponents of their own; query features likewise, which
+ * only those below 2^-28 of the largest of their (token, head) feel; probabilities by 2^-11 of themselves, or, for an
+ * output, by 2^-36 of the largest feature that the token sees. The rest is in 32 bits.
  * Rows that a token does not see do not reach its output, whatever they hold; a token that sees a row with
  * a value that is no finite 32-bit number becomes NaN as a whole (a rotary feature that is not finite reaches the
  * logits as it is). Blocks outside the cache set KVIP_STATUS_BAD_BLOCK and

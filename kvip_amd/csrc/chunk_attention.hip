@@ -53,11 +53,11 @@ constexpr int kCaPartSteps = 10;                  // what storing and joining a 
 constexpr int kCaCus = 256;
 constexpr float kCaLog2e = 1.44269504088896341f;
 constexpr float kCaLn2 = 0.693147180559945309f;
-constexpr float kCaMargin = 8.0f * kCaLog2e;
+constexpr float kCaMargin = 3.0f * kCaLog2e;
 constexpr int kCaTop = 14;                        // exponent of the largest feature in an image, and of a row's largest query
 constexpr int kCaSpread = 12;                     // rows of a tile whose exponents differ by more keep their own
 constexpr int kCaSoftmax = 19;                    // pieces of a tile's softmax
-constexpr int kCaLift = 4;                        // exponent that probabilities are lifted by: 2^(kCaMargin + kCaLift) fits fp16
+constexpr int kCaLift = 11;                       // exponent that probabilities are lifted by: 2^(kCaMargin + kCaLift) fits fp16
 static_assert(kCaLoads * 1024 * kCaWaves == kCaImage, "whole loads");
 static_assert(kCaSlots * kCaImage <= 160 * 1024, "LDS of a CU");
 

@@ -50,7 +50,7 @@ def features(rows, positions=None):
 def attention(query, key, value, scale):
     """query [heads, 576] of one token over the rows it sees. Returns (output [heads, 512], lse [heads], bound
     [heads, 512], lse bound [heads]): the bounds hold for probabilities rounded to fp16 (2^-11; the smallest, of tiles whose
-    exponent is up to 2 below others', 2^-27 of the maximum's), dot products of 576 terms, exponentials and sums of n
+    exponent is up to 2 below others', 2^-34 of the maximum's), dot products of 576 terms, exponentials and sums of n
     terms in 32 bits."""
     q, n = np.asarray(query, np.float64), len(key)
     if n == 0:
@@ -63,7 +63,7 @@ def attention(query, key, value, scale):
     p /= whole
     slip = abs(scale) * (np.abs(q) @ np.abs(key).T).max(1) * (576 + 8) * FP32 + np.abs(logits).max(1) * 8 * FP32
     sums = n * 2 * FP32 + 16 * FP32
-    bound = (p @ np.abs(value)) * (FP16 + 2 * slip + sums)[:, None] + 2.0 ** -27 * np.abs(value).sum(0) / whole
+    bound = (p @ np.abs(value)) * (FP16 + 2 * slip + sums)[:, None] + 2.0 ** -34 * np.abs(value).sum(0) / whole
     return p @ value, top[:, 0] + np.log(whole[:, 0]), bound, slip + sums + np.abs(top[:, 0]) * 4 * FP32
 
 

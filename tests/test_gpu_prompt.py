@@ -240,8 +240,9 @@ def test_chunk_attention_of_rows_of_other_sizes(torch_gpu, heads, counts, contex
         for i in sorted({0, 1, 7, n // 2, n - 7, n - 6}):
             row, sees = step.cu[b] + i, step.lens[b] - n + i + 1
             want, _, bound, _ = prompt.attention(q[row], key[:sees], value[:sees], SCALE)
-            # The probabilities' floor, under the largest exponent that a token has seen: 2^-29 of the largest value.
-            floor = 2.0 ** -28 * sees * np.abs(value[:sees]).max()
+            # The probabilities' floor, under the largest exponent that a token has seen: 2^-36 of the largest value, as the
+            # kernel's reference may be below the largest logit only, which raises them.
+            floor = 2.0 ** -36 * sees * np.abs(value[:sees]).max()
             assert np.all(np.abs(got[row] - want) <= bound + np.abs(want) * 2.0 ** -24 + floor), (b, i)
 
 
