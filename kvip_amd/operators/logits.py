@@ -31,7 +31,8 @@ class TokenHistory:
         self.seen = torch.zeros((batch, (vocab + 31) // 32), dtype=torch.int32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         p = abi.ptr
-        self._state = dict(counts=p(self.counts), seen=p(self.seen), status=p(self.status), batch=self.batch, vocab=self.vocab)
+        self._args = abi.HistoryArgs(counts=p(self.counts), seen=p(self.seen), status=p(self.status), batch=self.batch,
+                                     vocab=self.vocab)
 
     def _check(self, x, dtype, shape, what):
         abi.require(x.dtype == dtype and tuple(x.shape) == shape and x.is_contiguous() and x.device == self.device,
@@ -46,13 +47,14 @@ class TokenHistory:
         n = int(requests.shape[0]) if requests.dim() == 1 else 0
         abi.require(1 <= n <= abi.DRAFT_MAX_BATCH, f"requests must be int32 [1..{abi.DRAFT_MAX_BATCH}]")
         abi.require(tokens.dim() == 1 and tokens.shape[0] <= 0x7FFFFFFF, "tokens must be int64 [up to 2^31 - 1]")
+        a = self._args  # copied by the launch
+        a.requests, a.count = self._check(requests, t.int32, (n,), "requests"), n
+        a.cu_seqlens = self._check(cu_seqlens, t.int32, (n + 1,), "cu_seqlens")
+        a.prompt_lens = self._check(prompt_lens, t.int32, (n,), "prompt_lens")
+        a.max_tokens = int(tokens.shape[0])
         # Without tokens nothing is read: any address that is not null.
-        args = abi.HistoryArgs(
-            **self._state, requests=self._check(requests, t.int32, (n,), "requests"),
-            tokens=self._check(tokens, t.int64, tuple(tokens.shape), "tokens") or abi.ptr(self.counts),
-            cu_seqlens=self._check(cu_seqlens, t.int32, (n + 1,), "cu_seqlens"),
-            prompt_lens=self._check(prompt_lens, t.int32, (n,), "prompt_lens"), max_tokens=int(tokens.shape[0]), count=n)
-        abi.launch(t, self.device, self.library.kvip_hip_history_load, args, "token history")
+        a.tokens = self._check(tokens, t.int64, (a.max_tokens,), "tokens") or a.counts
+        abi.launch(t, self.device, self.library.kvip_hip_history_load, a, "token history")
         return self.counts
 
     def append(self, tokens, kept):
@@ -61,9 +63,10 @@ class TokenHistory:
         t = self.torch
         places = int(tokens.shape[1]) if tokens.dim() == 2 else 0
         abi.require(1 <= places <= abi.DRAFT_MAX_NODES, f"tokens must be int64 [{self.batch}, 1..{abi.DRAFT_MAX_NODES}]")
-        args = abi.HistoryArgs(**self._state, tokens=self._check(tokens, t.int64, (self.batch, places), "tokens"),
-                               kept=self._check(kept, t.int32, (self.batch,), "kept"), token_stride=places)
-        abi.launch(t, self.device, self.library.kvip_hip_history_append, args, "token history")
+        a = self._args  # copied by the launch
+        a.tokens, a.token_stride = self._check(tokens, t.int64, (self.batch, places), "tokens"), places
+        a.kept = self._check(kept, t.int32, (self.batch,), "kept")
+        abi.launch(t, self.device, self.library.kvip_hip_history_append, a, "token history")
         return self.counts
 
 
