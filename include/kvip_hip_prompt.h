@@ -34,7 +34,7 @@ extern "C" {
  *   output = sum_j p_j value_j / sum_j p_j, p_j = exp(s_j - max s), s_j = scale <query, key_j>
  * over the rows it sees (0 where it sees none), lse = log sum_j exp(s_j) (-infinity).
  * Features times their scales (products in 32 bits) are rounded once to fp16 under an exponent that the rows of 32
- * positions share, their largest feature being 2^14 .. 2^15 there: by 2^-11 of themselves, or 2^-39 of that largest;
+ * positions share, their largest feature being 2^11 .. 2^15 there: by 2^-11 of themselves, or 2^-36 of that largest;
  * rows whose largest features are more than 2^12 apart stand under exponents of their own; query features likewise, which
  * only those below 2^-28 of the largest of their (token, head) feel; probabilities by 2^-11 of themselves, or, for an
  * output, by 2^-36 of the largest feature that the token sees. The rest is in 32 bits.

@@ -77,8 +77,8 @@ struct ChunkPlan {
     int4 request[KVIP_DRAFT_MAX_BATCH];          // first token, tokens, cached rows, first image (-1: none)
 };
 
-// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, exponent and
-// whether its rows have their own) and the rows' exponents, then the images, then the parts: 32 rows x 512 sums per wave as its lanes hold them ([block][quarter][lane] 16 bytes),
+// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, code: four times the
+// exponent, plus 2 where there are such rows, plus 1 where its rows have exponents of their own) and the rows' exponents, then the images, then the parts: 32 rows x 512 sums per wave as its lanes hold them ([block][quarter][lane] 16 bytes),
 // then their (maximum, sum) pairs.
 struct ChunkWork {
     ChunkPlan* plan;
@@ -140,8 +140,10 @@ KVIP_DEVICE uint32_t ca_pack_half(float a, float b) {
     const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
     return __builtin_bit_cast(uint32_t, v);
 }
-// Exponent that takes the largest magnitude (of bits `most`, below infinity's) to 2^kCaTop .. 2^(kCaTop + 1).
+// Exponent that takes the largest magnitude (of bits `most`, below infinity's) to 2^kCaTop .. 2^(kCaTop + 1); for images
+// the next multiple of 4, so that most tiles have the same.
 KVIP_DEVICE int ca_exponent(uint32_t most) { return static_cast<int>(most >> 23) - 127 - kCaTop; }
+KVIP_DEVICE int ca_image_exponent(uint32_t most) { return (ca_exponent(most) + 3) & ~3; }
 
 // Plan and images. Every workgroup sums the requests' tiles for itself; the first one leaves the plan, the others take
 // images in turn. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8 rotary features.
@@ -332,9 +334,9 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
         }
         // One exponent for all rows, unless that would cost the smaller ones their bits: what a token sees must not
         // depend on rows that it does not.
-        const int tile_exponent = ca_exponent(flags.z);
-        const bool spread = flags.z != 0 && tile_exponent - ca_exponent(flags.w) > kCaSpread;
-        const int exponent = !spread ? tile_exponent : most_row > 0.f ? ca_exponent(__float_as_uint(most_row)) : -200;
+        const int tile_exponent = ca_image_exponent(flags.z);
+        const bool spread = flags.z != 0 && tile_exponent - ca_image_exponent(flags.w) > kCaSpread;
+        const int exponent = !spread ? tile_exponent : most_row > 0.f ? ca_image_exponent(__float_as_uint(most_row)) : -200;
         if (spread && piece == 0) work.exponents[static_cast<int64_t>(image) * kCaTile + t] = static_cast<int16_t>(exponent);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
         v4i* to = reinterpret_cast<v4i*>(work.images + static_cast<int64_t>(image) * kCaImage);
 #pragma unroll
         for (int i = 0; i < kCaImage / 16 / kCaThreads; ++i) to[tid + i * kCaThreads] = *reinterpret_cast<const v4i*>(s_image + 16 * (tid + i * kCaThreads));
-        if (tid == 0) work.flags[image] = make_uint4(flags.x, flags.y, static_cast<uint32_t>(tile_exponent * 2 + (spread ? 1 : 0)), 0);
+        if (tid == 0) work.flags[image] = make_uint4(flags.x, flags.y, static_cast<uint32_t>(tile_exponent * 4 + ((flags.x | flags.y) != 0 ? 2 : 0) + (spread ? 1 : 0)), 0);
     }
 }
 
@@ -534,25 +536,10 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     v16f s;
     v4i pb[2];  // probabilities of the tile whose values come next
 
-    // The flags of 64 tiles, which the lanes hold.
+    // The codes of 64 tiles, which the lanes hold.
     int held_first = t0;
-    uint4 held = work.flags[image0 + min(t0 + lane, reach - 1)];
-    asm volatile("" : "+v"(held.x), "+v"(held.y), "+v"(held.z));
-    struct Flags {
-        uint32_t odd, gone;
-        int exponent;
-        bool spread;
-    };
-    auto flags_of = [&](int t) {
-        if (t >= held_first + 64) {
-            held_first = t;
-            held = work.flags[image0 + min(t + lane, reach - 1)];
-            asm volatile("" : "+v"(held.x), "+v"(held.y), "+v"(held.z));  // waited for here, not at every use
-        }
-        const int at = t - held_first, last = __builtin_amdgcn_readlane(static_cast<int>(held.z), at);
-        return Flags{static_cast<uint32_t>(__builtin_amdgcn_readlane(held.x, at)), static_cast<uint32_t>(__builtin_amdgcn_readlane(held.y, at)),
-                     last >> 1, (last & 1) != 0};
-    };
+    int held = static_cast<int>(work.flags[image0 + min(t0 + lane, reach - 1)].z);
+    asm volatile("" : "+v"(held));
 
     // Operands are read from LDS kAhead products before their use, across the borders of logits and values too.
     constexpr int kAhead = 4;
@@ -585,12 +572,18 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     auto row_exponent = [&](int t, int i) {
         return static_cast<int>(work.exponents[static_cast<int64_t>(image0 + t) * kCaTile + 8 * (i >> 2) + 4 * hk + (i & 3)]);
     };
-    Flags flags;
-    int of_tile;
+    int of_tile, tile_exponent, calm = 0x7FFFFFFF;  // calm: the exponent that leaves these as they are
+    bool special;
     auto look = [&](int t) {  // does not need the logits
-        flags = flags_of(t);
-        of_tile = flags.exponent;
-        spread = flags.spread;
+        if (t >= held_first + 64) {
+            held_first = t;
+            held = static_cast<int>(work.flags[image0 + min(t + lane, reach - 1)].z);
+            asm volatile("" : "+v"(held));  // waited for here, not at every use
+        }
+        const int code = __builtin_amdgcn_readlane(held, t - held_first);
+        tile_exponent = code >> 2;
+        spread = (code & 1) != 0;
+        special = (code & 3) != 0 || t >= t_mask;
     };
     // Logits of a tile, whose first operands are under way; the loads that are aimed at stand between the products, the
     // first value operands of the tile at `next` behind them.
@@ -612,11 +605,13 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     };
     static_assert(kCaLoads * 4 == kCaFrags, "a load every four products");
     auto mask = [&](int t) {
-        if (t >= t_mask || flags.odd != 0 || flags.gone != 0 || spread) {
+        of_tile = tile_exponent;
+        if (special) {
+            const uint4 flags = work.flags[image0 + t];
             const int left = sees - t * kCaTile;
             uint32_t seen = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-            seen &= ~flags.gone;
-            if (seen & flags.odd) l_sum = NAN;
+            seen &= ~flags.y;
+            if (seen & flags.x) l_sum = NAN;
             if (seen == 0) of_tile = exponent;
             seen >>= 4 * hk;
             if (spread) {
@@ -641,12 +636,14 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     bool raise;
     auto softmax = [&](int piece) {
         if (piece == 0) {
-            shift = max(of_tile - exponent, 0);
-            exponent += shift;
-            lower = max(of_tile - exponent, -100);
-            // A scale so small that the logits vanish still leaves a number, which what is masked stays below.
-            factor = fmaxf(ldexpf(scale2, q_exponent + of_tile), 0x1p-126f);
-            asm volatile("" : "+v"(factor), "+v"(lower));
+            if (special || tile_exponent != calm) {
+                shift = max(of_tile - exponent, 0);
+                exponent += shift;
+                lower = max(of_tile - exponent, -100);
+                // A scale so small that the logits vanish still leaves a number, which what is masked stays below.
+                factor = fmaxf(ldexpf(scale2, q_exponent + of_tile), 0x1p-126f);
+                calm = !spread && __ballot(shift != 0 || lower != 0 || of_tile != tile_exponent) == 0ull ? tile_exponent : 0x7FFFFFFF;
+            }
         } else if (piece == 1) {
             mx = s[0];
 #pragma unroll
@@ -658,12 +655,23 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
             const float m_new = raise ? mx : m_run;
             alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : raise ? 0.f : 1.f;
             m_run = m_new;
-            bias = (m_new == -INFINITY ? 0.f : -m_new) + static_cast<float>(kCaLift + lower);
-            asm volatile("" : "+v"(bias));
+            const float lift = static_cast<float>(kCaLift + lower);
+            bias = (m_new == -INFINITY ? 0.f : -m_new) + lift;
+            if (__ballot(fabsf(m_new) > 0x1p20f && m_new != -INFINITY) != 0ull) {
+                // Logits whose rounding a fused product would show: the difference from the maximum, rounded as that was.
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[i] * factor;
+                    asm volatile("" : "+v"(x));
+                    s[i] = m_new == -INFINITY ? x : x - m_new;
+                }
+                factor = 1.f;
+                bias = lift;
+                calm = 0x7FFFFFFF;
+            }
+            asm volatile("" : "+v"(bias), "+v"(factor));
         } else {
-            float p1 = s[piece - 3] * factor;  // rounded as the maximum was, however large the logits are
-            asm volatile("" : "+v"(p1));
-            p1 = __builtin_amdgcn_exp2f(p1 + bias);
+            float p1 = __builtin_amdgcn_exp2f(fmaf(s[piece - 3], factor, bias));
             fresh_sum += p1;
             asm volatile("" : "+v"(p1), "+v"(fresh_sum));  // here, not behind the products
             s[piece - 3] = p1;

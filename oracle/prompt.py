@@ -27,8 +27,8 @@ FP16 = 2.0 ** -11
 def features(rows, positions=None):
     """rows uint8 [n, >= 656] of one request, at positions 0, 1, ... or as given -> (key [n, 576], value [n, 512], odd [n]: a
     value is no finite number). Products in 32 bits, rounded to fp16 under the exponent that takes the largest finite
-    feature of the 32 positions' rows (those that are odd left out) to 2^14 .. 2^15, or, where the rows' own exponents
-    differ by more than 12, each under its own."""
+    feature of the 32 positions' rows (those that are odd left out) to 2^11 .. 2^15 (a multiple of 4), or, where the rows'
+    own exponents differ by more than 12, each under its own."""
     positions = np.arange(len(rows)) if positions is None else np.asarray(positions)
     with np.errstate(over="ignore", invalid="ignore"):
         nope, rope, scales = draft.row_parts(rows)
@@ -39,7 +39,7 @@ def features(rows, positions=None):
         for tile in np.unique(positions // 32):
             at = np.flatnonzero(positions // 32 == tile)
             sizes = np.abs(np.where(np.isfinite(key[at]), key[at], 0)).max(1)
-            exponents = np.where(sizes >= 2.0 ** -126, np.frexp(sizes)[1] - 1, -127) - 14
+            exponents = -(-(np.where(sizes >= 2.0 ** -126, np.frexp(sizes)[1] - 1, -127) - 14) // 4) * 4
             if np.any(sizes > 0) and exponents.max() - exponents[sizes > 0].min() <= 12:
                 exponents[:] = exponents.max()
             for i, exponent in zip(at, exponents):
@@ -50,7 +50,7 @@ def features(rows, positions=None):
 def attention(query, key, value, scale):
     """query [heads, 576] of one token over the rows it sees. Returns (output [heads, 512], lse [heads], bound
     [heads, 512], lse bound [heads]): the bounds hold for probabilities rounded to fp16 (2^-11; the smallest, of tiles whose
-    exponent is up to 2 below others', 2^-34 of the maximum's), dot products of 576 terms, exponentials and sums of n
+    exponent is 4 below others', 2^-31 of the maximum's), dot products of 576 terms, exponentials and sums of n
     terms in 32 bits."""
     q, n = np.asarray(query, np.float64), len(key)
     if n == 0:
@@ -63,7 +63,7 @@ def attention(query, key, value, scale):
     p /= whole
     slip = abs(scale) * (np.abs(q) @ np.abs(key).T).max(1) * (576 + 8) * FP32 + np.abs(logits).max(1) * 8 * FP32
     sums = n * 2 * FP32 + 16 * FP32
-    bound = (p @ np.abs(value)) * (FP16 + 2 * slip + sums)[:, None] + 2.0 ** -34 * np.abs(value).sum(0) / whole
+    bound = (p @ np.abs(value)) * (FP16 + 2 * slip + sums)[:, None] + 2.0 ** -31 * np.abs(value).sum(0) / whole
     return p @ value, top[:, 0] + np.log(whole[:, 0]), bound, slip + sums + np.abs(top[:, 0]) * 4 * FP32
 
 

@@ -14,12 +14,15 @@ def test_features_round_to_eleven_bits():
     rows[0, 640:644] = np.asarray([1 + 2.0 ** -11 + 2.0 ** -20], "<f4").view(np.uint8)  # rounds up
     rows[1, 640:644] = np.asarray([1 + 2.0 ** -11], "<f4").view(np.uint8)               # halves to the even step
     rows[:, :512] = draft.e4m3_bytes(np.ones((40, 512), np.float32))
-    rows[35, 640:644] = np.asarray([3e38], "<f4").view(np.uint8)                        # another tile's exponent
+    rows[35, 640:644] = np.asarray([3e38], "<f4").view(np.uint8)  # its tile's rows keep exponents of their own
     rows[36, 0:1] = draft.e4m3_bytes(np.asarray([2.0 ** -9], np.float32))
+    rows[3, 640:656] = np.asarray([2.0 ** -9] * 4, "<f4").view(np.uint8)  # one exponent
+    rows[3, 0:1] = draft.e4m3_bytes(np.asarray([2.0 ** -9], np.float32))
+    rows[3, 512:514] = np.asarray([0x3F81], "<u2").view(np.uint8)  # bf16 1 + 2^-7
     key, value, odd = prompt.features(rows)
     assert value[0, 0] == 1 + 2.0 ** -10 and value[1, 0] == 1.0 and value[2, 0] == 1.0 and not odd.any()
-    assert value[35, 0] == float(np.float32(3e38).astype(np.float64)) or abs(value[35, 0] / 3e38 - 1) <= 2.0 ** -11
-    assert value[36, 0] == 0.0 and value[36, 200] == 0.0  # far below the largest of their 32 rows
+    assert abs(value[35, 0] / 3e38 - 1) <= 2.0 ** -11 and value[36, 0] == 2.0 ** -9 and value[36, 200] == 1.0
+    assert value[3, 0] == 2.0 ** -18 and value[3, 1] == 2.0 ** -9 and key[3, 512] == 1 + 2.0 ** -7
     assert np.array_equal(key[:, :512], value) and np.array_equal(prompt.features(rows[:32])[1], value[:32])
 
 
