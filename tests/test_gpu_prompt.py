@@ -162,8 +162,35 @@ def test_chunk_attention_options(torch_gpu):
             device(torch, step.lens, torch.int32), device(torch, step.cu, torch.int32))
     again = kvip_amd.chunk_attention(*args, scale=0.11, output_dtype=torch.float32)
     assert torch.equal(again[:92], op.output[:92])
-    for scale in (-0.05, 0.0, 1e-30):
+    for scale in (-0.05, 0.0, 1e-30, 3e6):
         step.check(step.run(scale=scale), scale=scale, every=23)
+
+
+@pytest.mark.parametrize("heads,counts,contexts", [(16, [40], [500]), (16, [9, 60], [9000, 0])])
+def test_chunk_attention_of_huge_logits(torch_gpu, heads, counts, contexts):
+    """Logits of 10^7 and more: all weight is on the largest, and nothing overflows on the way."""
+    torch = torch_gpu
+    say(f"case chunk huge logits counts={counts}")
+    step = Chunks(torch, np.random.default_rng(3), counts, contexts, heads)
+    step.query = (step.query.float() * 2.0 ** 26).to(torch.bfloat16)
+    op = step.run(output="fp32")
+    got, lse, q, sure = host(op()), host(op.lse), step.query.double().numpy(), 0
+    assert np.all(np.isfinite(got)) and np.all(np.isfinite(lse))
+    for b, n in enumerate(counts):
+        key, value, _ = prompt.features(step.rows[[step.slot(b, p) for p in range(step.lens[b])]])
+        for i in range(0, n, 7):
+            row, sees = step.cu[b] + i, step.lens[b] - n + i + 1
+            logits = SCALE * (q[row] @ key[:sees].T)
+            slip = SCALE * (np.abs(q[row]) @ np.abs(key[:sees]).T).max(1) * 584 * 2.0 ** -24
+            top = logits.argmax(1)
+            for h in range(heads):
+                others = np.delete(logits[h], top[h])
+                if len(others) and logits[h, top[h]] - others.max() < 2 * slip[h] + 100:
+                    continue  # rounding may choose another
+                sure += 1
+                assert np.all(np.abs(got[row, h] - value[top[h]]) <= np.abs(value[top[h]]) * 2.0 ** -10), (b, i, h)
+                assert abs(lse[row, h] - logits[h, top[h]]) <= slip[h] + abs(logits[h, top[h]]) * 2.0 ** -21
+    assert sure > 50
 
 
 def test_chunk_attention_equals_tree_attention_of_chains(torch_gpu):
