@@ -6,6 +6,20 @@
 // tokens of a vocabulary) need more, and each of these is worked out by one thread on its own: a bit in LDS takes
 // the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing, and a
 // token named several times gets the same sum, in the list's order, whichever thread has it.
+//
+// A row is read twice: for its maximum and sum, a part of the vocabulary per workgroup, then, in a second launch, for its
+// probabilities, each workgroup putting the parts' statistics together for itself. (A row that is one part takes one launch.) The
+// first reading is the running maximum and sum of a softmax, per thread, without a branch; NaN and infinities are
+// looked for only where the sum is no number.
+//
+// What bounds it. 320 rows of 131072 bf16 logits: 34 + 52 us. The second launch moves 252 MB at 4.8 TB/s; the first is
+// bound by vector instructions (25 per token and lane, of which 9 are the penalties, worked out for a whole wave wherever
+// one of its 512 tokens is held) and by its last round of workgroups. 176 constrained rows of 32000 with 64 biases
+// 10.5 + 13.5 us, one row of 131072 fp32 logits 5.4 + 6 us: chains of latencies (request, its numbers, lists, bits, counts).
+// A token takes its bias from the entry that names it; the list is gone through only where two entries met (11.5 + 15 before).
+// Dropped after measuring: held tokens taken out of the dense pass and worked out from a list (39 + 87 us; the scattered stores
+// cost more than the penalties), biases staged in LDS (20 % more for the constrained rows), 256 or 1024
+// threads per workgroup (-2 %, +25 %).
 #include "kvip_hip_prompt.h"
 #include "lane_groups.h"
 
@@ -146,32 +160,40 @@ struct LogitPart {
         }
     }
 
-    // Token v with its biases and the row's ancestors.
-    KVIP_DEVICE float one(int v, int b, const int* way, int ways) {
-        bool held = seen != nullptr && (seen[v >> 3] >> (v & 7) & 1);
-        int n = held ? counts[v] : 0;
-        for (int i = 0; i < ways; ++i) {
-            n += way[i] == v;
-            held = held || way[i] == v;
-        }
-        float x = static_cast<float>(logits[v]);
-        if (held) x *= x > 0.f ? row.inverse : row.repetition;
-        if (n > 0) x -= fmaf(row.frequency, static_cast<float>(n), row.presence);
+    // Token v, which entry `bias` of the request's list or (bias below 0) one of the row's ancestors names; `again`: several
+    // entries may, so that both lists are gone through.
+    KVIP_DEVICE float one(int v, int b, int bias, bool again, const int* way, int ways) {
         const int32_t* names = p.bias_tokens + static_cast<int64_t>(b) * p.biases;
         const float* values = p.bias_values + static_cast<int64_t>(b) * p.biases;
-        int i = 0;
-        for (; i + kLgListed <= p.biases; i += kLgListed) {  // in one go, as each load is waited for
-            int name[kLgListed];
-            float value[kLgListed];
-#pragma unroll
-            for (int j = 0; j < kLgListed; ++j) {
-                name[j] = names[i + j];
-                value[j] = values[i + j];
+        const float own = bias >= 0 ? values[bias] : 0.f;
+        float x = static_cast<float>(logits[v]);
+        bool held = seen != nullptr && (seen[v >> 3] >> (v & 7) & 1);
+        int n = held ? counts[v] : 0;
+        if (again || bias < 0) {
+            for (int i = 0; i < ways; ++i) {
+                n += way[i] == v;
+                held = held || way[i] == v;
             }
-#pragma unroll
-            for (int j = 0; j < kLgListed; ++j) x = name[j] == v ? x + value[j] : x;
         }
-        for (; i < p.biases; ++i) x = names[i] == v ? x + values[i] : x;
+        if (held) x *= x > 0.f ? row.inverse : row.repetition;
+        if (n > 0) x -= fmaf(row.frequency, static_cast<float>(n), row.presence);
+        if (again) {
+            int i = 0;
+            for (; i + kLgListed <= p.biases; i += kLgListed) {  // in one go, as each load is waited for
+                int name[kLgListed];
+                float value[kLgListed];
+#pragma unroll
+                for (int j = 0; j < kLgListed; ++j) {
+                    name[j] = names[i + j];
+                    value[j] = values[i + j];
+                }
+#pragma unroll
+                for (int j = 0; j < kLgListed; ++j) x = name[j] == v ? x + value[j] : x;
+            }
+            for (; i < p.biases; ++i) x = names[i] == v ? x + values[i] : x;
+        } else if (bias >= 0) {
+            x += own;
+        }
         if (allowed != nullptr && !(allowed[v >> 3] >> (v & 7) & 1)) return -INFINITY;
         if (x == x) return x;
         err |= KVIP_STATUS_BAD_PROBS;
@@ -186,7 +208,7 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     __shared__ uint32_t s_special[kLgMaxPart / 32];
     __shared__ LogitStat s_stats[kLgWaves];
     __shared__ int s_way[64];
-    __shared__ int s_ways, s_request;
+    __shared__ int s_ways, s_request, s_again;
     const int tid = threadIdx.x, lane = tid & 63;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
     const int words = (p.vocab + 31) / 32;
@@ -202,7 +224,10 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     LogitStat stat = {-INFINITY, 0.f, p.vocab, 0};
     if (MODE == kLgWrite && tid < parts) stat = stats[tid];
 
-    if (tid == 0) s_request = p.batch;
+    if (tid == 0) {
+        s_request = p.batch;
+        s_again = 0;
+    }
     const int listed = (p.visible == nullptr ? 0 : 63) + p.biases;
     if (listed > 0) {
         for (int i = tid; i < (at.end - at.begin + 31) / 32; i += kLgThreads) s_special[i] = 0;
@@ -256,14 +281,22 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
             if (v >= p.vocab) err |= KVIP_STATUS_BAD_TOKEN;
             if (v < at.begin || v >= at.end) continue;
             const uint32_t bit = 1u << (v & 31);
-            if (!(atomicOr(&s_special[(v - at.begin) >> 5], bit) & bit)) mine |= 1ull << k;
+            if (!(atomicOr(&s_special[(v - at.begin) >> 5], bit) & bit)) {
+                mine |= 1ull << k;
+            } else {
+                s_again = 1;
+            }
         }
         __syncthreads();
         at.special = s_special;
     }
-    auto named = [&](int k) {
-        const int e = tid + k * kLgThreads, ways = s_ways;
-        return e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
+    // f(x, token) of this thread's tokens.
+    auto for_mine = [&](auto f) {
+        for (uint64_t left = mine; left != 0; left &= left - 1) {
+            const int e = tid + (__ffsll(static_cast<unsigned long long>(left)) - 1) * kLgThreads, ways = s_ways;
+            const int v = e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
+            f(at.one(v, b, e - ways, s_again != 0, s_way, ways), v);
+        }
     };
 
     if constexpr ((MODE & kLgStats) != 0) {
@@ -309,16 +342,14 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
                 for (int i = 0; i < kLgVec; ++i) stat.l += weight_of(x[i], stat.m, at.row);
             }
         }
-        for (uint64_t left = mine; left != 0; left &= left - 1) {
-            const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
-            const float x = at.one(v, b, s_way, s_ways);
+        for_mine([&](float x, int v) {
             if (x > stat.m) {
                 stat = {x, (stat.m == -INFINITY ? 0.f : stat.l * weight_of(stat.m, x, at.row)) + 1.f, v, 0};
             } else if (x != -INFINITY) {
                 stat.l += weight_of(x, stat.m, at.row);
                 if (x == stat.m) stat.first = min(stat.first, v);
             }
-        }
+        });
         merge_block(stat, s_stats, at.row);
         if constexpr (MODE == kLgStats) {
             if (tid == 0) stats[part] = stat;
@@ -362,10 +393,7 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
         }
         if (listed > 0) {
             __syncthreads();  // the dense pass's zeros are in place
-            for (uint64_t left = mine; left != 0; left &= left - 1) {
-                const int v = named(__ffsll(static_cast<unsigned long long>(left)) - 1);
-                out[v] = static_cast<O>(prob(at.one(v, b, s_way, s_ways), v));
-            }
+            for_mine([&](float x, int v) { out[v] = static_cast<O>(prob(x, v)); });
         }
     }
     report(p.status, err);
@@ -407,7 +435,8 @@ void launch_logits(const KvipLogitArgs& a, hipStream_t s) {
 }
 
 // A request's counts over one part of the vocabulary, counted in LDS and written whole, so that nothing has to be
-// cleared before.
+// cleared before. 32 requests of 1000-30000 tokens and 131072 counts take 12 us: each part reads all of a request's tokens
+// (from the L2 but for the first), eight per thread at a time; parts of half the size took 14.5.
 constexpr int kHistThreads = 1024;
 constexpr int kHistPart = 1 << 14;  // 64 KB of counts
 constexpr int kHistAtOnce = 8;      // tokens of a thread whose loads are issued together

@@ -809,6 +809,32 @@ def test_masked_and_odd_logits(torch_gpu, vocab):
     assert int(op.status.item()) == 0
 
 
+@pytest.mark.parametrize("counts,vocab,biases", [([1], 9001, 30), ([6, 1], 32000, 64), ([5], 5000, 4096), ([3, 3], 140001, 4096), ([20], 64, 20)])
+def test_lists_of_tokens_named_once_or_more(torch_gpu, counts, vocab, biases):
+    """Biases of tokens that nothing else names, of drafted tokens, and of a token named by every third entry."""
+    torch = torch_gpu
+    say(f"case lists counts={counts} vocab={vocab} biases={biases}")
+    rng = np.random.default_rng(vocab + biases)
+    s = Sampling(torch, rng, counts, vocab, "fp32", biases=biases, masked=True)
+    s.numbers["temperature"][:] = 0.8
+    s.allowed[:, 0] |= 1
+    drafted = set(s.tokens.tolist())
+    for _ in range(2):
+        for b in range(len(counts)):
+            s.names[b] = rng.permutation([v for v in range(vocab) if v not in drafted or vocab < 100])[:biases]
+        op = s.op()
+        s.check(op())
+        assert int(op.status.item()) == 0
+        drafted = set()
+    s.names[:, 1:biases // 2:7] = s.tokens[s.cu[:-1], None]
+    op = s.op()
+    s.check(op())
+    s.names[:, ::3] = s.names[:, :1]
+    op = s.op()
+    s.check(op())
+    assert int(op.status.item()) == 0
+
+
 def test_logits_report(torch_gpu):
     torch = torch_gpu
     say("case logits report")
