@@ -138,8 +138,9 @@ typedef struct KvipHistoryArgs {
 } KvipHistoryArgs;
 
 /* Probabilities of the next token from logits, row by row of a packed step. With n how often the request
- * wrote token v (counts, and the row's ancestors among the step's tokens 1 .. 63: bit i of visible[row] names token
- * i, token 0 being in the history already; without visible there are none) and x the logit in 32 bits:
+ * wrote token v (counts, read for the tokens of seen alone, and the row's ancestors among the step's tokens 1 .. 63:
+ * bit i of visible[row] names token i, token 0 being in the history already; without visible, as for the last rows of
+ * prompt chunks, there are none) and x the logit in 32 bits:
  *   x = x > 0 ? x / repetition : x * repetition   where the request holds v (seen, or an ancestor);
  *   x = x - presence - frequency * n              where n > 0;
  *   x = x + the biases of v in the request's list (in the list's order; token negative: none);

@@ -2,18 +2,40 @@
 //
 // The rows of the problem are a request's (chunk token, head) pairs. There are many per cached row, so a cached row
 // is read by many workgroups, and converting its fp8 features in every one of them costs more than the products
-// (attention of a few step tokens over the same rows spends 10 vector instructions per MFMA that way). So the rows
-// are laid out once, as bf16, in the order in which the tile loop wants them in LDS (expand): a tile of 32 rows is an
-// image of 72 pieces x 32 rows x 16 bytes that direct-to-LDS loads copy as it stands.
+// (attention of a few step tokens over the same rows spends 10 vector instructions per MFMA that way and reaches 795
+// TFLOP/s). So the rows are laid out once, as fp16, in the order in which the tile loop wants them in LDS (expand): a
+// tile of 32 rows is an image of 72 pieces x 32 rows x 16 bytes that direct-to-LDS loads copy as it stands.
+//
+// fp16 and not bf16, as a feature is an fp8 number times a 32-bit scale and a probability any number: in bf16 the
+// roundings of keys, values and probabilities each add 0.0012 to an output's 0.0017 of error on 1030 cached rows (less on
+// more rows, which average them); in fp16 nothing is left of them. What fp16 lacks is range, so an image stands under the
+// exponent of its largest feature, each row under its own where the rows are far apart (what a token sees must not depend
+// on what it does not); the sums of a row of the problem stand under the largest exponent of the cached rows that
+// it has seen, and probabilities are lifted to the top of the range. bf16 was 10 % faster (6.83 instead of 7.63
+// ms on the second of the cases below): the card holds 1.8 GHz under either, as little as its power allows.
 //
 // A workgroup of 4 waves takes 128 rows of the problem, 32 per wave; a wave keeps its queries (144 registers) and its
-// 32 x 512 sums (the 256 accumulation registers). Logits are computed transposed (cached rows x rows of the problem), so
-// that a lane holds one row's logits of 16 cached rows: the softmax takes one lane swap per tile, and the
-// probabilities, rounded to bf16, are the value product's operand in the lane that has them, as the order of cached
+// 32 x 512 sums (the 256 accumulation registers; one wave per SIMD has 512 in all). Logits are computed transposed (cached
+// rows x rows of the problem), so that a lane holds one row's logits of 16 cached rows: the softmax takes one lane swap
+// per tile, and the probabilities are the value product's operand in the lane that has them, as the order of cached
 // rows along K is free. The value operand is read transposed from the same image. The running maximum is raised
 // lazily, when a tile exceeds it by kCaMargin.
+// One wave per SIMD hides nothing by itself, so the loop is one stretch of 68 MFMAs with everything else in between: the
+// logits of tile t + 1, then the values of tile t with the softmax of tile t + 1 beside them. Operands are read from
+// LDS four products ahead, across the borders of the two; the barrier for the tile after next stands where a tile's last
+// reads are done.
 //
-// Few row tiles over long contexts are cut along the context into segments, whose parts a third launch joins.
+// Few row tiles over long contexts are cut along the context into segments, whose parts a third launch joins. Requests
+// are taken the longest first.
+//
+// What bounds it. 2048 tokens x 128 heads on 8192 rows: 3.52 ms, 1160 TFLOP/s, and 4096 tokens x 16 heads on 65536
+// rows: 7.63 ms, 1180 TFLOP/s, of the 1360 of a large fp16 product: power (an MFMA is under way in 64 % of the cycles
+// at 1.78 GHz; fewer cycles per tile lower the clock); laying the rows out takes 11 and 26 us of that. 12 requests of
+// 1-700 tokens x 16 heads on up to 16000 rows: 1.21 ms, 980 TFLOP/s, as the longest workgroup takes as long as the
+// mean CU. 130 tokens x 16 heads on 1030 rows: 6 + 24 + 9 us, chains of latencies (plan, images, queries to fp16,
+// five tiles, parts, join).
+// Dropped after measuring: operands eight products ahead and two accumulators for the logits in turn (both +-0 %), other
+// prices of a part in the plan (+-2 % on small calls).
 #include <type_traits>
 #include <utility>
 
@@ -77,9 +99,10 @@ struct ChunkPlan {
     int4 request[KVIP_DRAFT_MAX_BATCH];          // first token, tokens, cached rows, first image (-1: none)
 };
 
-// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, code: four times the
-// exponent, plus 2 where there are such rows, plus 1 where its rows have exponents of their own) and the rows' exponents, then the images, then the parts: 32 rows x 512 sums per wave as its lanes hold them ([block][quarter][lane] 16 bytes),
-// then their (maximum, sum) pairs.
+// Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, code: four times
+// the exponent, plus 2 where there are such rows, plus 1 where its rows have exponents of their own) and the rows'
+// exponents, then the images, then the parts: 32 rows x 512 sums per wave as its lanes hold them
+// ([block][quarter][lane] 16 bytes), then their (maximum, sum) pairs.
 struct ChunkWork {
     ChunkPlan* plan;
     uint4* flags;
@@ -146,7 +169,8 @@ KVIP_DEVICE int ca_exponent(uint32_t most) { return static_cast<int>(most >> 23)
 KVIP_DEVICE int ca_image_exponent(uint32_t most) { return (ca_exponent(most) + 3) & ~3; }
 
 // Plan and images. Every workgroup sums the requests' tiles for itself; the first one leaves the plan, the others take
-// images in turn. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8 rotary features.
+// images in turn. A thread takes 64 features of a row (16 of each scale group, so that 8 threads read whole lines) and 8
+// rotary features.
 __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChunkAttnArgs p) {
     __shared__ __align__(16) uint8_t s_image[kCaImage];
     __shared__ int s_before[KVIP_DRAFT_MAX_BATCH + 1];
@@ -865,7 +889,8 @@ bool ca_sizes(int32_t batch, int32_t heads, int32_t max_tokens, int64_t max_rows
 // Few rows of the problem per request are the business of kvip_hip_tree_attention, which reads the cache as it is: here
 // the images cost 1808 bytes of traffic per cached row. One request of 16 heads on 16000 rows, 1 / 16 / 64 tokens: 25.6 / 46.9 /
 // 69.7 us there, 52.3 / 55.1 / 69.8 here; of 128 heads, 4 / 16 / 64 tokens: 50.3 / 105 / 318 and 56.5 / 95.9 / 258; 8
-// requests of 16 heads x 8 tokens on 8000 rows: 55.0 and 80.4, of 128 heads: 190 and 166.
+// requests of 16 heads x 8 tokens on 8000 rows: 55.0 and 80.4, of 128 heads: 190 and 166. (A workspace of this file's, of 269 MB or
+// more, would do there too: 135 MB at most. So a call may have a narrower block table than its workspace was sized for.)
 bool ca_few(int32_t batch, int32_t heads, int32_t max_tokens, int32_t max_blocks) {
     return max_tokens <= KVIP_DRAFT_MAX_NODES && static_cast<int64_t>(max_tokens) * heads <= 512ll * batch &&
            kvip_hip_tree_attention_workspace_bytes(batch, heads, max_tokens, max_blocks) != 0;

@@ -25,8 +25,8 @@ class ChunkAttention:
     workspace allocated once; `bind` validates a call's tensors, `__call__` enqueues it on the current stream
     (capturable; one object's calls follow one another, as they share its workspace). max_tokens: tokens of a call;
     max_context: cached rows of a request, the chunk's among them; max_rows: cached rows of a call's requests
-    together (default batch * max_context), which the workspace holds as bf16, 1152 bytes each. A request past
-    that gets zeros and sets a status bit."""
+    together (default batch * max_context), which the workspace holds as fp16, 1152 bytes each (small calls read the
+    cache itself). A request past that gets zeros and sets a status bit."""
 
     def __init__(self, torch, *, batch, heads, max_tokens, max_context, device, max_rows=None, output_dtype=None, lse=False):
         abi.require(1 <= batch <= abi.DRAFT_MAX_BATCH, f"batch must be in 1..{abi.DRAFT_MAX_BATCH}")
