@@ -490,14 +490,14 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     const bool whole = reach <= cut;
     const int hn = lane & 31, hk = lane >> 5;
     const int row = first_row + hn, node = min(row, rows - 1) / p.heads;
-    const int64_t out_row = static_cast<int64_t>(q.begin) * p.heads + row;
+    const int64_t out_first = static_cast<int64_t>(q.begin) * p.heads + first_row;
     if (t0 >= t1) {
         if (unit.seg != 0 || reach > 0) return;  // nothing of the row tile is here
         for (int i = tid; i < kCaTileRows * (kCaValue / 4); i += kCaThreads) {  // rows that see nothing
             const int r = unit.rt * kCaTileRows + i / (kCaValue / 4);
             if (r < rows) ca_store(p, (static_cast<int64_t>(q.begin) * p.heads + r) * kCaValue + i % (kCaValue / 4) * 4, f32x4{0.f, 0.f, 0.f, 0.f});
         }
-        if (p.lse != nullptr && hk == 0 && row < rows) p.lse[out_row] = -INFINITY;
+        if (p.lse != nullptr && hk == 0 && row < rows) p.lse[out_first + hn] = -INFINITY;
         return;
     }
     const int sees = min(max(q.past() + node + 1, 0), q.length);  // cached rows that the lane's row sees
@@ -516,17 +516,24 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         constexpr int i = decltype(which)::value;
         ca_dma16<i % 4 * 1024>(from + i / 4 * 4096, lane * 16, to + i / 4 * 4096);
     };
+    // Queries of the wave's rows (rows past the last: the last again; their outputs are not written) come through a slot of its
+    // own, in groups of 8 pieces x 32 rows, in which piece j of row r stands in place j ^ (r & 7) of the row's 8: whole lines
+    // from memory, and reads of a piece of 32 rows on all banks. (130 tokens x 16 heads on 130 / 1030 / 4130 rows 19.7 / 23.5 / 36.4 us with loads of each lane's own
+    // row, 17.3 / 22.1 / 34.9 so; nothing where every CU is busy.) The largest feature is looked for while they arrive.
+    constexpr int kGroups = kCaPieces / 8, kGroupLoads = kCaRows / 8, kGroupFrags = 4;
+    const uint32_t mine = ring + w * kCaImage;
+    {
+        const int last = max(rows - 1 - first_row, 0);  // row of the wave
+        const uint8_t* query = reinterpret_cast<const uint8_t*>(p.query) + (static_cast<int64_t>(q.begin) * p.heads + min(first_row, rows - 1)) * (2 * kCaKey);
+        uint32_t from_row[kGroupLoads];
 #pragma unroll
-    for (int t = 0; t < kCaSlots - 2; ++t) {
-        aim(t0 + t);
-        for_all(fetch, std::make_integer_sequence<int, kCaLoads>{});
+        for (int k = 0; k < kGroupLoads; ++k) from_row[k] = min(8 * k + (lane >> 3), last) * (2 * kCaKey) + ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+            for (int k = 0; k < kGroupLoads; ++k) ca_dma16<0>(query + g * 128, from_row[k], mine + (g * kGroupLoads + k) * 1024);
+        }
     }
-    // Queries of the wave's rows (rows past the last read it again; their outputs are not written): fragment i holds
-    // features 16 i + 8 (lane / 32) .. + 7.
-    const uint16_t* query = p.query + (static_cast<int64_t>(q.begin) * p.heads + min(row, rows - 1)) * kCaKey + hk * 8;
-    v4i qf[kCaFrags];
-#pragma unroll
-    for (int i = 0; i < kCaFrags; ++i) qf[i] = *reinterpret_cast<const v4i*>(query + i * 16);
     v16f o[kCaBlocks];
 #pragma unroll
     for (int f = 0; f < kCaBlocks; ++f) {
@@ -534,14 +541,35 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
         ca_hold(o[f]);
     }
+    v4i qf[kCaFrags];  // fragment i: features 16 i + 8 (lane / 32) .. + 7
+    u16x2 most_q = {};
+    uint32_t piece_at[kGroupFrags];
+#pragma unroll
+    for (int i = 0; i < kGroupFrags; ++i) {
+        piece_at[i] = mine + hn * 128 + ((2 * i + hk) ^ (hn & 7)) * 16;
+        asm volatile("" : "+v"(piece_at[i]));
+    }
+    for_all([&](auto which) {
+        constexpr int g = decltype(which)::value;
+        asm volatile("s_waitcnt vmcnt(%0)" : : "n"((kGroups - 1 - g) * kGroupLoads) : "memory");
+#pragma unroll
+        for (int i = g * kGroupFrags; i < (g + 1) * kGroupFrags; ++i) {
+            qf[i] = *(LdsV4i)(piece_at[i % kGroupFrags] + g * 4096);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most_q = __builtin_elementwise_max(most_q, __builtin_bit_cast(u16x2, qf[i][j] & 0x7FFF7FFF));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }, std::make_integer_sequence<int, kGroups>{});
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+#pragma unroll
+    for (int t = 0; t < kCaSlots - 2; ++t) {
+        aim(t0 + t);
+        for_all(fetch, std::make_integer_sequence<int, kCaLoads>{});
+    }
     // They become fp16 under an exponent of their row's, exactly but for features below 2^-28 of its largest. A negative
     // scale turns their signs.
-    u16x2 most_q = {};
-#pragma unroll
-    for (int i = 0; i < kCaFrags; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) most_q = __builtin_elementwise_max(most_q, __builtin_bit_cast(u16x2, qf[i][j] & 0x7FFF7FFF));
-    }
     uint32_t most_bits = static_cast<uint32_t>(max(most_q[0], most_q[1])) << 16;
     most_bits = __float_as_uint(ca_half_max(__uint_as_float(most_bits < 0x7F800000u ? most_bits : 0u)));
     const int q_exponent = max(ca_exponent(most_bits), -126);
@@ -782,6 +810,8 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
 
     const float l_all = ldexpf(ca_half_sum(l_sum), -kCaLift);
     const float share = ldexpf(whole ? ca_share(l_all) : 1.f, exponent - kCaLift);
+    int hn_ = hn;
+    asm volatile("" : "+v"(hn_));  // what comes of it is not held over the tile loop
     f32x4* part = work.sums + (static_cast<int64_t>(blockIdx.x) * kCaWaves + w) * (kCaBlocks * 4 * 64) + lane;
 #pragma unroll
     for (int f = 0; f < kCaBlocks; ++f) {
@@ -802,18 +832,18 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
                     v[e] = pair[0];
                     v[e + 2] = pair[1];
                 }
-                if (row < rows) *reinterpret_cast<v4i*>(static_cast<__bf16*>(p.output) + out_row * kCaValue + 32 * f + 8 * a + 8 * hk) = v;
+                if (hn_ < rows - first_row) *reinterpret_cast<v4i*>(static_cast<__bf16*>(p.output) + (out_first + hn_) * kCaValue + 32 * f + 8 * a + 8 * hk) = v;
             }
-        } else if (row < rows) {
+        } else if (hn_ < rows - first_row) {
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                ca_store(p, out_row * kCaValue + 32 * f + 8 * a + 4 * hk, f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]});
+                ca_store(p, (out_first + hn_) * kCaValue + 32 * f + 8 * a + 4 * hk, f32x4{x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]});
             }
         }
     }
     if (hk == 0) {
-        if (!whole) work.states[static_cast<int64_t>(blockIdx.x) * kCaTileRows + w * kCaRows + hn] = make_float2(m_run, l_all);
-        else if (p.lse != nullptr && row < rows) p.lse[out_row] = ca_lse(m_run, l_all);
+        if (!whole) work.states[static_cast<int64_t>(blockIdx.x) * kCaTileRows + w * kCaRows + hn_] = make_float2(m_run, l_all);
+        else if (p.lse != nullptr && hn_ < rows - first_row) p.lse[out_first + hn_] = ca_lse(m_run, l_all);
     }
 }
 
