@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_kernel(const KvipNormR
     const int64_t first = static_cast<int64_t>(blockIdx.x) * run;
     const int tokens = static_cast<int>(min(static_cast<int64_t>(run), p.tokens - first));
     for (int i = tid; i < tokens * pairs; i += kNrThreads) {
-        s_turn[i] = turn_of(p.positions[first + i / pairs], p.frequencies[i % pairs], p.magnitude, false);
+        s_turn[i] = fine_turn_of(p.positions[first + i / pairs], p.frequencies[i % pairs], p.magnitude);
     }
     const int j = tid % G;
     const bool live = j * kNrLane < p.dim, turned = j * kNrLane < p.rotary_dim;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rotary_any_kernel(const KvipN
             const int pair = p.half ? f % pairs : f / 2;
             const bool second = p.half ? f >= pairs : (f & 1) != 0;
             const float other = s_head[w][p.half ? (second ? f - pairs : f + pairs) : f ^ 1];
-            const float2 turn = turn_of(p.positions[token], p.frequencies[pair], p.magnitude, false);
+            const float2 turn = fine_turn_of(p.positions[token], p.frequencies[pair], p.magnitude);
             x[i] = x[i] * turn.x + (second ? other : -other) * turn.y;
         }
         largest = fmaxf(largest, fabsf(x[i]));
