@@ -32,7 +32,7 @@
 // rows: 7.63 ms, 1180 TFLOP/s, of the 1360 of a large fp16 product: power (an MFMA is under way in 64 % of the cycles
 // at 1.78 GHz; fewer cycles per tile lower the clock); laying the rows out takes 11 and 26 us of that. 12 requests of
 // 1-700 tokens x 16 heads on up to 16000 rows: 1.17 ms, 1010 TFLOP/s, as the longest workgroup takes as long as the
-// mean CU. 130 tokens x 16 heads on 1030 rows: 6 + 24 + 9 us, chains of latencies (plan, images, queries to fp16,
+// mean CU. 130 tokens x 16 heads on 1030 rows: 6 + 22 + 8 us, chains of latencies (plan, images, queries to fp16,
 // five tiles, parts, join).
 // Dropped after measuring: operands eight products ahead and two accumulators for the logits in turn (both +-0 %), other
 // prices of a part in the plan (+-2 % on small calls).
