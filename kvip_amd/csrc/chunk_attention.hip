@@ -74,6 +74,7 @@ constexpr int kCaMostCuts = 32;
 constexpr int kCaPartSteps = 10;                  // what storing and joining a part costs, in tiles
 constexpr int kCaCus = 256;
 constexpr float kCaLog2e = 1.44269504088896341f;
+constexpr float kCaLargest = 3.402823466e38f;
 constexpr float kCaLn2 = 0.693147180559945309f;
 constexpr float kCaMargin = 3.0f * kCaLog2e;
 constexpr int kCaTop = 14;                        // exponent of the largest feature in an image, and of a row's largest query
@@ -583,7 +584,8 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
         }
         asm volatile("" : "+v"(qf[i]));  // worked out here, not in the tile loop
     }
-    const float scale2 = fabsf(p.scale * kCaLog2e);
+    int scale_exponent;  // the scale in log2 units is scale2 times 2 to this
+    const float scale2 = frexpf(fabsf(p.scale), &scale_exponent) * kCaLog2e;
     float m_run = -INFINITY, l_sum = 0.f;
     v16f s;
     v4i pb[2];  // probabilities of the tile whose values come next
@@ -692,8 +694,9 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
                 shift = max(of_tile - exponent, 0);
                 exponent += shift;
                 lower = max(of_tile - exponent, -100);
-                // A scale so small that the logits vanish still leaves a number, which what is masked stays below.
-                factor = fmaxf(ldexpf(scale2, q_exponent + of_tile), 0x1p-126f);
+                // A scale so small that the logits vanish still leaves a number, which what is masked stays below, and one so
+                // large that they overflow leaves those that are 0.
+                factor = fminf(fmaxf(ldexpf(scale2, scale_exponent + q_exponent + of_tile), 0x1p-126f), kCaLargest);
                 calm = !spread && __ballot(shift != 0 || lower != 0 || of_tile != tile_exponent) == 0ull ? tile_exponent : 0x7FFFFFFF;
             }
         } else if (piece == 1) {

@@ -166,6 +166,33 @@ def test_chunk_attention_options(torch_gpu):
         step.check(step.run(scale=scale), scale=scale, every=23)
 
 
+def test_chunk_attention_of_nothing_but_zeros(torch_gpu):
+    """Queries of zero weigh every row alike, under any scale."""
+    torch = torch_gpu
+    say("case chunk zero queries")
+    step = Chunks(torch, np.random.default_rng(6), [50, 30], [200, 4000], 6)
+    step.query[::2] = 0
+    step.query[1::2] *= 1e-38  # logits that no scale brings to more than some units
+    for scale in (3e38, -3e38, 1.0):
+        step.check(step.run(scale=scale), scale=scale, every=7)
+
+
+@pytest.mark.parametrize("heads,counts,contexts", [(4, [3], [200]), (16, [70, 9], [100, 700])])
+def test_chunk_attention_takes_narrower_tables(torch_gpu, heads, counts, contexts):
+    """An object for long contexts, bound to block tables of the step's."""
+    torch = torch_gpu
+    say(f"case chunk narrow table counts={counts}")
+    step = Chunks(torch, np.random.default_rng(7), counts, contexts, heads, pad=0 if max(counts) < 64 else 70)
+    first = step.run()()
+    op = kvip_amd.ChunkAttention(torch, batch=len(counts), heads=heads, max_tokens=step.tokens, max_context=20000, max_rows=3000, device="cuda")
+    args = (step.query.cuda(), step.kv, device(torch, step.table, torch.int32), device(torch, step.lens, torch.int32),
+            device(torch, step.cu, torch.int32))
+    got = op.bind(*args)()
+    assert torch.equal(got[:sum(counts)], first[:sum(counts)])
+    with pytest.raises(ValueError):
+        op.bind(args[0], step.kv, torch.zeros((len(counts), 158), dtype=torch.int32, device="cuda"), *args[3:])
+
+
 @pytest.mark.parametrize("heads,counts,contexts", [(16, [40], [500]), (16, [9, 60], [9000, 0])])
 def test_chunk_attention_of_huge_logits(torch_gpu, heads, counts, contexts):
     """Logits of 10^7 and more: all weight is on the largest, and nothing overflows on the way."""
