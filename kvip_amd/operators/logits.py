@@ -35,23 +35,25 @@ class TokenHistory:
                                      vocab=self.vocab)
 
     def _check(self, x, dtype, shape, what):
-        abi.require(x.dtype == dtype and tuple(x.shape) == shape and x.is_contiguous() and x.device == self.device,
-                    f"{what} must be contiguous {dtype} {list(shape)} on {self.device}")
-        return abi.ptr(x)
+        # Worded only where it fails: with a message made for every check a call took 9.4 us of the host instead of 6.4.
+        if x.dtype is not dtype or x.shape != shape or not x.is_contiguous() or x.device != self.device:
+            raise ValueError(f"{what} must be contiguous {dtype} {list(shape)} on {self.device}")
+        return x.data_ptr()
 
     def load(self, requests, tokens, cu_seqlens, prompt_lens):
         """Replaces what requests[i] (int32 [n] in 0 .. batch - 1, none twice; negative: none) holds by the tokens
         cu_seqlens[i] .. cu_seqlens[i + 1] (int64, packed), the first prompt_lens[i] (int32 [n]) of which are its
         prompt; no tokens: it holds none. Returns counts."""
         t = self.torch
-        n = int(requests.shape[0]) if requests.dim() == 1 else 0
-        abi.require(1 <= n <= abi.DRAFT_MAX_BATCH, f"requests must be int32 [1..{abi.DRAFT_MAX_BATCH}]")
-        abi.require(tokens.dim() == 1 and tokens.shape[0] <= 0x7FFFFFFF, "tokens must be int64 [up to 2^31 - 1]")
+        n = requests.numel()
+        if requests.dim() != 1 or not 1 <= n <= abi.DRAFT_MAX_BATCH:
+            raise ValueError(f"requests must be int32 [1..{abi.DRAFT_MAX_BATCH}]")
+        abi.require(tokens.dim() == 1 and tokens.numel() <= 0x7FFFFFFF, "tokens must be int64 [up to 2^31 - 1]")
         a = self._args  # copied by the launch
         a.requests, a.count = self._check(requests, t.int32, (n,), "requests"), n
         a.cu_seqlens = self._check(cu_seqlens, t.int32, (n + 1,), "cu_seqlens")
         a.prompt_lens = self._check(prompt_lens, t.int32, (n,), "prompt_lens")
-        a.max_tokens = int(tokens.shape[0])
+        a.max_tokens = tokens.numel()
         # Without tokens nothing is read: any address that is not null.
         a.tokens = self._check(tokens, t.int64, (a.max_tokens,), "tokens") or a.counts
         abi.launch(t, self.device, self.library.kvip_hip_history_load, a, "token history")
@@ -61,8 +63,9 @@ class TokenHistory:
         """Adds the first kept[b] (int32 [batch]) of tokens[b] (int64 [batch, up to 64]) to request b, as
         `kvip_amd.DraftVerifier` returns them. Returns counts."""
         t = self.torch
-        places = int(tokens.shape[1]) if tokens.dim() == 2 else 0
-        abi.require(1 <= places <= abi.DRAFT_MAX_NODES, f"tokens must be int64 [{self.batch}, 1..{abi.DRAFT_MAX_NODES}]")
+        places = tokens.shape[1] if tokens.dim() == 2 else 0
+        if not 1 <= places <= abi.DRAFT_MAX_NODES:
+            raise ValueError(f"tokens must be int64 [{self.batch}, 1..{abi.DRAFT_MAX_NODES}]")
         a = self._args  # copied by the launch
         a.tokens, a.token_stride = self._check(tokens, t.int64, (self.batch, places), "tokens"), places
         a.kept = self._check(kept, t.int32, (self.batch,), "kept")
