@@ -137,11 +137,12 @@ struct LogitPart {
                 for (int i = 0; i < kLgVec; ++i) n[i] = v + i < end ? counts[v + i] : 0;
             }
 #pragma unroll
-            for (int i = 0; i < kLgVec; ++i) {  // a token that is not held has a count of 0
+            for (int i = 0; i < kLgVec; ++i) {  // a count counts with its bit alone
                 const uint32_t on = bit_mask(held, i);
+                const int written = n[i] & static_cast<int>(on);
                 const float factor = __uint_as_float(pick(on, __float_as_uint(x[i] > 0.f ? row.inverse : row.repetition), 0x3F800000u));
-                const float less = fmaf(row.frequency, static_cast<float>(n[i]), row.presence);
-                x[i] = fmaf(x[i], factor, n[i] > 0 ? -less : -0.f);
+                const float less = fmaf(row.frequency, static_cast<float>(written), row.presence);
+                x[i] = fmaf(x[i], factor, written > 0 ? -less : -0.f);
             }
         }
         if (raw.may != 0xFFu) {
