@@ -18,7 +18,8 @@ def _codes(torch):
 
 class TokenHistory:
     """counts int32 [batch, vocab] (how often a request wrote a token), seen int32 [batch, (vocab + 31) / 32] (bits: it
-    wrote the token or its prompt has it) and status, allocated once and empty."""
+    wrote the token or its prompt has it) and status, allocated once and empty. Calls may come from several threads and
+    streams as long as they are for different requests."""
 
     def __init__(self, torch, *, batch, vocab, device):
         abi.require(1 <= batch <= abi.DRAFT_MAX_BATCH, f"batch must be in 1..{abi.DRAFT_MAX_BATCH}")
@@ -49,7 +50,7 @@ class TokenHistory:
         if requests.dim() != 1 or not 1 <= n <= abi.DRAFT_MAX_BATCH:
             raise ValueError(f"requests must be int32 [1..{abi.DRAFT_MAX_BATCH}]")
         abi.require(tokens.dim() == 1 and tokens.numel() <= 0x7FFFFFFF, "tokens must be int64 [up to 2^31 - 1]")
-        a = self._args  # copied by the launch
+        a = abi.HistoryArgs.from_buffer_copy(self._args)  # this call's: the entry runs without the interpreter's lock
         a.requests, a.count = self._check(requests, t.int32, (n,), "requests"), n
         a.cu_seqlens = self._check(cu_seqlens, t.int32, (n + 1,), "cu_seqlens")
         a.prompt_lens = self._check(prompt_lens, t.int32, (n,), "prompt_lens")
@@ -66,7 +67,7 @@ class TokenHistory:
         places = tokens.shape[1] if tokens.dim() == 2 else 0
         if not 1 <= places <= abi.DRAFT_MAX_NODES:
             raise ValueError(f"tokens must be int64 [{self.batch}, 1..{abi.DRAFT_MAX_NODES}]")
-        a = self._args  # copied by the launch
+        a = abi.HistoryArgs.from_buffer_copy(self._args)  # this call's: the entry runs without the interpreter's lock
         a.tokens, a.token_stride = self._check(tokens, t.int64, (self.batch, places), "tokens"), places
         a.kept = self._check(kept, t.int32, (self.batch,), "kept")
         abi.launch(t, self.device, self.library.kvip_hip_history_append, a, "token history")
