@@ -4,8 +4,9 @@
 // Nearly all of a row is alike: a logit, a bit whether the request holds the token, for those it holds a count, a
 // bit whether the grammar allows it. Only the row's drafted ancestors and the request's biases (some hundred
 // tokens of a vocabulary) need more, and each of these is worked out by one thread on its own: a bit in LDS takes
-// the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing, and a
-// token named several times gets the same sum, in the list's order, whichever thread has it.
+// the token out of the dense pass, the thread puts it back. So lists of any length cost the dense pass nothing. A
+// token named several times has a second bit: the thread of the first entry that names it has it, and its wave goes through the
+// list together, so that neither its sum nor the order of the row's depends on which thread comes first.
 //
 // A row is read twice: for its maximum and sum, a part of the vocabulary per workgroup, then, in a second launch, for its
 // probabilities, each workgroup putting the parts' statistics together for itself. (A row that is one part takes one launch.) The
@@ -30,8 +31,8 @@ constexpr int kLgThreads = 512;
 constexpr int kLgWaves = kLgThreads / 64;
 constexpr int kLgVec = 8;                      // tokens of a thread at a time: a byte of the bit masks
 constexpr int kLgRun = kLgThreads * kLgVec;
-constexpr int kLgListed = 16;                  // biases looked at together
-constexpr int kLgMaxPart = 1 << 17;            // tokens of a workgroup (16 KB of bits)
+constexpr int kLgListed = 4;                   // entries of a lane looked at together
+constexpr int kLgMaxPart = 1 << 17;            // tokens of a workgroup (twice 16 KB of bits)
 constexpr float kLgLog2e = 1.44269504088896341f;
 constexpr float kLgLargest = 3.402823466e38f;
 
@@ -161,40 +162,48 @@ struct LogitPart {
         }
     }
 
-    // Token v, which entry `bias` of the request's list or (bias below 0) one of the row's ancestors names; `again`: several
-    // entries may, so that both lists are gone through.
-    KVIP_DEVICE float one(int v, int b, int bias, bool again, const int* way, int ways) {
-        const int32_t* names = p.bias_tokens + static_cast<int64_t>(b) * p.biases;
-        const float* values = p.bias_values + static_cast<int64_t>(b) * p.biases;
-        const float own = bias >= 0 ? values[bias] : 0.f;
+    // x of token v, which entry e names (the row's ancestors first, then the request's list), before its mask and, where other
+    // entries name it (`again`), before its biases. False where an ancestor before e names it, which has it then.
+    KVIP_DEVICE bool named(int v, int b, int e, bool again, const int* way, int ways, float* out) const {
+        const int bias = e - ways;
+        const float own = bias >= 0 ? p.bias_values[static_cast<int64_t>(b) * p.biases + bias] : 0.f;
         float x = static_cast<float>(logits[v]);
         bool held = seen != nullptr && (seen[v >> 3] >> (v & 7) & 1);
         int n = held ? counts[v] : 0;
         if (again || bias < 0) {
             for (int i = 0; i < ways; ++i) {
+                if (way[i] == v && i < e) return false;
                 n += way[i] == v;
                 held = held || way[i] == v;
             }
         }
         if (held) x *= x > 0.f ? row.inverse : row.repetition;
         if (n > 0) x -= fmaf(row.frequency, static_cast<float>(n), row.presence);
-        if (again) {
-            int i = 0;
-            for (; i + kLgListed <= p.biases; i += kLgListed) {  // in one go, as each load is waited for
-                int name[kLgListed];
-                float value[kLgListed];
+        *out = !again && bias >= 0 ? x + own : x;
+        return true;
+    }
+    // All biases of token v added to x in the list's order, by a whole wave, whose lanes all pass the same. False where an entry
+    // of the list before `bias` names it, which has it then.
+    KVIP_DEVICE bool add_biases(int v, int b, int bias, float* x) const {
+        const int lane = threadIdx.x & 63;
+        const int32_t* names = p.bias_tokens + static_cast<int64_t>(b) * p.biases;
+        const float* values = p.bias_values + static_cast<int64_t>(b) * p.biases;
+        for (int i = 0; i < p.biases; i += 64 * kLgListed) {
+            int name[kLgListed];
 #pragma unroll
-                for (int j = 0; j < kLgListed; ++j) {
-                    name[j] = names[i + j];
-                    value[j] = values[i + j];
+            for (int j = 0; j < kLgListed; ++j) name[j] = i + 64 * j + lane < p.biases ? names[i + 64 * j + lane] : -1;
+#pragma unroll
+            for (int j = 0; j < kLgListed; ++j) {
+                for (uint64_t found = __ballot(name[j] == v); found != 0; found &= found - 1) {
+                    const int e = i + 64 * j + __builtin_ctzll(found);
+                    if (e < bias) return false;
+                    *x += values[e];
                 }
-#pragma unroll
-                for (int j = 0; j < kLgListed; ++j) x = name[j] == v ? x + value[j] : x;
             }
-            for (; i < p.biases; ++i) x = names[i] == v ? x + values[i] : x;
-        } else if (bias >= 0) {
-            x += own;
         }
+        return true;
+    }
+    KVIP_DEVICE float masked(int v, float x) {
         if (allowed != nullptr && !(allowed[v >> 3] >> (v & 7) & 1)) return -INFINITY;
         if (x == x) return x;
         err |= KVIP_STATUS_BAD_PROBS;
@@ -202,14 +211,16 @@ struct LogitPart {
     }
 };
 
+static_assert((63 + KVIP_LOGIT_MAX_BIASES + kLgThreads - 1) / kLgThreads <= 32, "bits of a thread's entries");
+
 enum { kLgStats = 1, kLgWrite = 2 };  // both: a row is one part
 
 template <typename T, typename O, int MODE>
 __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs p, int parts, int part_size) {
-    __shared__ uint32_t s_special[kLgMaxPart / 32];
+    __shared__ uint32_t s_special[kLgMaxPart / 32], s_twice[kLgMaxPart / 32];
     __shared__ LogitStat s_stats[kLgWaves];
     __shared__ int s_way[64];
-    __shared__ int s_ways, s_request, s_again;
+    __shared__ int s_ways, s_request;
     const int tid = threadIdx.x, lane = tid & 63;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts;
     const int words = (p.vocab + 31) / 32;
@@ -225,13 +236,10 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     LogitStat stat = {-INFINITY, 0.f, p.vocab, 0};
     if (MODE == kLgWrite && tid < parts) stat = stats[tid];
 
-    if (tid == 0) {
-        s_request = p.batch;
-        s_again = 0;
-    }
+    if (tid == 0) s_request = p.batch;
     const int listed = (p.visible == nullptr ? 0 : 63) + p.biases;
     if (listed > 0) {
-        for (int i = tid; i < (at.end - at.begin + 31) / 32; i += kLgThreads) s_special[i] = 0;
+        for (int i = tid; i < (at.end - at.begin + 31) / 32; i += kLgThreads) s_special[i] = s_twice[i] = 0;
     }
     __syncthreads();
     for (int b = tid; b < p.batch; b += kLgThreads) {
@@ -261,7 +269,7 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
     at.row.plain = at.row.c > 0.f && at.row.c < INFINITY;
 
     // The row's ancestors, and which tokens of this part are not the dense pass's.
-    uint64_t mine = 0;  // bit k: this thread has the token that entry tid + 512 k names
+    uint32_t mine = 0;  // bit k: entry tid + 512 k names a token of this part
     if (listed > 0) {
         if (tid < 64) {
             const int begin = min(max(p.cu_seqlens[b], 0), p.max_tokens), behind = min(max(p.cu_seqlens[b + 1], begin), p.max_tokens);
@@ -282,21 +290,34 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const KvipLogitArgs 
             if (v >= p.vocab) err |= KVIP_STATUS_BAD_TOKEN;
             if (v < at.begin || v >= at.end) continue;
             const uint32_t bit = 1u << (v & 31);
-            if (!(atomicOr(&s_special[(v - at.begin) >> 5], bit) & bit)) {
-                mine |= 1ull << k;
-            } else {
-                s_again = 1;
-            }
+            mine |= 1u << k;
+            if (atomicOr(&s_special[(v - at.begin) >> 5], bit) & bit) atomicOr(&s_twice[(v - at.begin) >> 5], bit);
         }
         __syncthreads();
         at.special = s_special;
     }
     // f(x, token) of this thread's tokens.
     auto for_mine = [&](auto f) {
-        for (uint64_t left = mine; left != 0; left &= left - 1) {
-            const int e = tid + (__ffsll(static_cast<unsigned long long>(left)) - 1) * kLgThreads, ways = s_ways;
-            const int v = e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
-            f(at.one(v, b, e - ways, s_again != 0, s_way, ways), v);
+        for (uint32_t rest = mine; __ballot(rest != 0) != 0; rest &= rest - 1) {  // lanes without a token go along
+            const int ways = s_ways, e = tid + (__ffs(rest) - 1) * kLgThreads;
+            bool have = rest != 0, again = false;
+            int v = 0;
+            float x = 0.f;
+            if (have) {
+                v = e < ways ? s_way[e] : p.bias_tokens[static_cast<int64_t>(b) * p.biases + e - ways];
+                again = (s_twice[(v - at.begin) >> 5] >> (v & 31) & 1) != 0;
+                have = at.named(v, b, e, again, s_way, ways, &x);
+            }
+            for (uint64_t several = __ballot(have && again); several != 0; several &= several - 1) {
+                const int l = __builtin_ctzll(several);
+                float sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
+                const bool first_named = at.add_biases(__builtin_amdgcn_readlane(v, l), b, __builtin_amdgcn_readlane(e, l) - ways, &sum);
+                if (lane == l) {
+                    x = sum;
+                    have = first_named;
+                }
+            }
+            if (have) f(at.masked(v, x), v);
         }
     };
 
