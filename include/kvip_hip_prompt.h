@@ -147,7 +147,8 @@ typedef struct KvipHistoryArgs {
  *   x = -infinity                                 where bit v % 32 of allowed[row][v / 32] is 0;
  *   probs = exp((x - max x) / temperature) / their sum, or, where temperature is not above 0, 1 at the first of the
  *   largest x and 0 elsewhere.
- * Each array is optional (repetition 1, the others 0, temperature 1). Sums are 32-bit, over at most 2^17 terms per
+ * Each array is optional (repetition 1, the others 0, temperature 1). In 32 bits; where temperature is above 0, x / repetition may
+ * be x times the rounded reciprocal, where it is not, numbers that are 32-bit ones stay exact, so that tokens tie. Sums are 32-bit, over at most 2^17 terms per
  * run and then over the runs; probabilities are rounded once. An x that is NaN counts as -infinity and sets
  * KVIP_STATUS_BAD_PROBS, as does a row that is -infinity everywhere, which gets 0 everywhere; tokens at +infinity
  * share the row. Drafted or bias tokens past vocab - 1 (drafted: or negative) set KVIP_STATUS_BAD_TOKEN and are left out;

@@ -122,7 +122,19 @@ struct LogitPart {
         return raw;
     }
 
-    // Their x, -infinity for those that are not the dense pass's; CAREFUL: and for NaN, which is noted.
+    // x of a held token that the request wrote n times, as exact as 32 bits are: where quotient and difference are 32-bit
+    // numbers they come out as these, so that tokens whose x are equal tie. (The quotient by the reciprocal and what that leaves,
+    // where it leaves a number.)
+    KVIP_DEVICE float penalised(float x, int n) const {
+        const float less = n > 0 ? fmaf(row.frequency, static_cast<float>(n), row.presence) : 0.f;
+        const float product = x * row.inverse, rest = fmaf(-product, row.repetition, x);
+        const float quotient = fabsf(rest) < INFINITY ? fmaf(rest, row.inverse, product) : product;
+        return x > 0.f ? quotient - less : fmaf(x, row.repetition, -less);
+    }
+
+    // Their x, -infinity for those that are not the dense pass's; CAREFUL: and for NaN, which is noted. Without CAREFUL a
+    // quotient is a product with the rounded reciprocal, off by 2^-23 at most, which no probability shows; CAREFUL is the way
+    // of rows that look for their largest x alone, where a tie has to be one.
     template <bool CAREFUL>
     KVIP_DEVICE void adjust(int v, Raw raw, float (&x)[kLgVec]) {
 #pragma unroll
@@ -141,6 +153,11 @@ struct LogitPart {
             for (int i = 0; i < kLgVec; ++i) {  // a count counts with its bit alone
                 const uint32_t on = bit_mask(held, i);
                 const int written = n[i] & static_cast<int>(on);
+                if constexpr (CAREFUL) {
+                    x[i] = __uint_as_float(pick(on, __float_as_uint(penalised(x[i], written)), __float_as_uint(x[i])));
+                    asm volatile("" : "+v"(x[i]));  // one after another, for fewer registers
+                    continue;
+                }
                 const float factor = __uint_as_float(pick(on, __float_as_uint(x[i] > 0.f ? row.inverse : row.repetition), 0x3F800000u));
                 const float less = fmaf(row.frequency, static_cast<float>(written), row.presence);
                 x[i] = fmaf(x[i], factor, written > 0 ? -less : -0.f);
@@ -177,8 +194,7 @@ struct LogitPart {
                 held = held || way[i] == v;
             }
         }
-        if (held) x *= x > 0.f ? row.inverse : row.repetition;
-        if (n > 0) x -= fmaf(row.frequency, static_cast<float>(n), row.presence);
+        if (held) x = penalised(x, n);
         *out = !again && bias >= 0 ? x + own : x;
         return true;
     }

@@ -39,6 +39,74 @@ def test_counts_without_their_bit_are_not_read(torch_gpu, vocab, biases):
     assert int(op.status.item()) == 0
 
 
+def odd_reciprocals():
+    """Numbers of 8 bits in 1..2 whose rounded reciprocal times themselves is not 1 in 32 bits."""
+    r = (np.arange(129, 256) / 128).astype(np.float32)
+    return r[r * (np.float32(1) / r) != 1]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("vocab", [700, 30000])
+@pytest.mark.parametrize("listed", [None, "first", "second", "drafted"])
+def test_the_first_of_equal_logits_wins(torch_gpu, dtype, vocab, listed):
+    """A held token whose logit over the repetition penalty is exactly another's logit, whichever of them a bias of 0 or a
+    draft names. Every number here is exact in 32 bits, so that there is one answer."""
+    torch = torch_gpu
+    say(f"case equal logits {dtype} vocab={vocab} listed={listed}")
+    r = odd_reciprocals()[:30]
+    n, first, second = len(r), 5, 600
+    drafted = listed == "drafted"
+    rows = 2 * n if drafted else n
+    last = np.arange(1, rows, 2) if drafted else np.arange(n)  # the row of each request that is looked at
+    x = np.full((rows, vocab), -9.0, np.float32)
+    x[last, first], x[last, second] = r, 1.0
+    history = kvip_amd.TokenHistory(torch, batch=n, vocab=vocab, device="cuda")
+    tokens, visible = np.full(rows, 77), np.ones(rows, np.int64)
+    kw = {}
+    if drafted:  # row 1 comes behind the drafted token
+        tokens[last], visible[last] = first, 3
+        kw = dict(tokens=device(torch, tokens, torch.int64), visible=device(torch, visible, torch.int64))
+    else:
+        history.load(device(torch, range(n), torch.int32), torch.full((n,), first, dtype=torch.int64, device="cuda"),
+                     device(torch, range(n + 1), torch.int32), device(torch, [1] * n, torch.int32))
+    if listed in ("first", "second"):
+        kw = dict(bias_tokens=torch.full((n, 1), first if listed == "first" else second, dtype=torch.int32, device="cuda"),
+                  bias_values=torch.zeros((n, 1), device="cuda"))
+    op = kvip_amd.LogitProcessor(torch, batch=n, max_tokens=rows, vocab=vocab, device="cuda")
+    op.bind(device(torch, x, dtype_of(torch, dtype)), device(torch, np.arange(n + 1) * (rows // n), torch.int32), history=history,
+            temperature=torch.zeros(n, device="cuda"), repetition=device(torch, r, torch.float32), **kw)
+    got = host(op())[last]
+    assert np.array_equal(got.argmax(1), np.full(n, first)) and np.all(np.count_nonzero(got, axis=1) == 1)
+    assert int(op.status.item()) == 0
+
+
+@pytest.mark.parametrize("vocab", [700, 30000])
+def test_equal_tokens_get_equal_sums(torch_gpu, vocab):
+    """Tokens of one logit, all held and written as often, of which a bias of 0 names some: the first wins, whether it is
+    named or not, with penalties that no 32-bit number is."""
+    torch = torch_gpu
+    say(f"case equal sums vocab={vocab}")
+    rng = np.random.default_rng(vocab)
+    n = 64
+    x = np.full((n, vocab), -30.0, np.float32)
+    held = np.sort(np.stack([rng.permutation(vocab)[:6] for _ in range(n)]), axis=1)
+    x[np.arange(n)[:, None], held] = rng.uniform(0.5, 9, (n, 1)).astype(np.float32)
+    history = kvip_amd.TokenHistory(torch, batch=n, vocab=vocab, device="cuda")
+    history.load(device(torch, range(n), torch.int32), device(torch, np.repeat(held, 3, axis=1).reshape(-1), torch.int64),
+                 device(torch, np.arange(n + 1) * 18, torch.int32), torch.zeros(n, dtype=torch.int32, device="cuda"))
+    numbers = {k: device(torch, rng.uniform(low, high, n), torch.float32) for k, low, high in
+               (("repetition", 1.01, 1.9), ("presence", 0.01, 0.9), ("frequency", 0.01, 0.3))}
+    for named in ((0,), (1, 3), (0, 1, 2, 3, 4, 5), ()):
+        kw = {}
+        if named:
+            kw = dict(bias_tokens=device(torch, held[:, list(named)], torch.int32), bias_values=torch.zeros((n, len(named)), device="cuda"))
+        op = kvip_amd.LogitProcessor(torch, batch=n, max_tokens=n, vocab=vocab, device="cuda")
+        op.bind(device(torch, x, torch.float32), device(torch, range(n + 1), torch.int32), history=history,
+                temperature=torch.zeros(n, device="cuda"), **numbers, **kw)
+        got = host(op())
+        assert np.array_equal(got.argmax(1), held[:, 0]) and np.all(np.count_nonzero(got, axis=1) == 1), named
+
+
 @pytest.mark.parametrize("vocab,biases", [(20000, 4096), (140001, 2000), (3000, 600)])
 def test_tokens_named_twice_repeat_themselves(torch_gpu, vocab, biases):
     """Lists whose entries meet in pairs, from other threads and other waves: every call gives the same bits."""
