@@ -58,7 +58,8 @@ KVIP_DEVICE uint32_t pick(uint32_t on, uint32_t a, uint32_t b) { return (a & on)
 
 KVIP_DEVICE float weight_of(float x, float m, const LogitRow& r) {
     if (r.plain && m < INFINITY) return __builtin_amdgcn_exp2f((x - m) * r.c);
-    return x == m ? 1.f : x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaxf(x - m, -kLgLargest) * r.c);
+    // Beside an infinite m nothing has weight but its equals, at any temperature.
+    return x == m ? 1.f : x == -INFINITY || m == INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaxf(x - m, -kLgLargest) * r.c);
 }
 
 // All threads' statistics put together, in every thread: largest first, then sums and places under it.

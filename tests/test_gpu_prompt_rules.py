@@ -145,3 +145,24 @@ def test_one_token_of_many_named_twice(torch_gpu):
     op = s.op()
     s.check(op())
     assert int(op.status.item()) == 0
+
+
+@pytest.mark.parametrize("vocab", [40, 30000])
+@pytest.mark.parametrize("listed", [False, True])
+def test_infinite_logits_take_the_row_at_any_temperature(torch_gpu, vocab, listed):
+    """Tokens at +infinity share their row, others get nothing, under temperatures up to infinity."""
+    torch = torch_gpu
+    say(f"case infinite logits vocab={vocab} listed={listed}")
+    t = device(torch, [math.inf, 3.4e38, 1e37, 1e30, 1.0, 1e-30, 1e-42, 0.0], torch.float32)
+    x = torch.randn((8, vocab), generator=torch.Generator().manual_seed(2)).cuda()
+    kw = {}
+    if listed:
+        kw = dict(bias_tokens=device(torch, [[7, 30]] * 8, torch.int32), bias_values=torch.full((8, 2), math.inf, device="cuda"))
+    else:
+        x[:, 7] = x[:, 30] = math.inf
+    op = kvip_amd.LogitProcessor(torch, batch=8, max_tokens=8, vocab=vocab, device="cuda")
+    got = host(op.bind(x, device(torch, range(9), torch.int32), temperature=t, **kw)())
+    want = np.zeros((8, vocab))
+    want[:, 7] = want[:, 30] = 0.5
+    want[7, 7], want[7, 30] = 1.0, 0.0
+    assert np.array_equal(got, want) and int(op.status.item()) == 0
