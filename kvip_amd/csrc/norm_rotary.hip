@@ -34,14 +34,19 @@ KVIP_DEVICE float under_scale(float x, float scale) {  // for any scale
     x /= scale;
     return x > 448.f ? 448.f : x < -448.f ? -448.f : x;
 }
-// Four features' codes. Times the scale's reciprocal a feature is off by two roundings of 2^-24, far less than what
-// its code can hold, and at most 448 but for those, which the conversion rounds away; a scale below the normal
-// range has no exact enough reciprocal.
+// Four features' codes. A quotient is the product with the scale's reciprocal and what that leaves over, which is the rounded
+// quotient, and at most 448 but for a rounding, which the conversion rounds away. (The product alone is off by two roundings
+// and sends features that are half-way between two codes to either.) A scale so small that what is left over would be below the
+// normal range, or one that is infinite, takes divisions.
+KVIP_DEVICE float by_reciprocal(float x, float scale, float reciprocal) {
+    const float product = x * reciprocal;
+    return fmaf(fmaf(-product, scale, x), reciprocal, product);
+}
 KVIP_DEVICE int head_codes(const float (&x)[4], float scale, float reciprocal) {
     int packed = 0;
-    if (scale >= 0x1p-126f && scale < INFINITY) {
-        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * reciprocal, x[1] * reciprocal, packed, false);
-        return __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * reciprocal, x[3] * reciprocal, packed, true);
+    if (scale >= 0x1p-100f && scale < INFINITY) {
+        packed = __builtin_amdgcn_cvt_pk_fp8_f32(by_reciprocal(x[0], scale, reciprocal), by_reciprocal(x[1], scale, reciprocal), packed, false);
+        return __builtin_amdgcn_cvt_pk_fp8_f32(by_reciprocal(x[2], scale, reciprocal), by_reciprocal(x[3], scale, reciprocal), packed, true);
     }
     packed = __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[0], scale), under_scale(x[1], scale), packed, false);
     return __builtin_amdgcn_cvt_pk_fp8_f32(under_scale(x[2], scale), under_scale(x[3], scale), packed, true);

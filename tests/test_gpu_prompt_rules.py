@@ -166,3 +166,37 @@ def test_infinite_logits_take_the_row_at_any_temperature(torch_gpu, vocab, liste
     want[:, 7] = want[:, 30] = 0.5
     want[7, 7], want[7, 30] = 1.0, 0.0
     assert np.array_equal(got, want) and int(op.status.item()) == 0
+
+
+# --- norm and rotation -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("exponent", [0, 3, -40, 90, -105, -124])
+@pytest.mark.parametrize("half", [False, True])
+def test_codes_of_features_half_way_between_two(torch_gpu, exponent, half):
+    """Features that are exactly half-way between two codes times the head's scale go to the even one, whatever the scale.
+    Every number is exact in 32 bits, so that there is one answer."""
+    torch = torch_gpu
+    say(f"case half-way codes 2^{exponent} half={half}")
+    scales = (np.arange(128, 256) / 128).astype(np.float32)
+    scales = scales[scales * np.float32(448) / np.float32(448) == scales]
+    values = np.concatenate([np.arange(17, 32, 2) * 2.0 ** k for k in (-3, 0, 3)] + [[448.0, 0.0]])
+    heads = np.zeros((len(scales), 128))
+    heads[:, :len(values)] = values
+    heads[:, 64:64 + len(values)] = -values
+    x = (heads * scales[:, None] * 2.0 ** exponent).astype(np.float32)
+    assert np.array_equal(x.astype(np.float64), heads * scales[:, None] * 2.0 ** exponent)
+    want, scale = prompt.codes(heads)
+    assert np.all(scale == 1)
+    n = len(scales)
+    turn = kvip_amd.Rotary(torch, rotary_dim=64, layout="half" if half else "interleaved", device="cuda")
+    op = kvip_amd.NormRotary(torch, rotary=turn, dim=128)
+    codes, factor = torch.zeros((n, 1, 128), dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros((n, 1), device="cuda")
+    pages, page_scales = torch.zeros((1, 128, 128), dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros((1, 128), device="cuda")
+    heads = device(torch, x[:, None], torch.float32)
+    op.bind(torch.zeros(n, dtype=torch.int64, device="cuda"), heads, heads.clone(), query_out=codes, query_scale=factor,
+            slots=torch.arange(n, device="cuda"), key_cache=pages, key_scales=page_scales)()
+    for got, s in ((codes[:, 0], factor[:, 0]), (pages[0, :n], page_scales[0, :n])):
+        assert np.array_equal(host(s), scales * 2.0 ** exponent)
+        assert np.array_equal(host(got.float()), want)
+    assert int(op.status.item()) == 0
