@@ -42,7 +42,8 @@ extern "C" {
  * a value that is no finite 32-bit number becomes NaN as a whole (a rotary feature that is not finite reaches the
  * logits as it is). Blocks outside the cache set KVIP_STATUS_BAD_BLOCK and
  * count as not there; lengths outside 0 .. max_blocks * 128, fewer rows than chunk tokens, or cu_seqlens that
- * fall or leave 0 .. max_tokens set KVIP_STATUS_BAD_LENGTH (they are cut to the range). So does a request
+ * fall or leave 0 .. max_tokens set KVIP_STATUS_BAD_LENGTH (they are cut to the range; a row of several requests goes with
+ * the first of them, but where kvip_hip_tree_attention does the work, see below). So does a request
  * whose rows and those of the requests before it, each request's rounded up to 32, are more than max_rows rounded up
  * to 32 plus 32 * batch: it sees nothing. With steps, a request with steps[b] <= 0 (one that
  * kvip_hip_page_tables_extend refused) sees nothing: output 0, lse -infinity. Rows of output and lse behind

@@ -152,6 +152,13 @@ KVIP_DEVICE ChunkRequest ca_request(const KvipChunkAttnArgs& p, int b, uint32_t*
     }
     return q;
 }
+// Without the rows that an earlier request has, which come first (cu_seqlens that fall): `from` is the first row that is its own.
+KVIP_DEVICE ChunkRequest ca_own(ChunkRequest q, int from) {
+    const int taken = min(max(from - q.begin, 0), q.tokens);
+    q.begin += taken;
+    q.tokens -= taken;
+    return q;
+}
 KVIP_DEVICE int ca_row_tiles(const ChunkRequest& q, int heads) { return (q.tokens * heads + kCaTileRows - 1) / kCaTileRows; }
 KVIP_DEVICE int ca_steps(const ChunkRequest& q) { return q.tokens > 0 ? (q.length + kCaTile - 1) / kCaTile : 0; }
 
@@ -184,6 +191,7 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
     uint32_t err = 0;
     int steps[kPer];
     uint32_t sum = 0, sum_tiles = 0, total, total_tiles;
+    bool fall = false;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = tid * kPer + i;
@@ -192,6 +200,7 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
             const ChunkRequest q = ca_request(p, b, &err);
             steps[i] = ca_steps(q);
             sum_tiles += ca_row_tiles(q, p.heads);
+            fall |= p.cu_seqlens[b + 1] < p.cu_seqlens[b];
         }
         sum += steps[i];
     }
@@ -214,13 +223,36 @@ __global__ __launch_bounds__(kCaThreads) void chunk_expand_kernel(const KvipChun
             s_work = 0;
         }
         if (tid < kCaMostCuts) s_units[tid] = 0;
-        __syncthreads();
+        // Where cu_seqlens fall, several requests have the same rows, and the launches have no workgroups for more than max_tokens:
+        // each row goes with the first of them. (The images are laid out all the same.)
+        int* s_own = reinterpret_cast<int*>(s_image);  // first row of each request's own, where they fall
+        const bool falls = __syncthreads_or(fall) != 0;
+        if (falls) {
+            if (tid == 0) {
+                int behind = 0;
+                for (int b = 0; b < p.batch; ++b) {
+                    uint32_t none = 0;
+                    const ChunkRequest q = ca_request(p, b, &none);
+                    s_own[b] = behind;
+                    behind = max(behind, q.begin + q.tokens);
+                }
+            }
+            __syncthreads();
+            sum_tiles = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int b = tid * kPer + i;
+                uint32_t none = 0;
+                if (b < p.batch) sum_tiles += ca_row_tiles(ca_own(ca_request(p, b, &none), s_own[b]), p.heads);
+            }
+        }
         block_exclusive_scan(sum_tiles, s_sums, &total_tiles);
         // Requests by their context, the longest first, so that what is left at the end is short.
         for (int b = tid; b < p.batch; b += kCaThreads) {
             uint32_t none = 0;
-            const ChunkRequest q = ca_request(p, b, &none);
+            ChunkRequest q = ca_request(p, b, &none);
             const int steps_b = ca_steps(q);
+            if (falls) q = ca_own(q, s_own[b]);
             int rank = 0;
             for (int i = 0; i < p.batch; ++i) {
                 const int other = s_before[i + 1] - s_before[i];

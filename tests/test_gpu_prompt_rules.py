@@ -200,3 +200,32 @@ def test_codes_of_features_half_way_between_two(torch_gpu, exponent, half):
         assert np.array_equal(host(s), scales * 2.0 ** exponent)
         assert np.array_equal(host(got.float()), want)
     assert int(op.status.item()) == 0
+
+
+# --- attention -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,counts,contexts,cu", [
+    (128, [1000, 0, 900, 0, 1000], [1000, 0, 600, 0, 100], [0, 1000, 100, 1000, 100, 1100]),
+    (16, [100, 0, 90, 0, 90, 0, 100], [9000, 0, 9000, 0, 9000, 0, 8000], [0, 100, 10, 100, 10, 100, 10, 110])])
+def test_rows_that_several_requests_claim_are_the_first_ones(torch_gpu, heads, counts, contexts, cu):
+    """cu_seqlens that fall: every row is written, by the first request that has it, and the status says so."""
+    torch = torch_gpu
+    say(f"case claimed rows heads={heads} cu={cu}")
+    step = Chunks(torch, np.random.default_rng(heads), counts, contexts, heads)
+    step.cu, step.tokens = np.asarray(cu, np.int32), cu[-1] + 5
+    step.query = step.query[:step.tokens].contiguous()
+    op = step.run()
+    got, lse, q = host(op()), host(op.lse), step.query.double().numpy()
+    assert int(op.status.item()) == abi.STATUS_BAD_LENGTH
+    last, shared = len(counts) - 1, max(cu[:-1])
+    for b, rows in ((0, (0, cu[2] - 1, cu[2], cu[1] - 1)), (last, (shared, shared + 3, cu[-1] - 1))):
+        key, value, odd = prompt.features(step.rows[[step.slot(b, p) for p in range(step.lens[b])]])
+        assert not odd.any()
+        for row in rows:
+            sees = step.lens[b] - (cu[b + 1] - row) + 1
+            want, want_lse, bound, lse_bound = prompt.attention(q[row], key[:sees], value[:sees], SCALE)
+            assert np.all(np.abs(got[row] - want) <= bound + np.abs(want) * 2.0 ** -8), (b, row)
+            assert np.all(np.abs(lse[row] - want_lse) <= lse_bound), (b, row)
+    assert not np.any(np.all(got[:cu[-1]] == 3.0, axis=(1, 2)))
+    assert np.all(got[cu[-1]:] == 3.0) and np.all(lse[cu[-1]:] == 3.0)
