@@ -229,3 +229,30 @@ def test_rows_that_several_requests_claim_are_the_first_ones(torch_gpu, heads, c
             assert np.all(np.abs(lse[row] - want_lse) <= lse_bound), (b, row)
     assert not np.any(np.all(got[:cu[-1]] == 3.0, axis=(1, 2)))
     assert np.all(got[cu[-1]:] == 3.0) and np.all(lse[cu[-1]:] == 3.0)
+
+
+def test_a_long_request_keeps_its_sums(torch_gpu):
+    """2^20 rows, one page over and over: that page's attention, with log(2^13) more in the log-sum-exp.
+
+    The plan cuts a lone long request into 32 segments of 1024 tiles of 32 rows. A sum of probabilities is 16 terms per tile and
+    lane, then 1024 additions, then 2 lanes and 32 parts, each off by 2^-24 of the sum at most: (16 + 1024 + 33) 2^-24 <
+    2^-13.8. An output sum is 2 matrix products per tile with at most 16 roundings each: 2^15 2^-24 = 2^-9 of the
+    sum of magnitudes; features are positive here, so that this is the output's own size."""
+    torch = torch_gpu
+    say("case long sums")
+    rng = np.random.default_rng(31)
+    step = Chunks(torch, rng, [1], [127], 16, spare=0)
+    step.rows[:, :512] &= 0x7F  # positive features
+    key, value, odd = prompt.features(step.rows)
+    assert not odd.any() and len(step.rows) == 128 and np.all(value >= 0)
+    length = 1 << 20
+    op = kvip_amd.ChunkAttention(torch, batch=1, heads=16, max_tokens=71, max_context=length, device="cuda", output_dtype=torch.float32, lse=True)
+    op.bind(step.query.cuda(), torch.from_numpy(step.rows).cuda().view(1, 128, -1), torch.zeros((1, length // 128), dtype=torch.int32, device="cuda"),
+            device(torch, [length], torch.int32), device(torch, [0, 1], torch.int32))
+    got, lse = host(op())[0], host(op.lse)[0]
+    # Each probability's rounding to fp16 is in the page's own bound: it is the same one in every repetition, 2^-36 of the largest
+    # feature per row among the smallest.
+    want, want_lse, bound, lse_bound = prompt.attention(step.query.double().numpy()[0], key, value, SCALE)
+    assert np.all(np.abs(got - want) <= bound + want * (2.0 ** -9 + 2.0 ** -13.8))
+    assert np.all(np.abs(lse - (want_lse + math.log(length // 128))) <= lse_bound + 2.0 ** -13.8 + 20 * 2.0 ** -23)
+    assert int(op.status.item()) == 0
