@@ -844,7 +844,17 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the loads past the last tile
 
     const float l_all = ldexpf(ca_half_sum(l_sum), -kCaLift);
-    const float share = ldexpf(whole ? ca_share(l_all) : 1.f, exponent - kCaLift);
+    // The smallest exponents are taken in two steps, so that the share is an ordinary number.
+    const int below = min(exponent + 64, 0);
+    if (__ballot(below != 0) != 0ull) {
+#pragma unroll
+        for (int f = 0; f < kCaBlocks; ++f) {
+            ca_hold(o[f]);
+            o[f] *= ldexpf(1.f, below);
+            ca_hold(o[f]);
+        }
+    }
+    const float share = ldexpf(whole ? ca_share(l_all) : 1.f, exponent - below - kCaLift);
     int hn_ = hn;
     asm volatile("" : "+v"(hn_));  // what comes of it is not held over the tile loop
     f32x4* part = work.sums + (static_cast<int64_t>(blockIdx.x) * kCaWaves + w) * (kCaBlocks * 4 * 64) + lane;

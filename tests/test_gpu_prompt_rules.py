@@ -9,8 +9,8 @@ import pytest
 import kvip_amd
 from kvip_amd.runtime import abi
 from oracle import prompt
-from tests.test_gpu_draft import SCALE, device, dtype_of, host, say
-from tests.test_gpu_prompt import Chunks, Sampling
+from tests.test_gpu_draft import HALF_STEP, SCALE, device, dtype_of, host, say
+from tests.test_gpu_prompt import LOWEST, Chunks, Sampling
 
 pytestmark = pytest.mark.gpu
 
@@ -256,3 +256,30 @@ def test_a_long_request_keeps_its_sums(torch_gpu):
     assert np.all(np.abs(got - want) <= bound + want * (2.0 ** -9 + 2.0 ** -13.8))
     assert np.all(np.abs(lse - (want_lse + math.log(length // 128))) <= lse_bound + 2.0 ** -13.8 + 20 * 2.0 ** -23)
     assert int(op.status.item()) == 0
+
+
+@pytest.mark.parametrize("power", [-60, -112, -120, -126, -133])
+@pytest.mark.parametrize("output", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads,counts,contexts", [(16, [70, 3], [900, 40]), (4, [20, 50], [9000, 10])])
+def test_chunk_attention_of_rows_near_the_end_of_the_range(torch_gpu, power, output, heads, counts, contexts):
+    """Rows whose features come near the smallest normal number, and pass it: outputs as exact as elsewhere, but
+    for a step of 2^-149 (bf16: 2^-133) at each of two roundings."""
+    torch = torch_gpu
+    say(f"case chunk small rows 2^{power} {output} counts={counts}")
+    step = Chunks(torch, np.random.default_rng(heads), counts, contexts, heads)
+    scales = step.rows[:, 640:656].copy().view("<f4")
+    used = np.isfinite(scales).all(1)
+    scales[used] = 2.0 ** power
+    step.rows[:, 640:656] = scales.astype("<f4").view(np.uint8)
+    step.rows[used, 512:640] = 0  # rotary features
+    op = step.run(output=output)
+    got, q = host(op()), step.query.double().numpy()
+    for b, n in enumerate(counts):
+        key, value, odd = prompt.features(step.rows[[step.slot(b, p) for p in range(step.lens[b])]])
+        assert not odd.any()
+        for i in sorted({0, n // 2, n - 1}):
+            row, sees = step.cu[b] + i, step.lens[b] - n + i + 1
+            want, _, bound, _ = prompt.attention(q[row], key[:sees], value[:sees], SCALE)
+            bound = bound + np.abs(want) * HALF_STEP[output] + 2 * LOWEST[output] + 2.0 ** -148
+            assert np.all(np.abs(got[row] - want) <= bound), (b, i, float((np.abs(got[row] - want) / bound).max()))
+            assert np.abs(want).max() > 2.0 ** (power - 3)
