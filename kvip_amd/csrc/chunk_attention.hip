@@ -102,14 +102,14 @@ struct ChunkPlan {
 
 // Workspace: plan, then per image (rows with values that are no finite numbers, rows that are not there, code: four times
 // the exponent, plus 2 where there are such rows, plus 1 where its rows have exponents of their own) and the rows'
-// exponents, then the images, then the parts: 32 rows x 512 sums per wave as its lanes hold them
+// exponents, then the images, then the parts: 32 rows x 512 outputs of the part per wave as its lanes hold them
 // ([block][quarter][lane] 16 bytes), then their (maximum, sum) pairs.
 struct ChunkWork {
     ChunkPlan* plan;
     uint4* flags;
     int16_t* exponents;
     uint8_t* images;
-    f32x4* sums;
+    f32x4* outputs;
     float2* states;
 };
 __host__ __device__ inline int64_t ca_images(int64_t max_rows, int batch) { return (max_rows + kCaTile - 1) / kCaTile + batch; }
@@ -127,7 +127,7 @@ __host__ __device__ inline ChunkWork ca_work(void* base, int64_t images, size_t*
     w.flags = reinterpret_cast<uint4*>(take(static_cast<size_t>(images) * sizeof(uint4)));
     w.exponents = reinterpret_cast<int16_t*>(take(static_cast<size_t>(images) * kCaTile * sizeof(int16_t)));
     w.images = take(static_cast<size_t>(images) * kCaImage);
-    w.sums = reinterpret_cast<f32x4*>(take(static_cast<size_t>(kCaUnits) * kCaWaves * kCaBlocks * 4 * 64 * sizeof(f32x4)));
+    w.outputs = reinterpret_cast<f32x4*>(take(static_cast<size_t>(kCaUnits) * kCaWaves * kCaBlocks * 4 * 64 * sizeof(f32x4)));
     w.states = reinterpret_cast<float2*>(take(static_cast<size_t>(kCaUnits) * kCaTileRows * sizeof(float2)));
     if (bytes != nullptr) *bytes = at;
     return w;
@@ -854,10 +854,10 @@ __global__ __launch_bounds__(kCaThreads, 1) void chunk_attention_kernel(const Kv
             ca_hold(o[f]);
         }
     }
-    const float share = ldexpf(whole ? ca_share(l_all) : 1.f, exponent - below - kCaLift);
+    const float share = ldexpf(ca_share(l_all), exponent - below - kCaLift);
     int hn_ = hn;
     asm volatile("" : "+v"(hn_));  // what comes of it is not held over the tile loop
-    f32x4* part = work.sums + (static_cast<int64_t>(blockIdx.x) * kCaWaves + w) * (kCaBlocks * 4 * 64) + lane;
+    f32x4* part = work.outputs + (static_cast<int64_t>(blockIdx.x) * kCaWaves + w) * (kCaBlocks * 4 * 64) + lane;
 #pragma unroll
     for (int f = 0; f < kCaBlocks; ++f) {
         ca_hold(o[f]);
@@ -910,7 +910,7 @@ __global__ __launch_bounds__(kCaThreads) void chunk_join_kernel(const KvipChunkA
     constexpr int kRun = kCaBlocks / 4;  // fours of features of a wave
     constexpr int kAtOnce = 4;           // parts whose loads are issued together
     const int at = (slice * kCaWaves + w) * kRun;
-    const f32x4* sums = work.sums + (static_cast<int64_t>(unit) * kCaWaves + rg) * (kCaBlocks * 4 * 64) + at * 64 + lane;
+    const f32x4* outputs = work.outputs + (static_cast<int64_t>(unit) * kCaWaves + rg) * (kCaBlocks * 4 * 64) + at * 64 + lane;
     float m = -INFINITY, l = 0.f;
     f32x4 x[kRun] = {};
     for (int first = 0; first < parts; first += kAtOnce) {
@@ -923,31 +923,36 @@ __global__ __launch_bounds__(kCaThreads) void chunk_join_kernel(const KvipChunkA
             if (first + i >= parts) continue;
             state[i] = states[(first + i) * kCaTileRows];
 #pragma unroll
-            for (int j = 0; j < kRun; ++j) y[i][j] = __builtin_nontemporal_load(sums + (static_cast<int64_t>(first + i) * kCaWaves * (kCaBlocks * 4) + j) * 64);
+            for (int j = 0; j < kRun; ++j) y[i][j] = __builtin_nontemporal_load(outputs + (static_cast<int64_t>(first + i) * kCaWaves * (kCaBlocks * 4) + j) * 64);
         }
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) most = fmaxf(most, state[i].x);
-        const float keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - most);
-        l *= keep;
+        const float keep = most == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - most);
+        l = keep;
+        float weight[kAtOnce];
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) x[j] *= keep;
+        for (int i = 0; i < kAtOnce; ++i) {
+            // A part without a maximum has no outputs, but may be NaN as a whole.
+            weight[i] = state[i].x == -INFINITY ? state[i].y : state[i].y * __builtin_amdgcn_exp2f(state[i].x - most);
+            l += weight[i];
+        }
+        // Outputs so far are outputs, not sums: no row is too large for them.
+        const float share = ca_share(l);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) x[j] *= keep * share;
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
             if (first + i >= parts) break;
-            // A part without a maximum has no sums, but may be NaN as a whole.
-            const float weight = state[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[i].x - most);
-            l += state[i].x == -INFINITY ? state[i].y : state[i].y * weight;
 #pragma unroll
-            for (int j = 0; j < kRun; ++j) x[j] += y[i][j] * weight;
+            for (int j = 0; j < kRun; ++j) x[j] += y[i][j] * (weight[i] * share);
         }
         m = most;
     }
-    const float factor = ca_share(l);
     const int64_t out_row = static_cast<int64_t>(q.begin) * p.heads + row;
     if (row >= rows) return;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-        ca_store(p, out_row * kCaValue + (at + j) / 4 * 32 + (at + j) % 4 * 8 + (lane >> 5) * 4, x[j] * factor);
+        ca_store(p, out_row * kCaValue + (at + j) / 4 * 32 + (at + j) % 4 * 8 + (lane >> 5) * 4, x[j]);
     }
     if (slice == 0 && threadIdx.x < kCaRows && p.lse != nullptr) p.lse[out_row] = ca_lse(m, l);
 }

@@ -258,20 +258,23 @@ def test_a_long_request_keeps_its_sums(torch_gpu):
     assert int(op.status.item()) == 0
 
 
-@pytest.mark.parametrize("power", [-60, -112, -120, -126, -133])
+@pytest.mark.parametrize("power", [-60, -112, -120, -126, -133, 112, 118])
 @pytest.mark.parametrize("output", ["fp32", "bf16"])
 @pytest.mark.parametrize("heads,counts,contexts", [(16, [70, 3], [900, 40]), (4, [20, 50], [9000, 10])])
-def test_chunk_attention_of_rows_near_the_end_of_the_range(torch_gpu, power, output, heads, counts, contexts):
-    """Rows whose features come near the smallest normal number, and pass it: outputs as exact as elsewhere, but
+def test_chunk_attention_of_rows_near_the_ends_of_the_range(torch_gpu, power, output, heads, counts, contexts):
+    """Rows whose features come near the smallest normal number, and pass it, or near the largest (under queries that keep the
+    logits ordinary): outputs as exact as elsewhere, but
     for a step of 2^-149 (bf16: 2^-133) at each of two roundings."""
     torch = torch_gpu
-    say(f"case chunk small rows 2^{power} {output} counts={counts}")
+    say(f"case chunk rows of 2^{power} {output} counts={counts}")
     step = Chunks(torch, np.random.default_rng(heads), counts, contexts, heads)
     scales = step.rows[:, 640:656].copy().view("<f4")
     used = np.isfinite(scales).all(1)
     scales[used] = 2.0 ** power
     step.rows[:, 640:656] = scales.astype("<f4").view(np.uint8)
     step.rows[used, 512:640] = 0  # rotary features
+    if power > 0:
+        step.query = (step.query.float() * 2.0 ** -power).to(torch.bfloat16)
     op = step.run(output=output)
     got, q = host(op()), step.query.double().numpy()
     for b, n in enumerate(counts):
@@ -283,3 +286,16 @@ def test_chunk_attention_of_rows_near_the_end_of_the_range(torch_gpu, power, out
             bound = bound + np.abs(want) * HALF_STEP[output] + 2 * LOWEST[output] + 2.0 ** -148
             assert np.all(np.abs(got[row] - want) <= bound), (b, i, float((np.abs(got[row] - want) / bound).max()))
             assert np.abs(want).max() > 2.0 ** (power - 3)
+
+
+def test_chunk_attention_of_nothing_but_nan(torch_gpu):
+    """Long contexts whose rotary features are all NaN, or NaN in one row of the first segment, cut into many parts."""
+    torch = torch_gpu
+    say("case chunk NaN parts")
+    step = Chunks(torch, np.random.default_rng(17), [2, 3], [9000, 9000], 4)
+    used = [step.slot(0, p) for p in range(step.lens[0])]
+    step.rows[used, 512:640] = 0xFF
+    step.rows[step.slot(1, 5), 512:514] = [0xC0, 0x7F]
+    op = step.run()
+    got, lse = host(op()), host(op.lse)
+    assert np.all(np.isnan(got[:5])) and np.all(np.isnan(lse[:5])) and int(op.status.item()) == 0
