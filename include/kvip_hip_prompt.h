@@ -50,7 +50,9 @@ extern "C" {
  * cu_seqlens[batch] are left as they were. A workspace serves one call at a time, and the lengths stay as
  * they are while it runs.
  * Where max_tokens is at most 64 and max_tokens * heads at most 512 * batch, kvip_hip_tree_attention does the work
- * (without visible): it rounds probabilities times scales, not features, and max_rows does not count. */
+ * (without visible): it rounds probabilities times scales to bf16 (2^-8), not features, holds weighted sums of values as they are
+ * (which values of 10^35 and more on some rows take past 32 bits), and max_rows does not count. Elsewhere the workspace has 1152
+ * bytes for each of max_rows and of 32 rows per request, and 269 MB for the parts of contexts that are cut. */
 typedef struct KvipChunkAttnArgs {
     const uint16_t* query;        /* [max_tokens, heads, 576] bf16, 16-byte aligned */
     const uint8_t* kv_cache;      /* 16-byte aligned */

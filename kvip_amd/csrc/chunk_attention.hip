@@ -12,7 +12,7 @@
 // exponent of its largest feature, each row under its own where the rows are far apart (what a token sees must not depend
 // on what it does not); the sums of a row of the problem stand under the largest exponent of the cached rows that
 // it has seen, and probabilities are lifted to the top of the range. bf16 was 10 % faster (6.83 instead of 7.63
-// ms on the second of the cases below): the card holds 1.8 GHz under either, as little as its power allows.
+// ms on the second of the cases below), the card at 1.8 GHz under either.
 //
 // A workgroup of 4 waves takes 128 rows of the problem, 32 per wave; a wave keeps its queries (144 registers) and its
 // 32 x 512 sums (the 256 accumulation registers; one wave per SIMD has 512 in all). Logits are computed transposed (cached
@@ -25,15 +25,21 @@
 // LDS four products ahead, across the borders of the two; the barrier for the tile after next stands where a tile's last
 // reads are done.
 //
-// Few row tiles over long contexts are cut along the context into segments, whose parts a third launch joins. Requests
-// are taken the longest first.
+// Few row tiles over long contexts are cut along the context into segments, whose parts a third launch joins: outputs of the
+// segment's rows alone with their sums, as weighted sums of large values would pass 32 bits. Requests are taken the longest
+// first.
 //
-// What bounds it. 2048 tokens x 128 heads on 8192 rows: 3.52 ms, 1160 TFLOP/s, and 4096 tokens x 16 heads on 65536
-// rows: 7.63 ms, 1180 TFLOP/s, of the 1360 of a large fp16 product: power (an MFMA is under way in 64 % of the cycles
-// at 1.78 GHz; fewer cycles per tile lower the clock); laying the rows out takes 11 and 26 us of that. 12 requests of
-// 1-700 tokens x 16 heads on up to 16000 rows: 1.17 ms, 1010 TFLOP/s, as the longest workgroup takes as long as the
-// mean CU. 130 tokens x 16 heads on 1030 rows: 6 + 22 + 8 us, chains of latencies (plan, images, queries to fp16,
-// five tiles, parts, join).
+// What bounds it. 2048 tokens x 128 heads on 8192 rows: 3.4-3.5 ms, 1170-1200 TFLOP/s, and 4096 tokens x 16 heads on 65536
+// rows: 7.4-7.7 ms, 1170-1220 TFLOP/s, of the 1360 of a large fp16 product (on another card 4.0 and 8.7 ms): an MFMA is under
+// way in 64 % of the cycles, at 1.78 GHz. The LDS is as busy, since every MFMA takes 1 KB from it, which four SIMDs without a pause
+// would make all of its 128 bytes a cycle; without half of these reads the second case took 6 % less (wrong results, for
+// the time alone). The clock is the card's answer to its power, and waves wait in 26 % of their cycles. Laying the rows out takes 11
+// and 26 us. 12 requests of 1-700 tokens x 16 heads on up to 16000 rows: 1.14-1.17 ms, 1030 TFLOP/s, as the last workgroup
+// ends 10 % after the mean CU's work. 130 tokens x 16 heads on 1030 rows: 6.5 + 22 + 8.5 us, chains of latencies (plan, images,
+// queries to fp16, five tiles, parts, join).
+// What it does not do: contexts are cut only where the whole batch has at most 512 row tiles, so that one long context among
+// more of them is walked by its workgroups alone, some 1.9 us for every 32 rows; and few-row requests beside others
+// are laid out like these (see ca_few).
 // Dropped after measuring: operands eight products ahead and two accumulators for the logits in turn (both +-0 %), other
 // prices of a part in the plan (+-2 % on small calls).
 #include <type_traits>

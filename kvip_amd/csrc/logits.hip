@@ -13,11 +13,13 @@
 // first reading is the running maximum and sum of a softmax, per thread, without a branch; NaN and infinities are
 // looked for only where the sum is no number.
 //
-// What bounds it. 320 rows of 131072 bf16 logits: 34 + 52 us. The second launch moves 252 MB at 4.8 TB/s; the first is
-// bound by vector instructions (25 per token and lane, of which 9 are the penalties, worked out for a whole wave wherever
-// one of its 512 tokens is held) and by its last round of workgroups. 176 constrained rows of 32000 with 64 biases
-// 10.5 + 13.5 us, one row of 131072 fp32 logits 5.4 + 6 us: chains of latencies (request, its numbers, lists, bits, counts).
-// A token takes its bias from the entry that names it; the list is gone through only where two entries met (11.5 + 15 before).
+// What bounds it. 320 rows of 131072 bf16 logits: 37 + 52 us in turn over one input (some of which the last cache keeps; 104 a
+// pass over others). The second launch moves 252 MB at 4.8 TB/s; the first is bound by vector instructions (28 per token and lane,
+// of which 10 are the penalties, worked out for a whole wave wherever one of its 512 tokens is held) and by its last round
+// of workgroups. 176 constrained rows of 32000 with 64 biases 11 + 14 us, one row of 131072 fp32 logits 5.3 + 6.1 us: chains of
+// latencies (request, its numbers, lists, bits, counts). 8 rows of 30000 with 4096 biases take 18.5 us, 26 with one token
+// named twice, 580 with all of them.
+// A token takes its bias from the entry that names it; the list is gone through only where several entries name one.
 // Dropped after measuring: held tokens taken out of the dense pass and worked out from a list (39 + 87 us; the scattered stores
 // cost more than the penalties), biases staged in LDS (20 % more for the constrained rows), 256 or 1024
 // threads per workgroup (-2 %, +25 %).

@@ -8,8 +8,8 @@
 // head's features under way. Few tokens' heads go over several workgroups, their keys to one of their own.
 //
 // What bounds it: memory for many tokens. 4001 tokens of 32 + 8 normed heads of 128 take 15.5 us (5.3 TB/s; a large copy
-// reaches 5.1), 8192 tokens of 64 index heads 46.5 (4.4 TB/s; 160 vector instructions per 512 features hold the SIMDs for
-// some 36 of these, 305 with exact quotients for every feature's code took 71). 256 tokens of 64 index heads take 5.3
+// reaches 5.1), 8192 tokens of 64 index heads 49 (4.2 TB/s; 177 vector instructions per 512 features hold the SIMDs for
+// some 40 of these, 305 with a division for every feature's code took 71). 256 tokens of 64 index heads take 5.5
 // us, one token 3.5: angles, features, codes, one after the other.
 #include "kvip_hip_prompt.h"
 #include "lane_groups.h"

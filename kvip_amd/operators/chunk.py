@@ -25,8 +25,10 @@ class ChunkAttention:
     workspace allocated once; `bind` validates a call's tensors, `__call__` enqueues it on the current stream
     (capturable; one object's calls follow one another, as they share its workspace). max_tokens: tokens of a call;
     max_context: cached rows of a request, the chunk's among them; max_rows: cached rows of a call's requests
-    together (default batch * max_context), which the workspace holds as fp16, 1152 bytes each (small calls read the
-    cache itself). A request past that gets zeros and sets a status bit."""
+    together (default batch * max_context), which the workspace holds as fp16, 1152 bytes each, beside 269 MB for the parts
+    of contexts that are cut (objects for few rows, up to 64 tokens and 512 * batch of tokens times heads, have neither: up to
+    135 MB, and the cache is read as it is). One object serves layer after layer. A request past max_rows gets zeros and sets a
+    status bit."""
 
     def __init__(self, torch, *, batch, heads, max_tokens, max_context, device, max_rows=None, output_dtype=None, lse=False):
         abi.require(1 <= batch <= abi.DRAFT_MAX_BATCH, f"batch must be in 1..{abi.DRAFT_MAX_BATCH}")
@@ -95,7 +97,9 @@ class ChunkAttention:
 
 def chunk_attention(query, kv_cache, block_table, seq_lens, cu_seqlens, scale=KEY_DIM ** -0.5, *, max_rows=None,
                     output_dtype=None, steps=None):
-    """One chunk-attention call (arguments as `ChunkAttention`); returns [rows, heads, 512]."""
+    """One chunk-attention call (arguments as `ChunkAttention`, whose buffers it allocates); returns [rows, heads, 512]. What is
+    wrong with tables and lengths, requests past max_rows among it, shows in an object's status alone: without max_rows there is
+    room for every request."""
     import torch
 
     op = ChunkAttention(torch, batch=int(seq_lens.shape[0]), heads=int(query.shape[1]), max_tokens=int(query.shape[0]),
